@@ -561,6 +561,25 @@ int sf_from_heads(const void* g, int dtype, int64_t B, int64_t S, int64_t H, int
                   const float* sin, int rotate, int transposed, float scale, void* x_grad, void* stream);
 
 /*
+ * Rotary positions (no counterpart in the reference): the first rotary_dim
+ * elements of every head of q [B, S, heads, D] and k [B, S, kv_heads, D] turn
+ * in pairs (i, i + rotary_dim / 2), or (2 i, 2 i + 1) when `interleaved`, by
+ * the angle of their position, a' = a c - b s, b' = b c + a s in f32, one
+ * rounding; the others are copied.  cos, sin: f32 [table_rows, rotary_dim / 2].
+ * positions: int32 or int64 (position_bytes 4 or 8), entry b * position_sb + s
+ * (position_sb 0: shared by the batch), or null: the position is s.  A position
+ * that the tables do not hold gives NaN.  `inverse` turns the other way: the
+ * adjoint, which carries gradients back.  q and k may be strided (batch,
+ * sequence and head strides in elements; elements of a head contiguous); q_out
+ * and k_out are contiguous.  heads or kv_heads may be 0.  dtype f32 or bf16.
+ */
+int sf_rotary(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, int64_t heads, const void* k, int64_t k_sb,
+              int64_t k_ss, int64_t k_sh, int64_t kv_heads, int dtype, int64_t B, int64_t S, int64_t D,
+              int64_t rotary_dim, int interleaved, const float* cos, const float* sin, int64_t table_rows,
+              const void* positions, int position_bytes, int64_t position_sb, int inverse, void* q_out, void* k_out,
+              void* stream);
+
+/*
  * Causal softmax attention of the retrained model in bf16 with no S x S tensor
  * in memory (HuggingFace's eager attention of the LlamaForCausalLM that
  * legacy/model_llama.py:39-55 wraps, and its first derivative).  q, k, v, out
