@@ -580,6 +580,68 @@ int sf_rotary(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, int64_t h
               void* stream);
 
 /*
+ * A cache of keys and values held in 8 bits (no counterpart in the reference),
+ * for generating with a model.  64 consecutive positions of one sequence and
+ * head are a block: int8 codes with one f32 scale for its keys and one for its
+ * values (value = code * scale, scale = max |x| / 127, code = x / scale rounded
+ * to the nearest, ties to even).  A sequence's last block is held in bf16, as
+ * the rows came, until it is whole, so what the cache holds does not depend on
+ * how many rows are appended at a time.  A token whose key or value of a head
+ * holds a NaN or an infinity becomes NaN there, and so does the block that it
+ * is in once that is whole.
+ * starts and ends [batch] int32 on the device count the tokens held before the
+ * newest ones and with them; the caller advances them.  All entries of a cache
+ * for one layer; sizes in bytes, with Dp = head_dim rounded up to 64:
+ *   codes batch * kv_heads * blocks * 64 * Dp, scales batch * kv_heads * blocks
+ *   * 4, tails batch * kv_heads * 64 * Dp * 2 (codes and tails 16-byte aligned)
+ * head_dim: a multiple of 8 up to 256.
+ */
+typedef struct sf_kv8_cache {
+  void* k_codes;
+  void* v_codes;
+  float* k_scales;
+  float* v_scales;
+  void* k_tail;
+  void* v_tail;
+  const int32_t* starts;
+  const int32_t* ends;
+  int64_t batch, kv_heads, head_dim;
+  int64_t blocks; /* capacity of a sequence in blocks */
+} sf_kv8_cache;
+
+/*
+ * The newest rows of every sequence, positions starts[b] .. ends[b] - 1, from
+ * the first rows of k, v [batch, n, kv_heads, head_dim] bf16 (strides in
+ * elements, heads contiguous, rows 16-byte aligned; at most n per sequence).
+ */
+int sf_kv8_append(const sf_kv8_cache* cache, const void* k, int64_t k_sb, int64_t k_ss, int64_t k_sh, const void* v,
+                  int64_t v_sb, int64_t v_ss, int64_t v_sh, int64_t n, void* stream);
+
+/*
+ * What the cache stands for, f32 k, v [batch, tokens, kv_heads, head_dim]: the
+ * positions from first[b] (null: first_all) on, 0 past a sequence's end.
+ */
+int sf_kv8_values(const sf_kv8_cache* cache, const int32_t* first, int64_t first_all, int64_t tokens, float* k,
+                  float* v, void* stream);
+
+/*
+ * out [batch, n, heads, head_dim] bf16 = softmax(scale q k^T) v of the newest
+ * queries q [batch, n, heads, head_dim] bf16 (strided as k in sf_kv8_append)
+ * over the cached keys: query i of a sequence is at position starts[b] + i and
+ * sees the keys up to it, the last `window` of them if window > 0.  Rows from
+ * ends[b] - starts[b] on are 0.  heads is a multiple of kv_heads: query head h
+ * reads key-value head h / (heads / kv_heads).  bound: an upper bound of ends
+ * known to the host; it sizes the launch (more keys are read correctly, with
+ * fewer workgroups than they deserve).  Scores, sums and outputs are f32, the
+ * probabilities bf16 as operands of the second product.
+ */
+size_t sf_kv8_attend_workspace_size(int64_t batch, int64_t kv_heads, int64_t heads, int64_t head_dim, int64_t n,
+                                    int64_t bound);
+int sf_kv8_attend(const sf_kv8_cache* cache, const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, int64_t n,
+                  int64_t heads, float scale, int64_t window, int64_t bound, void* out, void* workspace,
+                  size_t workspace_bytes, void* stream);
+
+/*
  * Causal softmax attention of the retrained model in bf16 with no S x S tensor
  * in memory (HuggingFace's eager attention of the LlamaForCausalLM that
  * legacy/model_llama.py:39-55 wraps, and its first derivative).  q, k, v, out

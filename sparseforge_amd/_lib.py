@@ -206,6 +206,25 @@ class HutchTensor(ctypes.Structure):
     ]
 
 
+class Kv8Cache(ctypes.Structure):
+    """Mirror of ``sf_kv8_cache``."""
+
+    _fields_ = [
+        ("k_codes", ctypes.c_void_p),
+        ("v_codes", ctypes.c_void_p),
+        ("k_scales", ctypes.c_void_p),
+        ("v_scales", ctypes.c_void_p),
+        ("k_tail", ctypes.c_void_p),
+        ("v_tail", ctypes.c_void_p),
+        ("starts", ctypes.c_void_p),
+        ("ends", ctypes.c_void_p),
+        ("batch", ctypes.c_int64),
+        ("kv_heads", ctypes.c_int64),
+        ("head_dim", ctypes.c_int64),
+        ("blocks", ctypes.c_int64),
+    ]
+
+
 class AdamwParams(ctypes.Structure):
     """Mirror of ``sf_adamw_params``."""
 
@@ -272,6 +291,10 @@ SIGNATURES = {
     "sf_attention_backward": (_I, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _F, _P, _P, _P, _P, _P]),
     "sf_rotary": (_I, [_P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I, _I64, _I64, _I64, _I64, _I, _P, _P,
                        _I64, _P, _I, _I64, _I, _P, _P, _P]),
+    "sf_kv8_append": (_I, [ctypes.POINTER(Kv8Cache), _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P]),
+    "sf_kv8_values": (_I, [ctypes.POINTER(Kv8Cache), _P, _I64, _I64, _P, _P, _P]),
+    "sf_kv8_attend_workspace_size": (_SZ, [_I64, _I64, _I64, _I64, _I64, _I64]),
+    "sf_kv8_attend": (_I, [ctypes.POINTER(Kv8Cache), _P, _I64, _I64, _I64, _I64, _I64, _F, _I64, _I64, _P, _P, _SZ, _P]),
     "sf_transpose_batched": (_I, [_P, _I, _I64, _I64, _I64, _P, _P]),
     "sf_softmax_rows": (_I, [_P, _I, _I64, _I64, _I, _P, _P]),
     "sf_softmax_rows_backward": (_I, [_P, _P, _I, _I64, _I64, _I, _P, _P]),
