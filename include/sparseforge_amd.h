@@ -580,6 +580,27 @@ int sf_rotary(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, int64_t h
               void* stream);
 
 /*
+ * Logits before a token is drawn (no counterpart in the reference): for token t
+ * of a row, in f32 and in this order, rounded once to the dtype (f32 or bf16)
+ *   t occurs c > 0 times in the row's history: x = x > 0 ? x / repetition :
+ *   x * repetition; x -= frequency * c; x -= presence
+ *   x += bias[t];  x = -inf where t is not allowed
+ * logits, out: [rows, vocab], row strides in elements (out may be logits).
+ * history: int32 or int64 ids [rows, history_len] (history_bytes 4 or 8; null:
+ * none), the first history_lengths[row] of a row (null: all) counted, ids
+ * outside the vocabulary not.  repetition, presence, frequency: f32 [rows], or
+ * null: the number beside it.  bias: f32 rows (stride 0: shared), or null.
+ * allowed: bytes (0: not), or with allowed_bits one bit a token, lowest first;
+ * its row stride in bytes (0: shared); null: all.  rows < 65536.
+ */
+int sf_process_logits(const void* logits, int64_t logits_stride, int dtype, int64_t rows, int64_t vocab,
+                      const void* history, int64_t history_stride, int64_t history_len, int history_bytes,
+                      const int32_t* history_lengths, const float* repetition, float repetition_all,
+                      const float* presence, float presence_all, const float* frequency, float frequency_all,
+                      const float* bias, int64_t bias_stride, const void* allowed, int64_t allowed_stride,
+                      int allowed_bits, void* out, int64_t out_stride, void* stream);
+
+/*
  * A cache of keys and values held in 8 bits (no counterpart in the reference),
  * for generating with a model.  64 consecutive positions of one sequence and
  * head are a block: int8 codes with one f32 scale for its keys and one for its

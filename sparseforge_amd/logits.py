@@ -1,0 +1,101 @@
+"""Logits before a token is drawn (sf_process_logits): penalties for repeated tokens, a bias, a mask of the tokens that
+may follow.  No counterpart in the reference, which scores text and does not shape what a model answers.
+
+For token t of a row, in float32 and in this order, rounded once to the logits' type:
+
+    t occurs c > 0 times in the row's history:  x = x / repetition if x > 0 else x * repetition
+                                                x = x - frequency * c;  x = x - presence
+    x = x + bias[t]
+    x = -inf if t is not allowed
+
+A row whose mask allows nothing is -inf throughout.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib as L
+from . import profiling as _prof
+
+
+def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
+                   history_lengths: torch.Tensor | None = None, *, repetition=1.0, presence=0.0, frequency=0.0,
+                   bias: torch.Tensor | None = None, allowed: torch.Tensor | None = None,
+                   out: torch.Tensor | None = None) -> torch.Tensor:
+    """logits [B, V] (bf16 or float32, rows contiguous, e.g. all_logits[:, -1]) -> the processed logits, in `out` if
+    given (logits itself may be given), else in a new tensor.
+
+    history: int32 / int64 [B, n] token ids, the first history_lengths[b] (int32 [B], all where None) of a row counted;
+    ids outside 0 .. V - 1 (padding) are not.  repetition, presence, frequency: a number, or float32 [B] on the device.
+    bias: float32 [V] or [B, V].  allowed: bool [V] or [B, V], or its bits as int32 [ceil(V / 32)] or [B, ceil(V / 32)]
+    (token t is bit t % 32 of word t // 32)."""
+    dev = L.require_device_only(logits, history, history_lengths, bias, allowed, out)
+    dt = L.dtype_code(logits)
+    if logits.dim() != 2:
+        raise ValueError(f"process_logits: logits must be [B, V], got {tuple(logits.shape)}")
+    B, V = logits.shape
+    if logits.stride(1) != 1 and V > 1:
+        logits = logits.contiguous()
+    if out is None:
+        out = torch.empty((B, V), dtype=logits.dtype, device=dev)
+    elif out.shape != (B, V) or out.dtype != logits.dtype or not (out.stride(1) == 1 or V <= 1) \
+            or (B > 1 and out.stride(0) < V):
+        raise ValueError(f"process_logits: out must be {logits.dtype} [{B}, {V}] with rows of its own")
+    n = 0
+    if history is not None:
+        if history.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"process_logits: the history is {history.dtype} (int32 / int64 only)")
+        if history.dim() != 2 or history.shape[0] != B:
+            raise ValueError(f"process_logits: history {tuple(history.shape)} for {B} rows")
+        history = _rows(history)
+        n = history.shape[1]
+        if history_lengths is not None and (history_lengths.dtype != torch.int32 or history_lengths.shape != (B,)):
+            raise ValueError(f"process_logits: history_lengths must be int32 [{B}]")
+    elif history_lengths is not None:
+        raise ValueError("process_logits: history_lengths without a history")
+    given = [_per_row(x, name, B, dev) for x, name in ((repetition, "repetition"), (presence, "presence"),
+                                                       (frequency, "frequency"))]
+    if not torch.is_tensor(repetition) and not repetition > 0:
+        raise ValueError(f"process_logits: a repetition penalty of {repetition}")
+    if bias is not None:
+        if bias.dtype != torch.float32:
+            raise TypeError(f"process_logits: the bias is {bias.dtype} (float32 only)")
+        if bias.shape not in ((V,), (B, V)):
+            raise ValueError(f"process_logits: bias {tuple(bias.shape)} for logits {(B, V)}")
+        bias = _rows(bias)
+    bits = 0
+    if allowed is not None:
+        if allowed.dtype not in (torch.bool, torch.int32):
+            raise TypeError(f"process_logits: allowed is {allowed.dtype} (bool, or int32 words of bits)")
+        bits = int(allowed.dtype == torch.int32)
+        wide = -(-V // 32) if bits else V
+        if allowed.shape not in ((wide,), (B, wide)):
+            raise ValueError(f"process_logits: allowed {tuple(allowed.shape)} for logits {(B, V)}")
+        allowed = _rows(allowed)
+    lengths = history_lengths.contiguous() if history_lengths is not None else None
+    with _prof.region("sf_process_logits", 2 * logits.numel() * logits.element_size(), "B", dev):
+        L.check(L.lib().sf_process_logits(
+            L.ptr(logits), logits.stride(0) if B > 1 else V, dt, B, V, L.ptr(history) if n else None,
+            history.stride(0) if n else 0, n, history.element_size() if n else 0, L.ptr(lengths) if n else None,
+            *given[0], *given[1], *given[2], L.ptr(bias), bias.stride(0) if bias is not None and bias.dim() == 2 else 0,
+            L.ptr(allowed),
+            allowed.stride(0) * allowed.element_size() if allowed is not None and allowed.dim() == 2 else 0, bits,
+            L.ptr(out), out.stride(0) if B > 1 else V, L.stream(dev)), "sf_process_logits")
+    return out
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """t with contiguous rows (any row stride that goes forward)."""
+    return t if t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
+
+
+def _per_row(x, name: str, B: int, dev) -> tuple:
+    """A penalty as the kernel takes it: a pointer to one for each row, or a number."""
+    if not torch.is_tensor(x):
+        return None, float(x)
+    if x.device != dev:
+        L.require_device_only(x)
+        raise ValueError(f"process_logits: {name} is on {x.device}, the logits on {dev}")
+    if x.dtype != torch.float32 or x.shape != (B,) or not (x.is_contiguous()):
+        raise ValueError(f"process_logits: {name} must be a number or a contiguous float32 [{B}]")
+    return x.data_ptr(), 0.0
