@@ -30,10 +30,10 @@ struct AttendArgs {
   int n, heads, group;
   int window;         // 0: none
   float scale;        // times log2 e
-  int tiles;          // of 16 RT rows
+  int rows, tiles;    // rows of a workgroup, and how many times that a (sequence, head) has
   int splits, chunk;  // key blocks of a workgroup: at least `chunk`
-  float* po;          // [B H tiles][splits][16 RT][Dp] unnormalised outputs
-  float* pml;         // [B H tiles][splits][2][16 RT] maxima, sums
+  float* po;          // [B H tiles][splits][rows][Dp] unnormalised outputs
+  float* pml;         // [B H tiles][splits][2][rows] maxima, sums
 };
 
 // What a tile of rows sees.
@@ -44,13 +44,12 @@ struct TileRange {
   int per;                 // blocks of a split
   __device__ __forceinline__ int used() const { return b1 > b0 ? (b1 - b0 + per - 1) / per : 0; }
 };
-template <int ROWS>
-__device__ __forceinline__ TileRange tile_range(const AttendArgs& a, int b, int tile) {
+__device__ __forceinline__ TileRange tile_range(const AttendArgs& a, int rows, int b, int tile) {
   TileRange r;
   kv_range(a.c, b, a.n, r.start, r.end);
   const int cnt = r.end - r.start;
-  r.i0 = tile * ROWS / a.group;
-  r.i1 = min(cnt, (tile * ROWS + ROWS - 1) / a.group + 1);
+  r.i0 = tile * rows / a.group;
+  r.i1 = min(cnt, (tile * rows + rows - 1) / a.group + 1);
   r.b0 = r.b1 = 0;
   r.per = 1;
   if (r.i0 >= r.i1) return r;
@@ -119,6 +118,25 @@ struct TailBlock {
   }
 };
 
+// What a block's scales do to its scores and probabilities.  The value scale goes into the exponent, which costs
+// nothing for each key, and the sum of a row takes it out again.  Where it is far from 1 and the smaller of those
+// probabilities leave the range of floats, the sum is taken without it.  A scale of 0 has codes of 0, for which any
+// other does as well.
+struct BlockScale {
+  float ks;      // of the scores, with log2 e; positive
+  float lv, rv;  // log2 of the value scale, and its reciprocal
+  bool far;
+  bool nan;      // a block of NaN: its scores become NaN
+  __device__ __forceinline__ BlockScale(float k, float v, float scale) {
+    nan = k != k;  // both are
+    ks = k > 0.0f ? k * scale : 1.0f;
+    v = v > 0.0f ? v : 1.0f;
+    far = v < 0x1p-64f || v > 0x1p64f;
+    lv = log2f(v);
+    rv = far ? 0.0f : __builtin_amdgcn_rcpf(v);
+  }
+};
+
 // A wave's rows: queries, running softmax and output, transposed (lane: row lane % 16 of each 16).
 template <int DB, int RT>
 struct RowState {
@@ -127,9 +145,80 @@ struct RowState {
   float m[RT], l[RT];  // l: of the keys this lane's group holds
   int pos[RT];         // position of the row's query, -1: no such row
 
-  template <class Block>
-  __device__ __forceinline__ void block(const Block& x, int blk, float ks, float vs, int window, bool masked) {
+  // The queries of rows row0 + 16 r + lane % 16 (below `rows`) of key-value head h.
+  __device__ __forceinline__ void start(const AttendArgs& a, const TileRange& tr, int b, int h, int row0) {
+    const int lane = threadIdx.x & 63, g = lane >> 4;
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const int row = row0 + r * 16 + (lane & 15), i = row / a.group, hq = h * a.group + row % a.group;
+      const bool real = i < tr.i1;
+      pos[r] = real ? tr.start + i : -1;
+      const uint16_t* src = a.q + b * a.qsb + i * a.qss + hq * a.qsh;
+#pragma unroll
+      for (int hh = 0; hh < DB; ++hh)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int d = hh * 64 + g * 16 + x * 8;
+          const V4 w = real && d < a.c.D ? ld16(src + d) : zero16();
+          q[r][hh][x] = __builtin_bit_cast(bf16x8_t, make_uint4(w.w[0], w.w[1], w.w[2], w.w[3]));
+        }
+#pragma unroll
+      for (int dt = 0; dt < DB * 4; ++dt) o[r][dt] = f32x4_t{};
+      m[r] = kAtnLow;
+      l[r] = 0.0f;
+    }
+  }
+
+  // Scores of a block that some row does not see whole, or that is NaN.
+  __device__ __forceinline__ void hide(int r, f32x4_t (&s)[4], int blk, bool nan, int window) {
     const int g = (threadIdx.x & 63) >> 4;
+    const int hi = pos[r] - blk * kKvBlock - 4 * g, lo = window ? hi - window : -1 - 4 * g;  // seen: lo < key <= hi
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int key = 16 * (i / 4) + i % 4;
+      float x = s[i / 4][i % 4];
+      x = nan ? __builtin_nanf("") : x;
+      s[i / 4][i % 4] = key <= hi && key > lo ? x : -INFINITY;
+    }
+  }
+
+  // Scores of 64 keys of 16 rows -> operands of the second product.
+  __device__ __forceinline__ void softmax(int r, const f32x4_t (&s)[4], const BlockScale& sc, bf16x8_t (&p)[2]) {
+    float mx = s[0][0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i / 4][i % 4]);
+    mx *= sc.ks;
+    if (__builtin_amdgcn_ballot_w64(mx > m[r] + kAtnSlack)) {
+      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+      const float mn = fmaxf(m[r], mx), f = __builtin_amdgcn_exp2f(m[r] - mn);
+      m[r] = mn;
+      l[r] *= f;
+#pragma unroll
+      for (int dt = 0; dt < DB * 4; ++dt) o[r][dt] *= f;
+    }
+    if (sc.far) {
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sum += __builtin_amdgcn_exp2f(fmaf(s[i / 4][i % 4], sc.ks, -m[r]));
+      l[r] += sum;
+    }
+    const float off = sc.lv - m[r];
+    float e[16], sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      e[i] = __builtin_amdgcn_exp2f(fmaf(s[i / 4][i % 4], sc.ks, off));
+      sum += e[i];
+    }
+    l[r] = fmaf(sum, sc.rv, l[r]);
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      p[u] = __builtin_bit_cast(bf16x8_t, make_uint4(pack2(e[8 * u], e[8 * u + 1]), pack2(e[8 * u + 2], e[8 * u + 3]),
+                                                     pack2(e[8 * u + 4], e[8 * u + 5]), pack2(e[8 * u + 6], e[8 * u + 7])));
+  }
+
+  template <class Block>
+  __device__ __forceinline__ void block(const Block& x, int blk, const BlockScale& sc, int window, bool masked) {
     f32x4_t s[RT][4];
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
@@ -144,48 +233,13 @@ struct RowState {
           for (int r = 0; r < RT; ++r) s[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[r][hh][a], s[r][t], 0, 0, 0);
         }
     }
+    if (masked || sc.nan) {
+#pragma unroll
+      for (int r = 0; r < RT; ++r) hide(r, s[r], blk, sc.nan, window);
+    }
     bf16x8_t p[RT][2];
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      uint32_t seen = 0xffffu;  // bit 4 t + e: the row sees key 16 t + 4 g + e
-      if (masked) {
-        seen = 0;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = blk * kKvBlock + 16 * (i / 4) + 4 * g + i % 4;
-          const bool in = key <= pos[r] && (!window || key > pos[r] - window);
-          seen |= in ? 1u << i : 0u;
-        }
-      }
-      float mx = kAtnLow;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const float x = s[r][i / 4][i % 4] * ks;
-        mx = fmaxf(mx, !masked || (seen >> i & 1) ? x : kAtnLow);
-      }
-      if (__builtin_amdgcn_ballot_w64(mx > m[r] + kAtnSlack)) {
-        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        const float mn = fmaxf(m[r], mx), f = __builtin_amdgcn_exp2f(m[r] - mn);
-        m[r] = mn;
-        l[r] *= f;
-#pragma unroll
-        for (int dt = 0; dt < DB * 4; ++dt) o[r][dt] *= f;
-      }
-      float e[16];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        e[i] = __builtin_amdgcn_exp2f(fmaf(s[r][i / 4][i % 4], ks, -m[r]));
-        if (masked && !(seen >> i & 1)) e[i] = 0.0f;
-        l[r] += e[i];
-        e[i] *= vs;
-        if (masked && !(seen >> i & 1)) e[i] = 0.0f;  // vs may be NaN
-      }
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        p[r][u] = __builtin_bit_cast(bf16x8_t, make_uint4(pack2(e[8 * u], e[8 * u + 1]), pack2(e[8 * u + 2], e[8 * u + 3]),
-                                                          pack2(e[8 * u + 4], e[8 * u + 5]), pack2(e[8 * u + 6], e[8 * u + 7])));
-    }
+    for (int r = 0; r < RT; ++r) softmax(r, s[r], sc, p[r]);
 #pragma unroll
     for (int dt = 0; dt < DB * 4; ++dt)
 #pragma unroll
@@ -195,11 +249,20 @@ struct RowState {
         for (int r = 0; r < RT; ++r) o[r][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, p[r][u], o[r][dt], 0, 0, 0);
       }
   }
+
+  // Sums of whole rows.
+  __device__ __forceinline__ void finish() {
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      l[r] += __shfl_xor(l[r], 16, 64);
+      l[r] += __shfl_xor(l[r], 32, 64);
+    }
+  }
 };
 
 // One split of one tile of rows: the waves take its blocks in turn and join at the end.
 template <int DB, int RT>
-__global__ void __launch_bounds__(kAtnWaves * 64, 2) kv8_attend_kernel(AttendArgs a) {
+__global__ void __launch_bounds__(kAtnWaves * 64, DB * RT > 2 ? 1 : 2) kv8_attend_kernel(AttendArgs a) {
   constexpr int ROWS = 16 * RT, Dp = DB * 64;
   __shared__ float sml[2][kAtnWaves][ROWS];
   __shared__ __align__(16) float so[kAtnWaves][ROWS][Dp + 4];
@@ -208,31 +271,12 @@ __global__ void __launch_bounds__(kAtnWaves * 64, 2) kv8_attend_kernel(AttendArg
   const int b = static_cast<int>(bh / a.c.H), h = static_cast<int>(bh % a.c.H);
   const int lane = threadIdx.x & 63, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const TileRange tr = tile_range<ROWS>(a, b, tile);
+  const TileRange tr = tile_range(a, ROWS, b, tile);
   const int used = tr.used();
   if (split >= used && split > 0) return;
   RowState<DB, RT> st;
-  int first_pos = INT32_MAX, last_pos = -1;  // of the tile's queries
-  if (used) first_pos = tr.start + tr.i0, last_pos = tr.start + tr.i1 - 1;
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    const int row = tile * ROWS + r * 16 + (lane & 15), i = row / a.group, hq = h * a.group + row % a.group;
-    const bool real = i < tr.i1;
-    st.pos[r] = real ? tr.start + i : -1;
-    const uint16_t* q = a.q + b * a.qsb + i * a.qss + hq * a.qsh;
-#pragma unroll
-    for (int hh = 0; hh < DB; ++hh)
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int d = hh * 64 + g * 16 + x * 8;
-        const V4 w = real && d < a.c.D ? ld16(q + d) : zero16();
-        st.q[r][hh][x] = __builtin_bit_cast(bf16x8_t, make_uint4(w.w[0], w.w[1], w.w[2], w.w[3]));
-      }
-#pragma unroll
-    for (int dt = 0; dt < DB * 4; ++dt) st.o[r][dt] = f32x4_t{};
-    st.m[r] = kAtnLow;
-    st.l[r] = 0.0f;
-  }
+  st.start(a, tr, b, h, tile * ROWS);
+  const int first_pos = tr.start + tr.i0, last_pos = tr.start + tr.i1 - 1;  // of the tile's queries
   if (used) {
     const int whole = tr.end / kKvBlock;  // blocks of codes
     const int bs = tr.b0 + split * tr.per, be = min(tr.b1, bs + tr.per);
@@ -248,20 +292,19 @@ __global__ void __launch_bounds__(kAtnWaves * 64, 2) kv8_attend_kernel(AttendArg
     for (; blk < ce; blk += kAtnWaves) {
       const int nb = blk + kAtnWaves;
       if (nb < ce) next.load(kc + (int64_t)nb * kKvBlock * Dp, vc + (int64_t)nb * kKvBlock * Dp);
-      const float ks = a.c.ks[bh * a.c.blocks + blk] * a.scale, vs = a.c.vs[bh * a.c.blocks + blk];
-      st.block(cur, blk, ks, vs, a.window, masked(blk));
+      const BlockScale sc(a.c.ks[bh * a.c.blocks + blk], a.c.vs[bh * a.c.blocks + blk], a.scale);
+      st.block(cur, blk, sc, a.window, masked(blk));
       cur = next;
     }
     if (blk < be) {  // the incomplete block
       const TailBlock<DB> tail{a.c.kt + bh * kKvBlock * Dp, a.c.vt + bh * kKvBlock * Dp, tr.end - blk * kKvBlock};
-      st.block(tail, blk, a.scale, 1.0f, a.window, true);
+      st.block(tail, blk, BlockScale(1.0f, 1.0f, a.scale), a.window, true);
     }
   }
   // join the waves
+  st.finish();
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
-    st.l[r] += __shfl_xor(st.l[r], 16, 64);
-    st.l[r] += __shfl_xor(st.l[r], 32, 64);
     const int row = r * 16 + (lane & 15);
     if (g == 0) {
       sml[0][wave][row] = st.m[r];
@@ -307,69 +350,225 @@ __global__ void __launch_bounds__(kAtnWaves * 64, 2) kv8_attend_kernel(AttendArg
   }
 }
 
-// Joins the splits of one tile.
-template <int DB, int RT>
-__global__ void __launch_bounds__(256) kv8_join_kernel(AttendArgs a) {
-  constexpr int ROWS = 16 * RT, Dp = DB * 64;
-  const int tile = blockIdx.x % a.tiles;
+// Many rows: the waves of a workgroup share the blocks.  Each converts its part of a block into LDS once, in the
+// operands' order (a fragment of 16 bytes a lane, 1 KB, is written and read in a row, without bank conflicts), and
+// takes all of it for its own 16 RT rows.  The next block's codes are on their way meanwhile.
+template <int DB, int RT, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64, 2) kv8_chunk_kernel(AttendArgs a) {
+  constexpr int ROWS = 16 * RT * WAVES, Dp = DB * 64, N = DB * 8 / WAVES;  // chunks of a lane: keys', then values'
+  __shared__ __align__(16) unsigned char lds[2][DB * 16][1024];           // fragments (hh, t, a) of keys, (dt, u) of values
+  const int tile = blockIdx.x % a.tiles, split = blockIdx.y;
   const int64_t bh = blockIdx.x / a.tiles;
   const int b = static_cast<int>(bh / a.c.H), h = static_cast<int>(bh % a.c.H);
-  const TileRange tr = tile_range<ROWS>(a, b, tile);
+  const int lane = threadIdx.x & 63, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const TileRange tr = tile_range(a, ROWS, b, tile);
   const int used = tr.used();
-  const int64_t part0 = (int64_t)blockIdx.x * a.splits;
-  for (int at = threadIdx.x; at < ROWS * (Dp / 4); at += 256) {
-    const int row = at / (Dp / 4), d = (at - row * (Dp / 4)) * 4;
-    const int gr = tile * ROWS + row, i = gr / a.group, hq = h * a.group + gr % a.group;
-    if (i >= a.n || d >= a.c.D) continue;
-    float m = kAtnLow, l = 0.0f, o[4] = {0, 0, 0, 0};
-    if (i < tr.i1) {
-      for (int s = 0; s < used; ++s) m = fmaxf(m, a.pml[((part0 + s) * 2) * ROWS + row]);
-      for (int s = 0; s < used; ++s) {
-        const float f = __builtin_amdgcn_exp2f(a.pml[((part0 + s) * 2) * ROWS + row] - m);
-        const float4 x = *reinterpret_cast<const float4*>(a.po + ((part0 + s) * ROWS + row) * Dp + d);
-        l += f * a.pml[((part0 + s) * 2 + 1) * ROWS + row];
-        o[0] += f * x.x;
-        o[1] += f * x.y;
-        o[2] += f * x.z;
-        o[3] += f * x.w;
+  if (split >= used && split > 0) return;
+  const int row0 = tile * ROWS + wave * 16 * RT;
+  RowState<DB, RT> st;
+  st.start(a, tr, b, h, row0);
+  // positions of the wave's queries
+  const int first_pos = tr.start + row0 / a.group;
+  const int last_pos = row0 / a.group < tr.i1 ? tr.start + min(tr.i1 - 1, (row0 + 16 * RT - 1) / a.group) : -kKvBlock;
+  if (used) {
+    const int whole = tr.end / kKvBlock;
+    const int bs = tr.b0 + split * tr.per, be = min(tr.b1, bs + tr.per), ce = min(be, whole);
+    const int8_t* kc = a.c.k + bh * a.c.blocks * kKvBlock * Dp;
+    const int8_t* vc = a.c.v + bh * a.c.blocks * kKvBlock * Dp;
+    const float* ks = a.c.ks + bh * a.c.blocks;
+    const float* vs = a.c.vs + bh * a.c.blocks;
+    V4 w[N];
+    auto load = [&](int blk) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const int c = j * WAVES + wave;  // of DB * 8: codes of keys, then of values
+        const int8_t* src = c < DB * 4 ? kc + c * 1024 : vc + (c - DB * 4) * 1024;
+        w[j] = ld16(src + (int64_t)blk * kKvBlock * Dp + (lane & 15) * 64 + g * 16);
+      }
+    };
+    struct {
+      const unsigned char* p;
+      int lane;
+      __device__ __forceinline__ bf16x8_t key(int hh, int t, int x) const {
+        return *reinterpret_cast<const bf16x8_t*>(p + ((hh * 4 + t) * 2 + x) * 1024 + lane * 16);
+      }
+      __device__ __forceinline__ bf16x8_t value(int dt, int u) const {
+        return *reinterpret_cast<const bf16x8_t*>(p + (DB * 8 + dt * 2 + u) * 1024 + lane * 16);
+      }
+    } frags;
+    frags.lane = lane;
+    auto stage = [&](int blk) {
+      unsigned char(*buf)[1024] = lds[blk & 1];
+      if (blk < ce) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const int c = j * WAVES + wave;
+          *reinterpret_cast<bf16x8_t*>(&buf[2 * c][lane * 16]) = codes_to_bf16(w[j].w[0], w[j].w[1]);
+          *reinterpret_cast<bf16x8_t*>(&buf[2 * c + 1][lane * 16]) = codes_to_bf16(w[j].w[2], w[j].w[3]);
+        }
+      } else {  // the incomplete block
+        const TailBlock<DB> tail{a.c.kt + bh * kKvBlock * Dp, a.c.vt + bh * kKvBlock * Dp, tr.end - blk * kKvBlock};
+#pragma unroll 1
+        for (int j = 0; j < N; ++j) {
+          const int c = j * WAVES + wave, f = c % (DB * 4);
+#pragma unroll 1
+          for (int x = 0; x < 2; ++x)
+            *reinterpret_cast<bf16x8_t*>(&buf[2 * c + x][lane * 16]) =
+                c < DB * 4 ? tail.key(f / 4, f % 4, x) : tail.value(f, x);
+        }
+      }
+      __syncthreads();  // also: every wave is done with the block before the last, whose buffer is next
+      if (blk + 1 < ce) load(blk + 1);
+    };
+    // blocks that some row of this wave sees
+    const int from = a.window ? min(be, max(bs, (first_pos - a.window + 1) / kKvBlock)) : bs;
+    const int to = max(from, min(be, last_pos / kKvBlock + 1));
+    int blk = bs;
+    if (bs < ce) load(bs);
+    for (; blk < from; ++blk) stage(blk);
+    for (; blk < to; ++blk) {
+      stage(blk);
+      const bool coded = blk < ce;
+      const BlockScale sc(coded ? ks[blk] : 1.0f, coded ? vs[blk] : 1.0f, a.scale);
+      frags.p = lds[blk & 1][0];
+      st.block(frags, blk, sc, a.window,
+               blk * kKvBlock + kKvBlock - 1 > first_pos || (a.window && blk * kKvBlock <= last_pos - a.window));
+    }
+    for (; blk < be; ++blk) stage(blk);
+  }
+  st.finish();
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const int row = row0 + r * 16 + (lane & 15), i = row / a.group, hq = h * a.group + row % a.group;
+    if (a.splits > 1) {
+      const int64_t part = (int64_t)blockIdx.x * a.splits + split;
+      const int tr_row = row - tile * ROWS;
+#pragma unroll
+      for (int dt = 0; dt < DB * 4; ++dt)
+        *reinterpret_cast<float4*>(a.po + (part * ROWS + tr_row) * Dp + dt * 16 + 4 * g) =
+            make_float4(st.o[r][dt][0], st.o[r][dt][1], st.o[r][dt][2], st.o[r][dt][3]);
+      if (g == 0) {
+        a.pml[(part * 2 + 0) * ROWS + tr_row] = st.m[r];
+        a.pml[(part * 2 + 1) * ROWS + tr_row] = st.l[r];
+      }
+    } else if (i < a.n) {
+      uint16_t* dst = a.out + (((int64_t)b * a.n + i) * a.heads + hq) * a.c.D;
+      const float f = 1.0f / st.l[r];
+#pragma unroll
+      for (int dt = 0; dt < DB * 4; ++dt) {
+        const int d = dt * 16 + 4 * g;
+        if (d < a.c.D)
+          *reinterpret_cast<uint2*>(dst + d) =
+              i < tr.i1 ? make_uint2(pack2(st.o[r][dt][0] * f, st.o[r][dt][1] * f),
+                                     pack2(st.o[r][dt][2] * f, st.o[r][dt][3] * f))
+                        : make_uint2(0, 0);
       }
     }
-    const float f = 1.0f / l;
-    uint2 w = make_uint2(0, 0);
-    if (i < tr.i1) w = make_uint2(pack2(o[0] * f, o[1] * f), pack2(o[2] * f, o[3] * f));
-    *reinterpret_cast<uint2*>(a.out + (((int64_t)b * a.n + i) * a.heads + hq) * a.c.D + d) = w;
   }
 }
 
-template <int DB, int RT>
-void launch_attend(const AttendArgs& a, hipStream_t st) {
-  const unsigned tiles = static_cast<unsigned>((int64_t)a.c.B * a.c.H * a.tiles);
-  kv8_attend_kernel<DB, RT><<<dim3(tiles, a.splits), kAtnWaves * 64, 0, st>>>(a);
-  if (a.splits > 1) kv8_join_kernel<DB, RT><<<tiles, 256, 0, st>>>(a);
+// Joins the splits of output rows: `teams` groups of Dp / 4 threads take those of one row in turn.
+template <int DB>
+__global__ void __launch_bounds__(256) kv8_join_kernel(AttendArgs a, int teams) {
+  constexpr int L = DB * 16, G = DB == 3 ? 4 : 256 / L, Dp = DB * 64;
+  __shared__ __align__(16) float so[G][Dp + 4];
+  __shared__ float sml[2][G];
+  const int t = threadIdx.x, grp = t / L, team = grp % teams, first = grp - team;
+  const int64_t out_row = (int64_t)blockIdx.x * (G / teams) + grp / teams;
+  const bool real = grp < G && out_row < (int64_t)a.c.B * a.n * a.heads;
+  const int hq = static_cast<int>(out_row % a.heads);
+  const int64_t bi = real ? out_row / a.heads : 0;
+  const int b = static_cast<int>(bi / a.n), i = static_cast<int>(bi % a.n);
+  const int gr = i * a.group + hq % a.group, tile = gr / a.rows, row = gr - tile * a.rows;
+  const TileRange tr = tile_range(a, a.rows, b, tile);
+  const int used = i < tr.i1 ? tr.used() : 0, d = (t - grp * L) * 4;
+  const int64_t part0 = (((int64_t)b * a.c.H + hq / a.group) * a.tiles + tile) * a.splits;
+  float m = kAtnLow, l = 0.0f, o[4] = {0, 0, 0, 0};
+  if (real) {
+#pragma unroll 4
+    for (int s = team; s < used; s += teams) {
+      const float ms = a.pml[(part0 + s) * 2 * a.rows + row], ls = a.pml[((part0 + s) * 2 + 1) * a.rows + row];
+      const float4 x = *reinterpret_cast<const float4*>(a.po + ((part0 + s) * a.rows + row) * Dp + d);
+      const float mn = fmaxf(m, ms), f = __builtin_amdgcn_exp2f(m - mn), fs = __builtin_amdgcn_exp2f(ms - mn);
+      m = mn;
+      l = l * f + ls * fs;
+      o[0] = o[0] * f + x.x * fs;
+      o[1] = o[1] * f + x.y * fs;
+      o[2] = o[2] * f + x.z * fs;
+      o[3] = o[3] * f + x.w * fs;
+    }
+    *reinterpret_cast<float4*>(&so[grp][d]) = make_float4(o[0], o[1], o[2], o[3]);
+    if (d == 0) {
+      sml[0][grp] = m;
+      sml[1][grp] = l;
+    }
+  }
+  __syncthreads();
+  if (!real || team != 0 || d >= a.c.D) return;
+  m = kAtnLow;
+  l = o[0] = o[1] = o[2] = o[3] = 0.0f;
+  for (int k = first; k < first + teams; ++k) m = fmaxf(m, sml[0][k]);
+  for (int k = first; k < first + teams; ++k) {
+    const float f = __builtin_amdgcn_exp2f(sml[0][k] - m);
+    const float4 x = *reinterpret_cast<const float4*>(&so[k][d]);
+    l += f * sml[1][k];
+    o[0] += f * x.x;
+    o[1] += f * x.y;
+    o[2] += f * x.z;
+    o[3] += f * x.w;
+  }
+  const float f = i < tr.i1 ? 1.0f / l : 0.0f;
+  *reinterpret_cast<uint2*>(a.out + (bi * a.heads + hq) * a.c.D + d) =
+      make_uint2(pack2(o[0] * f, o[1] * f), pack2(o[2] * f, o[3] * f));
 }
 
-// How a call is cut: rows of a tile and key splits.
+// How a call is cut: waves of a workgroup that share blocks (0: each takes its own), 16-row pieces of a wave, rows of a
+// workgroup, key splits.
 struct AttendPlan {
-  int rt;
+  int waves, rt, rows;
   int64_t tiles;  // of one (sequence, head)
   int splits, chunk;
   size_t bytes;
 };
 AttendPlan attend_plan(int64_t B, int64_t H, int64_t heads, int64_t Dp, int64_t n, int64_t bound) {
   AttendPlan p;
-  const int64_t rows = n * (heads / H);
+  const int64_t rows = n * (heads / H), blocks = ceil_div(bound, kKvBlock);
   p.rt = rows <= 16 || Dp > 128 ? 1 : 2;
-  p.tiles = ceil_div(rows, 16 * p.rt);
-  const int64_t wgs = B * H * p.tiles, blocks = ceil_div(bound, kKvBlock);
-  // enough workgroups for two on every CU, none with less than two blocks for each of its waves
-  int64_t s = ceil_div(1024, wgs);
+  p.waves = rows <= 16 * p.rt ? 0 : B * H * ceil_div(rows, 128 * p.rt) >= 256 ? 8 : 4;
+  p.rows = 16 * p.rt * (p.waves ? p.waves : 1);
+  p.tiles = ceil_div(rows, p.rows);
+  const int64_t wgs = B * H * p.tiles;
+  // enough workgroups for two on every CU and some to spare, none with less than two blocks for each of its waves
+  int64_t s = ceil_div(p.waves == 8 ? 256 : p.waves == 4 ? 512 : 1024, wgs);
   const int64_t most = ceil_div(blocks, 2 * kAtnWaves);
   if (s > most) s = most;
   if (s < 1) s = 1;
   p.splits = static_cast<int>(s);
   p.chunk = static_cast<int>(blocks > 0 ? ceil_div(blocks, s) : 1);
-  p.bytes = s > 1 ? static_cast<size_t>(wgs) * s * (16 * p.rt) * (Dp + 2) * 4 : 0;
+  p.bytes = s > 1 ? static_cast<size_t>(wgs) * s * p.rows * (Dp + 2) * 4 : 0;
   return p;
+}
+
+template <int DB>
+void launch_attend(const AttendArgs& a, const AttendPlan& p, hipStream_t st) {
+  constexpr int RT = DB <= 2 ? 2 : 1;  // of the shared form: what the registers hold twice a SIMD
+  const dim3 grid(static_cast<unsigned>((int64_t)a.c.B * a.c.H * a.tiles), a.splits);
+  if (p.waves == 8)
+    kv8_chunk_kernel<DB, RT, 8><<<grid, 512, 0, st>>>(a);
+  else if (p.waves == 4)
+    kv8_chunk_kernel<DB, RT, 4><<<grid, 256, 0, st>>>(a);
+  else if (p.rt == RT)
+    kv8_attend_kernel<DB, RT><<<grid, kAtnWaves * 64, 0, st>>>(a);
+  else
+    kv8_attend_kernel<DB, 1><<<grid, kAtnWaves * 64, 0, st>>>(a);
+  if (a.splits > 1) {
+    constexpr int G = DB == 3 ? 4 : 16 / DB;
+    int teams = 1;
+    while (teams < G && teams < a.splits) teams *= 2;
+    const int64_t rows = (int64_t)a.c.B * a.n * a.heads;
+    kv8_join_kernel<DB><<<static_cast<unsigned>(ceil_div(rows, G / teams)), 256, 0, st>>>(a, teams);
+  }
 }
 
 }  // namespace
@@ -406,7 +605,7 @@ extern "C" int sf_kv8_attend(const sf_kv8_cache* cache, const void* q, int64_t q
                workspace_bytes, p.bytes);
   SF_CHECK_ARG(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "sf_kv8_attend: workspace must be 16-byte aligned");
   const int64_t wgs = (int64_t)a.c.B * a.c.H * p.tiles;
-  SF_CHECK_ARG(wgs < (1ll << 31) && n * (heads / a.c.H) < (1ll << 30), "sf_kv8_attend: too many rows");
+  SF_CHECK_ARG(a.c.B * n * heads < (1ll << 31), "sf_kv8_attend: too many rows");
   a.q = static_cast<const uint16_t*>(q);
   a.qsb = q_sb, a.qss = q_ss, a.qsh = q_sh;
   a.out = static_cast<uint16_t*>(out);
@@ -415,19 +614,18 @@ extern "C" int sf_kv8_attend(const sf_kv8_cache* cache, const void* q, int64_t q
   a.group = static_cast<int>(heads / a.c.H);
   a.window = static_cast<int>(window < cap ? window : 0);
   a.scale = scale * kAtnLog2e;
+  a.rows = p.rows;
   a.tiles = static_cast<int>(p.tiles);
   a.splits = p.splits;
   a.chunk = p.chunk;
   a.po = static_cast<float*>(workspace);
-  a.pml = a.po ? a.po + wgs * p.splits * 16 * p.rt * a.c.Dp : nullptr;
+  a.pml = a.po ? a.po + wgs * p.splits * p.rows * a.c.Dp : nullptr;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  switch (a.c.Dp / 64 * 10 + p.rt) {
-    case 11: launch_attend<1, 1>(a, st); break;
-    case 12: launch_attend<1, 2>(a, st); break;
-    case 21: launch_attend<2, 1>(a, st); break;
-    case 22: launch_attend<2, 2>(a, st); break;
-    case 31: launch_attend<3, 1>(a, st); break;
-    case 41: launch_attend<4, 1>(a, st); break;
+  switch (a.c.Dp / 64) {
+    case 1: launch_attend<1>(a, p, st); break;
+    case 2: launch_attend<2>(a, p, st); break;
+    case 3: launch_attend<3>(a, p, st); break;
+    case 4: launch_attend<4>(a, p, st); break;
   }
   return launch_status("sf_kv8_attend");
 }
