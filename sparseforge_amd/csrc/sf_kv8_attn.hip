@@ -61,6 +61,20 @@ __device__ __forceinline__ TileRange tile_range(const AttendArgs& a, int rows, i
   return r;
 }
 
+// Workgroup -> tile: those of one (sequence, head) on one XCD, whose L2 then holds its codes, longest rows first.
+__device__ __forceinline__ void tile_of(const AttendArgs& a, int64_t& bh, int& tile) {
+  const int64_t id = blockIdx.x, all = (int64_t)a.c.B * a.c.H;
+  if (all % kXcds == 0) {
+    const int64_t r = id / kXcds;
+    bh = r / a.tiles * kXcds + id % kXcds;
+    tile = static_cast<int>(r % a.tiles);
+  } else {
+    bh = id / a.tiles;
+    tile = static_cast<int>(id % a.tiles);
+  }
+  tile = a.tiles - 1 - tile;
+}
+
 // 8 codes -> bf16, exact: a code has at most 8 significant bits, so the high half of its float is the bf16.
 __device__ __forceinline__ bf16x8_t codes_to_bf16(uint32_t w0, uint32_t w1) {
   uint32_t o[4];
@@ -132,7 +146,7 @@ struct BlockScale {
     ks = k > 0.0f ? k * scale : 1.0f;
     v = v > 0.0f ? v : 1.0f;
     far = v < 0x1p-64f || v > 0x1p64f;
-    lv = log2f(v);
+    lv = far ? log2f(v) : __builtin_amdgcn_logf(v);
     rv = far ? 0.0f : __builtin_amdgcn_rcpf(v);
   }
 };
@@ -142,7 +156,7 @@ template <int DB, int RT>
 struct RowState {
   bf16x8_t q[RT][DB][2];
   f32x4_t o[RT][DB * 4];
-  float m[RT], l[RT];  // l: of the keys this lane's group holds
+  float m[RT], l[RT];
   int pos[RT];         // position of the row's query, -1: no such row
 
   // The queries of rows row0 + 16 r + lane % 16 (below `rows`) of key-value head h.
@@ -182,44 +196,8 @@ struct RowState {
     }
   }
 
-  // Scores of 64 keys of 16 rows -> operands of the second product.
-  __device__ __forceinline__ void softmax(int r, const f32x4_t (&s)[4], const BlockScale& sc, bf16x8_t (&p)[2]) {
-    float mx = s[0][0];
-#pragma unroll
-    for (int i = 1; i < 16; ++i) mx = fmaxf(mx, s[i / 4][i % 4]);
-    mx *= sc.ks;
-    if (__builtin_amdgcn_ballot_w64(mx > m[r] + kAtnSlack)) {
-      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      const float mn = fmaxf(m[r], mx), f = __builtin_amdgcn_exp2f(m[r] - mn);
-      m[r] = mn;
-      l[r] *= f;
-#pragma unroll
-      for (int dt = 0; dt < DB * 4; ++dt) o[r][dt] *= f;
-    }
-    if (sc.far) {
-      float sum = 0.0f;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) sum += __builtin_amdgcn_exp2f(fmaf(s[i / 4][i % 4], sc.ks, -m[r]));
-      l[r] += sum;
-    }
-    const float off = sc.lv - m[r];
-    float e[16], sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      e[i] = __builtin_amdgcn_exp2f(fmaf(s[i / 4][i % 4], sc.ks, off));
-      sum += e[i];
-    }
-    l[r] = fmaf(sum, sc.rv, l[r]);
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-      p[u] = __builtin_bit_cast(bf16x8_t, make_uint4(pack2(e[8 * u], e[8 * u + 1]), pack2(e[8 * u + 2], e[8 * u + 3]),
-                                                     pack2(e[8 * u + 4], e[8 * u + 5]), pack2(e[8 * u + 6], e[8 * u + 7])));
-  }
-
   template <class Block>
-  __device__ __forceinline__ void block(const Block& x, int blk, const BlockScale& sc, int window, bool masked) {
-    f32x4_t s[RT][4];
+  __device__ __forceinline__ void scores(const Block& x, f32x4_t (&s)[RT][4]) const {
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
 #pragma unroll
@@ -233,13 +211,78 @@ struct RowState {
           for (int r = 0; r < RT; ++r) s[r][t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[r][hh][a], s[r][t], 0, 0, 0);
         }
     }
+  }
+
+  // What is rare before a block's probabilities: rows that do not see it whole, a maximum that has to rise, a value
+  // scale far from 1.
+  __device__ __forceinline__ void settle(f32x4_t (&s)[RT][4], int blk, const BlockScale& sc, int window, bool masked) {
     if (masked || sc.nan) {
 #pragma unroll
       for (int r = 0; r < RT; ++r) hide(r, s[r], blk, sc.nan, window);
     }
-    bf16x8_t p[RT][2];
+    float mx[RT];
+    bool rise = false;
 #pragma unroll
-    for (int r = 0; r < RT; ++r) softmax(r, s[r], sc, p[r]);
+    for (int r = 0; r < RT; ++r) {
+      mx[r] = s[r][0][0];
+#pragma unroll
+      for (int i = 1; i < 16; ++i) mx[r] = fmaxf(mx[r], s[r][i / 4][i % 4]);
+      mx[r] *= sc.ks;
+      rise |= mx[r] > m[r] + kAtnSlack;
+    }
+    if (__builtin_amdgcn_ballot_w64(rise)) {
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        float x = fmaxf(mx[r], __shfl_xor(mx[r], 16, 64));
+        x = fmaxf(x, __shfl_xor(x, 32, 64));
+        const float mn = fmaxf(m[r], x), f = __builtin_amdgcn_exp2f(m[r] - mn);
+        m[r] = mn;
+        l[r] *= f;
+#pragma unroll
+        for (int dt = 0; dt < DB * 4; ++dt) o[r][dt] *= f;
+      }
+    }
+    if (sc.far) {
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum += __builtin_amdgcn_exp2f(fmaf(s[r][i / 4][i % 4], sc.ks, -m[r]));
+        sum += __shfl_xor(sum, 16, 64);
+        l[r] += sum + __shfl_xor(sum, 32, 64);
+      }
+    }
+  }
+
+  // Probabilities times the value scale, as operands of the second product.
+  __device__ __forceinline__ void weights(const f32x4_t (&s)[RT][4], const BlockScale& sc, bf16x8_t (&p)[RT][2]) {
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const float off = sc.lv - m[r];
+      float e[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(s[r][i / 4][i % 4], sc.ks, off));
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        p[r][u] = __builtin_bit_cast(bf16x8_t, make_uint4(pack2(e[8 * u], e[8 * u + 1]), pack2(e[8 * u + 2], e[8 * u + 3]),
+                                                          pack2(e[8 * u + 4], e[8 * u + 5]), pack2(e[8 * u + 6], e[8 * u + 7])));
+    }
+  }
+
+  // The sums of the rows' probabilities, as a product with ones: the vector unit has more to do than the matrix unit,
+  // and the sums are those of the rounded probabilities that the output takes.
+  __device__ __forceinline__ void sums(const bf16x8_t (&p)[RT][2], const BlockScale& sc) {
+    const bf16x8_t ones = __builtin_bit_cast(bf16x8_t, make_uint4(0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u));
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      f32x4_t t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p[r][0], f32x4_t{}, 0, 0, 0);
+      t = __builtin_amdgcn_mfma_f32_16x16x32_bf16(ones, p[r][1], t, 0, 0, 0);
+      l[r] = fmaf(t[0], sc.rv, l[r]);
+    }
+  }
+
+  template <class Block>
+  __device__ __forceinline__ void output(const Block& x, const bf16x8_t (&p)[RT][2]) {
 #pragma unroll
     for (int dt = 0; dt < DB * 4; ++dt)
 #pragma unroll
@@ -250,13 +293,70 @@ struct RowState {
       }
   }
 
-  // Sums of whole rows.
-  __device__ __forceinline__ void finish() {
+  template <class Block>
+  __device__ __forceinline__ void block(const Block& x, int blk, const BlockScale& sc, int window, bool masked) {
+    f32x4_t s[RT][4];
+    bf16x8_t p[RT][2];
+    scores(x, s);
+    settle(s, blk, sc, window, masked);
+    weights(s, sc, p);
+    sums(p, sc);
+    output(x, p);
+  }
+
+  // scores(x, next), weights(s, sc, p) and output(x, p) as one stream of instructions: products of the next scores
+  // between exponentials, and `rest(i, n)`, i = 0 .. n - 1, between products of the output.
+  template <class Block, class Rest>
+  __device__ __forceinline__ void turn(const Block& x, const f32x4_t (&s)[RT][4], f32x4_t (&next)[RT][4],
+                                       const BlockScale& sc, const Rest& rest) {
+    constexpr int F = DB * 8;  // fragments of keys, and of values
+    float off[RT];
+    uint32_t pw[RT][8];
+    constexpr int A = 2;  // fragments read ahead
+    bf16x8_t f[A + 1];
+    auto key = [&](int i) { return x.key(i / 2 % DB, i / (2 * DB), i % 2); };
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      l[r] += __shfl_xor(l[r], 16, 64);
-      l[r] += __shfl_xor(l[r], 32, 64);
+      off[r] = sc.lv - m[r];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) next[r][t] = f32x4_t{};
     }
+#pragma unroll
+    for (int i = 0; i < A; ++i) f[i] = key(i);
+#pragma unroll
+    for (int i = 0; i < F; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+      f[(i + A) % (A + 1)] = i + A < F ? key(i + A) : x.value((i + A - F) / 2, (i + A - F) % 2);
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+        next[r][i / (2 * DB)] =
+            __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[i % (A + 1)], q[r][i / 2 % DB][i % 2], next[r][i / (2 * DB)], 0, 0, 0);
+      // pairs of weights: 8 RT of them over F places
+#pragma unroll
+      for (int j = i * 8 * RT / F; j < (i + 1) * 8 * RT / F; ++j) {
+        const int r = j / 8, e = j % 8 * 2;
+        const float a = __builtin_amdgcn_exp2f(fmaf(s[r][e / 4][e % 4], sc.ks, off[r]));
+        const float b = __builtin_amdgcn_exp2f(fmaf(s[r][e / 4][e % 4 + 1], sc.ks, off[r]));
+        pw[r][j % 8] = pack2(a, b);
+      }
+    }
+    bf16x8_t p[RT][2];
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        p[r][u] = __builtin_bit_cast(bf16x8_t, make_uint4(pw[r][4 * u], pw[r][4 * u + 1], pw[r][4 * u + 2], pw[r][4 * u + 3]));
+    sums(p, sc);
+#pragma unroll
+    for (int i = 0; i < F; ++i) {
+      __builtin_amdgcn_sched_barrier(0);
+      if (i + A < F) f[(F + i + A) % (A + 1)] = x.value((i + A) / 2, (i + A) % 2);
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+        o[r][i / 2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[(F + i) % (A + 1)], p[r][i % 2], o[r][i / 2], 0, 0, 0);
+      rest(i, F);
+    }
+    __builtin_amdgcn_sched_barrier(0);
   }
 };
 
@@ -302,7 +402,6 @@ __global__ void __launch_bounds__(kAtnWaves * 64, DB * RT > 2 ? 1 : 2) kv8_atten
     }
   }
   // join the waves
-  st.finish();
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     const int row = r * 16 + (lane & 15);
@@ -352,13 +451,16 @@ __global__ void __launch_bounds__(kAtnWaves * 64, DB * RT > 2 ? 1 : 2) kv8_atten
 
 // Many rows: the waves of a workgroup share the blocks.  Each converts its part of a block into LDS once, in the
 // operands' order (a fragment of 16 bytes a lane, 1 KB, is written and read in a row, without bank conflicts), and
-// takes all of it for its own 16 RT rows.  The next block's codes are on their way meanwhile.
+// takes all of it for its own 16 RT rows.  In a turn, the scores of the next block are products on the matrix unit
+// while the probabilities of this one are exponentials on the vector unit; the block after, its codes loaded at the
+// turn's start, is converted at its end.  Keys are staged one block further than values.
 template <int DB, int RT, int WAVES>
 __global__ void __launch_bounds__(WAVES * 64, 2) kv8_chunk_kernel(AttendArgs a) {
   constexpr int ROWS = 16 * RT * WAVES, Dp = DB * 64, N = DB * 8 / WAVES;  // chunks of a lane: keys', then values'
   __shared__ __align__(16) unsigned char lds[2][DB * 16][1024];           // fragments (hh, t, a) of keys, (dt, u) of values
-  const int tile = blockIdx.x % a.tiles, split = blockIdx.y;
-  const int64_t bh = blockIdx.x / a.tiles;
+  int tile, split = blockIdx.y;
+  int64_t bh;
+  tile_of(a, bh, tile);
   const int b = static_cast<int>(bh / a.c.H), h = static_cast<int>(bh % a.c.H);
   const int lane = threadIdx.x & 63, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -378,71 +480,99 @@ __global__ void __launch_bounds__(WAVES * 64, 2) kv8_chunk_kernel(AttendArgs a) 
     const int8_t* vc = a.c.v + bh * a.c.blocks * kKvBlock * Dp;
     const float* ks = a.c.ks + bh * a.c.blocks;
     const float* vs = a.c.vs + bh * a.c.blocks;
+    const int coded = max(bs, ce - 1);  // the last block of codes here, or any that exists
+    const TailBlock<DB> tail{a.c.kt + bh * kKvBlock * Dp, a.c.vt + bh * kKvBlock * Dp, tr.end - whole * kKvBlock};
     V4 w[N];
-    auto load = [&](int blk) {
+    // Chunk c of DB * 8 (codes of keys, then of values) of blocks kb and vb; past the codes it is read for nothing.
+    auto load = [&](int kb, int vb) {
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const int c = j * WAVES + wave;  // of DB * 8: codes of keys, then of values
+        const int c = j * WAVES + wave;
         const int8_t* src = c < DB * 4 ? kc + c * 1024 : vc + (c - DB * 4) * 1024;
-        w[j] = ld16(src + (int64_t)blk * kKvBlock * Dp + (lane & 15) * 64 + g * 16);
+        w[j] = ld16(src + (int64_t)min(c < DB * 4 ? kb : vb, coded) * kKvBlock * Dp + (lane & 15) * 64 + g * 16);
+      }
+    };
+    auto stage_half = [&](int j, int x, int kb, int vb) {
+      const int c = j * WAVES + wave;
+      *reinterpret_cast<bf16x8_t*>(&lds[(c < DB * 4 ? kb : vb) & 1][2 * c + x][lane * 16]) =
+          codes_to_bf16(w[j].w[2 * x], w[j].w[2 * x + 1]);
+    };
+    auto stage = [&](int kb, int vb) {
+#pragma unroll
+      for (int j = 0; j < 2 * N; ++j) stage_half(j / 2, j % 2, kb, vb);
+    };
+    auto stage_tail = [&](int kb, int vb) {
+      if (kb != whole && vb != whole) return;
+#pragma unroll 1
+      for (int j = 0; j < 2 * N; ++j) {
+        const int c = j / 2 * WAVES + wave, x = j % 2;
+        if ((c < DB * 4 ? kb : vb) != whole) continue;
+        *reinterpret_cast<bf16x8_t*>(&lds[whole & 1][2 * c + x][lane * 16]) =
+            c < DB * 4 ? tail.key(c / 4, c % 4, x) : tail.value(c - DB * 4, x);
       }
     };
     struct {
-      const unsigned char* p;
-      int lane;
+      const unsigned char* k;
+      const unsigned char* v;
       __device__ __forceinline__ bf16x8_t key(int hh, int t, int x) const {
-        return *reinterpret_cast<const bf16x8_t*>(p + ((hh * 4 + t) * 2 + x) * 1024 + lane * 16);
+        return *reinterpret_cast<const bf16x8_t*>(k + ((hh * 4 + t) * 2 + x) * 1024);
       }
       __device__ __forceinline__ bf16x8_t value(int dt, int u) const {
-        return *reinterpret_cast<const bf16x8_t*>(p + (DB * 8 + dt * 2 + u) * 1024 + lane * 16);
+        return *reinterpret_cast<const bf16x8_t*>(v + (DB * 8 + dt * 2 + u) * 1024);
       }
     } frags;
-    frags.lane = lane;
-    auto stage = [&](int blk) {
-      unsigned char(*buf)[1024] = lds[blk & 1];
-      if (blk < ce) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-          const int c = j * WAVES + wave;
-          *reinterpret_cast<bf16x8_t*>(&buf[2 * c][lane * 16]) = codes_to_bf16(w[j].w[0], w[j].w[1]);
-          *reinterpret_cast<bf16x8_t*>(&buf[2 * c + 1][lane * 16]) = codes_to_bf16(w[j].w[2], w[j].w[3]);
-        }
-      } else {  // the incomplete block
-        const TailBlock<DB> tail{a.c.kt + bh * kKvBlock * Dp, a.c.vt + bh * kKvBlock * Dp, tr.end - blk * kKvBlock};
-#pragma unroll 1
-        for (int j = 0; j < N; ++j) {
-          const int c = j * WAVES + wave, f = c % (DB * 4);
-#pragma unroll 1
-          for (int x = 0; x < 2; ++x)
-            *reinterpret_cast<bf16x8_t*>(&buf[2 * c + x][lane * 16]) =
-                c < DB * 4 ? tail.key(f / 4, f % 4, x) : tail.value(f, x);
-        }
-      }
-      __syncthreads();  // also: every wave is done with the block before the last, whose buffer is next
-      if (blk + 1 < ce) load(blk + 1);
-    };
     // blocks that some row of this wave sees
     const int from = a.window ? min(be, max(bs, (first_pos - a.window + 1) / kKvBlock)) : bs;
     const int to = max(from, min(be, last_pos / kKvBlock + 1));
-    int blk = bs;
-    if (bs < ce) load(bs);
-    for (; blk < from; ++blk) stage(blk);
-    for (; blk < to; ++blk) {
-      stage(blk);
-      const bool coded = blk < ce;
-      const BlockScale sc(coded ? ks[blk] : 1.0f, coded ? vs[blk] : 1.0f, a.scale);
-      frags.p = lds[blk & 1][0];
-      st.block(frags, blk, sc, a.window,
-               blk * kKvBlock + kKvBlock - 1 > first_pos || (a.window && blk * kKvBlock <= last_pos - a.window));
+    load(bs, bs);
+    stage(bs, bs);
+    stage_tail(bs, bs);
+    int blk = bs - 1;
+    // Turn blk: the block's own products after the next one's scores.
+    auto turn_of_others = [&] {
+      __syncthreads();
+      load(blk + 2, blk + 1);
+      stage(blk + 2, blk + 1);
+      stage_tail(blk + 2, blk + 1);
+    };
+    for (; blk < from - 1; ++blk) turn_of_others();
+    f32x4_t s[RT][4];
+    if (to > from) {
+      __syncthreads();
+      load(blk + 2, blk + 1);
+      frags.k = &lds[from & 1][0][lane * 16];
+      st.scores(frags, s);
+      stage(blk + 2, blk + 1);
+      stage_tail(blk + 2, blk + 1);
+      float k1 = ks[min(from, coded)], v1 = vs[min(from, coded)];  // the next block's scales
+      for (++blk; blk < to; ++blk) {
+        __syncthreads();  // every wave is done with what this turn overwrites
+        load(blk + 2, blk + 1);
+        const BlockScale sc(blk < ce ? k1 : 1.0f, blk < ce ? v1 : 1.0f, a.scale);
+        k1 = ks[min(blk + 1, coded)], v1 = vs[min(blk + 1, coded)];
+        st.settle(s, blk, sc, a.window,
+                  blk * kKvBlock + kKvBlock - 1 > first_pos || (a.window && blk * kKvBlock <= last_pos - a.window));
+        frags.k = &lds[(blk + 1) & 1][0][lane * 16];
+        frags.v = &lds[blk & 1][0][lane * 16];
+        f32x4_t next[RT][4];  // past the last block: of what lies there, unused
+        st.turn(frags, s, next, sc, [&](int i, int n) {
+#pragma unroll
+          for (int j = i * 2 * N / n; j < (i + 1) * 2 * N / n; ++j) stage_half(j / 2, j % 2, blk + 2, blk + 1);
+        });
+        stage_tail(blk + 2, blk + 1);
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int t = 0; t < 4; ++t) s[r][t] = next[r][t];
+      }
     }
-    for (; blk < be; ++blk) stage(blk);
+    for (; blk < be; ++blk) turn_of_others();
   }
-  st.finish();
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     const int row = row0 + r * 16 + (lane & 15), i = row / a.group, hq = h * a.group + row % a.group;
     if (a.splits > 1) {
-      const int64_t part = (int64_t)blockIdx.x * a.splits + split;
+      const int64_t part = (bh * a.tiles + tile) * a.splits + split;
       const int tr_row = row - tile * ROWS;
 #pragma unroll
       for (int dt = 0; dt < DB * 4; ++dt)
