@@ -1,11 +1,10 @@
 // The 8-bit cache of keys and values (layout: sf_kv8.hpp): new rows appended, and what the cache stands for.
 //
 // A block that the new rows complete is coded: a = max |x| over its 64 x D elements, code = rint(127 x / a) (ties to
-// even), scale = a / 127.  127 x is exact in f32 for a bf16 x and the quotient, correctly rounded, lies on a
-// half-integer only where the exact one does, so the codes are those of exact arithmetic.  Rows of an incomplete
-// block are kept as they come until the block is whole: what the cache holds does not depend on how many rows came
-// at a time.  A token whose key or value (of a head) holds a NaN or an infinity is a NaN token: both its rows become
-// NaN, and the block it completes has NaN for its scales.
+// even), scale = a / 127; the codes are those of exact arithmetic (Coder).  Rows of an incomplete block are kept as
+// they come until the block is whole: what the cache holds does not depend on how many rows came at a time.  A token
+// whose key or value (of a head) holds a NaN or an infinity is a NaN token: both its rows become NaN, and the block it
+// completes has NaN for its scales.
 //
 // Both are bound by memory: append reads 4 D bytes per token and head and writes 2 D, values reads 2 D and writes
 // 8 D.
@@ -13,8 +12,6 @@
 
 namespace sf {
 namespace {
-
-constexpr int kAppBlock = 256;
 
 struct AppendArgs {
   KvCache c;
@@ -28,10 +25,27 @@ __device__ __forceinline__ bool nonfinite(uint32_t w) {  // either half of two b
   return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
 }
 
-// One workgroup per (block, head, sequence).  The first block's also keeps the rows of the last, incomplete one, after
+// rint(127 x / top) without a division for each element.  `unit` is 2^k and `c` 127 / (top unit): x unit c is off by
+// less than 2^-22 of itself.  The exact quotient of 15 bits by 8 is a half-integer or at least 2^-16 of itself away
+// from one, so rounding to 18 bits first (t - (t - y) with t = 65 y) gives half-integers where they are exact and
+// keeps the others on their side.
+struct Coder {
+  float unit, c;
+  __device__ __forceinline__ explicit Coder(float top) {
+    unit = top < 0x1p-60f ? 0x1p66f : top > 0x1p60f ? 0x1p-60f : 1.0f;
+    c = top > 0.0f ? 127.0f / (top * unit) : 0.0f;
+  }
+  __device__ __forceinline__ uint32_t operator()(float x) const {
+    const float y = x * unit * c, t = y * 65.0f;
+    return static_cast<uint32_t>(static_cast<int>(rintf(t - (t - y)))) & 255u;
+  }
+};
+
+// One workgroup per (block, head, sequence), a thread for 4 keys x 8 dims: its codes of values are dwords of their
+// lines, its rows of keys 8 bytes; a wave has 32 keys x 64 dims, whole lines of the rows it reads.  The first block's workgroup also keeps the rows of the last, incomplete block, after
 // it has read the tail that they replace.
-__global__ void __launch_bounds__(kAppBlock) kv8_append_kernel(AppendArgs a) {
-  __shared__ uint32_t top[2][kAppBlock / 64];
+__global__ void __launch_bounds__(2 * kKvMaxD) kv8_append_kernel(AppendArgs a) {
+  __shared__ uint32_t top[2][2 * kKvMaxD / 64];
   __shared__ uint32_t bad[kKvBlock];
   const KvCache& c = a.c;
   const int h = blockIdx.y, b = blockIdx.z, t = threadIdx.x;
@@ -39,39 +53,36 @@ __global__ void __launch_bounds__(kAppBlock) kv8_append_kernel(AppendArgs a) {
   kv_range(c, b, a.n, start, end);
   const int blk = start / kKvBlock + blockIdx.x, last = end / kKvBlock;
   const int64_t bh = (int64_t)b * c.H + h;
-  const int chunks = c.Dp / 8;  // of a row
-  const uint16_t* kin = a.k + b * a.ksb + h * a.ksh;
-  const uint16_t* vin = a.v + b * a.vsb + h * a.vsh;
+  const int wave = t / 64, lane = t % 64;
+  const int j0 = (wave % 2 * 8 + lane / 8) * 4, d = (wave / 2 * 8 + lane % 8) * 8;
+  const uint16_t* kin = a.k + b * a.ksb + h * a.ksh + d;
+  const uint16_t* vin = a.v + b * a.vsb + h * a.vsh + d;
   uint16_t* kt = c.kt + bh * kKvBlock * c.Dp;
   uint16_t* vt = c.vt + bh * kKvBlock * c.Dp;
-  auto new_row = [&](const uint16_t* in, int64_t ss, int row, int d) {
-    return d < c.D ? ld16(in + (row - start) * ss + d) : zero16();
-  };
+  V4 kx[4], vx[4];
   if (start < end && blk < last) {
-    constexpr int N = kKvBlock * kKvMaxD / 8 / kAppBlock;  // chunks of a thread at most
-    V4 kx[N], vx[N];
     uint32_t mk = 0, mv = 0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int at = t + i * kAppBlock;
-      if (at >= kKvBlock * chunks) break;
-      const int j = at / chunks, d = (at - j * chunks) * 8, row = blk * kKvBlock + j;
+    for (int i = 0; i < 4; ++i) {
+      const int row = blk * kKvBlock + j0 + i;
+      kx[i] = vx[i] = zero16();
       if (row < start) {
-        kx[i] = ld16(kt + kv_key_at(j, d));
+        kx[i] = ld16(kt + kv_key_at(j0 + i, d));
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          vx[i].w[q] = vt[kv_value_at(j, d + 2 * q)] | (uint32_t)vt[kv_value_at(j, d + 2 * q + 1)] << 16;
-      } else {
-        kx[i] = new_row(kin, a.kss, row, d);
-        vx[i] = new_row(vin, a.vss, row, d);
+        for (int q = 0; q < 8; ++q) vx[i].w[q / 2] |= (uint32_t)vt[kv_value_at(j0 + i, d + q)] << (16 * (q & 1));
+      } else if (d < c.D) {
+        kx[i] = ld16(kin + (row - start) * a.kss);
+        vx[i] = ld16(vin + (row - start) * a.vss);
       }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {  // magnitudes of bf16 order as integers, infinities and NaN at the top
         const uint32_t x = kx[i].w[q] & 0x7fff7fffu, y = vx[i].w[q] & 0x7fff7fffu;
         mk = max(mk, max(x & 0xffffu, x >> 16));
         mv = max(mv, max(y & 0xffffu, y >> 16));
       }
-    }
 #pragma unroll
     for (int m = 1; m < 64; m *= 2) {
       mk = max(mk, (uint32_t)__shfl_xor((int)mk, m, 64));
@@ -82,37 +93,33 @@ __global__ void __launch_bounds__(kAppBlock) kv8_append_kernel(AppendArgs a) {
       top[1][t >> 6] = mv;
     }
     __syncthreads();
-#pragma unroll
-    for (int w = 0; w < kAppBlock / 64; ++w) {
+    for (int w = 0; w < (int)blockDim.x / 64; ++w) {
       mk = max(mk, top[0][w]);
       mv = max(mv, top[1][w]);
     }
     const bool nan = mk >= 0x7f80u || mv >= 0x7f80u;
-    const float ak = __uint_as_float(mk << 16), av = __uint_as_float(mv << 16);
-    auto code = [&](uint32_t bits, float amax) -> int {
-      float x = __uint_as_float(bits), m = amax;
-      if (m >= 0x1p64f) {  // keep 127 x below the largest float
-        x *= 0x1p-16f;
-        m *= 0x1p-16f;
-      }
-      return m > 0.0f && !nan ? static_cast<int>(rintf(127.0f * x / m)) : 0;
-    };
+    const float ak = nan ? 0.0f : __uint_as_float(mk << 16), av = nan ? 0.0f : __uint_as_float(mv << 16);
     int8_t* kc = c.k + (bh * c.blocks + blk) * kKvBlock * c.Dp;
     int8_t* vc = c.v + (bh * c.blocks + blk) * kKvBlock * c.Dp;
+    if (nan) {  // no codes: x c would be NaN
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int at = t + i * kAppBlock;
-      if (at >= kKvBlock * chunks) break;
-      const int j = at / chunks, d = (at - j * chunks) * 8;
+      for (int i = 0; i < 4; ++i) kx[i] = vx[i] = zero16();
+    }
+    const Coder ck(ak), cv(av);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
       uint32_t w[2] = {0, 0};
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const uint32_t x = q & 1 ? kx[i].w[q / 2] & 0xffff0000u : kx[i].w[q / 2] << 16;
-        const uint32_t y = q & 1 ? vx[i].w[q / 2] & 0xffff0000u : vx[i].w[q / 2] << 16;
-        w[q / 4] |= (uint32_t)(code(x, ak) & 255) << (8 * (q & 3));
-        vc[kv_value_at(j, d + q)] = static_cast<int8_t>(code(y, av));
-      }
-      *reinterpret_cast<uint2*>(kc + kv_key_at(j, d)) = make_uint2(w[0], w[1]);
+      for (int q = 0; q < 8; ++q)
+        w[q / 4] |= ck(q & 1 ? hi_f(kx[i].w[q / 2]) : lo_f(kx[i].w[q / 2])) << (8 * (q & 3));
+      *reinterpret_cast<uint2*>(kc + kv_key_at(j0 + i, d)) = make_uint2(w[0], w[1]);
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {  // keys j0 .. j0 + 3 lie side by side
+      uint32_t w = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w |= cv(q & 1 ? hi_f(vx[i].w[q / 2]) : lo_f(vx[i].w[q / 2])) << (8 * i);
+      *reinterpret_cast<uint32_t*>(vc + kv_value_at(j0, d + q)) = w;
     }
     if (t == 0) {
       c.ks[bh * c.blocks + blk] = nan ? __builtin_nanf("") : ak / 127.0f;
@@ -120,27 +127,33 @@ __global__ void __launch_bounds__(kAppBlock) kv8_append_kernel(AppendArgs a) {
     }
   }
   if (blockIdx.x != 0 || start >= end || end % kKvBlock == 0) return;
-  const int from = max(start, last * kKvBlock);
   if (t < kKvBlock) bad[t] = 0;
   __syncthreads();  // also: the tail has been read
-  const int rows = end - from, j0 = from % kKvBlock;
-  for (int at = t; at < rows * chunks; at += kAppBlock) {
-    const int j = at / chunks, d = (at - j * chunks) * 8;
-    const V4 kx = new_row(kin, a.kss, from + j, d), vx = new_row(vin, a.vss, from + j, d);
+  bool in[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = last * kKvBlock + j0 + i;
+    in[i] = row >= start && row < end;
+    kx[i] = vx[i] = zero16();
+    if (in[i] && d < c.D) {
+      kx[i] = ld16(kin + (row - start) * a.kss);
+      vx[i] = ld16(vin + (row - start) * a.vss);
+    }
     bool any = false;
 #pragma unroll
-    for (int q = 0; q < 4; ++q) any |= nonfinite(kx.w[q]) || nonfinite(vx.w[q]);
-    if (any) bad[j] = 1;  // every writer writes 1
+    for (int q = 0; q < 4; ++q) any |= nonfinite(kx[i].w[q]) || nonfinite(vx[i].w[q]);
+    if (any) bad[j0 + i] = 1;  // every writer writes 1
   }
   __syncthreads();
-  for (int at = t; at < rows * chunks; at += kAppBlock) {
-    const int j = at / chunks, d = (at - j * chunks) * 8;
-    V4 kx = new_row(kin, a.kss, from + j, d), vx = new_row(vin, a.vss, from + j, d);
-    if (bad[j]) kx.w[0] = kx.w[1] = kx.w[2] = kx.w[3] = vx.w[0] = vx.w[1] = vx.w[2] = vx.w[3] = 0x7fc07fc0u;
-    *reinterpret_cast<uint4*>(kt + kv_key_at(j0 + j, d)) = make_uint4(kx.w[0], kx.w[1], kx.w[2], kx.w[3]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (!in[i]) continue;
+    V4 x = kx[i], y = vx[i];
+    if (bad[j0 + i]) x.w[0] = x.w[1] = x.w[2] = x.w[3] = y.w[0] = y.w[1] = y.w[2] = y.w[3] = 0x7fc07fc0u;
+    *reinterpret_cast<uint4*>(kt + kv_key_at(j0 + i, d)) = make_uint4(x.w[0], x.w[1], x.w[2], x.w[3]);
 #pragma unroll
     for (int q = 0; q < 8; ++q)
-      vt[kv_value_at(j0 + j, d + q)] = static_cast<uint16_t>(q & 1 ? vx.w[q / 2] >> 16 : vx.w[q / 2]);
+      vt[kv_value_at(j0 + i, d + q)] = static_cast<uint16_t>(q & 1 ? y.w[q / 2] >> 16 : y.w[q / 2]);
   }
 }
 
@@ -153,48 +166,60 @@ struct ValuesArgs {
   float* v;
 };
 
-// A thread takes 4 dims of one token and head.
+// One workgroup per (block, head, sequence), a thread for 4 keys x 4 dims: 16 bytes of 4 rows of each output.
 __global__ void __launch_bounds__(256) kv8_values_kernel(ValuesArgs a) {
   const KvCache& c = a.c;
-  const int quads = (c.D + 3) / 4;
-  const int64_t per_seq = a.tokens * c.H * quads;
-  const int b = blockIdx.y;
-  const int64_t at = blockIdx.x * 256ll + threadIdx.x;
-  if (at >= per_seq) return;
-  const int64_t row = at / quads;  // (token, head)
-  const int d = static_cast<int>(at - row * quads) * 4;
-  const int64_t tok = row / c.H;
-  const int h = static_cast<int>(row - tok * c.H);
-  const int64_t pos = (a.first ? a.first[b] : a.first_all) + tok;
+  const int h = blockIdx.y, b = blockIdx.z;
+  const int64_t first = a.first ? a.first[b] : a.first_all;
+  const int64_t blk = (first >> 6) + blockIdx.x;
   int start, end;
   kv_range(c, b, INT32_MAX, start, end);
-  float k[4] = {0, 0, 0, 0}, v[4] = {0, 0, 0, 0};
-  if (pos >= 0 && pos < end) {
-    const int64_t bh = (int64_t)b * c.H + h;
-    const int blk = static_cast<int>(pos / kKvBlock), j = static_cast<int>(pos % kKvBlock);
-    if (blk < end / kKvBlock) {
-      const int64_t g = bh * c.blocks + blk;
-      const float ks = c.ks[g], vs = c.vs[g];
+  const int64_t bh = (int64_t)b * c.H + h, at = (bh * c.blocks + blk) * kKvBlock * c.Dp;
+  const bool held = blk >= 0 && blk < (end + kKvBlock - 1) / kKvBlock, coded = held && blk < end / kKvBlock;
+  const float ks = coded ? c.ks[bh * c.blocks + blk] : 1.0f, vs = coded ? c.vs[bh * c.blocks + blk] : 1.0f;
+  const int quads = c.D / 4;
+  for (int item = threadIdx.x; item < quads * (kKvBlock / 4); item += 256) {
+    const int kg = item / quads, d = (item - kg * quads) * 4, j0 = kg * 4;
+    float k[4][4] = {}, v[4][4] = {};
+    if (coded) {
+      uint32_t kw[4], vw[4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        k[q] = ks * c.k[g * kKvBlock * c.Dp + kv_key_at(j, d + q)];
-        v[q] = vs * c.v[g * kKvBlock * c.Dp + kv_value_at(j, d + q)];
+      for (int i = 0; i < 4; ++i) {
+        kw[i] = *reinterpret_cast<const uint32_t*>(c.k + at + kv_key_at(j0 + i, d));
+        vw[i] = *reinterpret_cast<const uint32_t*>(c.v + at + kv_value_at(j0, d + i));
       }
-    } else {
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        k[q] = bf16_to_f32(c.kt[bh * kKvBlock * c.Dp + kv_key_at(j, d + q)]);
-        v[q] = bf16_to_f32(c.vt[bh * kKvBlock * c.Dp + kv_value_at(j, d + q)]);
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          k[i][q] = ks * static_cast<float>(static_cast<int8_t>(kw[i] >> (8 * q)));
+          v[i][q] = vs * static_cast<float>(static_cast<int8_t>(vw[q] >> (8 * i)));
+        }
+    } else if (held) {
+      const uint16_t* kt = c.kt + bh * kKvBlock * c.Dp;
+      const uint16_t* vt = c.vt + bh * kKvBlock * c.Dp;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint2 x = *reinterpret_cast<const uint2*>(kt + kv_key_at(j0 + i, d));
+        const uint2 y = *reinterpret_cast<const uint2*>(vt + kv_value_at(j0, d + i));
+        k[i][0] = lo_f(x.x), k[i][1] = hi_f(x.x), k[i][2] = lo_f(x.y), k[i][3] = hi_f(x.y);
+        v[0][i] = lo_f(y.x), v[1][i] = hi_f(y.x), v[2][i] = lo_f(y.y), v[3][i] = hi_f(y.y);
       }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t pos = blk * kKvBlock + j0 + i, tok = pos - first;
+      if (tok < 0 || tok >= a.tokens) continue;
+      const bool in = pos < end;
+      const int64_t o = ((b * a.tokens + tok) * c.H + h) * c.D + d;
+      typedef float f4 __attribute__((ext_vector_type(4)));
+      f4 x = {k[i][0], k[i][1], k[i][2], k[i][3]}, y = {v[i][0], v[i][1], v[i][2], v[i][3]};
+      if (!in) x = y = f4{};
+      // past the caches, which hold the rows and codes that come next: 145 -> 106 us for 268 MB an output
+      __builtin_nontemporal_store(x, reinterpret_cast<f4*>(a.k + o));
+      __builtin_nontemporal_store(y, reinterpret_cast<f4*>(a.v + o));
     }
   }
-  const int64_t o = ((b * a.tokens + tok) * c.H + h) * c.D + d;
-#pragma unroll
-  for (int q = 0; q < 4; ++q)
-    if (d + q < c.D) {
-      a.k[o + q] = k[q];
-      a.v[o + q] = v[q];
-    }
 }
 
 }  // namespace
@@ -239,7 +264,7 @@ extern "C" int sf_kv8_append(const sf_kv8_cache* cache, const void* k, int64_t k
   a.n = static_cast<int>(n);
   // blocks that n rows can touch from any start
   const int64_t touched = (n + kKvBlock - 2) / kKvBlock + 1;
-  kv8_append_kernel<<<dim3((unsigned)touched, a.c.H, a.c.B), kAppBlock, 0, static_cast<hipStream_t>(stream)>>>(a);
+  kv8_append_kernel<<<dim3((unsigned)touched, a.c.H, a.c.B), 2 * a.c.Dp, 0, static_cast<hipStream_t>(stream)>>>(a);
   return launch_status("sf_kv8_append");
 }
 
@@ -258,8 +283,7 @@ extern "C" int sf_kv8_values(const sf_kv8_cache* cache, const int32_t* first, in
   a.tokens = tokens;
   a.k = k;
   a.v = v;
-  const int64_t grid = ceil_div(tokens * a.c.H * ((a.c.D + 3) / 4), 256);
-  SF_CHECK_ARG(grid < (1ll << 31), "sf_kv8_values: too many tokens");
-  kv8_values_kernel<<<dim3((unsigned)grid, a.c.B), 256, 0, static_cast<hipStream_t>(stream)>>>(a);
+  const int64_t touched = (tokens + kKvBlock - 2) / kKvBlock + 1;
+  kv8_values_kernel<<<dim3((unsigned)touched, a.c.H, a.c.B), 256, 0, static_cast<hipStream_t>(stream)>>>(a);
   return launch_status("sf_kv8_values");
 }
