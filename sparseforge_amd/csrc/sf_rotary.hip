@@ -6,8 +6,9 @@
 // to the tensors' type (the model's own attention rounds each product to bf16, as HuggingFace's eager form does).
 //
 // Bound by memory: every element is read once and written once, and the 8 bytes of cos and sin per pair, which the
-// heads of a token share, come from the caches.  One launch takes queries and keys.  A thread turns V pairs: two
-// chunks of V elements with V the widest of 8, 4, 2, 1 that sizes, strides and addresses allow (`rotary_width`).
+// heads of a token share, come from the caches.  One launch takes queries and keys.  A thread turns two chunks of V
+// elements (one of 2 V / 2 pairs when interleaved) or copies one of W, the widest of 8, 4, 2, 1 that sizes, strides and
+// addresses allow, 16 bytes at most (`chunk_width`).
 #include "sf_common.hpp"
 
 namespace sf {
@@ -44,6 +45,7 @@ struct RotArgs {
   int64_t first;     // this launch's first token
   uint32_t items;
   int D, half, turn_units;  // units that turn pairs; the others copy
+  int copy_width;
   float sign;
   FastDiv per_token, per_head, seq;
 };
@@ -115,7 +117,14 @@ struct Chunk {
   }
 };
 
-// V = 1 reads interleaved pairs element by element.
+template <int DT, int W>
+__device__ __forceinline__ void copy_chunk(const void* x, int64_t src, void* y, int64_t dst) {
+  Chunk<DT, W> c;
+  c.load(x, src);
+  c.store(y, dst);
+}
+
+// V: elements of a chunk; a unit is two of them, one when interleaved (V = 1: two single elements).
 template <int DT, int V, bool ILV>
 __global__ void __launch_bounds__(kRotBlock) rotary_kernel(RotArgs a) {
   const uint32_t i = blockIdx.x * kRotBlock + threadIdx.x;
@@ -132,10 +141,15 @@ __global__ void __launch_bounds__(kRotBlock) rotary_kernel(RotArgs a) {
   const int64_t src = b * t.sb + s * t.ss + h * t.sh;
   const int64_t dst = (token * t.heads + h) * a.D;
   if (u >= a.turn_units) {  // the part of the head that does not turn
-    const int d = 2 * a.half + (u - a.turn_units) * V;
-    Chunk<DT, V> x;
-    x.load(t.x, src + d);
-    x.store(t.y, dst + d);
+    const int d = 2 * a.half + (u - a.turn_units) * a.copy_width;
+    if (a.copy_width == 8)
+      copy_chunk<DT, 8>(t.x, src + d, t.y, dst + d);
+    else if (a.copy_width == 4)
+      copy_chunk<DT, 4>(t.x, src + d, t.y, dst + d);
+    else if (a.copy_width == 2)
+      copy_chunk<DT, 2>(t.x, src + d, t.y, dst + d);
+    else
+      copy_chunk<DT, 1>(t.x, src + d, t.y, dst + d);
     return;
   }
   int64_t p = s;
@@ -143,32 +157,31 @@ __global__ void __launch_bounds__(kRotBlock) rotary_kernel(RotArgs a) {
     const int64_t at = b * a.pos_sb + s;
     p = a.pos_bytes == 8 ? static_cast<const int64_t*>(a.pos)[at] : static_cast<const int32_t*>(a.pos)[at];
   }
-  const int pair = u * V;
-  Chunk<SF_DTYPE_F32, V> c, sn;
+  constexpr bool ONE = ILV && V > 1;      // one chunk holds whole pairs
+  constexpr int PAIRS = ONE ? V / 2 : V;
+  const int pair = u * PAIRS;
+  Chunk<SF_DTYPE_F32, PAIRS> c, sn;
   if (p >= 0 && p < a.table_rows) {
     c.load(a.cos, p * a.half + pair);
     sn.load(a.sin, p * a.half + pair);
   } else {  // a position that the tables do not hold
 #pragma unroll
-    for (int k = 0; k < V; ++k) c.v[k] = sn.v[k] = __builtin_nanf("");
+    for (int k = 0; k < PAIRS; ++k) c.v[k] = sn.v[k] = __builtin_nanf("");
   }
-  const int d0 = ILV ? 2 * pair : pair, d1 = ILV ? 2 * pair + V : pair + a.half;
+  const int d0 = ILV ? 2 * pair : pair, d1 = ILV ? 2 * pair + 1 : pair + a.half;
   Chunk<DT, V> x0, x1, y0, y1;
   x0.load(t.x, src + d0);
-  x1.load(t.x, src + d1);
+  if constexpr (!ONE) x1.load(t.x, src + d1);
 #pragma unroll
-  for (int k = 0; k < V; ++k) {
-    // pair k: elements k of the two chunks, or 2 k and 2 k + 1 of both in a row
-    const int j = 2 * k;
-    const float e = !ILV ? x0.v[k] : j < V ? x0.v[j % V] : x1.v[j % V];
-    const float o = !ILV ? x1.v[k] : j + 1 < V ? x0.v[(j + 1) % V] : x1.v[(j + 1) % V];
+  for (int k = 0; k < PAIRS; ++k) {
+    const float e = ONE ? x0.v[2 * k % V] : x0.v[k % V], o = ONE ? x0.v[(2 * k + 1) % V] : x1.v[k % V];
     const float ss = a.sign * sn.v[k];
     const float e2 = e * c.v[k] - o * ss, o2 = o * c.v[k] + e * ss;
-    (!ILV ? y0.v[k] : j < V ? y0.v[j % V] : y1.v[j % V]) = e2;
-    (!ILV ? y1.v[k] : j + 1 < V ? y0.v[(j + 1) % V] : y1.v[(j + 1) % V]) = o2;
+    (ONE ? y0.v[2 * k % V] : y0.v[k % V]) = e2;
+    (ONE ? y0.v[(2 * k + 1) % V] : y1.v[k % V]) = o2;
   }
   y0.store(t.y, dst + d0);
-  y1.store(t.y, dst + d1);
+  if constexpr (!ONE) y1.store(t.y, dst + d1);
 }
 
 template <int DT, int V>
@@ -180,23 +193,28 @@ void launch_rotary(const RotArgs& a, bool ilv, hipStream_t st) {
     rotary_kernel<DT, V, false><<<grid, kRotBlock, 0, st>>>(a);
 }
 
-// The widest chunk that divides the half and the copied part and whose accesses are aligned: chunks of V elements
-// start at multiples of V within a head, heads at the strides' multiples.
-int rotary_width(const RotArgs& a, int size) {
-  int v = 8;
-  auto fits = [&](int64_t n) { return n % v == 0; };
+// The widest chunk, 16 bytes at most, that divides `part` and the head and whose accesses are aligned: it starts at
+// multiples of its width within a head, heads at the strides' multiples.
+int chunk_width(const RotArgs& a, int size, int part) {
+  int v = 16 / size;
   for (; v > 1; v /= 2) {
-    bool ok = fits(a.half) && fits(a.D);
-    for (const RotTensor& t : a.t) {
-      if (t.heads == 0) continue;
-      const int bytes = v * size < 16 ? v * size : 16;
-      ok = ok && fits(t.sb) && fits(t.ss) && fits(t.sh) && reinterpret_cast<uintptr_t>(t.x) % bytes == 0 &&
-           reinterpret_cast<uintptr_t>(t.y) % bytes == 0;
-    }
-    const int tb = v * 4 < 16 ? v * 4 : 16;
-    ok = ok && reinterpret_cast<uintptr_t>(a.cos) % tb == 0 && reinterpret_cast<uintptr_t>(a.sin) % tb == 0;
+    bool ok = part % v == 0 && a.D % v == 0;
+    for (const RotTensor& t : a.t)
+      ok = ok && (t.heads == 0 || ((t.sb | t.ss | t.sh) % v == 0 && reinterpret_cast<uintptr_t>(t.x) % (v * size) == 0 &&
+                                   reinterpret_cast<uintptr_t>(t.y) % (v * size) == 0));
     if (ok) break;
   }
+  return v;
+}
+// The same for pairs of `part` elements whose V (or V / 2) cosines are read as one too.
+int turn_width(const RotArgs& a, int size, bool ilv) {
+  int v = chunk_width(a, size, ilv ? 2 * a.half : a.half);
+  auto tables = [&] {
+    const int pairs = ilv && v > 1 ? v / 2 : v, bytes = pairs < 4 ? 4 * pairs : 16;
+    return a.half % pairs == 0 && reinterpret_cast<uintptr_t>(a.cos) % bytes == 0 &&
+           reinterpret_cast<uintptr_t>(a.sin) % bytes == 0;
+  };
+  while (!tables()) v /= 2;
   return v;
 }
 
@@ -236,9 +254,10 @@ extern "C" int sf_rotary(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh
   a.D = static_cast<int>(D);
   a.half = static_cast<int>(rotary_dim / 2);
   a.sign = inverse ? -1.0f : 1.0f;
-  const int v = rotary_width(a, dtype == SF_DTYPE_BF16 ? 2 : 4);
-  a.turn_units = a.half / v;
-  const int64_t per_head = a.turn_units + (D - rotary_dim) / v;
+  const int size = dtype == SF_DTYPE_BF16 ? 2 : 4, v = turn_width(a, size, interleaved);
+  a.copy_width = chunk_width(a, size, 2 * a.half);
+  a.turn_units = interleaved && v > 1 ? 2 * a.half / v : a.half / v;
+  const int64_t per_head = a.turn_units + (D - rotary_dim) / a.copy_width;
   const int64_t per_token = per_head * (heads + kv_heads);
   SF_CHECK_ARG(per_token <= (1ll << 31) - kRotBlock, "sf_rotary: a token's heads are too large");
   a.per_head = fast_div(static_cast<uint32_t>(per_head));
@@ -255,8 +274,7 @@ extern "C" int sf_rotary(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh
       else if (v == 2) launch_rotary<SF_DTYPE_BF16, 2>(a, interleaved, st);
       else launch_rotary<SF_DTYPE_BF16, 1>(a, interleaved, st);
     } else {
-      if (v == 8) launch_rotary<SF_DTYPE_F32, 8>(a, interleaved, st);
-      else if (v == 4) launch_rotary<SF_DTYPE_F32, 4>(a, interleaved, st);
+      if (v == 4) launch_rotary<SF_DTYPE_F32, 4>(a, interleaved, st);
       else if (v == 2) launch_rotary<SF_DTYPE_F32, 2>(a, interleaved, st);
       else launch_rotary<SF_DTYPE_F32, 1>(a, interleaved, st);
     }
