@@ -573,11 +573,22 @@ int sf_from_heads(const void* g, int dtype, int64_t B, int64_t S, int64_t H, int
  * sequence and head strides in elements; elements of a head contiguous); q_out
  * and k_out are contiguous.  heads or kv_heads may be 0.  dtype f32 or bf16.
  */
-int sf_rotary(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, int64_t heads, const void* k, int64_t k_sb,
-              int64_t k_ss, int64_t k_sh, int64_t kv_heads, int dtype, int64_t B, int64_t S, int64_t D,
-              int64_t rotary_dim, int interleaved, const float* cos, const float* sin, int64_t table_rows,
-              const void* positions, int position_bytes, int64_t position_sb, int inverse, void* q_out, void* k_out,
-              void* stream);
+typedef struct sf_rotary_desc {
+  const void* q;
+  void* q_out;
+  int64_t q_sb, q_ss, q_sh, heads;
+  const void* k;
+  void* k_out;
+  int64_t k_sb, k_ss, k_sh, kv_heads;
+  int64_t B, S, D, rotary_dim;
+  const float* cos;
+  const float* sin;
+  int64_t table_rows;
+  const void* positions;
+  int64_t position_sb;
+  int position_bytes, dtype, interleaved, inverse;
+} sf_rotary_desc;
+int sf_rotary(const sf_rotary_desc* desc, void* stream);
 
 /*
  * Logits before a token is drawn (no counterpart in the reference): for token t
@@ -593,12 +604,24 @@ int sf_rotary(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, int64_t h
  * allowed: bytes (0: not), or with allowed_bits one bit a token, lowest first;
  * its row stride in bytes (0: shared); null: all.  rows < 65536.
  */
-int sf_process_logits(const void* logits, int64_t logits_stride, int dtype, int64_t rows, int64_t vocab,
-                      const void* history, int64_t history_stride, int64_t history_len, int history_bytes,
-                      const int32_t* history_lengths, const float* repetition, float repetition_all,
-                      const float* presence, float presence_all, const float* frequency, float frequency_all,
-                      const float* bias, int64_t bias_stride, const void* allowed, int64_t allowed_stride,
-                      int allowed_bits, void* out, int64_t out_stride, void* stream);
+typedef struct sf_logits_desc {
+  const void* logits;
+  void* out;
+  int64_t logits_stride, out_stride, rows, vocab;
+  const void* history;
+  int64_t history_stride, history_len;
+  const int32_t* history_lengths;
+  const float* repetition;
+  const float* presence;
+  const float* frequency;
+  const float* bias;
+  int64_t bias_stride;
+  const void* allowed;
+  int64_t allowed_stride;
+  float repetition_all, presence_all, frequency_all;
+  int history_bytes, allowed_bits, dtype;
+} sf_logits_desc;
+int sf_process_logits(const sf_logits_desc* desc, void* stream);
 
 /*
  * A cache of keys and values held in 8 bits (no counterpart in the reference),

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 import torch
@@ -242,6 +243,11 @@ class AdamwParams(ctypes.Structure):
     ]
 
 
+# sf_rotary_desc and sf_logits_desc, which a decode step fills anew on every call: packed into bytes in 1 us, where the
+# fields of a ctypes Structure (or as many arguments) take 6.  Pointers and int64 are q.
+ROTARY_DESC = struct.Struct("@21q4i")
+LOGITS_DESC = struct.Struct("@17q3f3i")
+
 byref = ctypes.byref
 
 _P = ctypes.c_void_p
@@ -289,14 +295,12 @@ SIGNATURES = {
     "sf_from_heads": (_I, [_P, _I, _I64, _I64, _I64, _I64, _P, _P, _I, _I, _F, _P, _P]),
     "sf_attention_forward": (_I, [_P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _F, _P, _P, _P, _P, _P, _P]),
     "sf_attention_backward": (_I, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _F, _P, _P, _P, _P, _P]),
-    "sf_rotary": (_I, [_P, _I64, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _I, _I64, _I64, _I64, _I64, _I, _P, _P,
-                       _I64, _P, _I, _I64, _I, _P, _P, _P]),
+    "sf_rotary": (_I, [_P, _P]),
     "sf_kv8_append": (_I, [ctypes.POINTER(Kv8Cache), _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P]),
     "sf_kv8_values": (_I, [ctypes.POINTER(Kv8Cache), _P, _I64, _I64, _P, _P, _P]),
     "sf_kv8_attend_workspace_size": (_SZ, [_I64, _I64, _I64, _I64, _I64, _I64]),
     "sf_kv8_attend": (_I, [ctypes.POINTER(Kv8Cache), _P, _I64, _I64, _I64, _I64, _I64, _F, _I64, _I64, _P, _P, _SZ, _P]),
-    "sf_process_logits": (_I, [_P, _I64, _I, _I64, _I64, _P, _I64, _I64, _I, _P, _P, _F, _P, _F, _P, _F, _P, _I64, _P,
-                               _I64, _I, _P, _I64, _P]),
+    "sf_process_logits": (_I, [_P, _P]),
     "sf_transpose_batched": (_I, [_P, _I, _I64, _I64, _I64, _P, _P]),
     "sf_softmax_rows": (_I, [_P, _I, _I64, _I64, _I, _P, _P]),
     "sf_softmax_rows_backward": (_I, [_P, _P, _I, _I64, _I64, _I, _P, _P]),

@@ -138,32 +138,30 @@ __global__ void __launch_bounds__(kLgBlock) logits_kernel(LogitsArgs a) {
 
 using namespace sf;
 
-extern "C" int sf_process_logits(const void* logits, int64_t logits_stride, int dtype, int64_t rows, int64_t vocab,
-                                 const void* history, int64_t history_stride, int64_t history_len, int history_bytes,
-                                 const int32_t* history_lengths, const float* repetition, float repetition_all,
-                                 const float* presence, float presence_all, const float* frequency,
-                                 float frequency_all, const float* bias, int64_t bias_stride, const void* allowed,
-                                 int64_t allowed_stride, int allowed_bits, void* out, int64_t out_stride,
-                                 void* stream) {
-  SF_CHECK_ARG(dtype == SF_DTYPE_F32 || dtype == SF_DTYPE_BF16, "sf_process_logits: unknown dtype %d", dtype);
+extern "C" int sf_process_logits(const sf_logits_desc* desc, void* stream) {
+  SF_CHECK_ARG(desc, "sf_process_logits: null descriptor");
+  const sf_logits_desc& d = *desc;
+  const int64_t rows = d.rows, vocab = d.vocab;
+  SF_CHECK_ARG(d.dtype == SF_DTYPE_F32 || d.dtype == SF_DTYPE_BF16, "sf_process_logits: unknown dtype %d", d.dtype);
   SF_CHECK_ARG(rows >= 0 && rows < 65536 && vocab >= 0 && vocab < (1ll << 31), "sf_process_logits: %lld rows of %lld",
                (long long)rows, (long long)vocab);
   if (rows == 0 || vocab == 0) return SF_OK;
-  SF_CHECK_ARG(logits && out, "sf_process_logits: null pointer");
-  SF_CHECK_ARG(logits_stride >= 0 && out_stride >= vocab, "sf_process_logits: strides %lld, %lld for rows of %lld",
-               (long long)logits_stride, (long long)out_stride, (long long)vocab);
-  SF_CHECK_ARG(!history || ((history_bytes == 4 || history_bytes == 8) && history_len >= 0),
+  SF_CHECK_ARG(d.logits && d.out, "sf_process_logits: null pointer");
+  SF_CHECK_ARG(d.logits_stride >= 0 && d.out_stride >= vocab, "sf_process_logits: strides %lld, %lld for rows of %lld",
+               (long long)d.logits_stride, (long long)d.out_stride, (long long)vocab);
+  SF_CHECK_ARG(!d.history || ((d.history_bytes == 4 || d.history_bytes == 8) && d.history_len >= 0),
                "sf_process_logits: the history must be int32 or int64");
-  SF_CHECK_ARG(repetition || repetition_all > 0.0f, "sf_process_logits: a repetition penalty of %g", repetition_all);
+  SF_CHECK_ARG(d.repetition || d.repetition_all > 0.0f, "sf_process_logits: a repetition penalty of %g",
+               d.repetition_all);
   LogitsArgs a;
-  a.x = logits, a.y = out, a.xs = logits_stride, a.ys = out_stride;
+  a.x = d.logits, a.y = d.out, a.xs = d.logits_stride, a.ys = d.out_stride;
   a.V = vocab;
-  a.hist = history, a.hs = history_stride, a.hlen = history_len, a.hist_bytes = history_bytes;
-  a.lengths = history_lengths;
-  a.rep = repetition, a.pres = presence, a.freq = frequency;
-  a.rep1 = repetition_all, a.pres1 = presence_all, a.freq1 = frequency_all;
-  a.bias = bias, a.bs = bias_stride;
-  a.mask = static_cast<const uint8_t*>(allowed), a.ms = allowed_stride, a.mask_bits = allowed_bits;
+  a.hist = d.history, a.hs = d.history_stride, a.hlen = d.history_len, a.hist_bytes = d.history_bytes;
+  a.lengths = d.history_lengths;
+  a.rep = d.repetition, a.pres = d.presence, a.freq = d.frequency;
+  a.rep1 = d.repetition_all, a.pres1 = d.presence_all, a.freq1 = d.frequency_all;
+  a.bias = d.bias, a.bs = d.bias_stride;
+  a.mask = static_cast<const uint8_t*>(d.allowed), a.ms = d.allowed_stride, a.mask_bits = d.allowed_bits;
   // slices small enough that the rows fill the card, not so small that reading the history again outweighs a slice
   int64_t slices = ceil_div(1024, rows);
   const int64_t fewest = ceil_div(vocab, kLgMaxSlice), most = ceil_div(vocab, 8 * kLgBlock);
@@ -172,9 +170,9 @@ extern "C" int sf_process_logits(const void* logits, int64_t logits_stride, int 
   a.slice = ceil_div(ceil_div(vocab, slices), 32) * 32;
   slices = ceil_div(vocab, a.slice);
   const dim3 grid(static_cast<unsigned>(slices), static_cast<unsigned>(rows));
-  const size_t lds = history ? static_cast<size_t>(a.slice) * 4 : 0;
+  const size_t lds = d.history ? static_cast<size_t>(a.slice) * 4 : 0;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == SF_DTYPE_BF16)
+  if (d.dtype == SF_DTYPE_BF16)
     logits_kernel<SF_DTYPE_BF16><<<grid, kLgBlock, lds, st>>>(a);
   else
     logits_kernel<SF_DTYPE_F32><<<grid, kLgBlock, lds, st>>>(a);

@@ -223,42 +223,43 @@ int turn_width(const RotArgs& a, int size, bool ilv) {
 
 using namespace sf;
 
-extern "C" int sf_rotary(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh, int64_t heads, const void* k,
-                         int64_t k_sb, int64_t k_ss, int64_t k_sh, int64_t kv_heads, int dtype, int64_t B, int64_t S,
-                         int64_t D, int64_t rotary_dim, int interleaved, const float* cos, const float* sin,
-                         int64_t table_rows, const void* positions, int position_bytes, int64_t position_sb,
-                         int inverse, void* q_out, void* k_out, void* stream) {
-  SF_CHECK_ARG(dtype == SF_DTYPE_F32 || dtype == SF_DTYPE_BF16, "sf_rotary: unknown dtype %d", dtype);
-  SF_CHECK_ARG(B >= 0 && S >= 0 && heads >= 0 && kv_heads >= 0, "sf_rotary: negative size");
-  SF_CHECK_ARG(B * S < (1ll << 31) && heads < (1 << 20) && kv_heads < (1 << 20), "sf_rotary: too many tokens or heads");
+extern "C" int sf_rotary(const sf_rotary_desc* desc, void* stream) {
+  SF_CHECK_ARG(desc, "sf_rotary: null descriptor");
+  const sf_rotary_desc& d = *desc;
+  const int64_t B = d.B, S = d.S, D = d.D;
+  SF_CHECK_ARG(d.dtype == SF_DTYPE_F32 || d.dtype == SF_DTYPE_BF16, "sf_rotary: unknown dtype %d", d.dtype);
+  SF_CHECK_ARG(B >= 0 && S >= 0 && d.heads >= 0 && d.kv_heads >= 0, "sf_rotary: negative size");
+  SF_CHECK_ARG((B == 0 || S < (1ll << 31) / B) && d.heads < (1 << 20) && d.kv_heads < (1 << 20),
+               "sf_rotary: too many tokens or heads");
   SF_CHECK_ARG(D >= 1 && D <= 4096, "sf_rotary: head dimension %lld outside 1 .. 4096", (long long)D);
-  SF_CHECK_ARG(rotary_dim >= 2 && rotary_dim % 2 == 0 && rotary_dim <= D,
-               "sf_rotary: rotary_dim %lld must be even, at least 2 and at most the head's %lld", (long long)rotary_dim,
-               (long long)D);
-  SF_CHECK_ARG(!positions || position_bytes == 4 || position_bytes == 8, "sf_rotary: positions must be int32 or int64");
-  if (B == 0 || S == 0 || heads + kv_heads == 0) return SF_OK;
-  SF_CHECK_ARG(cos && sin && table_rows >= 1, "sf_rotary: no tables");
-  SF_CHECK_ARG(heads == 0 || (q && q_out), "sf_rotary: null pointer");
-  SF_CHECK_ARG(kv_heads == 0 || (k && k_out), "sf_rotary: null pointer");
-  SF_CHECK_ARG(positions || S <= table_rows, "sf_rotary: %lld positions, the tables hold %lld", (long long)S,
-               (long long)table_rows);
+  SF_CHECK_ARG(d.rotary_dim >= 2 && d.rotary_dim % 2 == 0 && d.rotary_dim <= D,
+               "sf_rotary: rotary_dim %lld must be even, at least 2 and at most the head's %lld",
+               (long long)d.rotary_dim, (long long)D);
+  SF_CHECK_ARG(!d.positions || d.position_bytes == 4 || d.position_bytes == 8,
+               "sf_rotary: positions must be int32 or int64");
+  if (B == 0 || S == 0 || d.heads + d.kv_heads == 0) return SF_OK;
+  SF_CHECK_ARG(d.cos && d.sin && d.table_rows >= 1, "sf_rotary: no tables");
+  SF_CHECK_ARG(d.heads == 0 || (d.q && d.q_out), "sf_rotary: null pointer");
+  SF_CHECK_ARG(d.kv_heads == 0 || (d.k && d.k_out), "sf_rotary: null pointer");
+  SF_CHECK_ARG(d.positions || S <= d.table_rows, "sf_rotary: %lld positions, the tables hold %lld", (long long)S,
+               (long long)d.table_rows);
   RotArgs a{};
-  a.t[0] = {q, q_out, q_sb, q_ss, q_sh, static_cast<int>(heads)};
-  a.t[1] = {k, k_out, k_sb, k_ss, k_sh, static_cast<int>(kv_heads)};
-  a.cos = cos;
-  a.sin = sin;
-  a.pos = positions;
-  a.pos_bytes = position_bytes;
-  a.pos_sb = position_sb;
-  a.table_rows = table_rows;
+  a.t[0] = {d.q, d.q_out, d.q_sb, d.q_ss, d.q_sh, static_cast<int>(d.heads)};
+  a.t[1] = {d.k, d.k_out, d.k_sb, d.k_ss, d.k_sh, static_cast<int>(d.kv_heads)};
+  a.cos = d.cos;
+  a.sin = d.sin;
+  a.pos = d.positions;
+  a.pos_bytes = d.position_bytes;
+  a.pos_sb = d.position_sb;
+  a.table_rows = d.table_rows;
   a.D = static_cast<int>(D);
-  a.half = static_cast<int>(rotary_dim / 2);
-  a.sign = inverse ? -1.0f : 1.0f;
-  const int size = dtype == SF_DTYPE_BF16 ? 2 : 4, v = turn_width(a, size, interleaved);
+  a.half = static_cast<int>(d.rotary_dim / 2);
+  a.sign = d.inverse ? -1.0f : 1.0f;
+  const int size = d.dtype == SF_DTYPE_BF16 ? 2 : 4, v = turn_width(a, size, d.interleaved);
   a.copy_width = chunk_width(a, size, 2 * a.half);
-  a.turn_units = interleaved && v > 1 ? 2 * a.half / v : a.half / v;
-  const int64_t per_head = a.turn_units + (D - rotary_dim) / a.copy_width;
-  const int64_t per_token = per_head * (heads + kv_heads);
+  a.turn_units = d.interleaved && v > 1 ? 2 * a.half / v : a.half / v;
+  const int64_t per_head = a.turn_units + (D - d.rotary_dim) / a.copy_width;
+  const int64_t per_token = per_head * (d.heads + d.kv_heads);
   SF_CHECK_ARG(per_token <= (1ll << 31) - kRotBlock, "sf_rotary: a token's heads are too large");
   a.per_head = fast_div(static_cast<uint32_t>(per_head));
   a.per_token = fast_div(static_cast<uint32_t>(per_token));
@@ -268,15 +269,15 @@ extern "C" int sf_rotary(const void* q, int64_t q_sb, int64_t q_ss, int64_t q_sh
   for (a.first = 0; a.first < B * S; a.first += most) {
     const int64_t n = B * S - a.first < most ? B * S - a.first : most;
     a.items = static_cast<uint32_t>(n * per_token);
-    if (dtype == SF_DTYPE_BF16) {
-      if (v == 8) launch_rotary<SF_DTYPE_BF16, 8>(a, interleaved, st);
-      else if (v == 4) launch_rotary<SF_DTYPE_BF16, 4>(a, interleaved, st);
-      else if (v == 2) launch_rotary<SF_DTYPE_BF16, 2>(a, interleaved, st);
-      else launch_rotary<SF_DTYPE_BF16, 1>(a, interleaved, st);
+    if (d.dtype == SF_DTYPE_BF16) {
+      if (v == 8) launch_rotary<SF_DTYPE_BF16, 8>(a, d.interleaved, st);
+      else if (v == 4) launch_rotary<SF_DTYPE_BF16, 4>(a, d.interleaved, st);
+      else if (v == 2) launch_rotary<SF_DTYPE_BF16, 2>(a, d.interleaved, st);
+      else launch_rotary<SF_DTYPE_BF16, 1>(a, d.interleaved, st);
     } else {
-      if (v == 4) launch_rotary<SF_DTYPE_F32, 4>(a, interleaved, st);
-      else if (v == 2) launch_rotary<SF_DTYPE_F32, 2>(a, interleaved, st);
-      else launch_rotary<SF_DTYPE_F32, 1>(a, interleaved, st);
+      if (v == 4) launch_rotary<SF_DTYPE_F32, 4>(a, d.interleaved, st);
+      else if (v == 2) launch_rotary<SF_DTYPE_F32, 2>(a, d.interleaved, st);
+      else launch_rotary<SF_DTYPE_F32, 1>(a, d.interleaved, st);
     }
   }
   return launch_status("sf_rotary");

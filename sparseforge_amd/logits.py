@@ -53,9 +53,9 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
             raise ValueError(f"process_logits: history_lengths must be int32 [{B}]")
     elif history_lengths is not None:
         raise ValueError("process_logits: history_lengths without a history")
-    given = [_per_row(x, name, B, dev) for x, name in ((repetition, "repetition"), (presence, "presence"),
-                                                       (frequency, "frequency"))]
-    if not torch.is_tensor(repetition) and not repetition > 0:
+    rep, pres, freq = (_per_row(repetition, "repetition", B, dev), _per_row(presence, "presence", B, dev),
+                       _per_row(frequency, "frequency", B, dev))
+    if not isinstance(repetition, torch.Tensor) and not repetition > 0:
         raise ValueError(f"process_logits: a repetition penalty of {repetition}")
     if bias is not None:
         if bias.dtype != torch.float32:
@@ -73,15 +73,22 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
             raise ValueError(f"process_logits: allowed {tuple(allowed.shape)} for logits {(B, V)}")
         allowed = _rows(allowed)
     lengths = history_lengths.contiguous() if history_lengths is not None else None
-    with _prof.region("sf_process_logits", 2 * logits.numel() * logits.element_size(), "B", dev):
-        L.check(L.lib().sf_process_logits(
-            L.ptr(logits), logits.stride(0) if B > 1 else V, dt, B, V, L.ptr(history) if n else None,
-            history.stride(0) if n else 0, n, history.element_size() if n else 0, L.ptr(lengths) if n else None,
-            *given[0], *given[1], *given[2], L.ptr(bias), bias.stride(0) if bias is not None and bias.dim() == 2 else 0,
-            L.ptr(allowed),
-            allowed.stride(0) * allowed.element_size() if allowed is not None and allowed.dim() == 2 else 0, bits,
-            L.ptr(out), out.stride(0) if B > 1 else V, L.stream(dev)), "sf_process_logits")
+    hist = (history.data_ptr(), history.stride(0), n, L.ptr(lengths) or 0) if n else (0, 0, 0, 0)
+    desc = L.LOGITS_DESC.pack(
+        logits.data_ptr(), out.data_ptr(), logits.stride(0) if B > 1 else V, out.stride(0) if B > 1 else V, B, V, *hist,
+        rep[0], pres[0], freq[0], *_strided(bias), *_strided(allowed), rep[1], pres[1], freq[1],
+        history.element_size() if n else 0, bits, dt)
+    with _prof.region("sf_process_logits", 2 * B * V * logits.element_size(), "B", dev):
+        L.check(L.lib().sf_process_logits(desc, L.stream(dev)), "sf_process_logits")
     return out
+
+
+def _strided(t: torch.Tensor | None) -> tuple[int, int]:
+    """Address and row stride (0: one row for all); the bias' in elements, the mask's in bytes."""
+    if t is None:
+        return 0, 0
+    step = t.stride(0) if t.dim() == 2 else 0
+    return t.data_ptr(), step * (1 if t.dtype == torch.float32 else t.element_size())
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -91,8 +98,8 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 
 def _per_row(x, name: str, B: int, dev) -> tuple:
     """A penalty as the kernel takes it: a pointer to one for each row, or a number."""
-    if not torch.is_tensor(x):
-        return None, float(x)
+    if not isinstance(x, torch.Tensor):
+        return 0, float(x)
     if x.device != dev:
         L.require_device_only(x)
         raise ValueError(f"process_logits: {name} is on {x.device}, the logits on {dev}")

@@ -123,29 +123,26 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(3) == 1 or t.shape[3] == 1 else t.contiguous()
 
 
+_NONE = (0, 0, 0, 0, 0, 0)
+
+
 def _launch(q, k, cos, sin, positions, interleaved: bool, inverse: bool):
-    dev = q.device if q is not None else k.device
     some = q if q is not None else k
+    dev = some.device
     B, S, _, D = some.shape
     cos, sin = cos.contiguous(), sin.contiguous()
+    at = (0, 0, 0)
     if positions is not None:
         positions = positions.contiguous()
-    outs, args, n = [], [], 0
+        at = positions.data_ptr(), S if positions.dim() == 2 else 0, positions.element_size()
     rows = [None if t is None else _rows(t) for t in (q, k)]  # held until the launch
-    for t in rows:
-        if t is None:
-            outs.append(None)
-            args.append((None, 0, 0, 0, 0))
-            continue
-        outs.append(torch.empty(t.shape, dtype=t.dtype, device=dev))
-        args.append((t.data_ptr(), t.stride(0), t.stride(1), t.stride(2), t.shape[2]))
-        n += t.numel()
-    with _prof.region("sf_rotary", 2 * n * some.element_size(), "B", dev):
-        L.check(L.lib().sf_rotary(*args[0], *args[1], L.dtype_code(some), B, S, D, 2 * cos.shape[1], int(interleaved),
-                                  L.ptr(cos), L.ptr(sin), cos.shape[0], L.ptr(positions),
-                                  positions.element_size() if positions is not None else 0,
-                                  S if positions is not None and positions.dim() == 2 else 0, int(inverse),
-                                  L.ptr(outs[0]), L.ptr(outs[1]), L.stream(dev)), "sf_rotary")
+    outs = [None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format) for t in rows]
+    args = [_NONE if t is None else (t.data_ptr(), y.data_ptr(), *t.stride()[:3], t.shape[2])
+            for t, y in zip(rows, outs)]
+    desc = L.ROTARY_DESC.pack(*args[0], *args[1], B, S, D, 2 * cos.shape[1], cos.data_ptr(), sin.data_ptr(),
+                              cos.shape[0], at[0], at[1], at[2], L.dtype_code(some), interleaved, inverse)
+    with _prof.region("sf_rotary", 2 * (args[0][5] + args[1][5]) * B * S * D * some.element_size(), "B", dev):
+        L.check(L.lib().sf_rotary(desc, L.stream(dev)), "sf_rotary")
     return outs[0], outs[1]
 
 

@@ -82,3 +82,18 @@ def test_product_package_never_uses_the_oracle_or_scratch_files():
         assert "_work/" not in path.read_text(), f"{path} refers to _work/"
     for path in list(pkg.rglob("*.hip")) + list(pkg.rglob("*.hpp")):
         assert "_work/" not in path.read_text(), f"{path} refers to _work/"
+
+
+def test_packed_descriptors_match_the_header():
+    """sf_rotary_desc and sf_logits_desc field by field against the struct formats that the binding packs."""
+    from sparseforge_amd import _lib as L
+
+    text = re.sub(r"/\*.*?\*/", "", open(HEADER).read(), flags=re.S)
+    for name, fmt in (("sf_rotary_desc", L.ROTARY_DESC), ("sf_logits_desc", L.LOGITS_DESC)):
+        body = re.search(r"typedef struct %s \{(.*?)\}" % name, text, flags=re.S).group(1)
+        got = ""
+        for field in filter(None, (f.strip() for f in body.split(";"))):
+            code = "q" if "*" in field or field.startswith("int64_t") else {"int": "i", "float": "f"}[field.split()[0]]
+            got += code * (field.count(",") + 1)
+        want = "".join(c * int(n or 1) for n, c in re.findall(r"(\d*)([qif])", fmt.format))
+        assert got == want, name
