@@ -634,8 +634,9 @@ int sf_process_logits(const sf_logits_desc* desc, void* stream);
  * holds a NaN or an infinity becomes NaN there, and so does the block that it
  * is in once that is whole.
  * starts and ends [batch] int32 on the device count the tokens held before the
- * newest ones and with them; the caller advances them.  All entries of a cache
- * for one layer; sizes in bytes, with Dp = head_dim rounded up to 64:
+ * newest ones and with them; sf_kv8_extend advances them, and layers may share
+ * them.  All entries of a cache for one layer; sizes in bytes, with Dp =
+ * head_dim rounded up to 64:
  *   codes batch * kv_heads * blocks * 64 * Dp, scales batch * kv_heads * blocks
  *   * 4, tails batch * kv_heads * 64 * Dp * 2 (codes and tails 16-byte aligned)
  * head_dim: a multiple of 8 up to 256.
@@ -647,11 +648,17 @@ typedef struct sf_kv8_cache {
   float* v_scales;
   void* k_tail;
   void* v_tail;
-  const int32_t* starts;
-  const int32_t* ends;
+  int32_t* starts;
+  int32_t* ends;
   int64_t batch, kv_heads, head_dim;
   int64_t blocks; /* capacity of a sequence in blocks */
 } sf_kv8_cache;
+
+/*
+ * A step of n tokens a sequence: starts = ends, ends += counts[b] (clamped to
+ * 0 .. n; null: n), up to the capacity.
+ */
+int sf_kv8_extend(const sf_kv8_cache* cache, int64_t n, const int32_t* counts, void* stream);
 
 /*
  * The newest rows of every sequence, positions starts[b] .. ends[b] - 1, from

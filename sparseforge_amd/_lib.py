@@ -296,6 +296,7 @@ SIGNATURES = {
     "sf_attention_forward": (_I, [_P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _F, _P, _P, _P, _P, _P, _P]),
     "sf_attention_backward": (_I, [_P, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _P, _P, _F, _P, _P, _P, _P, _P]),
     "sf_rotary": (_I, [_P, _P]),
+    "sf_kv8_extend": (_I, [ctypes.POINTER(Kv8Cache), _I64, _P, _P]),
     "sf_kv8_append": (_I, [ctypes.POINTER(Kv8Cache), _P, _I64, _I64, _I64, _P, _I64, _I64, _I64, _I64, _P]),
     "sf_kv8_values": (_I, [ctypes.POINTER(Kv8Cache), _P, _I64, _I64, _P, _P, _P]),
     "sf_kv8_attend_workspace_size": (_SZ, [_I64, _I64, _I64, _I64, _I64, _I64]),

@@ -13,6 +13,16 @@
 namespace sf {
 namespace {
 
+__global__ void __launch_bounds__(256) kv8_extend_kernel(KvCache c, int n, const int32_t* __restrict__ counts) {
+  const int b = blockIdx.x * 256 + threadIdx.x;
+  if (b >= c.B) return;
+  const int cap = static_cast<int>(c.blocks * kKvBlock);
+  const int count = counts ? min(max(counts[b], 0), n) : n;
+  const int start = min(max(c.ends[b], 0), cap);
+  c.starts[b] = start;
+  c.ends[b] = min(start + count, cap);
+}
+
 struct AppendArgs {
   KvCache c;
   const uint16_t* k;  // [B, n, H, D]
@@ -246,6 +256,16 @@ int kv8_cache(const sf_kv8_cache* d, const char* what, KvCache& c) {
 }  // namespace sf
 
 using namespace sf;
+
+extern "C" int sf_kv8_extend(const sf_kv8_cache* cache, int64_t n, const int32_t* counts, void* stream) {
+  KvCache c;
+  if (int rc = kv8_cache(cache, "sf_kv8_extend", c)) return rc;
+  SF_CHECK_ARG(n >= 0 && n <= c.blocks * kKvBlock, "sf_kv8_extend: %lld tokens for a capacity of %lld", (long long)n,
+               (long long)(c.blocks * kKvBlock));
+  kv8_extend_kernel<<<static_cast<unsigned>(ceil_div(c.B, 256)), 256, 0, static_cast<hipStream_t>(stream)>>>(
+      c, static_cast<int>(n), counts);
+  return launch_status("sf_kv8_extend");
+}
 
 extern "C" int sf_kv8_append(const sf_kv8_cache* cache, const void* k, int64_t k_sb, int64_t k_ss, int64_t k_sh,
                              const void* v, int64_t v_sb, int64_t v_ss, int64_t v_sh, int64_t n, void* stream) {

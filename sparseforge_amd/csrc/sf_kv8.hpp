@@ -36,9 +36,9 @@ struct KvCache {
   float* vs;
   uint16_t* kt;  // tails
   uint16_t* vt;
-  const int32_t* starts;  // [B]: tokens held before the newest
-  const int32_t* ends;    // [B]: and with them
-  int64_t blocks;         // capacity of a sequence in blocks
+  int32_t* starts;  // [B]: tokens held before the newest
+  int32_t* ends;    // [B]: and with them
+  int64_t blocks;   // capacity of a sequence in blocks
   int B, H, D, Dp;
 };
 

@@ -29,7 +29,11 @@ BLOCK = 64  # tokens that share a scale
 class KVCache8:
     """Keys and values of `batch` sequences of at most `capacity` tokens (rounded up to whole blocks) for `layers`
     layers.  `ends` [batch] int32 holds the sequences' lengths on the device, `bound` what the host knows them to be
-    at most (exact when every counts[b] is n)."""
+    at most (exact when every counts[b] is n).
+
+    A step may be captured in a graph and replayed: the lengths advance on the device, and the kernels read them and
+    stay inside the capacity.  `bound`, which sizes attend's launch, is that of the capture: set it to the length that
+    the replays will reach before capturing."""
 
     def __init__(self, batch: int, kv_heads: int, head_dim: int, capacity: int, layers: int = 1, device="cuda"):
         if min(batch, kv_heads, capacity, layers) < 1:
@@ -84,8 +88,8 @@ class KVCache8:
                 raise ValueError("KVCache8.extend: counts are on another device")
             if counts.dtype != torch.int32 or counts.shape != (self.batch,):
                 raise ValueError(f"KVCache8.extend: counts must be int32 [{self.batch}]")
-        self.starts.copy_(self.ends)
-        self.ends.add_(n if counts is None else counts.clamp(0, n))
+        L.check(L.lib().sf_kv8_extend(ctypes.byref(self._descs[0]), n, L.ptr(counts), L.stream(self.ends.device)),
+                "sf_kv8_extend")
         self.bound += n
         self._new = n
 

@@ -44,6 +44,7 @@ from torch.nn import functional as F
 from . import _lib as L
 from . import profiling as _prof
 from .linear import apply_in_backward, plain_backward
+from .rotary import RotaryScaling, rotary_cos_sin
 from .sparse_modeling import SparseLinear, SparseLinearConfig
 
 
@@ -58,6 +59,7 @@ class LlamaShape:
     num_attention_heads: int = 32
     rms_norm_eps: float = 1e-5
     rope_theta: float = 10000.0
+    rope_scaling: RotaryScaling | None = None  # for contexts longer than the trained one
     output_hidden_state: bool = False  # set by Distill_Model
 
     @property
@@ -717,7 +719,12 @@ class LlamaDecoder(nn.Module):
     def _tables(self, seq: int, device):
         key = (seq, str(device))
         if key not in self._rope:
-            self._rope[key] = rotary_tables(seq, self.config.head_dim, self.config.rope_theta, device)
+            c = self.config
+            if c.rope_scaling is None:
+                self._rope[key] = rotary_tables(seq, c.head_dim, c.rope_theta, device)
+            else:
+                self._rope[key] = tuple(torch.cat([t, t], dim=-1) for t in rotary_cos_sin(
+                    seq, c.head_dim, c.rope_theta, c.rope_scaling, device))
         return self._rope[key]
 
     def forward(self, idx: torch.Tensor, targets: torch.Tensor | None = None):

@@ -282,6 +282,69 @@ def test_runaway_and_flat_scores(cuda_device):
         assert bool(((out - o).abs() <= bar).all())
 
 
+@pytest.mark.parametrize("n", [1, 40])
+def test_values_of_any_size(cuda_device, n):
+    """Blocks of values from 2^-100 to 2^110, of zeros, and all in one sequence: the smallest ones carry the weight of
+    their keys, and a block of large ones that has next to none of it adds next to nothing."""
+    from sparseforge_amd.kv_cache import KVCache8
+
+    g = torch.Generator(device=cuda_device).manual_seed(n)
+    T, H, Hk, D = 6 * BLOCK + 20, 4, 2, 64
+    k, v = _data(g, 1, T, Hk, D, cuda_device)
+    q = torch.randn(1, n, H, D, generator=g, device=cuda_device).bfloat16()
+    mixed = torch.tensor([2.0 ** e for e in (0, -100, 90, -66, 66, 0, 0)], device=cuda_device)
+    mixed[5] = 0.0
+    for size in (torch.full((7,), 2.0 ** -100, device=cuda_device), torch.full((7,), 2.0 ** 110, device=cuda_device),
+                 torch.zeros(7, device=cuda_device), mixed, mixed.flip(0)):
+        w = (v.float() * size.repeat_interleave(BLOCK)[:T, None, None]).bfloat16()
+        cache = KVCache8(1, Hk, D, T)
+        if T > n:
+            _fill(cache, k[:, :T - n], w[:, :T - n], [T - n])
+        cache.extend(n)
+        cache.append(k[:, T - n:], w[:, T - n:])
+        out = cache.attend(q).view(n, H, D).double()
+        o, bar = _attention(q[0], _stored(k[0], T), _stored(w[0], T), T - n, D ** -0.5, 0)
+        assert bool(((out - o).abs() <= bar).all())
+
+
+def test_captured_step_replayed(cuda_device):
+    """One token's step as a graph, replayed from 60 tokens to 70 (a block is completed on the way) with eager work and
+    waits between the replays, each against the same step without a graph."""
+    from sparseforge_amd.kv_cache import KVCache8
+
+    g = torch.Generator(device=cuda_device).manual_seed(12)
+    B, H, Hk, D, T = 2, 4, 2, 64, 72
+    k, v = _data(g, B, T, Hk, D, cuda_device)
+    q = torch.randn(T, B, 1, H, D, generator=g, device=cuda_device).bfloat16()
+    plain, caught = KVCache8(B, Hk, D, T), KVCache8(B, Hk, D, T)
+    for c in (plain, caught):
+        _fill(c, k[:, :60], v[:, :60], [60, 60])
+    now = [torch.empty_like(x) for x in (q[0], k[:, :1], v[:, :1])]
+
+    def step(c):
+        c.extend(1)
+        c.append(now[1], now[2])
+        return c.attend(now[0])
+
+    step(KVCache8(B, Hk, D, T))  # the kernels are loaded before the capture
+    torch.cuda.synchronize()
+    caught.bound = T - 1
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(caught)
+    for i in range(60, 70):
+        for x, y in zip(now, (q[i], k[:, i:i + 1], v[:, i:i + 1])):
+            x.copy_(y)
+        plain.bound = T - 1  # the same cut of the launch
+        want = step(plain)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+        torch.randn(1000, device=cuda_device).sum().item()
+    assert caught.ends.tolist() == [70, 70]
+    assert all(torch.equal(a, b) for a, b in zip(caught.values(0, 70), plain.values(0, 70)))
+
+
 def test_queries_that_are_not_finite_stay_with_their_rows(cuda_device):
     from sparseforge_amd.kv_cache import KVCache8
 
