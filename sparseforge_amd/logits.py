@@ -29,7 +29,10 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
     ids outside 0 .. V - 1 (padding) are not.  repetition, presence, frequency: a number, or float32 [B] on the device.
     bias: float32 [V] or [B, V].  allowed: bool [V] or [B, V], or its bits as int32 [ceil(V / 32)] or [B, ceil(V / 32)]
     (token t is bit t % 32 of word t // 32)."""
-    dev = L.require_device_only(logits, history, history_lengths, bias, allowed, out)
+    dev = logits.device
+    for t in (logits, history, history_lengths, bias, allowed, out):
+        if t is not None and (not t.is_cuda or t.get_device() != dev.index):
+            L.require_device_only(logits, history, history_lengths, bias, allowed, out)  # says which
     dt = L.dtype_code(logits)
     if logits.dim() != 2:
         raise ValueError(f"process_logits: logits must be [B, V], got {tuple(logits.shape)}")
@@ -37,7 +40,7 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
     if logits.stride(1) != 1 and V > 1:
         logits = logits.contiguous()
     if out is None:
-        out = torch.empty((B, V), dtype=logits.dtype, device=dev)
+        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
     elif out.shape != (B, V) or out.dtype != logits.dtype or not (out.stride(1) == 1 or V <= 1) \
             or (B > 1 and out.stride(0) < V):
         raise ValueError(f"process_logits: out must be {logits.dtype} [{B}, {V}] with rows of its own")

@@ -91,13 +91,17 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor, sin
 
 
 def _check(q, k, cos, sin, positions) -> None:
-    L.require_device_only(q, k, cos, sin, positions)
+    at = q.get_device()
+    if at < 0 or cos.get_device() != at or sin.get_device() != at or (k is not None and k.get_device() != at) \
+            or (positions is not None and positions.get_device() != at):
+        L.require_device_only(q, k, cos, sin, positions)  # says which
     if q.dim() != 4:
         raise ValueError(f"rotary_embed: q must be [B, S, H, D], got {tuple(q.shape)}")
     if q.dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"rotary_embed: q is {q.dtype} (bfloat16 / float32 only)")
+    B, S, _, D = q.shape
     if k is not None:
-        if k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3]:
+        if k.dim() != 4 or k.shape[0] != B or k.shape[1] != S or k.shape[3] != D:
             raise ValueError(f"rotary_embed: k {tuple(k.shape)} does not go with q {tuple(q.shape)}")
         if k.dtype != q.dtype:
             raise TypeError(f"rotary_embed: k is {k.dtype}, q {q.dtype}")
@@ -105,17 +109,17 @@ def _check(q, k, cos, sin, positions) -> None:
         raise TypeError("rotary_embed: cos and sin must be float32")
     if cos.dim() != 2 or cos.shape != sin.shape:
         raise ValueError(f"rotary_embed: cos {tuple(cos.shape)} and sin {tuple(sin.shape)} must be [P, r / 2] both")
-    if not 1 <= cos.shape[1] <= q.shape[3] // 2:
-        raise ValueError(f"rotary_embed: tables of {cos.shape[1]} pairs for heads of {q.shape[3]}")
+    if not 1 <= cos.shape[1] <= D // 2:
+        raise ValueError(f"rotary_embed: tables of {cos.shape[1]} pairs for heads of {D}")
     if cos.requires_grad or sin.requires_grad:
         raise ValueError("rotary_embed: cos and sin take no gradient")
-    if positions is not None:
-        if positions.dtype not in (torch.int32, torch.int64):
-            raise TypeError(f"rotary_embed: positions are {positions.dtype} (int32 / int64 only)")
-        if positions.shape not in (q.shape[:2], q.shape[1:2]):
-            raise ValueError(f"rotary_embed: positions {tuple(positions.shape)} for q {tuple(q.shape)}")
-    elif q.shape[1] > cos.shape[0]:
-        raise ValueError(f"rotary_embed: {q.shape[1]} positions, the tables hold {cos.shape[0]}")
+    if positions is None:
+        if S > cos.shape[0]:
+            raise ValueError(f"rotary_embed: {S} positions, the tables hold {cos.shape[0]}")
+    elif positions.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"rotary_embed: positions are {positions.dtype} (int32 / int64 only)")
+    elif positions.shape != (B, S) and positions.shape != (S,):
+        raise ValueError(f"rotary_embed: positions {tuple(positions.shape)} for q {tuple(q.shape)}")
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
@@ -126,24 +130,35 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
 _NONE = (0, 0, 0, 0, 0, 0)
 
 
+def _side(t: torch.Tensor, y: torch.Tensor) -> tuple:
+    sb, ss, sh, _ = t.stride()
+    return t.data_ptr(), y.data_ptr(), sb, ss, sh, t.shape[2]
+
+
 def _launch(q, k, cos, sin, positions, interleaved: bool, inverse: bool):
     some = q if q is not None else k
-    dev = some.device
     B, S, _, D = some.shape
     cos, sin = cos.contiguous(), sin.contiguous()
     at = (0, 0, 0)
     if positions is not None:
         positions = positions.contiguous()
         at = positions.data_ptr(), S if positions.dim() == 2 else 0, positions.element_size()
-    rows = [None if t is None else _rows(t) for t in (q, k)]  # held until the launch
-    outs = [None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format) for t in rows]
-    args = [_NONE if t is None else (t.data_ptr(), y.data_ptr(), *t.stride()[:3], t.shape[2])
-            for t, y in zip(rows, outs)]
-    desc = L.ROTARY_DESC.pack(*args[0], *args[1], B, S, D, 2 * cos.shape[1], cos.data_ptr(), sin.data_ptr(),
-                              cos.shape[0], at[0], at[1], at[2], L.dtype_code(some), interleaved, inverse)
-    with _prof.region("sf_rotary", 2 * (args[0][5] + args[1][5]) * B * S * D * some.element_size(), "B", dev):
+    q_out = k_out = None
+    q_side = k_side = _NONE
+    if q is not None:
+        q = _rows(q)
+        q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+        q_side = _side(q, q_out)
+    if k is not None:
+        k = _rows(k)
+        k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
+        k_side = _side(k, k_out)
+    desc = L.ROTARY_DESC.pack(*q_side, *k_side, B, S, D, 2 * cos.shape[1], cos.data_ptr(), sin.data_ptr(),
+                              cos.shape[0], *at, L.dtype_code(some), interleaved, inverse)
+    dev = some.device
+    with _prof.region("sf_rotary", 2 * (q_side[5] + k_side[5]) * B * S * D * some.element_size(), "B", dev):
         L.check(L.lib().sf_rotary(desc, L.stream(dev)), "sf_rotary")
-    return outs[0], outs[1]
+    return q_out, k_out
 
 
 class _Rotary(torch.autograd.Function):
