@@ -3,14 +3,25 @@
 // with i, j positions of a sequence.  A query that sees no key (its sequence has ended) gives 0.
 //
 // The query heads that share a key-value head are rows of one product with it: row r of (sequence, key-value head) is
-// query r / group of head r % group.  A wave takes 16 RT rows over whole blocks of 64 keys.  q codes and p codes are
-// products of bf16 operands (codes up to 127 are exact in bf16) with f32 sums; the block's key scale multiplies the
-// scores with the softmax's factor, its value scale the probabilities before they round to bf16.
+// query r / group of head r % group.  A wave takes 16 RT rows over whole blocks of 64 keys, one pass with a running
+// maximum and sum.  Both products are v_mfma_f32_16x16x32_bf16 on codes converted to bf16, which is exact (8 significant
+// bits), with f32 scores, sums and outputs.  The key scale multiplies the scores with the softmax's factor; the value
+// scale enters the exponent (BlockScale).  The probabilities round to bf16 as operands of the second product, which
+// moves an output by 2^-8 of its terms at most, as much as storing it in bf16 does; the sums are of the rounded ones.
 //
-// A wave's running maximum is one for all lanes of a row and is raised only when a score passes it by 8 (in log2):
-// probabilities up to 2^8 cost nothing in f32 or bf16, and most blocks need no exchange between lanes.
+// A row's running maximum is raised only when a score passes it by 8 (in log2): probabilities up to 2^8 cost nothing in
+// f32 or bf16, and most blocks need no exchange between lanes.
 //
-// Bound by memory for single tokens: every code is read once, 2 D bytes per key and head.
+// Two forms:
+//   up to 16 rows (32 with heads of at most 128): kv8_attend_kernel.  Bound by reading the codes, 2 D bytes per key and
+//     key-value head.  Each wave takes blocks of its own, converted in registers, and the keys are split over workgroups;
+//     kv8_join_kernel joins them.  Conversion and softmax, about 500 vector instructions a block and wave, stay under
+//     the memory's time.  Measured: 32 sequences of 1024 .. 4096, 32 heads of 128: 113 us, 5.8 TB/s; 2 of 131071, 32
+//     heads over 8: 85 us + 5 us for the join, 6.0 TB/s; one of 33 tokens, 32 heads of 64: 5.2 us.
+//   more: kv8_chunk_kernel.  Bound by the matrix unit and, as much, by the vector unit beside it (an exponential, its
+//     argument, a maximum and half a conversion to bf16 for each score): of its cycles the first is busy in 42 % and the
+//     second in 53 %, at 2.05 GHz under this load.  Measured: 2048 tokens over 18001, 32 heads of 128 over 8: 537 to
+//     625 us from one card to another, 910 to 1060 TFLOP/s, where a large library product of bf16 reaches 1234.
 #include "sf_kv8.hpp"
 
 namespace sf {
@@ -479,7 +490,7 @@ __global__ void __launch_bounds__(kAtnWaves * 64, DB * RT == 1 ? 4 : DB * RT == 
 // while the probabilities of this one are exponentials on the vector unit; the block after, its codes loaded at the
 // turn's start, is converted at its end.  Keys are staged one block further than values.
 template <int DB, int RT, int WAVES>
-__global__ void __launch_bounds__(WAVES * 64, 2) kv8_chunk_kernel(AttendArgs a) {
+__global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DB > 2 ? 1 : 2) kv8_chunk_kernel(AttendArgs a) {
   constexpr int ROWS = 16 * RT * WAVES, Dp = DB * 64, N = DB * 8 / WAVES;  // chunks of a lane: keys', then values'
   __shared__ __align__(16) unsigned char lds[2][DB * 16][1024];           // fragments (hh, t, a) of keys, (dt, u) of values
   int tile, split = blockIdx.y;
@@ -701,6 +712,8 @@ AttendPlan attend_plan(int64_t B, int64_t H, int64_t heads, int64_t Dp, int64_t 
   int64_t s = ceil_div(p.waves == 8 ? 256 : 512, wgs);
   const int64_t most = ceil_div(blocks, 2 * kAtnWaves);
   if (s > most) s = most;
+  // four blocks for each wave cost less than joining splits: 1000 tokens over 8 heads of 128 take 11.5 us, 16 us in two
+  if (!p.waves && blocks <= 4 * kAtnWaves) s = 1;
   if (s < 1) s = 1;
   p.splits = static_cast<int>(s);
   p.chunk = static_cast<int>(blocks > 0 ? ceil_div(blocks, s) : 1);
@@ -763,7 +776,7 @@ extern "C" int sf_kv8_attend(const sf_kv8_cache* cache, const void* q, int64_t q
                workspace_bytes, p.bytes);
   SF_CHECK_ARG(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, "sf_kv8_attend: workspace must be 16-byte aligned");
   const int64_t wgs = (int64_t)a.c.B * a.c.H * p.tiles;
-  SF_CHECK_ARG(a.c.B * n * heads < (1ll << 31), "sf_kv8_attend: too many rows");
+  SF_CHECK_ARG(a.c.B * n * heads < (1ll << 31) && wgs < (1ll << 23), "sf_kv8_attend: too many rows");
   a.q = static_cast<const uint16_t*>(q);
   a.qsb = q_sb, a.qss = q_ss, a.qsh = q_sh;
   a.out = static_cast<uint16_t*>(out);
