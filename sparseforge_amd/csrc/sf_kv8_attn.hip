@@ -16,8 +16,8 @@
 //   up to 16 rows (32 with heads of at most 128): kv8_attend_kernel.  Bound by reading the codes, 2 D bytes per key and
 //     key-value head.  Each wave takes blocks of its own, converted in registers, and the keys are split over workgroups;
 //     kv8_join_kernel joins them.  Conversion and softmax, about 500 vector instructions a block and wave, stay under
-//     the memory's time.  Measured: 32 sequences of 1024 .. 4096, 32 heads of 128: 113 us, 5.8 TB/s; 2 of 131071, 32
-//     heads over 8: 85 us + 5 us for the join, 6.0 TB/s; one of 33 tokens, 32 heads of 64: 5.2 us.
+//     the memory's time.  Measured: 32 sequences of 1024 .. 4096, 32 heads of 128: 111 us, 5.9 TB/s; 2 of 131071, 32
+//     heads over 8: 84 us + 5 us for the join, 6.0 TB/s; one of 33 tokens, 32 heads of 64: 5.1 us.
 //   more: kv8_chunk_kernel.  Bound by the matrix unit and, as much, by the vector unit beside it (an exponential, its
 //     argument, a maximum and half a conversion to bf16 for each score): of its cycles the first is busy in 42 % and the
 //     second in 53 %, at 2.05 GHz under this load.  Measured: 2048 tokens over 18001, 32 heads of 128 over 8: 537 to
@@ -380,8 +380,12 @@ struct RowState {
 };
 
 // One split of one tile of rows: the waves take its blocks in turn and join at the end.
+// Waves a SIMD that the registers hold without spilling (heads of 256 run 2 waves 20 % slower: they spill).
 template <int DB, int RT>
-__global__ void __launch_bounds__(kAtnWaves * 64, DB * RT == 1 ? 4 : DB * RT == 2 && RT == 1 ? 3 : 2) kv8_attend_kernel(AttendArgs a) {
+constexpr int attend_waves() { return DB * RT == 1 ? 4 : DB == 2 && RT == 1 ? 3 : DB == 4 ? 1 : 2; }
+
+template <int DB, int RT>
+__global__ void __launch_bounds__(kAtnWaves * 64, attend_waves<DB, RT>()) kv8_attend_kernel(AttendArgs a) {
   constexpr int ROWS = 16 * RT, Dp = DB * 64;
   __shared__ float sml[2][kAtnWaves][ROWS];
   __shared__ __align__(16) float so[kAtnWaves][ROWS][Dp + 4];
@@ -418,18 +422,20 @@ __global__ void __launch_bounds__(kAtnWaves * 64, DB * RT == 1 ? 4 : DB * RT == 
       k1 = ks[blk], v1 = vs[blk];
     }
     for (; blk < ce; blk += kAtnWaves) {
-      const int64_t next = min(blk + kAtnWaves, ce - 1);  // the last one is read again for nothing
+      const int64_t next = blk + kAtnWaves;
       f32x4_t s[RT][4];
       bf16x8_t p[RT][2];
       st.scores(x, s);
-      x.load(x.k, kc + next * kKvBlock * Dp);
       const BlockScale sc(k1, v1, a.scale);
-      k1 = ks[next], v1 = vs[next];
+      if (next < ce) {
+        x.load(x.k, kc + next * kKvBlock * Dp);
+        k1 = ks[next], v1 = vs[next];
+      }
       st.settle(s, blk, sc, a.window, masked(blk));
       st.weights(s, sc, p);
       st.sums(p, sc);
       st.output(x, p);
-      x.load(x.v, vc + next * kKvBlock * Dp);
+      if (next < ce) x.load(x.v, vc + next * kKvBlock * Dp);
     }
     if (blk < be) {  // the incomplete block
       const TailBlock<DB> tail{a.c.kt + bh * kKvBlock * Dp, a.c.vt + bh * kKvBlock * Dp, tr.end - blk * kKvBlock};
