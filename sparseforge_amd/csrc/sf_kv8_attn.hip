@@ -381,11 +381,10 @@ struct RowState {
 
 // One split of one tile of rows: the waves take its blocks in turn and join at the end.
 // Waves a SIMD that the registers hold without spilling (heads of 256 run 2 waves 20 % slower: they spill).
-template <int DB, int RT>
-constexpr int attend_waves() { return DB * RT == 1 ? 4 : DB == 2 && RT == 1 ? 3 : DB == 4 ? 1 : 2; }
+constexpr int attend_waves(int db, int rt) { return db * rt == 1 ? 4 : db == 2 && rt == 1 ? 3 : db == 4 ? 1 : 2; }
 
 template <int DB, int RT>
-__global__ void __launch_bounds__(kAtnWaves * 64, attend_waves<DB, RT>()) kv8_attend_kernel(AttendArgs a) {
+__global__ void __launch_bounds__(kAtnWaves * 64, attend_waves(DB, RT)) kv8_attend_kernel(AttendArgs a) {
   constexpr int ROWS = 16 * RT, Dp = DB * 64;
   __shared__ float sml[2][kAtnWaves][ROWS];
   __shared__ __align__(16) float so[kAtnWaves][ROWS][Dp + 4];
