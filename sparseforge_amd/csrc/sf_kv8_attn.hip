@@ -176,9 +176,9 @@ struct RowState {
   bf16x8_t q[RT][DB][2];
   f32x4_t o[RT][DB * 4];
   float m[RT], l[RT];
-  int pos[RT];         // position of the row's query, -1: no such row
+  int pos[RT];  // position of the row's query, -1: no such row
 
-  // The queries of rows row0 + 16 r + lane % 16 (below `rows`) of key-value head h.
+  // The queries of rows row0 + 16 r + lane % 16 of key-value head h; rows past the tile's queries are zeros.
   __device__ __forceinline__ void start(const AttendArgs& a, const TileRange& tr, int b, int h, int row0) {
     const int lane = threadIdx.x & 63, g = lane >> 4;
 #pragma unroll
@@ -379,10 +379,10 @@ struct RowState {
   }
 };
 
-// One split of one tile of rows: the waves take its blocks in turn and join at the end.
 // Waves a SIMD that the registers hold without spilling (heads of 256 run 2 waves 20 % slower: they spill).
 constexpr int attend_waves(int db, int rt) { return db * rt == 1 ? 4 : db == 2 && rt == 1 ? 3 : db == 4 ? 1 : 2; }
 
+// Few rows: one split of one tile.  The waves take its blocks in turn and join at the end.
 template <int DB, int RT>
 __global__ void __launch_bounds__(kAtnWaves * 64, attend_waves(DB, RT)) kv8_attend_kernel(AttendArgs a) {
   constexpr int ROWS = 16 * RT, Dp = DB * 64;

@@ -130,6 +130,20 @@ def test_values_that_are_not_finite(cuda_device):
         assert got[4] == -math.inf and got[5] == -math.inf and got[8] == 2.0
 
 
+def test_offsets_past_32_bits(cuda_device):
+    """2.2e9 logits: the last rows are processed as rows of their own."""
+    from sparseforge_amd.logits import process_logits
+
+    B, V = 17000, 131072
+    g = torch.Generator(device=cuda_device).manual_seed(4)
+    row = torch.randn(1, V, generator=g, device=cuda_device).bfloat16()
+    history = torch.randint(0, V, (B, 8), generator=g, device=cuda_device)
+    freq = torch.rand(B, generator=g, device=cuda_device)
+    got = process_logits(row.expand(B, V), history, frequency=freq)
+    for b in (0, 16383, 16384, 16385, B - 1):
+        assert torch.equal(got[b:b + 1], process_logits(row, history[b:b + 1], frequency=freq[b:b + 1].contiguous()))
+
+
 def test_empty_and_refusals(cuda_device):
     from sparseforge_amd.logits import process_logits
 
@@ -143,6 +157,8 @@ def test_empty_and_refusals(cuda_device):
         process_logits(x.half())
     with pytest.raises(ValueError):
         process_logits(x[0])
+    with pytest.raises(ValueError):
+        process_logits(torch.zeros(65536, 2, device=dev))
     with pytest.raises(TypeError):
         process_logits(x, ids.float())
     for bad in (ids[:1], ids[0]):

@@ -147,6 +147,19 @@ def test_positions_outside_the_tables_give_nan(cuda_device):
             assert not got[0, (0, 3)].isnan().any() and not got[..., 16:].isnan().any()
 
 
+def test_more_than_one_launch_and_offsets_past_32_bits(cuda_device):
+    """2.3e9 units of work and 3.5e9 elements: the last tokens are turned as the first ones."""
+    from sparseforge_amd.rotary import rotary_cos_sin, rotary_embed
+
+    S, H, D = 1 << 20, 1100, 3
+    g = torch.Generator(device=cuda_device).manual_seed(9)
+    cos, sin = rotary_cos_sin(S, 2, device=cuda_device)
+    row = torch.randn(1, 1, H, D, generator=g, device=cuda_device).bfloat16()
+    got = rotary_embed(row.expand(1, S, H, D), None, cos, sin)[0]
+    for at in (0, 1, (1 << 31) // (H * D) + 1, (1 << 31) // (2 * H), (1 << 31) // (2 * H) + 1, S - 1):
+        _check(got[:, at:at + 1].contiguous(), row, cos, sin, torch.tensor([[at]], device=cuda_device), False)
+
+
 def test_empty_and_refusals(cuda_device):
     from sparseforge_amd.rotary import rotary_cos_sin, rotary_embed
 
