@@ -18,10 +18,11 @@
 //     kv8_join_kernel joins them.  Conversion and softmax, about 500 vector instructions a block and wave, stay under
 //     the memory's time.  Measured: 32 sequences of 1024 .. 4096, 32 heads of 128: 111 us, 5.9 TB/s; 2 of 131071, 32
 //     heads over 8: 84 us + 5 us for the join, 6.0 TB/s; one of 33 tokens, 32 heads of 64: 5.1 us.
-//   more: kv8_chunk_kernel.  Bound by the matrix unit and, as much, by the vector unit beside it (an exponential, its
-//     argument, a maximum and half a conversion to bf16 for each score): of its cycles the first is busy in 42 % and the
-//     second in 53 %, at 2.05 GHz under this load.  Measured: 2048 tokens over 18001, 32 heads of 128 over 8: 537 to
-//     625 us from one card to another, 910 to 1060 TFLOP/s, where a large library product of bf16 reaches 1234.
+//   more: kv8_chunk_kernel.  Bound by power: the matrix unit is busy in 52 % of its cycles and the vector unit beside it
+//     (an exponential, its argument, a maximum and half a conversion to bf16 for each score) in 57 %, and the clock falls
+//     to 1.7 .. 2.0 GHz under that load.  Measured: 2048 tokens over 18001, 32 heads of 128 over 8: 536 us in a row of
+//     calls, 1063 TFLOP/s (557 to 650 us in the first dozen, while the clock settles), where a large library product of
+//     bf16 reaches 1130 to 1230.
 #include "sf_kv8.hpp"
 
 namespace sf {
@@ -323,15 +324,17 @@ struct RowState {
     output(x, p);
   }
 
-  // scores(x, next), weights(s, sc, p) and output(x, p) as one stream of instructions: products of the next scores
-  // between exponentials, and `rest(i, n)`, i = 0 .. n - 1, between products of the output.
+  // scores(x, next), weights(s, sc, p), sums(p, sc) and output(x, p) as one stream of instructions: products of the next
+  // scores between exponentials, and `rest(i, n)`, i = 0 .. n - 1, between products of the output.  The compiler may
+  // reorder four fragments' worth of it at a time (the whole of it: 760 us where this takes 536, single ones 555).  The
+  // products of the output, which have little beside them, go before what the other wave of the SIMD has.
   template <class Block, class Rest>
   __device__ __forceinline__ void turn(const Block& x, const f32x4_t (&s)[RT][4], f32x4_t (&next)[RT][4],
                                        const BlockScale& sc, const Rest& rest) {
     constexpr int F = DB * 8;  // fragments of keys, and of values
     float off[RT];
     uint32_t pw[RT][8];
-    constexpr int A = 2;  // fragments read ahead
+    constexpr int A = 4;  // fragments read ahead
     bf16x8_t f[A + 1];
     auto key = [&](int i) { return x.key(i / 2 % DB, i / (2 * DB), i % 2); };
 #pragma unroll
@@ -344,7 +347,7 @@ struct RowState {
     for (int i = 0; i < A; ++i) f[i] = key(i);
 #pragma unroll
     for (int i = 0; i < F; ++i) {
-      __builtin_amdgcn_sched_barrier(0);
+      if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);
       f[(i + A) % (A + 1)] = i + A < F ? key(i + A) : x.value((i + A - F) / 2, (i + A - F) % 2);
 #pragma unroll
       for (int r = 0; r < RT; ++r)
@@ -365,16 +368,18 @@ struct RowState {
 #pragma unroll
       for (int u = 0; u < 2; ++u)
         p[r][u] = __builtin_bit_cast(bf16x8_t, make_uint4(pw[r][4 * u], pw[r][4 * u + 1], pw[r][4 * u + 2], pw[r][4 * u + 3]));
+    __builtin_amdgcn_s_setprio(1);
     sums(p, sc);
 #pragma unroll
     for (int i = 0; i < F; ++i) {
-      __builtin_amdgcn_sched_barrier(0);
+      if (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);
       if (i + A < F) f[(F + i + A) % (A + 1)] = x.value((i + A) / 2, (i + A) % 2);
 #pragma unroll
       for (int r = 0; r < RT; ++r)
         o[r][i / 2] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f[(F + i) % (A + 1)], p[r][i % 2], o[r][i / 2], 0, 0, 0);
       rest(i, F);
     }
+    __builtin_amdgcn_s_setprio(0);
     __builtin_amdgcn_sched_barrier(0);
   }
 };
@@ -492,12 +497,16 @@ __global__ void __launch_bounds__(kAtnWaves * 64, attend_waves(DB, RT)) kv8_atte
 // Many rows: the waves of a workgroup share the blocks.  Each converts its part of a block into LDS once, in the
 // operands' order (a fragment of 16 bytes a lane, 1 KB, is written and read in a row, without bank conflicts), and
 // takes all of it for its own 16 RT rows.  In a turn, the scores of the next block are products on the matrix unit
-// while the probabilities of this one are exponentials on the vector unit; the block after, its codes loaded at the
+// while the probabilities of this one are exponentials on the vector unit; a block after, its codes loaded at the
 // turn's start, is converted at its end.  Keys are staged one block further than values.
 template <int DB, int RT, int WAVES>
 __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DB > 2 ? 1 : 2) kv8_chunk_kernel(AttendArgs a) {
   constexpr int ROWS = 16 * RT * WAVES, Dp = DB * 64, N = DB * 8 / WAVES;  // chunks of a lane: keys', then values'
-  __shared__ __align__(16) unsigned char lds[2][DB * 16][1024];           // fragments (hh, t, a) of keys, (dt, u) of values
+  // A barrier every other turn where there is room for it (4 % faster): a turn then stages what is read two turns later,
+  // into a slot whose block was read before the last barrier.
+  constexpr bool PAIR = WAVES == 8 && DB <= 2;
+  constexpr int AHEAD = PAIR ? 3 : 2, SLOTS = PAIR ? 4 : 2;
+  __shared__ __align__(16) unsigned char lds[SLOTS][DB * 16][1024];  // fragments (hh, t, a) of keys, (dt, u) of values
   int tile, split = blockIdx.y;
   int64_t bh;
   tile_of(a, bh, tile);
@@ -534,7 +543,7 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DB > 2 ? 1 : 2) kv8_
     };
     auto stage_half = [&](int j, int x, int kb, int vb) {
       const int c = j * WAVES + wave;
-      *reinterpret_cast<bf16x8_t*>(&lds[(c < DB * 4 ? kb : vb) & 1][2 * c + x][lane * 16]) =
+      *reinterpret_cast<bf16x8_t*>(&lds[(c < DB * 4 ? kb : vb) & (SLOTS - 1)][2 * c + x][lane * 16]) =
           codes_to_bf16(w[j].w[2 * x], w[j].w[2 * x + 1]);
     };
     auto stage = [&](int kb, int vb) {
@@ -547,7 +556,7 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DB > 2 ? 1 : 2) kv8_
       for (int j = 0; j < 2 * N; ++j) {
         const int c = j / 2 * WAVES + wave, x = j % 2;
         if ((c < DB * 4 ? kb : vb) != whole) continue;
-        *reinterpret_cast<bf16x8_t*>(&lds[whole & 1][2 * c + x][lane * 16]) =
+        *reinterpret_cast<bf16x8_t*>(&lds[whole & (SLOTS - 1)][2 * c + x][lane * 16]) =
             c < DB * 4 ? tail.key(c / 4, c % 4, x) : tail.value(c - DB * 4, x);
       }
     };
@@ -564,42 +573,48 @@ __global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DB > 2 ? 1 : 2) kv8_
     // blocks that some row of this wave sees
     const int from = a.window ? min(be, max(bs, (first_pos - a.window + 1) / kKvBlock)) : bs;
     const int to = max(from, min(be, last_pos / kKvBlock + 1));
-    load(bs, bs);
-    stage(bs, bs);
-    stage_tail(bs, bs);
+#pragma unroll 1
+    for (int i = 0; i < AHEAD - 1; ++i) {
+      load(bs + i, bs);
+      stage(bs + i, bs);
+      stage_tail(bs + i, bs);
+    }
     int blk = bs - 1;
+    auto meet = [&] {
+      if (!PAIR || ((blk ^ bs) & 1)) __syncthreads();
+    };
     // Turn blk: the block's own products after the next one's scores.
     auto turn_of_others = [&] {
-      __syncthreads();
-      load(blk + 2, blk + 1);
-      stage(blk + 2, blk + 1);
-      stage_tail(blk + 2, blk + 1);
+      meet();
+      load(blk + AHEAD, blk + AHEAD - 1);
+      stage(blk + AHEAD, blk + AHEAD - 1);
+      stage_tail(blk + AHEAD, blk + AHEAD - 1);
     };
     for (; blk < from - 1; ++blk) turn_of_others();
     f32x4_t s[RT][4];
     if (to > from) {
-      __syncthreads();
-      load(blk + 2, blk + 1);
-      frags.k = &lds[from & 1][0][lane * 16];
+      meet();
+      load(blk + AHEAD, blk + AHEAD - 1);
+      frags.k = &lds[from & (SLOTS - 1)][0][lane * 16];
       st.scores(frags, s);
-      stage(blk + 2, blk + 1);
-      stage_tail(blk + 2, blk + 1);
+      stage(blk + AHEAD, blk + AHEAD - 1);
+      stage_tail(blk + AHEAD, blk + AHEAD - 1);
       float k1 = ks[min(from, coded)], v1 = vs[min(from, coded)];  // the next block's scales
       for (++blk; blk < to; ++blk) {
-        __syncthreads();  // every wave is done with what this turn overwrites
-        load(blk + 2, blk + 1);
+        meet();  // every wave is done with what this turn overwrites
+        load(blk + AHEAD, blk + AHEAD - 1);
         const BlockScale sc(blk < ce ? k1 : 1.0f, blk < ce ? v1 : 1.0f, a.scale);
         k1 = ks[min(blk + 1, coded)], v1 = vs[min(blk + 1, coded)];
         st.settle(s, blk, sc, a.window,
                   blk * kKvBlock + kKvBlock - 1 > first_pos || (a.window && blk * kKvBlock <= last_pos - a.window));
-        frags.k = &lds[(blk + 1) & 1][0][lane * 16];
-        frags.v = &lds[blk & 1][0][lane * 16];
+        frags.k = &lds[(blk + 1) & (SLOTS - 1)][0][lane * 16];
+        frags.v = &lds[blk & (SLOTS - 1)][0][lane * 16];
         f32x4_t next[RT][4];  // past the last block: of what lies there, unused
         st.turn(frags, s, next, sc, [&](int i, int n) {
 #pragma unroll
-          for (int j = i * 2 * N / n; j < (i + 1) * 2 * N / n; ++j) stage_half(j / 2, j % 2, blk + 2, blk + 1);
+          for (int j = i * 2 * N / n; j < (i + 1) * 2 * N / n; ++j) stage_half(j / 2, j % 2, blk + AHEAD, blk + AHEAD - 1);
         });
-        stage_tail(blk + 2, blk + 1);
+        stage_tail(blk + AHEAD, blk + AHEAD - 1);
 #pragma unroll
         for (int r = 0; r < RT; ++r)
 #pragma unroll

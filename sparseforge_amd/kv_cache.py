@@ -61,6 +61,7 @@ class KVCache8:
         self.bound = 0
         self._new = 0  # tokens of the step under way
         self._descs = [self._desc(i, blocks) for i in range(layers)]
+        self._refs = [ctypes.byref(d) for d in self._descs]
 
     def _desc(self, i: int, blocks: int) -> L.Kv8Cache:
         d = L.Kv8Cache()
@@ -88,24 +89,26 @@ class KVCache8:
                 raise ValueError("KVCache8.extend: counts are on another device")
             if counts.dtype != torch.int32 or counts.shape != (self.batch,):
                 raise ValueError(f"KVCache8.extend: counts must be int32 [{self.batch}]")
-        L.check(L.lib().sf_kv8_extend(ctypes.byref(self._descs[0]), n, L.ptr(counts), L.stream(self.ends.device)),
-                "sf_kv8_extend")
+        dev = self.ends.device
+        with _prof.region("sf_kv8_extend", 12 * self.batch, "B", dev):
+            L.check(L.lib().sf_kv8_extend(self._refs[0], n, L.ptr(counts), L.stream(dev)), "sf_kv8_extend")
         self.bound += n
         self._new = n
 
     def _rows(self, t: torch.Tensor, name: str, heads: int | None) -> torch.Tensor:
         """t as the kernels read it: contiguous heads, rows at 16-byte aligned addresses."""
-        if t.device != self.ends.device:
+        if t.get_device() != self.ends.get_device():
             L.require_device_only(t)
             raise ValueError(f"KVCache8: {name} is on {t.device}, the cache on {self.ends.device}")
         if t.dtype != torch.bfloat16:
             raise TypeError(f"KVCache8: {name} is {t.dtype} (bfloat16 only)")
-        if t.dim() != 4 or t.shape[0] != self.batch or t.shape[3] != self.head_dim or \
-                (t.shape[2] != heads if heads else t.shape[2] % self.kv_heads or t.shape[2] == 0):
-            raise ValueError(f"KVCache8: {name} {tuple(t.shape)} does not go with {self.batch} sequences, "
+        shape = t.shape
+        if len(shape) != 4 or shape[0] != self.batch or shape[3] != self.head_dim or \
+                (shape[2] != heads if heads else shape[2] % self.kv_heads or shape[2] == 0):
+            raise ValueError(f"KVCache8: {name} {tuple(shape)} does not go with {self.batch} sequences, "
                              f"{self.kv_heads} heads of {self.head_dim}")
-        if t.shape[1] != self._new:
-            raise ValueError(f"KVCache8: {name} holds {t.shape[1]} tokens a sequence, the step has {self._new}")
+        if shape[1] != self._new:
+            raise ValueError(f"KVCache8: {name} holds {shape[1]} tokens a sequence, the step has {self._new}")
         sb, ss, sh, sd = t.stride()
         if sd != 1 or (sb | ss | sh) % 8 or t.data_ptr() % 16:
             t = t.clone(memory_format=torch.contiguous_format)
@@ -116,9 +119,8 @@ class KVCache8:
         k, v = self._rows(k, "k", self.kv_heads), self._rows(v, "v", self.kv_heads)
         dev = self.ends.device
         with _prof.region("sf_kv8_append", 3 * k.numel() * k.element_size(), "B", dev):
-            L.check(L.lib().sf_kv8_append(ctypes.byref(self._descs[layer]), k.data_ptr(), k.stride(0), k.stride(1),
-                                          k.stride(2), v.data_ptr(), v.stride(0), v.stride(1), v.stride(2), k.shape[1],
-                                          L.stream(dev)), "sf_kv8_append")
+            L.check(L.lib().sf_kv8_append(self._refs[layer], k.data_ptr(), *k.stride()[:3], v.data_ptr(),
+                                          *v.stride()[:3], self._new, L.stream(dev)), "sf_kv8_append")
 
     def attend(self, q: torch.Tensor, scale: float | None = None, window: int = 0, layer: int = 0) -> torch.Tensor:
         """Attention of the step's queries q [B, n, H, D] over the keys up to their own (the last `window` of them if
@@ -133,9 +135,8 @@ class KVCache8:
         size = lib.sf_kv8_attend_workspace_size(B, self.kv_heads, H, D, n, self.bound)
         ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
         with _prof.region("sf_kv8_attend", 4 * self.bound * n * B * H * D, "FLOP", dev):
-            L.check(lib.sf_kv8_attend(ctypes.byref(self._descs[layer]), q.data_ptr(), q.stride(0), q.stride(1),
-                                      q.stride(2), n, H, float(scale), int(window), self.bound, out.data_ptr(),
-                                      L.ptr(ws), size, L.stream(dev)), "sf_kv8_attend")
+            L.check(lib.sf_kv8_attend(self._refs[layer], q.data_ptr(), *q.stride()[:3], n, H, scale, window, self.bound,
+                                      out.data_ptr(), L.ptr(ws), size, L.stream(dev)), "sf_kv8_attend")
         return out
 
     def values(self, first: int | torch.Tensor = 0, tokens: int | None = None, layer: int = 0):
@@ -155,6 +156,6 @@ class KVCache8:
         k = torch.empty(shape, dtype=torch.float32, device=dev)
         v = torch.empty(shape, dtype=torch.float32, device=dev)
         with _prof.region("sf_kv8_values", 10 * k.numel(), "B", dev):
-            L.check(L.lib().sf_kv8_values(ctypes.byref(self._descs[layer]), L.ptr(at), first, tokens, k.data_ptr(),
+            L.check(L.lib().sf_kv8_values(self._refs[layer], L.ptr(at), first, tokens, k.data_ptr(),
                                           v.data_ptr(), L.stream(dev)), "sf_kv8_values")
         return k, v
