@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(kAtnWaves * 64, attend_waves(DB, RT)) kv8_atte
 // while the probabilities of this one are exponentials on the vector unit; a block after, its codes loaded at the
 // turn's start, is converted at its end.  Keys are staged one block further than values.
 template <int DB, int RT, int WAVES>
-__global__ void __launch_bounds__(WAVES * 64, WAVES == 4 && DB > 2 ? 1 : 2) kv8_chunk_kernel(AttendArgs a) {
+__global__ void __launch_bounds__(WAVES * 64, 2) kv8_chunk_kernel(AttendArgs a) {
   constexpr int ROWS = 16 * RT * WAVES, Dp = DB * 64, N = DB * 8 / WAVES;  // chunks of a lane: keys', then values'
   // A barrier every other turn where there is room for it (4 % faster): a turn then stages what is read two turns later,
   // into a slot whose block was read before the last barrier.
@@ -722,7 +722,10 @@ AttendPlan attend_plan(int64_t B, int64_t H, int64_t heads, int64_t Dp, int64_t 
   // Sharing pays from 33 rows on: 8 sequences of 16000, 8 heads of 128, 24 rows 59 us against 74 shared, 48 rows 98
   // against 91.
   p.rt = rows <= 16 || Dp > 128 ? 1 : 2;
-  p.waves = rows <= 16 * p.rt ? 0 : B * H * ceil_div(rows, 128 * p.rt) >= 256 ? 8 : 4;
+  // Eight waves convert a block once where four and four convert it twice; up to 128 rows half of them would have none
+  // of their own, and with heads above 128 four leave a SIMD one wave: 8 sequences of 4000, 2048 rows of 128 a head, 267
+  // us against 293; 2 of 8000, 150 rows, 52 against 56 and 60 rows, 37 against 34; 60 rows of 256, 31 against 35.
+  p.waves = rows <= 16 * p.rt ? 0 : rows <= 128 && Dp <= 128 ? 4 : 8;
   p.rows = 16 * p.rt * (p.waves ? p.waves : 1);
   p.tiles = ceil_div(rows, p.rows);
   const int64_t wgs = B * H * p.tiles;
@@ -745,16 +748,17 @@ template <int DB>
 void launch_attend(const AttendArgs& a, const AttendPlan& p, hipStream_t st) {
   constexpr int RT = DB <= 2 ? 2 : 1;  // of the shared form: what the registers hold twice a SIMD
   const dim3 grid(static_cast<unsigned>((int64_t)a.c.B * a.c.H * a.tiles), a.splits);
-  if (p.waves == 8)
+  if (p.waves == 8) {
     kv8_chunk_kernel<DB, RT, 8><<<grid, 512, 0, st>>>(a);
-  else if (p.waves == 4)
-    kv8_chunk_kernel<DB, RT, 4><<<grid, 256, 0, st>>>(a);
-  else if (p.rt == RT)
+  } else if (p.waves == 4) {
+    if constexpr (DB <= 2) kv8_chunk_kernel<DB, RT, 4><<<grid, 256, 0, st>>>(a);  // the plan's only such heads
+  } else if (p.rt == RT) {
     kv8_attend_kernel<DB, RT><<<grid, kAtnWaves * 64, 0, st>>>(a);
-  else
+  } else {
     kv8_attend_kernel<DB, 1><<<grid, kAtnWaves * 64, 0, st>>>(a);
+  }
   if (a.splits > 1) {
-    constexpr int G = DB == 3 ? 4 : 16 / DB;
+    constexpr int G = DB == 3 ? 4 : 16 / DB;  // groups of a workgroup: as many on a row as it has splits, else more rows
     int teams = 1;
     while (teams < G && teams < a.splits) teams *= 2;
     const int64_t rows = (int64_t)a.c.B * a.n * a.heads;
