@@ -166,6 +166,13 @@ CASES = [
 ]
 
 
+# every form of heads and rows: one row a head, 16, 17, 32, 33, 128, 129 and many, with keys in one piece and in several
+CASES += [(2, n, 2, 1, D, held, 0) for D in (64, 128, 136, 192, 248) for n, held in
+          ((1, (200, 3000)), (8, (2000, 5)), (9, (700, 64)), (16, (1300, 63)), (17, (2500, 1)), (64, (0, 900)),
+           (65, (400, 4000)), (150, (1, 1100)))]
+CASES += [(1, 100, 6, 2, D, (900,), 150) for D in (136, 256)]
+
+
 @pytest.mark.parametrize("B,n,H,Hk,D,held,window", CASES)
 def test_attend(cuda_device, B, n, H, Hk, D, held, window):
     from sparseforge_amd.kv_cache import KVCache8
