@@ -20,9 +20,9 @@
 //     heads over 8: 84 us + 5 us for the join, 6.0 TB/s; one of 33 tokens, 32 heads of 64: 5.1 us.
 //   more: kv8_chunk_kernel.  Bound by power: the matrix unit is busy in 52 % of its cycles and the vector unit beside it
 //     (an exponential, its argument, a maximum and half a conversion to bf16 for each score) in 57 %, and the clock falls
-//     to 1.7 .. 2.0 GHz under that load.  Measured: 2048 tokens over 18001, 32 heads of 128 over 8: 536 us in a row of
-//     calls, 1063 TFLOP/s (557 to 650 us in the first dozen, while the clock settles), where a large library product of
-//     bf16 reaches 1130 to 1230.
+//     to 1.7 .. 2.0 GHz under that load.  Measured: 2048 tokens over 18001, 32 heads of 128 over 8: 496 to 536 us from
+//     one card to another in a row of calls, 1063 to 1149 TFLOP/s (557 to 650 us in the first dozen, while the clock
+//     settles), where a large library product of bf16 reaches 1130 to 1230.
 #include "sf_kv8.hpp"
 
 namespace sf {
