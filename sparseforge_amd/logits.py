@@ -8,7 +8,7 @@ For token t of a row, in float32 and in this order, rounded once to the logits' 
     x = x + bias[t]
     x = -inf if t is not allowed
 
-A row whose mask allows nothing is -inf throughout.
+A row whose mask allows nothing is -inf throughout.  Forward only: the result takes no gradient.
 """
 from __future__ import annotations
 
