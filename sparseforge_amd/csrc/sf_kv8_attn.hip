@@ -6,7 +6,7 @@
 // query r / group of head r % group.  A wave takes 16 RT rows over whole blocks of 64 keys, one pass with a running
 // maximum and sum.  Both products are v_mfma_f32_16x16x32_bf16 on codes converted to bf16, which is exact (8 significant
 // bits), with f32 scores, sums and outputs.  The key scale multiplies the scores with the softmax's factor; the value
-// scale enters the exponent (BlockScale).  The probabilities round to bf16 as operands of the second product, which
+// scale enters the exponent, relative to a scale that the wave's output is held in (RowState::refer).  The probabilities round to bf16 as operands of the second product, which
 // moves an output by 2^-8 of its terms at most, as much as storing it in bf16 does; the sums are of the rounded ones.
 //
 // A row's running maximum is raised only when a score passes it by 8 (in log2): probabilities up to 2^8 cost nothing in
@@ -44,7 +44,7 @@ struct AttendArgs {
   float scale;        // times log2 e
   int rows, tiles;    // rows of a workgroup, and how many times that a (sequence, head) has
   int splits, chunk;  // key blocks of a workgroup: at least `chunk`
-  float* po;          // [B H tiles][splits][rows][Dp] unnormalised outputs
+  float* po;          // [B H tiles][splits][rows][Dp] outputs over a split's keys alone
   float* pml;         // [B H tiles][splits][2][rows] maxima, sums
 };
 
@@ -152,22 +152,19 @@ struct TailBlock {
   }
 };
 
-// What a block's scales do to its scores and probabilities.  The value scale goes into the exponent, which costs
-// nothing for each key, and the sum of a row takes it out again.  Where it is far from 1 and the smaller of those
-// probabilities leave the range of floats, the sum is taken without it.  A scale of 0 has codes of 0, for which any
-// other does as well.
+// What a block's scales do to its scores and probabilities.  The value scale, over the power of two that the wave holds
+// its output in (RowState::refer), goes into the exponent, which costs nothing for each key, and the sum of a row takes
+// it out again.  A scale of 0 has codes of 0, for which any other does as well.
 struct BlockScale {
   float ks;      // of the scores, with log2 e; positive
-  float lv, rv;  // log2 of the value scale, and its reciprocal
-  bool far;
+  float v;       // of the values, 0 where any does
+  float lv, rv;  // log2 of the value scale over the wave's power of two, and its reciprocal
+  bool far;      // much smaller than that: the sum is taken apart
   bool nan;      // a block of NaN: its scores become NaN
-  __device__ __forceinline__ BlockScale(float k, float v, float scale) {
+  __device__ __forceinline__ BlockScale(float k, float v, float scale)
+      : v(v > 0.0f ? v : 0.0f), lv(0.0f), rv(1.0f), far(false) {
     nan = k != k;  // both are
     ks = k > 0.0f ? k * scale : 1.0f;
-    v = v > 0.0f ? v : 1.0f;
-    far = v < 0x1p-64f || v > 0x1p64f;
-    lv = far ? log2f(v) : __builtin_amdgcn_logf(v);
-    rv = far ? 0.0f : __builtin_amdgcn_rcpf(v);
   }
 };
 
@@ -178,6 +175,9 @@ struct RowState {
   f32x4_t o[RT][DB * 4];
   float m[RT], l[RT];
   int pos[RT];  // position of the row's query, -1: no such row
+  // o is in terms of 2^(unit - 127) and stays inside the range of floats whatever the values are, the largest numbers of
+  // bf16 among them; 0: of nothing yet.  top: the largest that unit has been.
+  int unit, top;
 
   // The queries of rows row0 + 16 r + lane % 16 of key-value head h; rows past the tile's queries are zeros.
   __device__ __forceinline__ void start(const AttendArgs& a, const TileRange& tr, int b, int h, int row0) {
@@ -201,6 +201,31 @@ struct RowState {
       m[r] = kAtnLow;
       l[r] = 0.0f;
     }
+    unit = top = 0;
+  }
+
+  __device__ __forceinline__ static float pow2(int biased) { return __uint_as_float((uint32_t)max(biased, 0) << 23); }
+
+  // Takes the unit from the block's value scale, 1/8 to 2 of it (every fourth power of two: neighbouring blocks share one),
+  // so that what a block adds does not depend on other blocks and a change of unit is exact.  It does not fall below 2^-64
+  // of the largest; block scales far below add to the sum, and to the output what they still can.
+  __device__ __forceinline__ void refer(BlockScale& sc) {
+    if (!(sc.v > 0.0f)) return;
+    const int want = max(((int)(__float_as_uint(sc.v) >> 23) + 3) & ~3, 8);
+    if (want != unit) {
+      top = max(top, want);
+      const int to = max(want, top - 64);
+      const float f = pow2(127 + min(unit - to, 64));
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int dt = 0; dt < DB * 4; ++dt) o[r][dt] *= f;
+      unit = to;
+    }
+    sc.far = want != unit;
+    const float x = sc.v * pow2(254 - unit);
+    sc.lv = sc.far ? log2f(x) : __builtin_amdgcn_logf(x);
+    sc.rv = sc.far ? 0.0f : __builtin_amdgcn_rcpf(x);
   }
 
   // Scores of a block that some row does not see whole, or that is NaN.
@@ -234,8 +259,9 @@ struct RowState {
   }
 
   // What is rare before a block's probabilities: rows that do not see it whole, a maximum that has to rise, a value
-  // scale far from 1.
-  __device__ __forceinline__ void settle(f32x4_t (&s)[RT][4], int blk, const BlockScale& sc, int window, bool masked) {
+  // scale far from the wave's.
+  __device__ __forceinline__ void settle(f32x4_t (&s)[RT][4], int blk, BlockScale& sc, int window, bool masked) {
+    refer(sc);
     if (masked || sc.nan) {
 #pragma unroll
       for (int r = 0; r < RT; ++r) hide(r, s[r], blk, sc.nan, window);
@@ -263,15 +289,19 @@ struct RowState {
       }
     }
     if (sc.far) {
+      f32x4_t e[4];
 #pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        float sum = 0.0f;
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sum += __builtin_amdgcn_exp2f(fmaf(s[r][i / 4][i % 4], sc.ks, -m[r]));
-        sum += __shfl_xor(sum, 16, 64);
-        l[r] += sum + __shfl_xor(sum, 32, 64);
-      }
+      for (int r = 0; r < RT; ++r) l[r] += sum(s[r], sc, -m[r], e);
     }
+  }
+
+  // The exponentials of a row's scores, and their sum.
+  __device__ __forceinline__ static float sum(const f32x4_t (&s)[4], const BlockScale& sc, float off, f32x4_t (&e)[4]) {
+    float x = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) x += e[i / 4][i % 4] = __builtin_amdgcn_exp2f(fmaf(s[i / 4][i % 4], sc.ks, off));
+    x += __shfl_xor(x, 16, 64);
+    return x + __shfl_xor(x, 32, 64);
   }
 
   // Probabilities times the value scale, as operands of the second product.
@@ -313,14 +343,37 @@ struct RowState {
       }
   }
 
+  // The output over the wave's keys: o over its sum, in terms of 1.  Rows that have met no key are 0.
+  __device__ __forceinline__ void finish() {
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const float f = l[r] == 0.0f ? 0.0f : 1.0f / l[r];
+#pragma unroll
+      for (int dt = 0; dt < DB * 4; ++dt) o[r][dt] = o[r][dt] * f * pow2(unit);
+    }
+  }
+
+  // The incomplete block, which comes last, and finish(): its values, any bf16 numbers, are products with weights that
+  // are final, at most 1.  s: its scores.
   template <class Block>
-  __device__ __forceinline__ void block(const Block& x, int blk, const BlockScale& sc, int window, bool masked) {
-    f32x4_t s[RT][4];
+  __device__ __forceinline__ void last(const Block& x, f32x4_t (&s)[RT][4], int blk, float scale, int window) {
+    BlockScale sc(1.0f, 0.0f, scale);
+    settle(s, blk, sc, window, true);
+#pragma unroll
+    for (int r = 0; r < RT; ++r) l[r] += sum(s[r], sc, -m[r], s[r]);
+    finish();
     bf16x8_t p[RT][2];
-    scores(x, s);
-    settle(s, blk, sc, window, masked);
-    weights(s, sc, p);
-    sums(p, sc);
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const float f = l[r] == 0.0f ? 0.0f : 1.0f / l[r];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        uint32_t w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = pack2(f * s[r][2 * u + i / 2][i % 2 * 2], f * s[r][2 * u + i / 2][i % 2 * 2 + 1]);
+        p[r][u] = __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
+      }
+    }
     output(x, p);
   }
 
@@ -430,7 +483,7 @@ __global__ void __launch_bounds__(kAtnWaves * 64, attend_waves(DB, RT)) kv8_atte
       f32x4_t s[RT][4];
       bf16x8_t p[RT][2];
       st.scores(x, s);
-      const BlockScale sc(k1, v1, a.scale);
+      BlockScale sc(k1, v1, a.scale);
       if (next < ce) {
         x.load(x.k, kc + next * kKvBlock * Dp);
         k1 = ks[next], v1 = vs[next];
@@ -443,7 +496,11 @@ __global__ void __launch_bounds__(kAtnWaves * 64, attend_waves(DB, RT)) kv8_atte
     }
     if (blk < be) {  // the incomplete block
       const TailBlock<DB> tail{a.c.kt + bh * kKvBlock * Dp, a.c.vt + bh * kKvBlock * Dp, tr.end - blk * kKvBlock};
-      st.block(tail, blk, BlockScale(1.0f, 1.0f, a.scale), a.window, true);
+      f32x4_t s[RT][4];
+      st.scores(tail, s);
+      st.last(tail, s, blk, a.scale, a.window);
+    } else {
+      st.finish();
     }
   }
   // join the waves
@@ -462,18 +519,22 @@ __global__ void __launch_bounds__(kAtnWaves * 64, attend_waves(DB, RT)) kv8_atte
   __syncthreads();
   for (int at = threadIdx.x; at < ROWS * (Dp / 4); at += kAtnWaves * 64) {
     const int row = at / (Dp / 4), d = (at - row * (Dp / 4)) * 4;
-    float m = kAtnLow, l = 0.0f, o[4] = {0, 0, 0, 0};
+    float m = kAtnLow, l = 0.0f, o[4] = {0, 0, 0, 0}, c[kAtnWaves];
 #pragma unroll
     for (int w = 0; w < kAtnWaves; ++w) m = fmaxf(m, sml[0][w][row]);
 #pragma unroll
     for (int w = 0; w < kAtnWaves; ++w) {
-      const float f = __builtin_amdgcn_exp2f(sml[0][w][row] - m);
+      c[w] = __builtin_amdgcn_exp2f(sml[0][w][row] - m) * sml[1][w][row];
+      l += c[w];
+    }
+    const float f = l == 0.0f ? 0.0f : 1.0f / l;
+#pragma unroll
+    for (int w = 0; w < kAtnWaves; ++w) {
       const float4 x = *reinterpret_cast<const float4*>(&so[w][row][d]);
-      l += f * sml[1][w][row];
-      o[0] += f * x.x;
-      o[1] += f * x.y;
-      o[2] += f * x.z;
-      o[3] += f * x.w;
+      o[0] += c[w] * f * x.x;
+      o[1] += c[w] * f * x.y;
+      o[2] += c[w] * f * x.z;
+      o[3] += c[w] * f * x.w;
     }
     if (a.splits > 1) {
       const int64_t part = (int64_t)blockIdx.x * a.splits + split;
@@ -485,9 +546,9 @@ __global__ void __launch_bounds__(kAtnWaves * 64, attend_waves(DB, RT)) kv8_atte
     } else {
       const int gr = tile * ROWS + row, i = gr / a.group, hq = h * a.group + gr % a.group;
       if (i < a.n && d < a.c.D) {
-        const float f = i < tr.i1 ? 1.0f / l : 0.0f;  // a sum of 0 where every score is -inf: NaN, as 0 / 0
+        const float none = l == 0.0f ? __builtin_nanf("") : 0.0f;  // every score is -inf: NaN, as 0 / 0
         uint2 w = make_uint2(0, 0);
-        if (i < tr.i1) w = make_uint2(pack2(o[0] * f, o[1] * f), pack2(o[2] * f, o[3] * f));
+        if (i < tr.i1) w = make_uint2(pack2(o[0] + none, o[1] + none), pack2(o[2] + none, o[3] + none));
         *reinterpret_cast<uint2*>(a.out + (((int64_t)b * a.n + i) * a.heads + hq) * a.c.D + d) = w;
       }
     }
@@ -600,10 +661,10 @@ __global__ void __launch_bounds__(WAVES * 64, 2) kv8_chunk_kernel(AttendArgs a) 
       stage(blk + AHEAD, blk + AHEAD - 1);
       stage_tail(blk + AHEAD, blk + AHEAD - 1);
       float k1 = ks[min(from, coded)], v1 = vs[min(from, coded)];  // the next block's scales
-      for (++blk; blk < to; ++blk) {
+      for (++blk; blk < min(to, whole); ++blk) {
         meet();  // every wave is done with what this turn overwrites
         load(blk + AHEAD, blk + AHEAD - 1);
-        const BlockScale sc(blk < ce ? k1 : 1.0f, blk < ce ? v1 : 1.0f, a.scale);
+        BlockScale sc(k1, v1, a.scale);
         k1 = ks[min(blk + 1, coded)], v1 = vs[min(blk + 1, coded)];
         st.settle(s, blk, sc, a.window,
                   blk * kKvBlock + kKvBlock - 1 > first_pos || (a.window && blk * kKvBlock <= last_pos - a.window));
@@ -619,6 +680,14 @@ __global__ void __launch_bounds__(WAVES * 64, 2) kv8_chunk_kernel(AttendArgs a) 
         for (int r = 0; r < RT; ++r)
 #pragma unroll
           for (int t = 0; t < 4; ++t) s[r][t] = next[r][t];
+      }
+      if (blk < to) {  // the incomplete block, the last of all: nothing is staged after it
+        meet();
+        frags.v = &lds[blk & (SLOTS - 1)][0][lane * 16];
+        st.last(frags, s, blk, a.scale, a.window);
+        ++blk;
+      } else {
+        st.finish();
       }
     }
     for (; blk < be; ++blk) turn_of_others();
@@ -639,14 +708,14 @@ __global__ void __launch_bounds__(WAVES * 64, 2) kv8_chunk_kernel(AttendArgs a) 
       }
     } else if (i < a.n) {
       uint16_t* dst = a.out + (((int64_t)b * a.n + i) * a.heads + hq) * a.c.D;
-      const float f = 1.0f / st.l[r];
+      const float none = st.l[r] == 0.0f ? __builtin_nanf("") : 0.0f;  // every score is -inf: NaN, as 0 / 0
 #pragma unroll
       for (int dt = 0; dt < DB * 4; ++dt) {
         const int d = dt * 16 + 4 * g;
         if (d < a.c.D)
           *reinterpret_cast<uint2*>(dst + d) =
-              i < tr.i1 ? make_uint2(pack2(st.o[r][dt][0] * f, st.o[r][dt][1] * f),
-                                     pack2(st.o[r][dt][2] * f, st.o[r][dt][3] * f))
+              i < tr.i1 ? make_uint2(pack2(st.o[r][dt][0] + none, st.o[r][dt][1] + none),
+                                     pack2(st.o[r][dt][2] + none, st.o[r][dt][3] + none))
                         : make_uint2(0, 0);
       }
     }
@@ -675,13 +744,14 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(AttendArgs a, int teams) 
     for (int s = team; s < used; s += teams) {
       const float ms = a.pml[(part0 + s) * 2 * a.rows + row], ls = a.pml[((part0 + s) * 2 + 1) * a.rows + row];
       const float4 x = *reinterpret_cast<const float4*>(a.po + ((part0 + s) * a.rows + row) * Dp + d);
-      const float mn = fmaxf(m, ms), f = __builtin_amdgcn_exp2f(m - mn), fs = __builtin_amdgcn_exp2f(ms - mn);
+      const float mn = fmaxf(m, ms), c0 = __builtin_amdgcn_exp2f(m - mn) * l, c1 = __builtin_amdgcn_exp2f(ms - mn) * ls;
       m = mn;
-      l = l * f + ls * fs;
-      o[0] = o[0] * f + x.x * fs;
-      o[1] = o[1] * f + x.y * fs;
-      o[2] = o[2] * f + x.z * fs;
-      o[3] = o[3] * f + x.w * fs;
+      l = c0 + c1;
+      const float f = l == 0.0f ? 0.0f : __builtin_amdgcn_rcpf(l), f0 = c0 * f, f1 = c1 * f;
+      o[0] = o[0] * f0 + x.x * f1;
+      o[1] = o[1] * f0 + x.y * f1;
+      o[2] = o[2] * f0 + x.z * f1;
+      o[3] = o[3] * f0 + x.w * f1;
     }
     *reinterpret_cast<float4*>(&so[grp][d]) = make_float4(o[0], o[1], o[2], o[3]);
     if (d == 0) {
@@ -694,18 +764,18 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(AttendArgs a, int teams) 
   m = kAtnLow;
   l = o[0] = o[1] = o[2] = o[3] = 0.0f;
   for (int k = first; k < first + teams; ++k) m = fmaxf(m, sml[0][k]);
+  for (int k = first; k < first + teams; ++k) l += __builtin_amdgcn_exp2f(sml[0][k] - m) * sml[1][k];
+  const float f = 1.0f / l;  // a sum of 0: every score is -inf, and the row NaN, as 0 / 0
   for (int k = first; k < first + teams; ++k) {
-    const float f = __builtin_amdgcn_exp2f(sml[0][k] - m);
+    const float c = __builtin_amdgcn_exp2f(sml[0][k] - m) * sml[1][k] * f;
     const float4 x = *reinterpret_cast<const float4*>(&so[k][d]);
-    l += f * sml[1][k];
-    o[0] += f * x.x;
-    o[1] += f * x.y;
-    o[2] += f * x.z;
-    o[3] += f * x.w;
+    o[0] += c * x.x;
+    o[1] += c * x.y;
+    o[2] += c * x.z;
+    o[3] += c * x.w;
   }
-  const float f = i < tr.i1 ? 1.0f / l : 0.0f;
   *reinterpret_cast<uint2*>(a.out + (bi * a.heads + hq) * a.c.D + d) =
-      make_uint2(pack2(o[0] * f, o[1] * f), pack2(o[2] * f, o[3] * f));
+      i < tr.i1 ? make_uint2(pack2(o[0], o[1]), pack2(o[2], o[3])) : make_uint2(0, 0);
 }
 
 // How a call is cut: waves of a workgroup that share blocks (0: each takes its own), 16-row pieces of a wave, rows of a

@@ -1,0 +1,57 @@
+"""Attention over the 8-bit cache at the ends of the numbers' range: values as large as bf16 holds, value scales of
+neighbouring blocks far apart.  Oracle and bar are test_gpu_kv_cache.py's."""
+import pytest
+import torch
+from test_gpu_kv_cache import BLOCK, _attention, _data, _stored
+
+pytestmark = pytest.mark.gpu
+
+
+def _outputs(q, k, v, D):
+    """Attention of the last q.shape[1] tokens of k, v over all of them: (out, o, bar) [n, H, D]."""
+    from sparseforge_amd.kv_cache import KVCache8
+
+    n, H, T = q.shape[1], q.shape[2], k.shape[1]
+    cache = KVCache8(1, k.shape[2], D, T)
+    if T > n:
+        cache.extend(T - n)
+        cache.append(k[:, :T - n], v[:, :T - n])
+    cache.extend(n)
+    cache.append(k[:, T - n:], v[:, T - n:])
+    out = cache.attend(q).view(n, H, D).double()
+    return out, *_attention(q[0], _stored(k[0], T), _stored(v[0], T), T - n, D ** -0.5, 0)
+
+
+# few rows and many, one piece of the keys and several, ending on a block's edge and inside a block
+FORMS = [(1, 1, 64, 6 * BLOCK), (1, 4, 128, 6 * BLOCK + 20), (1, 1, 128, 5000), (24, 1, 128, 700), (40, 4, 64, 500),
+         (40, 4, 128, 6 * BLOCK), (150, 1, 128, 5000), (9, 2, 200, 2100), (200, 2, 256, 1000)]
+
+
+@pytest.mark.parametrize("n,group,D,T", FORMS)
+def test_largest_values(cuda_device, n, group, D, T):
+    """Values between half of and the largest that bf16 has: a sum of few of them passes the floats, their mean does not."""
+    g = torch.Generator(device=cuda_device).manual_seed(n + T)
+    Hk = 2
+    k, v = _data(g, 1, T, Hk, D, cuda_device)
+    v = ((1.0 + 0.98 * torch.rand(v.shape, generator=g, device=cuda_device)) * 2.0 ** 127).bfloat16()
+    v[:, :, 1] *= -1.0
+    q = torch.randn(1, n, group * Hk, D, generator=g, device=cuda_device).bfloat16()
+    for size in (1.0, 0.0):  # and all weights equal
+        out, o, bar = _outputs(q * size, k, v, D)
+        assert bool(((out - o).abs() <= bar).all()), float(((out - o).abs() / bar).max())
+
+
+@pytest.mark.parametrize("n,group,D,T", FORMS)
+def test_large_values_without_weight(cuda_device, n, group, D, T):
+    """A block in the middle whose values are 2^80 times the others' and whose keys score too low to have any weight."""
+    g = torch.Generator(device=cuda_device).manual_seed(n * T)
+    Hk = 2
+    k, v = _data(g, 1, T, Hk, D, cuda_device)
+    q = torch.randn(1, n, group * Hk, D, generator=g, device=cuda_device).bfloat16()
+    q[..., 0] = 64.0
+    k[..., 0] = 1.0
+    k[:, 2 * BLOCK:3 * BLOCK, :, 0] = -64.0
+    v[:, 2 * BLOCK:3 * BLOCK] = (v[:, 2 * BLOCK:3 * BLOCK].float() * 2.0 ** 80).bfloat16()
+    out, o, bar = _outputs(q, k, v, D)
+    assert float(o.abs().max()) < 100.0
+    assert bool(((out - o).abs() <= bar).all()), float(((out - o).abs() / bar).max())
