@@ -6,8 +6,13 @@
 // query r / group of head r % group.  A wave takes 16 RT rows over whole blocks of 64 keys, one pass with a running
 // maximum and sum.  Both products are v_mfma_f32_16x16x32_bf16 on codes converted to bf16, which is exact (8 significant
 // bits), with f32 scores, sums and outputs.  The key scale multiplies the scores with the softmax's factor; the value
-// scale enters the exponent, relative to a scale that the wave's output is held in (RowState::refer).  The probabilities round to bf16 as operands of the second product, which
-// moves an output by 2^-8 of its terms at most, as much as storing it in bf16 does; the sums are of the rounded ones.
+// scale enters the exponent, over the power of two that the wave holds its output in (RowState::refer).
+//
+// The probabilities round to bf16 as operands of the second product, which moves an output by 2^-8 of its terms at most,
+// as much as storing it in bf16 does; the sums are of the rounded ones.  f16 would hold three bits more at the same rate,
+// but nothing below 2^-39 of the largest (2^-25 whole): an output that only small weights make, because the largest has a
+// code of 0 there, would come out wrong by more than its rounding.  Two parts in bf16 take the single-token form 10 to
+// 25 % longer.
 //
 // A row's running maximum is raised only when a score passes it by 8 (in log2): probabilities up to 2^8 cost nothing in
 // f32 or bf16, and most blocks need no exchange between lanes.
@@ -47,6 +52,14 @@ struct AttendArgs {
   float* po;          // [B H tiles][splits][rows][Dp] outputs over a split's keys alone
   float* pml;         // [B H tiles][splits][2][rows] maxima, sums
 };
+
+// A scale, in a vector register until it is used: as a scalar, which the compiler makes of what all lanes load alike, it
+// would be waited for where it is loaded, a block early (10 % of a chunk with heads of 64).
+__device__ __forceinline__ float ld_scale(const float* p) {
+  int same = 0;
+  asm("" : "+v"(same));
+  return p[same];
+}
 
 // What a tile of rows sees.
 struct TileRange {
@@ -206,12 +219,13 @@ struct RowState {
 
   __device__ __forceinline__ static float pow2(int biased) { return __uint_as_float((uint32_t)max(biased, 0) << 23); }
 
-  // Takes the unit from the block's value scale, 1/8 to 2 of it (every fourth power of two: neighbouring blocks share one),
-  // so that what a block adds does not depend on other blocks and a change of unit is exact.  It does not fall below 2^-64
-  // of the largest; block scales far below add to the sum, and to the output what they still can.
+  // Takes the unit from the block's value scale: 2^-31 to 2 of it, one power of two of 32, so that neighbouring blocks
+  // share one, what a block adds does not depend on other blocks, and a change of unit is exact.  It does not fall below
+  // 2^-64 of the largest; blocks far below add to the sum, and to the output what they still can.
   __device__ __forceinline__ void refer(BlockScale& sc) {
-    if (!(sc.v > 0.0f)) return;
-    const int want = max(((int)(__float_as_uint(sc.v) >> 23) + 3) & ~3, 8);
+    const uint32_t bits = __builtin_amdgcn_readfirstlane(__float_as_uint(sc.v));  // not negative
+    if (bits == 0) return;
+    const int want = min(max(((int)(bits >> 23) + 31) & ~31, 32), 248);
     if (want != unit) {
       top = max(top, want);
       const int to = max(want, top - 64);
@@ -223,8 +237,8 @@ struct RowState {
       unit = to;
     }
     sc.far = want != unit;
-    const float x = sc.v * pow2(254 - unit);
-    sc.lv = sc.far ? log2f(x) : __builtin_amdgcn_logf(x);
+    const float x = __uint_as_float(bits) * pow2(254 - unit);
+    sc.lv = __builtin_amdgcn_logf(x);  // of next to nothing: -inf, and the block adds nothing
     sc.rv = sc.far ? 0.0f : __builtin_amdgcn_rcpf(x);
   }
 
@@ -476,7 +490,7 @@ __global__ void __launch_bounds__(kAtnWaves * 64, attend_waves(DB, RT)) kv8_atte
     if (blk < ce) {
       x.load(x.k, kc + (int64_t)blk * kKvBlock * Dp);
       x.load(x.v, vc + (int64_t)blk * kKvBlock * Dp);
-      k1 = ks[blk], v1 = vs[blk];
+      k1 = ld_scale(ks + blk), v1 = ld_scale(vs + blk);
     }
     for (; blk < ce; blk += kAtnWaves) {
       const int64_t next = blk + kAtnWaves;
@@ -486,7 +500,7 @@ __global__ void __launch_bounds__(kAtnWaves * 64, attend_waves(DB, RT)) kv8_atte
       BlockScale sc(k1, v1, a.scale);
       if (next < ce) {
         x.load(x.k, kc + next * kKvBlock * Dp);
-        k1 = ks[next], v1 = vs[next];
+        k1 = ld_scale(ks + next), v1 = ld_scale(vs + next);
       }
       st.settle(s, blk, sc, a.window, masked(blk));
       st.weights(s, sc, p);
@@ -660,12 +674,12 @@ __global__ void __launch_bounds__(WAVES * 64, 2) kv8_chunk_kernel(AttendArgs a) 
       st.scores(frags, s);
       stage(blk + AHEAD, blk + AHEAD - 1);
       stage_tail(blk + AHEAD, blk + AHEAD - 1);
-      float k1 = ks[min(from, coded)], v1 = vs[min(from, coded)];  // the next block's scales
+      float k1 = ld_scale(ks + min(from, coded)), v1 = ld_scale(vs + min(from, coded));  // the next block's scales
       for (++blk; blk < min(to, whole); ++blk) {
         meet();  // every wave is done with what this turn overwrites
         load(blk + AHEAD, blk + AHEAD - 1);
         BlockScale sc(k1, v1, a.scale);
-        k1 = ks[min(blk + 1, coded)], v1 = vs[min(blk + 1, coded)];
+        k1 = ld_scale(ks + min(blk + 1, coded)), v1 = ld_scale(vs + min(blk + 1, coded));
         st.settle(s, blk, sc, a.window,
                   blk * kKvBlock + kKvBlock - 1 > first_pos || (a.window && blk * kKvBlock <= last_pos - a.window));
         frags.k = &lds[(blk + 1) & (SLOTS - 1)][0][lane * 16];

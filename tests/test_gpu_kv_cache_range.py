@@ -55,3 +55,20 @@ def test_large_values_without_weight(cuda_device, n, group, D, T):
     out, o, bar = _outputs(q, k, v, D)
     assert float(o.abs().max()) < 100.0
     assert bool(((out - o).abs() <= bar).all()), float(((out - o).abs() / bar).max())
+
+
+@pytest.mark.parametrize("n", [1, 40])
+@pytest.mark.parametrize("down", [12, 24, 36, 60])
+def test_small_weights_beside_a_large_one(cuda_device, n, down):
+    """One key with values of 0 and nearly all of the weight, 60000 with 2^-down of it each: the output is what these add,
+    and the bar, which is in terms of what adds, holds for it."""
+    g = torch.Generator(device=cuda_device).manual_seed(down)
+    T, D = 60000, 64
+    k = torch.zeros(1, T, 1, D, dtype=torch.bfloat16, device=cuda_device)
+    k[0, 3, 0, 0] = 1.0
+    v = (1.0 + torch.rand(1, T, 1, D, generator=g, device=cuda_device)).bfloat16()
+    v[0, 3] = 0.0
+    q = torch.zeros(1, n, 2, D, dtype=torch.bfloat16, device=cuda_device)
+    q[..., 0] = 0.6931472 * down * D ** 0.5
+    out, o, bar = _outputs(q, k, v, D)
+    assert bool(((out - o).abs() <= bar).all()), float(((out - o).abs() / bar).max())
