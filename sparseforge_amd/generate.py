@@ -83,6 +83,8 @@ def generate(model: LlamaDecoder, prompts: torch.Tensor, new_tokens: int, length
         lengths = torch.full((B,), S, dtype=torch.int32, device=dev)
     elif lengths.shape != (B,) or lengths.dtype != torch.int32 or lengths.device != dev:
         raise ValueError(f"generate: lengths must be int32 [{B}] on {dev}")
+    elif bool(((lengths < 1) | (lengths > S)).any()):
+        raise ValueError(f"generate: lengths must lie in 1 .. {S}, got {lengths.tolist()}")
     lengths = lengths.clone()
     tokens = torch.zeros(B, S + new_tokens, dtype=torch.int64, device=dev)
     tokens[:, :S] = prompts
