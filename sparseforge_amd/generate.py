@@ -32,8 +32,8 @@ class Generator:
 
     @torch.no_grad()
     def step(self, tokens: torch.Tensor, counts: torch.Tensor | None = None) -> torch.Tensor:
-        """tokens [B, n], the first counts[b] (int32 [B], n where None) of a row real -> the logits [B, V] after each
-        row's last real token (of a row without one: without meaning)."""
+        """tokens [B, n], the first counts[b] (int32 [B], n where None) of a row real, any ids in the others -> the logits
+        [B, V] after each row's last real token (of a row without one: without meaning)."""
         m, cache = self.model, self.cache
         B, n = tokens.shape
         cache.extend(n, counts)
@@ -42,6 +42,9 @@ class Generator:
             # rows past a sequence's tokens, whose results are not used, stay inside the tables
             positions = (positions + torch.arange(n, device=self.device, dtype=torch.int32)).clamp_(
                 max=cache.capacity - 1)
+        if counts is not None:  # ids that pad a row may be none of the embedding's (-1, say)
+            real = torch.arange(n, device=self.device) < counts[:, None]
+            tokens = torch.where(real, tokens, tokens.clamp(0, m.config.vocab_size - 1))
         h = m.embed_tokens(tokens)
         for i, layer in enumerate(m.layers):
             a, f = layer.self_attn, layer.mlp
@@ -65,7 +68,8 @@ class Generator:
 def generate(model: LlamaDecoder, prompts: torch.Tensor, new_tokens: int, lengths: torch.Tensor | None = None, *,
              repetition=1.0, presence=0.0, frequency=0.0, bias: torch.Tensor | None = None, allowed=None, pick=None,
              end_token: int | None = None, chunk: int = 2048) -> tuple[torch.Tensor, torch.Tensor]:
-    """Continue prompts [B, S] (the first lengths[b], at least one, of a row) by up to new_tokens tokens each.
+    """Continue prompts [B, S] (the first lengths[b], at least one, of a row; what pads a row is not looked at) by up to
+    new_tokens tokens each.
 
     Returns (tokens int64 [B, S + new_tokens], lengths int32 [B]): each prompt with its continuation, and how many
     tokens that is; what lies past a row's length has no meaning.  The penalties, bias and allowed are process_logits';

@@ -14,3 +14,24 @@ def test_lengths_outside_the_prompts_are_refused(cuda_device, lengths):
     with pytest.raises(ValueError, match="lengths"):
         generate(_model(cuda_device), torch.zeros(2, 4, dtype=torch.int64, device=cuda_device), 3,
                  torch.tensor(lengths, dtype=torch.int32, device=cuda_device))
+
+
+@pytest.mark.parametrize("chunk", [2048, 7])
+def test_padding_may_be_any_id(cuda_device, chunk):
+    """-1 and ids past the vocabulary beyond a row's length give what zeros there give."""
+    from sparseforge_amd.generate import Generator, generate
+
+    m = _model(cuda_device)
+    g = torch.Generator(device=cuda_device).manual_seed(4)
+    prompts = torch.randint(0, 503, (3, 20), generator=g, device=cuda_device)
+    count = [20, 3, 9]
+    lengths = torch.tensor(count, dtype=torch.int32, device=cuda_device)
+    pad = torch.arange(20, device=cuda_device) >= lengths[:, None]
+    got = {}
+    for fill in (0, -1, -100, 503, 2 ** 40):
+        tokens, ends = generate(m, prompts.masked_fill(pad, fill), 12, lengths, chunk=chunk, repetition=1.2)
+        got[fill] = [row[:n].tolist() for row, n in zip(tokens, ends.tolist())]
+        assert got[fill] == got[0] and [len(row) for row in got[fill]] == [n + 12 for n in count]
+    for dtype in (torch.int32, torch.int64):
+        a, b = (Generator(m, 3, 40).step(prompts.masked_fill(pad, fill).to(dtype), lengths) for fill in (0, -7))
+        assert torch.equal(a, b)
