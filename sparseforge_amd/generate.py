@@ -35,6 +35,11 @@ class Generator:
         """tokens [B, n], the first counts[b] (int32 [B], n where None) of a row real, any ids in the others -> the logits
         [B, V] after each row's last real token (of a row without one: without meaning)."""
         m, cache = self.model, self.cache
+        if tokens.dim() != 2 or tokens.shape[0] != self.batch or tokens.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"Generator.step: tokens must be ids [{self.batch}, n], got {tokens.dtype} "
+                             f"{tuple(tokens.shape)}")
+        if tokens.device != self.device:
+            raise ValueError(f"Generator.step: tokens are on {tokens.device}, the model on {self.device}")
         B, n = tokens.shape
         cache.extend(n, counts)
         positions = cache.starts[:, None]

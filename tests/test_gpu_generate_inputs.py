@@ -35,3 +35,18 @@ def test_padding_may_be_any_id(cuda_device, chunk):
     for dtype in (torch.int32, torch.int64):
         a, b = (Generator(m, 3, 40).step(prompts.masked_fill(pad, fill).to(dtype), lengths) for fill in (0, -7))
         assert torch.equal(a, b)
+
+
+def test_a_refused_step_leaves_the_cache_as_it_was(cuda_device):
+    """Tokens of another batch, type or place are refused before the lengths advance, and the step may be taken again."""
+    from sparseforge_amd.generate import Generator
+
+    m = _model(cuda_device)
+    idx = torch.arange(10, device=cuda_device).view(2, 5)
+    want = Generator(m, 2, 64).step(idx)
+    gen = Generator(m, 2, 64)
+    for bad in (idx[:1], idx[0], idx.view(5, 2), idx.float(), idx.cpu(), idx[:, :0]):
+        with pytest.raises(ValueError):
+            gen.step(bad)
+        assert gen.cache.bound == 0 and gen.cache.ends.tolist() == [0, 0]
+    assert torch.equal(gen.step(idx), want)
