@@ -79,8 +79,9 @@ def generate(model: LlamaDecoder, prompts: torch.Tensor, new_tokens: int, length
     Returns (tokens int64 [B, S + new_tokens], lengths int32 [B]): each prompt with its continuation, and how many
     tokens that is; what lies past a row's length has no meaning.  The penalties, bias and allowed are process_logits';
     allowed may be a function of (tokens, lengths) that gives the mask of a step.  pick turns logits [B, V] into ids
-    [B]: the most likely token (the lowest id among equals) where None.  A sequence stops after end_token.  Prompts
-    are taken `chunk` tokens at a time."""
+    [B]: the most likely token (the lowest id among equals) where None.  A sequence stops after end_token, and where
+    its mask or bias lets nothing follow; the logits that pick sees of one that has stopped are zeros.  Prompts are
+    taken `chunk` tokens at a time."""
     if prompts.dim() != 2 or prompts.shape[1] < 1 or prompts.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"generate: prompts must be ids [B, S], got {prompts.dtype} {tuple(prompts.shape)}")
     if new_tokens < 0 or chunk < 1:
@@ -104,16 +105,23 @@ def generate(model: LlamaDecoder, prompts: torch.Tensor, new_tokens: int, length
         out = gen.step(tokens[:, at:at + n], counts)
         logits = out if logits is None else torch.where((counts > 0)[:, None], out, logits)
     alive = torch.ones(B, dtype=torch.int32, device=dev)
+    shaped = allowed is not None or bias is not None
+    stops = shaped or end_token is not None
     for i in range(new_tokens):
         mask = allowed(tokens, lengths) if callable(allowed) else allowed
         logits = process_logits(logits, tokens, lengths, repetition=repetition, presence=presence,
                                 frequency=frequency, bias=bias, allowed=mask, out=logits)
-        ids = logits.argmax(-1) if pick is None else pick(logits)
+        if shaped:
+            alive = alive * ~(logits == float("-inf")).all(-1)
+        if pick is None:
+            ids = logits.argmax(-1)
+        else:
+            ids = pick(logits.masked_fill(alive[:, None] == 0, 0.0) if stops else logits)
         at = lengths.long()[:, None]
         tokens.scatter_(1, at, torch.where(alive[:, None] > 0, ids[:, None].long(), tokens.gather(1, at)))
         lengths += alive
         if end_token is not None:
             alive = alive * (ids != end_token)
         if i + 1 < new_tokens:
-            logits = gen.step(ids[:, None], alive if end_token is not None else None)
+            logits = gen.step(ids[:, None], alive if stops else None)
     return tokens, lengths

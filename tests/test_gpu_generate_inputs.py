@@ -50,3 +50,35 @@ def test_a_refused_step_leaves_the_cache_as_it_was(cuda_device):
             gen.step(bad)
         assert gen.cache.bound == 0 and gen.cache.ends.tolist() == [0, 0]
     assert torch.equal(gen.step(idx), want)
+
+
+def _sample(logits):
+    """A pick that needs a distribution: multinomial refuses rows of NaN, which a softmax of -inf throughout gives."""
+    p = logits.float().softmax(-1)
+    assert not p.isnan().any()
+    return torch.multinomial(p, 1)[:, 0]
+
+
+@pytest.mark.parametrize("pick", [None, _sample])
+def test_a_sequence_stops_where_nothing_may_follow(cuda_device, pick):
+    """A grammar that counts up to a number of each sequence's own and is then complete, with and without a last token."""
+    from sparseforge_amd.generate import generate
+
+    m = _model(cuda_device)
+    prompts = torch.tensor([[7, 10], [7, 20], [3, 30], [3, 500]], device=cuda_device)
+    stop = torch.tensor([14, 20, 60, 502], device=cuda_device)
+    ids = torch.arange(503, device=cuda_device)[None]
+
+    def up(tokens, lengths):
+        last = tokens.gather(1, lengths.long()[:, None] - 1)
+        return (ids == last + 1) & (ids <= stop[:, None])
+
+    tokens, ends = generate(m, prompts, 8, allowed=up, pick=pick)
+    assert ends.tolist() == [6, 2, 10, 4]
+    for row, n, first in zip(tokens.tolist(), ends.tolist(), (10, 20, 30, 500)):
+        assert row[1:n] == list(range(first, first + n - 1))
+    tokens, ends = generate(m, prompts, 8, allowed=up, pick=pick, end_token=13)
+    assert ends.tolist() == [5, 2, 10, 4] and tokens[0, :5].tolist() == [7, 10, 11, 12, 13]
+    none = torch.full((503,), float("-inf"), device=cuda_device)
+    tokens, ends = generate(m, prompts, 3, bias=none, pick=pick)
+    assert ends.tolist() == [2, 2, 2, 2] and torch.equal(tokens[:, :2], prompts)
