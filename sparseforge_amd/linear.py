@@ -310,11 +310,16 @@ class _Unrecorded:
         pass
 
 
+def transforms_active() -> bool:
+    """Whether a functorch transform (torch.func, vmap) or a forward-mode level is there, which a call that passes by
+    autograd's Functions would pass by too."""
+    return forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active()
+
+
 def plain_backward() -> bool:
     """Whether a backward pass runs with nothing that looks into it: no create_graph (grad mode is on then), no
-    functorch transform (torch.func, vmap) and no forward-mode level, which a direct call would pass by."""
-    return not (torch.is_grad_enabled() or forward_ad._current_level >= 0
-                or torch._C._are_functorch_transforms_active())
+    functorch transform and no forward-mode level."""
+    return not (torch.is_grad_enabled() or transforms_active())
 
 
 def apply_in_backward(fn, *args):

@@ -25,7 +25,7 @@ import torch
 
 from . import _lib as L
 from . import profiling as _prof
-from .linear import plain_backward
+from .linear import plain_backward, transforms_active
 
 SCALINGS = ("linear", "ntk", "yarn")
 
@@ -83,9 +83,10 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor, sin
     cos, sin: float32 [P, r / 2] (rotary_cos_sin); the first r elements of a head turn, the others are copied.
     positions: int32 or int64 [B, S] or [S] on the device, None for 0 .. S - 1; one outside 0 .. P - 1 gives NaN.
     q and k are bf16 or float32 and may be views (columns of a fused projection); the turn is in float32, rounded
-    once.  Differentiable in q and k any number of times; the tables and positions take no gradient."""
+    once.  Differentiable in q and k any number of times, in reverse mode (forward mode raises); the tables and positions
+    take no gradient."""
     _check(q, k, cos, sin, positions)
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
+    if (torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad))) or transforms_active():
         return _Rotary.apply(q, k, cos, sin, positions, bool(interleaved), False)
     return _launch(q, k, cos, sin, positions, interleaved, False)
 
