@@ -18,9 +18,10 @@ from . import profiling as _prof
 
 def _written(*ts) -> None:
     """Bump the version counter of tensors a kernel wrote in place, as a torch in-place op would: caches
-    keyed on a mask's version (the forward's effective mask) then see the write."""
+    keyed on a mask's version (the forward's effective mask) then see the write, and so does a backward that
+    saved the tensor.  Tensors of inference mode have no version."""
     for t in ts:
-        if t is not None:
+        if t is not None and not t.is_inference():
             torch.autograd.graph.increment_version(t)
 
 

@@ -16,6 +16,7 @@ import torch
 
 from . import _lib as L
 from . import profiling as _prof
+from .kernels import _written
 
 
 def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
@@ -39,11 +40,14 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
     B, V = logits.shape
     if logits.stride(1) != 1 and V > 1:
         logits = logits.contiguous()
+    given = out
     if out is None:
         out = torch.empty_like(logits, memory_format=torch.contiguous_format)
     elif out.shape != (B, V) or out.dtype != logits.dtype or not (out.stride(1) == 1 or V <= 1) \
             or (B > 1 and out.stride(0) < V):
         raise ValueError(f"process_logits: out must be {logits.dtype} [{B}, {V}] with rows of its own")
+    elif out.requires_grad and torch.is_grad_enabled():
+        raise ValueError("process_logits: out requires grad, and what is written to it takes none")
     n = 0
     if history is not None:
         if history.dtype not in (torch.int32, torch.int64):
@@ -83,6 +87,7 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
         history.element_size() if n else 0, bits, dt)
     with _prof.region("sf_process_logits", 2 * B * V * logits.element_size(), "B", dev):
         L.check(L.lib().sf_process_logits(desc, L.stream(dev)), "sf_process_logits")
+    _written(given)
     return out
 
 
