@@ -48,6 +48,8 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
         raise ValueError(f"process_logits: out must be {logits.dtype} [{B}, {V}] with rows of its own")
     elif out.requires_grad and torch.is_grad_enabled():
         raise ValueError("process_logits: out requires grad, and what is written to it takes none")
+    elif _mixed(logits, out):
+        logits = logits.clone()
     n = 0
     if history is not None:
         if history.dtype not in (torch.int32, torch.int64):
@@ -89,6 +91,19 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
         L.check(L.lib().sf_process_logits(desc, L.stream(dev)), "sf_process_logits")
     _written(given)
     return out
+
+
+def _mixed(x: torch.Tensor, out: torch.Tensor) -> bool:
+    """Whether some row of out lies over another place of x's rows: it could be written before that is read."""
+    B, V = x.shape
+    by, start, end = x.element_size(), x.data_ptr(), out.data_ptr()
+    xs, os = (t.stride(0) if B > 1 else V for t in (x, out))
+    if start + by * (xs * (B - 1) + V) <= end or end + by * (os * (B - 1) + V) <= start:
+        return False
+    if xs != os or (end - start) % by:
+        return True
+    off = (end - start) // by
+    return off != 0 and not V <= off % xs <= xs - V
 
 
 def _strided(t: torch.Tensor | None) -> tuple[int, int]:

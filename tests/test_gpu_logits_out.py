@@ -40,3 +40,27 @@ def test_an_out_that_requires_grad(cuda_device):
         own = torch.empty_like(x)
         process_logits(x, out=own)
     assert process_logits(x, out=own) is own
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_an_out_that_lies_over_the_logits(cuda_device, dtype):
+    """Rows written where other rows are still to be read: shifted by a row, by a few elements, of another stride, of one
+    row for all; and the forms that share memory without sharing an element."""
+    from sparseforge_amd.logits import process_logits
+
+    g = torch.Generator(device=cuda_device).manual_seed(8)
+    B, V = 300, 20001
+    history = torch.randint(0, V, (B, 9), generator=g, device=cuda_device)
+    data = torch.randn((B + 1) * (V + 7) * 2, generator=g, device=cuda_device).to(dtype)
+
+    def rows(first, stride):
+        return lambda t: t.as_strided((B, V), (stride, 1), first)
+
+    for x, y in ((rows(0, V), rows(V, V)), (rows(V, V), rows(0, V)), (rows(0, V), rows(3, V)), (rows(5, V), rows(0, V)),
+                 (rows(0, V + 7), rows(1, V)), (rows(0, V), rows(2, V + 7)), (rows(V, 0), rows(0, V)),
+                 (rows(0, 2 * V), rows(V, 2 * V)), (rows(V, 2 * V), rows(0, 2 * V)), (rows(0, V), rows(0, V)),
+                 (rows(0, 2 * V), rows(V - 1, 2 * V))):
+        want = process_logits(x(data).clone(), history, presence=0.5, frequency=0.25)
+        t = data.clone()
+        got = process_logits(x(t), history, presence=0.5, frequency=0.25, out=y(t))
+        assert torch.equal(got, want)
