@@ -22,6 +22,7 @@ import torch
 
 from . import _lib as L
 from . import profiling as _prof
+from .kernels import _written
 
 BLOCK = 64  # tokens that share a scale
 
@@ -92,6 +93,7 @@ class KVCache8:
         dev = self.ends.device
         with _prof.region("sf_kv8_extend", 12 * self.batch, "B", dev):
             L.check(L.lib().sf_kv8_extend(self._refs[0], n, L.ptr(counts), L.stream(dev)), "sf_kv8_extend")
+        _written(self.starts, self.ends)  # a backward may have saved starts as positions
         self.bound += n
         self._new = n
 
