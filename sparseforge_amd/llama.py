@@ -59,8 +59,8 @@ class LlamaShape:
     num_attention_heads: int = 32
     rms_norm_eps: float = 1e-5
     rope_theta: float = 10000.0
-    rope_scaling: RotaryScaling | None = None  # for contexts longer than the trained one
     output_hidden_state: bool = False  # set by Distill_Model
+    rope_scaling: RotaryScaling | None = None  # for contexts longer than the trained one
 
     @property
     def head_dim(self) -> int:
