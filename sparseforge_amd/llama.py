@@ -717,9 +717,9 @@ class LlamaDecoder(nn.Module):
                 normal_(mod.weight, std)
 
     def _tables(self, seq: int, device):
-        key = (seq, str(device))
+        c = self.config
+        key = (seq, str(device), c.head_dim, c.rope_theta, c.rope_scaling)
         if key not in self._rope:
-            c = self.config
             if c.rope_scaling is None:
                 self._rope[key] = rotary_tables(seq, c.head_dim, c.rope_theta, device)
             else:
