@@ -177,7 +177,7 @@ struct BlockScale {
   __device__ __forceinline__ BlockScale(float k, float v, float scale)
       : v(v > 0.0f ? v : 0.0f), lv(0.0f), rv(1.0f), far(false) {
     nan = k != k;  // both are
-    ks = k > 0.0f ? k * scale : 1.0f;
+    ks = k > 0.0f ? fmaxf(k * scale, 0x1p-149f) : 1.0f;  // not 0, which makes NaN of a hidden score's -inf
   }
 };
 

@@ -72,3 +72,25 @@ def test_small_weights_beside_a_large_one(cuda_device, n, down):
     q[..., 0] = 0.6931472 * down * D ** 0.5
     out, o, bar = _outputs(q, k, v, D)
     assert bool(((out - o).abs() <= bar).all()), float(((out - o).abs() / bar).max())
+
+
+@pytest.mark.parametrize("n,group,D,T", FORMS)
+def test_scores_of_next_to_nothing(cuda_device, n, group, D, T):
+    """Keys and a scale whose product no float holds: every score is 0 within 2^-100, hidden keys stay hidden."""
+    from sparseforge_amd.kv_cache import KVCache8
+
+    g = torch.Generator(device=cuda_device).manual_seed(n + D)
+    k, v = _data(g, 1, T, 2, D, cuda_device)
+    k = (k.float() * 1e-38 * 1e-2).bfloat16()
+    assert 0 < float(k.abs().max()) < 1e-38
+    q = torch.randn(1, n, group * 2, D, generator=g, device=cuda_device).bfloat16()
+    cache = KVCache8(1, 2, D, T + n)
+    if T > n:
+        cache.extend(T - n)
+        cache.append(k[:, :T - n], v[:, :T - n])
+    cache.extend(n)
+    cache.append(k[:, T - n:], v[:, T - n:])
+    for window in (0, 100):
+        out = cache.attend(q, scale=1e-12, window=window).view(n, 2 * group, D).double()
+        o, bar = _attention(q[0] * 0, _stored(k[0], T), _stored(v[0], T), T - n, 1.0, window)
+        assert bool(((out - o).abs() <= bar).all())
