@@ -186,9 +186,11 @@ extern "C" int sf_process_logits(const sf_logits_desc* desc, void* stream) {
   const dim3 grid(static_cast<unsigned>(slices), static_cast<unsigned>(rows));
   const size_t lds = d.history ? static_cast<size_t>(a.slice) * 4 : 0;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  // an output larger than the L2s together only pushes out of them what else is read: 512 rows of 131072 f32 take 128 us
-  // through them and 113 us past them
-  const bool past = rows * vocab * (d.dtype == SF_DTYPE_BF16 ? 2 : 4) > (32ll << 20);
+  // An output that the last-level cache (256 MB) does not hold beside the logits only pushes out of it what else is read,
+  // and is not found there by who reads it next. 512 rows of 131072 f32: 88 us past the caches, 101 through them, with an
+  // argmax of the result after it 162 and 166; 1024 of 50257 bf16 (103 MB): 50 and 51, 83 and 82; 256 of 131072 bf16 (67
+  // MB): 31 and 31, 82 and 72.
+  const bool past = rows * vocab * (d.dtype == SF_DTYPE_BF16 ? 2 : 4) > (128ll << 20);
   if (d.dtype == SF_DTYPE_BF16) {
     if (past)
       logits_kernel<SF_DTYPE_BF16, true><<<grid, kLgBlock, lds, st>>>(a);

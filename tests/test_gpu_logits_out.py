@@ -64,3 +64,20 @@ def test_an_out_that_lies_over_the_logits(cuda_device, dtype):
         t = data.clone()
         got = process_logits(x(t), history, presence=0.5, frequency=0.25, out=y(t))
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("B", [100, 300, 600])
+def test_rows_do_not_depend_on_how_many_there_are(cuda_device, dtype, B):
+    """Outputs on both sides of what is written past the caches: each row as it is alone."""
+    from sparseforge_amd.logits import process_logits
+
+    g = torch.Generator(device=cuda_device).manual_seed(B)
+    V = 131072
+    x = torch.randn(B, V, generator=g, device=cuda_device).to(dtype)
+    history = torch.randint(0, V, (B, 200), generator=g, device=cuda_device)
+    allowed = torch.rand(V, generator=g, device=cuda_device) < 0.7
+    got = process_logits(x, history, repetition=1.3, frequency=0.5, allowed=allowed)
+    for b in (0, 1, B // 2, B - 1):
+        want = process_logits(x[b:b + 1], history[b:b + 1], repetition=1.3, frequency=0.5, allowed=allowed)
+        assert torch.equal(got[b:b + 1], want)
