@@ -82,3 +82,41 @@ def test_a_sequence_stops_where_nothing_may_follow(cuda_device, pick):
     none = torch.full((503,), float("-inf"), device=cuda_device)
     tokens, ends = generate(m, prompts, 3, bias=none, pick=pick)
     assert ends.tolist() == [2, 2, 2, 2] and torch.equal(tokens[:, :2], prompts)
+
+
+@pytest.mark.parametrize("ragged", [False, True])
+def test_a_captured_step_replayed(cuda_device, ragged):
+    """One token a sequence as a graph, replayed over a block's edge with eager work and waits between the replays, each
+    against the same step without a graph."""
+    from sparseforge_amd.generate import Generator
+
+    m = _model(cuda_device)
+    g = torch.Generator(device=cuda_device).manual_seed(6)
+    idx = torch.randint(0, 503, (2, 72), generator=g, device=cuda_device)
+    plain, caught = Generator(m, 2, 80), Generator(m, 2, 80)
+    for gen in (plain, caught):
+        gen.step(idx[:, :60])
+    now = torch.zeros(2, 1, dtype=torch.int64, device=cuda_device)
+    counts = torch.ones(2, dtype=torch.int32, device=cuda_device) if ragged else None
+    warm = Generator(m, 2, 80)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):  # the kernels are loaded before the capture
+        warm.step(now, counts)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    caught.cache.bound = 78
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = caught.step(now, counts)
+    for i in range(60, 70):
+        now.copy_(idx[:, i:i + 1])
+        if ragged:
+            counts[1] = i % 2
+        plain.cache.bound = 78  # the same cut of the launch
+        want = plain.step(now, counts)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want) if not ragged or i % 2 else torch.equal(got[0], want[0])
+        torch.randn(1000, device=cuda_device).sum().item()
+    assert caught.cache.ends.tolist() == plain.cache.ends.tolist() == ([70, 65] if ragged else [70, 70])
