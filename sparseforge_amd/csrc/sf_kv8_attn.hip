@@ -177,7 +177,8 @@ struct BlockScale {
   __device__ __forceinline__ BlockScale(float k, float v, float scale)
       : v(v > 0.0f ? v : 0.0f), lv(0.0f), rv(1.0f), far(false) {
     nan = k != k;  // both are
-    ks = k > 0.0f ? fmaxf(k * scale, 0x1p-149f) : 1.0f;  // not 0, which makes NaN of a hidden score's -inf
+    // neither 0, which makes NaN of a hidden score's -inf, nor infinite, which does of a score of 0
+    ks = k > 0.0f ? __builtin_amdgcn_fmed3f(k * scale, 0x1p-149f, 3.0e38f) : 1.0f;
   }
 };
 
@@ -892,7 +893,7 @@ extern "C" int sf_kv8_attend(const sf_kv8_cache* cache, const void* q, int64_t q
   a.heads = static_cast<int>(heads);
   a.group = static_cast<int>(heads / a.c.H);
   a.window = static_cast<int>(window < cap ? window : 0);
-  a.scale = scale * kAtnLog2e;
+  a.scale = scale < 2.0e38f ? scale * kAtnLog2e : 3.0e38f;
   a.rows = p.rows;
   a.tiles = static_cast<int>(p.tiles);
   a.splits = p.splits;

@@ -94,3 +94,24 @@ def test_scores_of_next_to_nothing(cuda_device, n, group, D, T):
         out = cache.attend(q, scale=1e-12, window=window).view(n, 2 * group, D).double()
         o, bar = _attention(q[0] * 0, _stored(k[0], T), _stored(v[0], T), T - n, 1.0, window)
         assert bool(((out - o).abs() <= bar).all())
+
+
+@pytest.mark.parametrize("n,group,D,T", FORMS)
+def test_scales_past_the_floats(cuda_device, n, group, D, T):
+    """A scale, or a scale times a key's, above every float: rows that score 0 everywhere weigh all keys alike."""
+    from sparseforge_amd.kv_cache import KVCache8
+
+    g = torch.Generator(device=cuda_device).manual_seed(n - D)
+    k, v = _data(g, 1, T, 2, D, cuda_device)
+    q = torch.zeros(1, n, group * 2, D, dtype=torch.bfloat16, device=cuda_device)
+    for size, scale in ((1.0, 3e38), (1e-3, 2.9e38), (1e30, 1e30)):
+        cache = KVCache8(1, 2, D, T + n)
+        x = (k.float() * size).bfloat16()
+        if T > n:
+            cache.extend(T - n)
+            cache.append(x[:, :T - n], v[:, :T - n])
+        cache.extend(n)
+        cache.append(x[:, T - n:], v[:, T - n:])
+        out = cache.attend(q, scale=scale).view(n, 2 * group, D).double()
+        o, bar = _attention(q[0], _stored(k[0], T), _stored(v[0], T), T - n, 1.0, 0)
+        assert bool(((out - o).abs() <= bar).all())
