@@ -11,8 +11,8 @@
 // The probabilities round to bf16 as operands of the second product, which moves an output by 2^-8 of its terms at most,
 // as much as storing it in bf16 does; the sums are of the rounded ones.  f16 would hold three bits more at the same rate,
 // but nothing below 2^-39 of the largest (2^-25 whole): an output that only small weights make, because the largest has a
-// code of 0 there, would come out wrong by more than its rounding.  Two parts in bf16 take the single-token form 10 to
-// 25 % longer.
+// code of 0 there, would come out wrong by more than its rounding.  Two parts in bf16, 16 bits, take the single-token form
+// 10 to 25 % longer; the incomplete block's weights, one block of many, are such.
 //
 // A row's running maximum is raised only when a score passes it by 8 (in log2): probabilities up to 2^8 cost nothing in
 // f32 or bf16, and most blocks need no exchange between lanes.
@@ -346,15 +346,17 @@ struct RowState {
     }
   }
 
-  template <class Block>
-  __device__ __forceinline__ void output(const Block& x, const bf16x8_t (&p)[RT][2]) {
+  // Weights in one part or in several.
+  template <class Block, class... Parts>
+  __device__ __forceinline__ void output(const Block& x, const Parts&... parts) {
 #pragma unroll
     for (int dt = 0; dt < DB * 4; ++dt)
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const bf16x8_t vf = x.value(dt, u);
 #pragma unroll
-        for (int r = 0; r < RT; ++r) o[r][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, p[r][u], o[r][dt], 0, 0, 0);
+        for (int r = 0; r < RT; ++r)
+          ((o[r][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, parts[r][u], o[r][dt], 0, 0, 0)), ...);
       }
   }
 
@@ -369,7 +371,8 @@ struct RowState {
   }
 
   // The incomplete block, which comes last, and finish(): its values, any bf16 numbers, are products with weights that
-  // are final, at most 1.  s: its scores.
+  // are final, at most 1, in a high and a low part (16 bits together; one block, so this costs next to nothing).  s: its
+  // scores.
   template <class Block>
   __device__ __forceinline__ void last(const Block& x, f32x4_t (&s)[RT][4], int blk, float scale, int window) {
     BlockScale sc(1.0f, 0.0f, scale);
@@ -377,19 +380,30 @@ struct RowState {
 #pragma unroll
     for (int r = 0; r < RT; ++r) l[r] += sum(s[r], sc, -m[r], s[r]);
     finish();
-    bf16x8_t p[RT][2];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
       const float f = l[r] == 0.0f ? 0.0f : 1.0f / l[r];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = pack2(f * s[r][2 * u + i / 2][i % 2 * 2], f * s[r][2 * u + i / 2][i % 2 * 2 + 1]);
-        p[r][u] = __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
-      }
+      for (int t = 0; t < 4; ++t) s[r][t] *= f;
     }
-    output(x, p);
+    bf16x8_t p[2][RT][2];
+#pragma unroll
+    for (int part = 0; part < 2; ++part)
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          uint32_t w[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            f32x4_t& e = s[r][2 * u + i / 2];
+            w[i] = pack2(e[i % 2 * 2], e[i % 2 * 2 + 1]);
+            e[i % 2 * 2] -= lo_f(w[i]);
+            e[i % 2 * 2 + 1] -= hi_f(w[i]);
+          }
+          p[part][r][u] = __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
+        }
+    output(x, p[0], p[1]);
   }
 
   // scores(x, next), weights(s, sc, p), sums(p, sc) and output(x, p) as one stream of instructions: products of the next
