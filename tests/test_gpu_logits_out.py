@@ -81,3 +81,25 @@ def test_rows_do_not_depend_on_how_many_there_are(cuda_device, dtype, B):
     for b in (0, 1, B // 2, B - 1):
         want = process_logits(x[b:b + 1], history[b:b + 1], repetition=1.3, frequency=0.5, allowed=allowed)
         assert torch.equal(got[b:b + 1], want)
+
+
+def test_repetition_over_one_history_and_the_rest_over_another(cuda_device):
+    """Two calls in float32 are one definition: with one history for both they are a single call, bit for bit."""
+    from sparseforge_amd.logits import process_logits
+
+    g = torch.Generator(device=cuda_device).manual_seed(5)
+    x = torch.randn(3, 1003, generator=g, device=cuda_device)
+    history = torch.randint(0, 1003, (3, 400), generator=g, device=cuda_device)
+    bias = torch.randn(1003, generator=g, device=cuda_device)
+    allowed = torch.rand(1003, generator=g, device=cuda_device) < 0.8
+    rest = dict(presence=0.7, frequency=0.3, bias=bias, allowed=allowed)
+    once = process_logits(x, history, repetition=1.4, **rest)
+    assert torch.equal(process_logits(process_logits(x, history, repetition=1.4), history, **rest), once)
+    # the answer is the last 100 tokens
+    got = process_logits(process_logits(x, history, repetition=1.4), history[:, 300:], **rest)
+    count = torch.zeros(3, 1003, device=cuda_device).scatter_add_(1, history[:, 300:], torch.ones(3, 100, device=cuda_device))
+    met = torch.zeros(3, 1003, dtype=torch.bool, device=cuda_device).scatter_(1, history, True)
+    y = torch.where(met, torch.where(x > 0, x.double() / 1.4, x.double() * 1.4), x.double())
+    y = y - torch.where(count > 0, 0.3 * count.double() + 0.7, 0.0) + bias
+    assert bool(((got.double() - y).abs()[:, allowed] <= 1e-6 * (y.abs() + 10.0)[:, allowed]).all())
+    assert bool((got[:, ~allowed] == -float("inf")).all())
