@@ -664,6 +664,8 @@ int sf_kv8_extend(const sf_kv8_cache* cache, int64_t n, const int32_t* counts, v
  * The newest rows of every sequence, positions starts[b] .. ends[b] - 1, from
  * the first rows of k, v [batch, n, kv_heads, head_dim] bf16 (strides in
  * elements, heads contiguous, rows 16-byte aligned; at most n per sequence).
+ * Once between two calls of sf_kv8_extend: rows of the incomplete block that a
+ * call completes give way to those after it.
  */
 int sf_kv8_append(const sf_kv8_cache* cache, const void* k, int64_t k_sb, int64_t k_ss, int64_t k_sh, const void* v,
                   int64_t v_sb, int64_t v_ss, int64_t v_sh, int64_t n, void* stream);

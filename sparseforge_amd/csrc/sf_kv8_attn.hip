@@ -21,13 +21,14 @@
 //   up to 16 rows (32 with heads of at most 128): kv8_attend_kernel.  Bound by reading the codes, 2 D bytes per key and
 //     key-value head.  Each wave takes blocks of its own, converted in registers, and the keys are split over workgroups;
 //     kv8_join_kernel joins them.  Conversion and softmax, about 500 vector instructions a block and wave, stay under
-//     the memory's time.  Measured: 32 sequences of 1024 .. 4096, 32 heads of 128: 111 us, 5.9 TB/s; 2 of 131071, 32
-//     heads over 8: 84 us + 5 us for the join, 6.0 TB/s; one of 33 tokens, 32 heads of 64: 5.1 us.
-//   more: kv8_chunk_kernel.  Bound by power: the matrix unit is busy in 52 % of its cycles and the vector unit beside it
-//     (an exponential, its argument, a maximum and half a conversion to bf16 for each score) in 57 %, and the clock falls
-//     to 1.7 .. 2.0 GHz under that load.  Measured: 2048 tokens over 18001, 32 heads of 128 over 8: 496 to 536 us from
-//     one card to another in a row of calls, 1063 to 1149 TFLOP/s (557 to 650 us in the first dozen, while the clock
-//     settles), where a large library product of bf16 reaches 1130 to 1230.
+//     the memory's time.  Measured: 32 sequences of 1024 .. 4096, 32 heads of 128: 112 us, 5.8 TB/s; 2 of 131071, 32
+//     heads over 8: 84 us + 5 us for the join, 6.0 TB/s; one of 33 tokens, 32 heads of 64: 5.4 us.
+//   more: kv8_chunk_kernel.  Bound by power: the matrix unit is busy in 51 % of its cycles and the vector unit beside it
+//     (an exponential, its argument, a maximum and half a conversion to bf16 for each score) in 56 %, and the clock falls
+//     to 1.9 .. 2.1 GHz under that load.  Measured: 2048 tokens over 18001, 32 heads of 128 over 8: 495 to 526 us from
+//     one card to another in a row of calls, 1083 to 1150 TFLOP/s (554 to 610 us in the first dozen, while the clock
+//     settles), where a large library product of bf16 reaches 1130 to 1330; 32 heads of 64 over 18048: 342 us, 835
+//     TFLOP/s; from an empty cache, where the tiles are unequal, 32 heads of 128: 64 us, 540 TFLOP/s.
 #include "sf_kv8.hpp"
 
 namespace sf {

@@ -17,7 +17,10 @@ from .rotary import rotary_cos_sin, rotary_embed
 
 
 class Generator:
-    """A LlamaDecoder (bfloat16, on the GPU) with the caches of a batch of sequences of at most `capacity` tokens."""
+    """A LlamaDecoder (bfloat16, on the GPU) with the caches of a batch of sequences of at most `capacity` tokens.
+
+    A step calls the norms and projections of the model's layers itself, with the cached attention between them: forward
+    hooks of these run, those of a layer or of the model do not."""
 
     def __init__(self, model: LlamaDecoder, batch: int, capacity: int):
         weight = model.embed_tokens.weight
@@ -77,7 +80,8 @@ def generate(model: LlamaDecoder, prompts: torch.Tensor, new_tokens: int, length
     new_tokens tokens each.
 
     Returns (tokens int64 [B, S + new_tokens], lengths int32 [B]): each prompt with its continuation, and how many
-    tokens that is; what lies past a row's length has no meaning.  The penalties, bias and allowed are process_logits';
+    tokens that is; what lies past a row's length has no meaning.  The penalties, bias and allowed are process_logits',
+    with the prompt and the answer so far as the history;
     allowed may be a function of (tokens, lengths) that gives the mask of a step.  pick turns logits [B, V] into ids
     [B]: the most likely token (the lowest id among equals) where None.  A sequence stops after end_token, and where
     its mask or bias lets nothing follow; the logits that pick sees of one that has stopped are zeros.  Prompts are

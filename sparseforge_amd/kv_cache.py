@@ -117,7 +117,8 @@ class KVCache8:
         return t
 
     def append(self, k: torch.Tensor, v: torch.Tensor, layer: int = 0) -> None:
-        """The step's keys and values [B, n, Hk, D] of one layer."""
+        """The step's keys and values [B, n, Hk, D] of one layer, once in a step: where they complete a block, its kept
+        rows give way to those after it, and a second call would code these instead."""
         k, v = self._rows(k, "k", self.kv_heads), self._rows(v, "v", self.kv_heads)
         dev = self.ends.device
         with _prof.region("sf_kv8_append", 3 * k.numel() * k.element_size(), "B", dev):

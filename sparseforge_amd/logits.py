@@ -8,6 +8,10 @@ For token t of a row, in float32 and in this order, rounded once to the logits' 
     x = x + bias[t]
     x = -inf if t is not allowed
 
+One history serves all three penalties.  Where presence and frequency are to count the answer alone and repetition the
+prompt too, two calls in float32 are the definition: one with the whole history and repetition, one of its result with
+the answer and the rest.
+
 A row whose mask allows nothing is -inf throughout.  Forward only: the result takes no gradient.
 """
 from __future__ import annotations
@@ -24,7 +28,7 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
                    bias: torch.Tensor | None = None, allowed: torch.Tensor | None = None,
                    out: torch.Tensor | None = None) -> torch.Tensor:
     """logits [B, V] (bf16 or float32, rows contiguous, e.g. all_logits[:, -1]) -> the processed logits, in `out` if
-    given (logits itself may be given), else in a new tensor.
+    given (logits itself may be given, or memory that overlaps it), else in a new tensor.
 
     history: int32 / int64 [B, n] token ids, the first history_lengths[b] (int32 [B], all where None) of a row counted;
     ids outside 0 .. V - 1 (padding) are not.  repetition, presence, frequency: a number, or float32 [B] on the device.

@@ -11,7 +11,9 @@ Scalings for a context `factor` times the trained one:
     ntk     theta factor^(r / (r - 2)) for theta, r = rotary_dim: the slowest pair interpolates, the fastest stays
     yarn    f_i (g + (1 - g) / factor), g = clamp((L f_i / 2 pi - beta_slow) / (beta_fast - beta_slow), 0, 1), L the
             trained context: pairs that turn often within it stay, those that turn less than once interpolate;
-            m = 0.1 ln(factor) + 1 (Peng et al., 2023).  m is 1 otherwise.
+            m = 0.1 ln(factor) + 1 (Peng et al., 2023).  m is 1 otherwise.  The ramp g is linear in a pair's turns, as
+            in the paper; a model trained with one linear in the pair's index i has other frequencies inside the ramp
+            and needs tables made for it, which rotary_embed takes like these.
 
 There is no counterpart in the reference, whose attention rotates whole heads by the positions 0 .. S - 1 in half
 pairs (HuggingFace's eager attention, legacy/model_llama.py:39-55; llama.causal_attention does that).
