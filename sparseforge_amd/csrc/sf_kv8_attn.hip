@@ -6,7 +6,7 @@
 // query r / group of head r % group.  A wave takes 16 RT rows over whole blocks of 64 keys, one pass with a running
 // maximum and sum.  Both products are v_mfma_f32_16x16x32_bf16 on codes converted to bf16, which is exact (8 significant
 // bits), with f32 scores, sums and outputs.  The key scale multiplies the scores with the softmax's factor; the value
-// scale enters the exponent, over the power of two that the wave holds its output in (RowState::refer).
+// scale enters the exponent (BlockScale).
 //
 // The probabilities round to bf16 as operands of the second product, which moves an output by 2^-8 of its terms at most,
 // as much as storing it in bf16 does; the sums are of the rounded ones.  f16 would hold three bits more at the same rate,
@@ -38,6 +38,7 @@ constexpr int kAtnWaves = 4;
 constexpr float kAtnLog2e = 1.4426950408889634f;
 constexpr float kAtnLow = -3.0e38f;  // below every score that counts
 constexpr float kAtnSlack = 8.0f;
+constexpr float kAtnHuge = 0x1p40f;
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 struct AttendArgs {
@@ -166,14 +167,14 @@ struct TailBlock {
   }
 };
 
-// What a block's scales do to its scores and probabilities.  The value scale, over the power of two that the wave holds
-// its output in (RowState::refer), goes into the exponent, which costs nothing for each key, and the sum of a row takes
-// it out again.  A scale of 0 has codes of 0, for which any other does as well.
+// What a block's scales do to its scores and probabilities.  The value scale, in the wave's terms (RowState::refer), goes
+// into the exponent, which costs nothing for each key, and the sum of a row takes it out again.  A scale of 0 has codes
+// of 0, for which any other does as well.
 struct BlockScale {
   float ks;      // of the scores, with log2 e; positive
   float v;       // of the values, 0 where any does
-  float lv, rv;  // log2 of the value scale over the wave's power of two, and its reciprocal
-  bool far;      // much smaller than that: the sum is taken apart
+  float lv, rv;  // log2 of the value scale in the wave's terms, and its reciprocal
+  bool far;      // so small that the sum is taken apart
   bool nan;      // a block of NaN: its scores become NaN
   __device__ __forceinline__ BlockScale(float k, float v, float scale)
       : v(v > 0.0f ? v : 0.0f), lv(0.0f), rv(1.0f), far(false) {
@@ -190,9 +191,7 @@ struct RowState {
   f32x4_t o[RT][DB * 4];
   float m[RT], l[RT];
   int pos[RT];  // position of the row's query, -1: no such row
-  // o is in terms of 2^(unit - 127) and stays inside the range of floats whatever the values are, the largest numbers of
-  // bf16 among them; 0: of nothing yet.  top: the largest that unit has been.
-  int unit, top;
+  bool huge;    // o is in terms of kAtnHuge
 
   // The queries of rows row0 + 16 r + lane % 16 of key-value head h; rows past the tile's queries are zeros.
   __device__ __forceinline__ void start(const AttendArgs& a, const TileRange& tr, int b, int h, int row0) {
@@ -216,30 +215,25 @@ struct RowState {
       m[r] = kAtnLow;
       l[r] = 0.0f;
     }
-    unit = top = 0;
+    huge = false;
   }
 
-  __device__ __forceinline__ static float pow2(int biased) { return __uint_as_float((uint32_t)max(biased, 0) << 23); }
-
-  // Takes the unit from the block's value scale: 2^-31 to 2 of it, one power of two of 32, so that neighbouring blocks
-  // share one, what a block adds does not depend on other blocks, and a change of unit is exact.  It does not fall below
-  // 2^-64 of the largest; blocks far below add to the sum, and to the output what they still can.
+  // The block's value scale in the wave's terms.  A probability (up to 2^8), a code and the number of keys take up to 40
+  // powers of two beside it, so from the first scale of 2^80 on o is held in terms of 2^40: the largest values of bf16 stay
+  // inside the range of floats in products and sums, as their mean does, and rows that do not see them keep theirs (down
+  // to 2^-86).  Probabilities times scales below 2^-64 may leave the floats: their sum is taken without the scale.
   __device__ __forceinline__ void refer(BlockScale& sc) {
-    const uint32_t bits = __builtin_amdgcn_readfirstlane(__float_as_uint(sc.v));  // not negative
-    if (bits == 0) return;
-    const int want = min(max(((int)(bits >> 23) + 31) & ~31, 32), 248);
-    if (want != unit) {
-      top = max(top, want);
-      const int to = max(want, top - 64);
-      const float f = pow2(127 + min(unit - to, 64));
+    const float v = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(sc.v)));
+    if (!(v > 0.0f)) return;
+    if (v >= 0x1p80f && !huge) {
+      huge = true;
 #pragma unroll
       for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int dt = 0; dt < DB * 4; ++dt) o[r][dt] *= f;
-      unit = to;
+        for (int dt = 0; dt < DB * 4; ++dt) o[r][dt] *= 1.0f / kAtnHuge;
     }
-    sc.far = want != unit;
-    const float x = __uint_as_float(bits) * pow2(254 - unit);
+    const float x = huge ? v * (1.0f / kAtnHuge) : v;
+    sc.far = x < 0x1p-64f;
     sc.lv = __builtin_amdgcn_logf(x);  // of next to nothing: -inf, and the block adds nothing
     sc.rv = sc.far ? 0.0f : __builtin_amdgcn_rcpf(x);
   }
@@ -275,7 +269,7 @@ struct RowState {
   }
 
   // What is rare before a block's probabilities: rows that do not see it whole, a maximum that has to rise, a value
-  // scale far from the wave's.
+  // scale far from 1.
   __device__ __forceinline__ void settle(f32x4_t (&s)[RT][4], int blk, BlockScale& sc, int window, bool masked) {
     refer(sc);
     if (masked || sc.nan) {
@@ -365,9 +359,9 @@ struct RowState {
   __device__ __forceinline__ void finish() {
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
-      const float f = l[r] == 0.0f ? 0.0f : 1.0f / l[r];
+      const float f = l[r] == 0.0f ? 0.0f : (huge ? kAtnHuge : 1.0f) / l[r];
 #pragma unroll
-      for (int dt = 0; dt < DB * 4; ++dt) o[r][dt] = o[r][dt] * f * pow2(unit);
+      for (int dt = 0; dt < DB * 4; ++dt) o[r][dt] *= f;
     }
   }
 

@@ -128,3 +128,29 @@ def test_an_incomplete_block_alone(cuda_device, n, group, D, T):
     out, o, _ = _outputs(q, k, v, D)
     least = (o.bfloat16().double() - o).pow(2).mean().sqrt()
     assert float((out - o).pow(2).mean().sqrt() / least) < 1.01
+
+
+@pytest.mark.parametrize("n,group,D,window", [(200, 1, 128, 0), (90, 2, 64, 0), (24, 4, 128, 0), (60, 2, 200, 0),
+                                              (200, 1, 64, 100), (8, 2, 128, 40)])
+@pytest.mark.parametrize("size", [1.0, 2.0 ** -60])
+def test_largest_values_out_of_sight(cuda_device, n, group, D, window, size):
+    """The largest numbers of bf16 in tokens that some rows see and others of the same wave do not: theirs are as they are
+    without them."""
+    from sparseforge_amd.kv_cache import KVCache8
+
+    g = torch.Generator(device=cuda_device).manual_seed(n + D)
+    T, Hk = 260 + n, 2
+    k, v = _data(g, 1, T, Hk, D, cuda_device)
+    v = (v.float() * size).bfloat16()
+    # the last block of codes but one, or the first that a window leaves
+    at = 192 if window else (T // BLOCK - 1) * BLOCK
+    v[:, at:at + BLOCK] = 3.3e38 * torch.sign(v[:, at:at + BLOCK])
+    q = torch.randn(1, n, group * Hk, D, generator=g, device=cuda_device).bfloat16()
+    cache = KVCache8(1, Hk, D, T)
+    cache.extend(T - n)
+    cache.append(k[:, :T - n], v[:, :T - n])
+    cache.extend(n)
+    cache.append(k[:, T - n:], v[:, T - n:])
+    out = cache.attend(q, window=window).view(n, group * Hk, D).double()
+    o, bar = _attention(q[0], _stored(k[0], T), _stored(v[0], T), T - n, D ** -0.5, window)
+    assert bool(((out - o).abs() <= bar).all()), float(((out - o).abs() / bar).max())
