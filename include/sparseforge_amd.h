@@ -435,6 +435,70 @@ int sf_kl_backward(const void* student, const void* teacher, int dtype, int64_t 
                    float temperature, const double* row_lse, const float* row_scale, const void* grad_out,
                    int grad_out_dtype, void* grad_student, void* stream);
 
+/* ---- the top of a row of logits (no counterpart in the reference) ---- */
+
+#define SF_TOP_MAX_VOCAB 262144 /* longest rows */
+#define SF_TOP_MAX_K 1024       /* most entries that sf_top_logits gives */
+
+/*
+ * The k largest logits of every row, falling, equal ones by rising id (NaN
+ * above all, -0 equal to 0), with their ids, and the log-sum-exp of the row at
+ * `temperature`.  Row r lies at (r / inner) * outer_stride + (r % inner) *
+ * row_stride elements.  values [rows, k] (the logits' dtype), ids int32 [rows,
+ * k], lse f32 [rows] or null.
+ */
+typedef struct sf_top_logits_desc {
+  const void* logits;
+  int64_t outer_stride, row_stride, inner, rows, vocab, k;
+  void* values;
+  int32_t* ids;
+  float* lse;
+  float temperature;
+  int dtype;
+} sf_top_logits_desc;
+int sf_top_logits(const sf_top_logits_desc* desc, void* stream);
+
+/*
+ * KL of a student from a teacher's recorded top logits.  At temperature T, for
+ * a row with student logits s (rows as in sf_top_logits_desc), listed ids i_k
+ * and teacher logits t_k (values, ids: [rows, k]; ids int32 or int64, those
+ * outside the vocabulary are padding):
+ *   a = s / T, q = softmax(a), p_k = exp(t_k / T - N)
+ *   N = log sum_k exp(t_k / T), or lse[row] where given; r = 1 - sum p (not
+ *   below 0) with lse, else 0; q_rest = sum of q over the unlisted tokens
+ *   KL = sum_k p_k (log p_k - log q_(i_k)) + r (log r - log q_rest)
+ *   loss = T^2 sum_rows w KL / sum_rows w      (w = weights, null: 1)
+ * Rows of weight 0 are not looked at; rows without entries add 0; without any
+ * weight the loss is 0.  An id that is listed twice counts twice.
+ * stats: device double[sf_top_kl_stats_size / 8] and norm: device double, both
+ * written by the forward and read by the others.  Sums of rows are formed in
+ * a fixed order.
+ * backward: grad_logits [rows, vocab] = grad_out * dloss/ds, contiguous.
+ * double_backward: along grad_grad [rows, vocab] (contiguous), grad2_logits =
+ * grad_out * d(grad_grad . dloss/ds)/ds, and dot (or null) = grad_grad .
+ * dloss/ds.  The workspace is for the forward and the double_backward.
+ */
+typedef struct sf_top_kl_desc {
+  const void* logits;
+  int64_t outer_stride, row_stride, inner, rows, vocab;
+  const void* values;
+  const void* ids;
+  int64_t k;
+  const float* lse;
+  const float* weights;
+  double* stats;
+  double* norm;
+  float temperature;
+  int dtype, value_dtype, id_bytes;
+} sf_top_kl_desc;
+size_t sf_top_kl_stats_size(int64_t rows);
+size_t sf_top_kl_workspace_size(int64_t rows);
+int sf_top_kl_forward(const sf_top_kl_desc* desc, float* loss, void* workspace, size_t workspace_bytes, void* stream);
+int sf_top_kl_backward(const sf_top_kl_desc* desc, const float* grad_out, void* grad_logits, void* stream);
+int sf_top_kl_double_backward(const sf_top_kl_desc* desc, const float* grad_out, const void* grad_grad,
+                              void* grad2_logits, float* dot, void* workspace, size_t workspace_bytes,
+                              void* stream);
+
 /*
  * Masked weight W_eff = (W * E).to(W dtype), then (W_eff * scale).to(W dtype)
  * when scale != 1: the `w = weight * mask_cast` (and `* scale_factor`) of
@@ -622,6 +686,35 @@ typedef struct sf_logits_desc {
   int history_bytes, allowed_bits, dtype;
 } sf_logits_desc;
 int sf_process_logits(const sf_logits_desc* desc, void* stream);
+
+/*
+ * A token for every row of logits [rows, vocab] (row stride in elements, 0: one
+ * row for all), drawn with the given uniform f32 [rows] in [0, 1) (no
+ * counterpart in the reference).  In the order of falling logit, equal ones by
+ * rising id, with w = exp((x - max) / temperature): the first top_k are kept
+ * (not above 0: all), of these the fewest first that hold top_p of their
+ * weight (1 and more: all; always one), of these the ones with w >= min_p.  The
+ * token is the first, by id, at which the weight of the kept ones up to it
+ * exceeds uniform times their whole weight.  temperature 0: the largest logit
+ * of the lowest id.  temperature, top_k, top_p, min_p: [rows], or null: the
+ * number beside it.  tokens: -1 where a row holds a NaN or nothing above -inf.
+ * logprobs: f32 [rows] or null: the logarithm of the token's share of the kept
+ * weight (NaN, -inf for rows without a token).
+ */
+typedef struct sf_sample_desc {
+  const void* logits;
+  int64_t logits_stride, rows, vocab;
+  const float* uniform;
+  int64_t* tokens;
+  float* logprobs;
+  const float* temperature;
+  const int32_t* top_k;
+  const float* top_p;
+  const float* min_p;
+  float temperature_all, top_p_all, min_p_all;
+  int top_k_all, dtype;
+} sf_sample_desc;
+int sf_sample_logits(const sf_sample_desc* desc, void* stream);
 
 /*
  * A cache of keys and values held in 8 bits (no counterpart in the reference),

@@ -11,6 +11,7 @@ op is not a contiguous tensor on a ROCm device, the call raises.
 from __future__ import annotations
 
 import ctypes
+import math
 import os
 import struct
 import threading
@@ -243,10 +244,13 @@ class AdamwParams(ctypes.Structure):
     ]
 
 
-# sf_rotary_desc and sf_logits_desc, which a decode step fills anew on every call: packed into bytes in 1 us, where the
-# fields of a ctypes Structure (or as many arguments) take 6.  Pointers and int64 are q.
+# sf_rotary_desc and its like, which a decode or training step fills anew on every call: packed into bytes in 1 us, where
+# the fields of a ctypes Structure (or as many arguments) take 6.  Pointers and int64 are q.
 ROTARY_DESC = struct.Struct("@21q4i")
 LOGITS_DESC = struct.Struct("@17q3f3i")
+SAMPLE_DESC = struct.Struct("@11q3f2i")
+TOP_LOGITS_DESC = struct.Struct("@10qfi")
+TOP_KL_DESC = struct.Struct("@13qf3i")
 
 byref = ctypes.byref
 
@@ -302,6 +306,13 @@ SIGNATURES = {
     "sf_kv8_attend_workspace_size": (_SZ, [_I64, _I64, _I64, _I64, _I64, _I64]),
     "sf_kv8_attend": (_I, [ctypes.POINTER(Kv8Cache), _P, _I64, _I64, _I64, _I64, _I64, _F, _I64, _I64, _P, _P, _SZ, _P]),
     "sf_process_logits": (_I, [_P, _P]),
+    "sf_sample_logits": (_I, [_P, _P]),
+    "sf_top_logits": (_I, [_P, _P]),
+    "sf_top_kl_stats_size": (_SZ, [_I64]),
+    "sf_top_kl_workspace_size": (_SZ, [_I64]),
+    "sf_top_kl_forward": (_I, [_P, _P, _P, _SZ, _P]),
+    "sf_top_kl_backward": (_I, [_P, _P, _P, _P]),
+    "sf_top_kl_double_backward": (_I, [_P, _P, _P, _P, _P, _P, _SZ, _P]),
     "sf_transpose_batched": (_I, [_P, _I, _I64, _I64, _I64, _P, _P]),
     "sf_softmax_rows": (_I, [_P, _I, _I64, _I64, _I, _P, _P]),
     "sf_softmax_rows_backward": (_I, [_P, _P, _I, _I64, _I64, _I, _P, _P]),
@@ -440,6 +451,31 @@ def require_device_only(*tensors: torch.Tensor | None) -> torch.device:
 
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
+
+
+def rows_of(t: torch.Tensor) -> tuple[torch.Tensor, int, int, int, int]:
+    """t [.., V] as rows of a descriptor: t (a contiguous copy where its strides do not fit), the strides of the outer and
+    the inner level of rows, rows of the inner level, rows."""
+    lead = t.shape[:-1]
+    rows = math.prod(lead)
+    if rows == 0:
+        return t, 0, 0, 1, 0
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        t = t.contiguous()
+    levels: list = []  # (size, stride), the innermost first
+    for size, step in zip(reversed(lead), reversed(t.stride()[:-1])):
+        if size == 1:
+            continue
+        if levels and step == levels[-1][0] * levels[-1][1]:
+            levels[-1] = (levels[-1][0] * size, levels[-1][1])
+        else:
+            levels.append((size, step))
+    if len(levels) > 2:
+        return rows_of(t.contiguous())
+    if not levels:
+        return t, 0, 0, 1, 1
+    (inner, step), outer = levels[0], levels[1][1] if len(levels) == 2 else 0
+    return t, outer, step, inner, rows
 
 
 def stream(device: torch.device) -> int:

@@ -13,8 +13,13 @@ prompt too, two calls in float32 are the definition: one with the whole history 
 the answer and the rest.
 
 A row whose mask allows nothing is -inf throughout.  Forward only: the result takes no gradient.
+
+sample_logits draws the token (sf_sample_logits): temperature, top-k, top-p and min-p, with random numbers that the caller
+gives.
 """
 from __future__ import annotations
+
+import math
 
 import torch
 
@@ -95,6 +100,59 @@ def process_logits(logits: torch.Tensor, history: torch.Tensor | None = None,
         L.check(L.lib().sf_process_logits(desc, L.stream(dev)), "sf_process_logits")
     _written(given)
     return out
+
+
+def sample_logits(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+                  logprobs: bool = False):
+    """A token for every row of logits [B, V] (bf16 or float32, any row stride, e.g. 0 for several draws from one row),
+    drawn with uniform float32 [B] in [0, 1): ids int64 [B], or with logprobs (ids, float32 [B]).
+
+    With w = exp((x - max x) / temperature), in the order of falling logit, equal ones by rising id, these are kept: the
+    first top_k (0: all); of them the fewest first that hold top_p of their weight, and always the first; of them the ones
+    with w >= min_p.  The token is the first, by id, at which the weight of the kept ones up to it exceeds uniform times
+    their whole weight, its log-probability the logarithm of its share.  Temperature 0 takes the largest logit of the
+    lowest id.  Each setting is a number, or a tensor [B] on the device (top_k int32, the others float32; what lies
+    outside a setting's range there counts as its nearest end).  A row that holds a NaN, or nothing above -inf (a mask that
+    allows nothing), has no token: -1, with a log-probability of NaN or -inf.  V is at most 262144."""
+    dev = logits.device
+    for t in (logits, uniform):
+        if not t.is_cuda or t.get_device() != dev.index:
+            L.require_device_only(logits, uniform)  # says which
+    dt = L.dtype_code(logits)
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError(f"sample_logits: logits must be [B, V], got {tuple(logits.shape)}")
+    B, V = logits.shape
+    if logits.stride(1) != 1 and V > 1:
+        logits = logits.contiguous()
+    if uniform.dtype != torch.float32 or uniform.shape != (B,):
+        raise ValueError(f"sample_logits: uniform must be float32 [{B}], got {uniform.dtype} {tuple(uniform.shape)}")
+    uniform = uniform.contiguous()
+    temp, p, least = (_setting(x, name, low, high, B, dev) for x, name, low, high in
+                      ((temperature, "temperature", 0.0, math.inf), (top_p, "top_p", 0.0, 1.0),
+                       (min_p, "min_p", 0.0, 1.0)))
+    k = _setting(top_k, "top_k", 0, 2 ** 31 - 1, B, dev, torch.int32)
+    ids = torch.empty(B, dtype=torch.int64, device=dev)
+    logp = torch.empty(B, dtype=torch.float32, device=dev) if logprobs else None
+    desc = L.SAMPLE_DESC.pack(logits.data_ptr(), logits.stride(0) if B > 1 else V, B, V, uniform.data_ptr(),
+                              ids.data_ptr(), L.ptr(logp) or 0, temp[0], k[0], p[0], least[0], temp[1], p[1], least[1],
+                              k[1], dt)
+    with torch.cuda.device_of(logits), _prof.region("sf_sample_logits", B * V * logits.element_size(), "B", dev):
+        L.check(L.lib().sf_sample_logits(desc, L.stream(dev)), "sf_sample_logits")
+    return (ids, logp) if logprobs else ids
+
+
+def _setting(x, name: str, low, high, B: int, dev, dtype=torch.float32) -> tuple:
+    """A setting as the kernel takes it: a pointer to one for each row, or a number."""
+    if not isinstance(x, torch.Tensor):
+        if not low <= x <= high:
+            raise ValueError(f"sample_logits: a {name} of {x}")
+        return 0, int(x) if dtype == torch.int32 else float(x)
+    if x.device != dev:
+        L.require_device_only(x)
+        raise ValueError(f"sample_logits: {name} is on {x.device}, the logits on {dev}")
+    if x.dtype != dtype or x.shape != (B,) or not x.is_contiguous():
+        raise ValueError(f"sample_logits: {name} must be a number or a contiguous {dtype} [{B}]")
+    return x.data_ptr(), 0
 
 
 def _mixed(x: torch.Tensor, out: torch.Tensor) -> bool:
