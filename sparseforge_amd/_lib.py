@@ -10,6 +10,7 @@ op is not a contiguous tensor on a ROCm device, the call raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import math
 import os
@@ -458,6 +459,8 @@ def rows_of(t: torch.Tensor) -> tuple[torch.Tensor, int, int, int, int]:
     the inner level of rows, rows of the inner level, rows."""
     lead = t.shape[:-1]
     rows = math.prod(lead)
+    if t.is_contiguous():
+        return t, 0, t.shape[-1], max(rows, 1), rows
     if rows == 0:
         return t, 0, 0, 1, 0
     if t.stride(-1) != 1 and t.shape[-1] > 1:
@@ -476,6 +479,14 @@ def rows_of(t: torch.Tensor) -> tuple[torch.Tensor, int, int, int, int]:
         return t, 0, 0, 1, 1
     (inner, step), outer = levels[0], levels[1][1] if len(levels) == 2 else 0
     return t, outer, step, inner, rows
+
+
+_HERE = contextlib.nullcontext()
+
+
+def on(device: torch.device):
+    """A context in which launches go to `device`: nothing to do where it is the current one."""
+    return _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def stream(device: torch.device) -> int:

@@ -11,12 +11,15 @@
 // The rest's sums are formed without the listed tokens (one bit for each of the vocabulary in LDS), not as a difference.
 //
 // One workgroup per row streams it once.  Listed tokens (at most a few hundred) are gathered and handled in f64.
+#include <type_traits>
+
 #include "sf_common.hpp"
 
 namespace sf {
 namespace {
 
-constexpr int kTkBlock = 256;
+constexpr int kTkForwardU = 3, kTkBackwardU = 4;  // pieces of a row a thread loads before using them
+constexpr int kTkSecond = 512;
 constexpr int kTkStats = 6;  // f64 of a row that the backward needs
 constexpr float kTkLow = -3.0e38f;  // start of a running maximum: finite, so that -inf minus it is -inf and not NaN
 
@@ -27,7 +30,7 @@ struct TopKlArgs {
   const void* ids;
   const float* lse;      // null: renormalised
   const float* weights;  // null: all 1
-  int64_t vocab;
+  int vocab;
   int k, vdt, id_bytes;
   double inv_t;
 };
@@ -37,48 +40,141 @@ struct RowStats {
   double twice;           // an id is listed more than once
 };
 
-__device__ __forceinline__ int64_t tk_id(const TopKlArgs& a, int64_t at) {
+// Words of a row's marks.
+__host__ __device__ __forceinline__ int mark_words(int vocab) { return (vocab + 8) / 32 + 1; }
+
+__device__ __forceinline__ int tk_id(const TopKlArgs& a, int64_t at) {
   const int64_t id = a.id_bytes == 8 ? static_cast<const int64_t*>(a.ids)[at] : static_cast<const int32_t*>(a.ids)[at];
-  return id >= 0 && id < a.vocab ? id : -1;
+  return id >= 0 && id < a.vocab ? static_cast<int>(id) : -1;
 }
 
-// n (at most 8) elements from any element's address.
+// 8 elements from any element's address, as they are stored.
 template <int DT>
-__device__ __forceinline__ void tk_load8(const void* p, int64_t i, int n, float (&v)[8]) {
-  if (n == 8) {
-    if constexpr (DT == SF_DTYPE_BF16) {
-      uint32_t w[4];
-      __builtin_memcpy(w, static_cast<const uint16_t*>(p) + i, 16);
+struct Raw8 {
+  uint32_t w[DT == SF_DTYPE_BF16 ? 4 : 8];
+  __device__ __forceinline__ void load(const void* row, int i) {
+    __builtin_memcpy(w, static_cast<const char*>(row) + static_cast<int64_t>(i) * (DT == SF_DTYPE_BF16 ? 2 : 4),
+                     sizeof(w));
+  }
+  __device__ __forceinline__ void get(float (&v)[8]) const {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        v[2 * k] = __uint_as_float(w[k] << 16);
-        v[2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
-      }
-    } else {
-      __builtin_memcpy(v, static_cast<const float*>(p) + i, 32);
+    for (int k = 0; k < 8; ++k) {
+      if constexpr (DT == SF_DTYPE_BF16)
+        v[k] = __uint_as_float(k & 1 ? w[k / 2] & 0xffff0000u : w[k / 2] << 16);
+      else
+        v[k] = __uint_as_float(w[k]);
     }
-  } else {
+  }
+};
+
+template <int DT>
+__device__ __forceinline__ void tk_store8(void* row, int i, int n, const float (&v)[8]) {
+  if (n == 8) {
+    uint32_t w[DT == SF_DTYPE_BF16 ? 4 : 8];
+    if constexpr (DT == SF_DTYPE_BF16) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = k < n ? load_as_f32(p, i + k, DT) : -INFINITY;
+      for (int k = 0; k < 4; ++k)
+        w[k] = static_cast<uint32_t>(f32_to_bf16(v[2 * k])) | static_cast<uint32_t>(f32_to_bf16(v[2 * k + 1])) << 16;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) w[k] = __float_as_uint(v[k]);
+    }
+    __builtin_memcpy(static_cast<char*>(row) + static_cast<int64_t>(i) * (DT == SF_DTYPE_BF16 ? 2 : 4), w, sizeof(w));
+  } else {
+    for (int k = 0; k < n; ++k) store_from_f32(row, i + k, DT, v[k]);
   }
 }
-template <int DT>
-__device__ __forceinline__ void tk_store8(void* p, int64_t i, int n, const float (&v)[8]) {
+
+// How a row is cut: `head` tokens before its first 16-byte boundary, pieces of 8, and the last few.  Thread t takes pieces
+// t, t + BLK, ..; n of them; the last threads take the odd tokens.
+struct Cut {
+  int vocab, head, n;
+  template <int DT, int BLK>
+  static __device__ __forceinline__ Cut of(const void* row, int vocab) {
+    constexpr int kBytes = DT == SF_DTYPE_BF16 ? 2 : 4;
+    Cut c;
+    c.vocab = vocab;
+    c.head = static_cast<int>((16 - reinterpret_cast<uintptr_t>(row) % 16) % 16) / kBytes;
+    if (c.head > vocab) c.head = vocab;
+    const int pieces = (vocab - c.head) / 8, t = threadIdx.x;
+    c.n = pieces > t ? (pieces - t - 1) / BLK + 1 : 0;
+    return c;
+  }
+  template <int BLK>
+  __device__ __forceinline__ int at(int p) const {
+    return head + (static_cast<int>(threadIdx.x) + p * BLK) * 8;
+  }
+  // Place of a token's mark: a piece's marks are a byte.
+  __device__ __forceinline__ int mark(int id) const { return id + 8 - head; }
+};
+
+// f(first id, number of elements, elements of each of N rows) over the odd tokens; what is missing of 8 is -inf.
+template <int DT, int BLK, int N, typename F>
+__device__ __forceinline__ void tk_odd(const void* const (&rows)[N], const Cut& c, F&& f) {
+  const int done = c.head + (c.vocab - c.head) / 8 * 8, t = threadIdx.x;
+  const int i = t == BLK - 1 ? 0 : done, n = t == BLK - 1 ? c.head : t == BLK - 2 ? c.vocab - done : 0;
+  if (n == 0) return;
+  float v[N][8];
 #pragma unroll
-  for (int k = 0; k < 8; ++k)
-    if (k < n) store_from_f32(p, i + k, DT, v[k]);
+  for (int j = 0; j < N; ++j)
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[j][k] = k < n ? load_as_f32(rows[j], i + k, DT) : -INFINITY;
+  f(i, n, v);
 }
 
-__device__ __forceinline__ double wave_sum(double x) {
-  for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
-  return x;
+// The same over the pieces from piece `from` of each thread on, and the odd tokens: U pieces are loaded before the first
+// is used; before() runs, in every thread, between the first loads and their use.
+template <int DT, int BLK, int U, int N, typename B, typename F>
+__device__ __forceinline__ void tk_stream(const void* const (&rows)[N], const Cut& c, int from, B&& before, F&& f) {
+  Raw8<DT> raw[U][N];
+  float v[N][8];
+  const auto load = [&](int p) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (p + u < c.n)
+#pragma unroll
+        for (int j = 0; j < N; ++j) raw[u][j].load(rows[j], c.at<BLK>(p + u));
+  };
+  load(from);
+  before();
+  for (int p = from; p < c.n; p += U) {
+    if (p > from) load(p);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (p + u < c.n) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) raw[u][j].get(v[j]);
+        f(c.at<BLK>(p + u), 8, v);
+      }
+  }
+  tk_odd<DT, BLK>(rows, c, f);
+}
+
+template <int DT>
+__device__ __forceinline__ const void* row_at(const void* p, int64_t at) {
+  return static_cast<const char*>(p) + at * (DT == SF_DTYPE_BF16 ? 2 : 4);
+}
+
+// Sums of N numbers over groups of W lanes, and maxima.
+template <int W = 64, int N>
+__device__ __forceinline__ void lanes_sum(double (&x)[N]) {
+#pragma unroll
+  for (int off = W / 2; off > 0; off >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] += __shfl_xor(x[i], off, 64);
+}
+template <int W = 64, int N>
+__device__ __forceinline__ void lanes_max(double (&x)[N]) {
+#pragma unroll
+  for (int off = W / 2; off > 0; off >>= 1)
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = fmax(x[i], __shfl_xor(x[i], off, 64));
 }
 
 // Sum of N numbers of every thread, in an order that does not vary; the result is in every thread.
 template <int N, int BLK>
 __device__ __forceinline__ void block_sum(double (&x)[N], double (&part)[BLK / 64][N]) {
-#pragma unroll
-  for (int i = 0; i < N; ++i) x[i] = wave_sum(x[i]);
+  lanes_sum(x);
   __syncthreads();
   if ((threadIdx.x & 63) == 0)
     for (int i = 0; i < N; ++i) part[threadIdx.x >> 6][i] = x[i];
@@ -89,74 +185,113 @@ __device__ __forceinline__ void block_sum(double (&x)[N], double (&part)[BLK / 6
     for (int w = 0; w < BLK / 64; ++w) x[i] += part[w][i];
   }
 }
+// Marks the row's listed ids in bits that are 0; per wave in flags: 1 if some are listed, 3 if one was marked already.
 template <int BLK>
-__device__ __forceinline__ double block_max(double x, double (&part)[BLK / 64]) {
-  for (int off = 32; off > 0; off >>= 1) x = fmax(x, __shfl_xor(x, off, 64));
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = x;
-  __syncthreads();
-  x = part[0];
-  for (int w = 1; w < BLK / 64; ++w) x = fmax(x, part[w]);
-  return x;
-}
-
-// Marks the row's listed ids; in every thread 1 if some are, 3 if one is listed twice.
-template <int BLK>
-__device__ __forceinline__ int mark_listed(const TopKlArgs& a, int64_t r, uint32_t* bits) {
-  for (int64_t i = threadIdx.x; i < a.vocab / 32 + 1; i += BLK) bits[i] = 0;
-  __syncthreads();
+__device__ __forceinline__ void mark_listed(const TopKlArgs& a, int64_t r, const Cut& c, uint32_t* bits, int* flags) {
   int any = 0, twice = 0;
   for (int k = threadIdx.x; k < a.k; k += BLK) {
-    const int64_t id = tk_id(a, r * a.k + k);
+    const int id = tk_id(a, r * a.k + k);
     if (id < 0) continue;
     any = 1;
-    twice |= atomicOr(&bits[id / 32], 1u << (id % 32)) >> (id % 32) & 1;
+    const int at = c.mark(id);
+    twice |= atomicOr(&bits[at / 32], 1u << (at % 32)) >> (at % 32) & 1;
   }
-  any = __syncthreads_or(any) ? 1 : 0;
-  return any | (__syncthreads_or(twice) ? 2 : 0);
+  const int f = (__ballot(any) ? 1 : 0) | (__ballot(twice) ? 2 : 0);
+  if ((threadIdx.x & 63) == 0) flags[threadIdx.x >> 6] = f;
+}
+template <int BLK>
+__device__ __forceinline__ int all_flags(const int* flags) {
+  int f = 0;
+  for (int w = 0; w < BLK / 64; ++w) f |= flags[w];
+  return f;
 }
 
-// The marks of 8 tokens from i on.
-__device__ __forceinline__ uint32_t marks8(const uint32_t* bits, int64_t i) {
-  return static_cast<uint32_t>((static_cast<uint64_t>(bits[i / 32 + 1]) << 32 | bits[i / 32]) >> (i % 32)) & 255u;
+// The marks of the up to 8 tokens from i on: of a piece, or of the odd ones.
+__device__ __forceinline__ uint32_t marks8(const uint32_t* bits, const Cut& c, int i) {
+  const int at = c.mark(i);
+  return reinterpret_cast<const uint8_t*>(bits)[at / 8] >> (at % 8);
 }
 
-template <int DT>
-__global__ void __launch_bounds__(kTkBlock) top_kl_kernel(TopKlArgs a, double* __restrict__ stats,
-                                                          double* __restrict__ row_kl) {
-  extern __shared__ uint32_t bits[];  // vocab / 32 + 2 words
-  __shared__ double part5[kTkBlock / 64][5];
-  __shared__ double part1[kTkBlock / 64];
+// Whether entry k of the row is the first with its id.
+__device__ __forceinline__ bool first_of_id(const TopKlArgs& a, int64_t r, int k, int id) {
+  for (int j = 0; j < k; ++j)
+    if (tk_id(a, r * a.k + j) == id) return false;
+  return true;
+}
+
+// What a wave finds of a row.
+struct WavePart {
+  double nb, e0, e1, e2;  // listed: sums of e = exp(b - nb), of e (b - nb), of e a
+  double ml, sl;          // listed students: maximum and sum of exponentials
+  float m, sum;           // tokens of the stream: maximum and sum of exponentials
+};
+
+// exp(x - top) for sums whose maximum is top; nothing counts 0.
+__device__ __forceinline__ double exp_from(double x, double top) { return x == -INFINITY ? 0.0 : exp(x - top); }
+
+// REST: with the teacher's log-sum-exp; the stream then leaves out the listed tokens.
+template <int DT, int BLK, bool REST>
+__global__ void __launch_bounds__(BLK) top_kl_kernel(TopKlArgs a, double* __restrict__ stats,
+                                                     double* __restrict__ row_kl) {
+  extern __shared__ uint32_t bits[];  // mark_words(vocab)
+  __shared__ WavePart parts[BLK / 64];
+  __shared__ int flags[BLK / 64];
   const int64_t r = blockIdx.x;
-  const int t = threadIdx.x;
-  RowStats st{};
+  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   if (a.weights && a.weights[r] == 0.0f) {
     if (t == 0) row_kl[r] = 0.0;
     return;
   }
-  const int64_t base = (r / a.inner) * a.s0 + (r % a.inner) * a.s1;
-  if (t == 0) bits[a.vocab / 32 + 1] = 0;
-  const int marked = mark_listed<kTkBlock>(a, r, bits);
-  if (!marked) {  // a row without entries adds nothing
-    if (t == 0) {
-      row_kl[r] = 0.0;
-      *reinterpret_cast<RowStats*>(stats + r * kTkStats) = st;
-    }
-    return;
-  }
-  st.twice = marked >> 1;
-  // the unlisted tokens: running maximum and sum of exponentials
+  const void* rows[1] = {row_at<DT>(a.s, (r / a.inner) * a.s0 + (r % a.inner) * a.s1)};
+  const Cut cut = Cut::of<DT, BLK>(rows[0], a.vocab);
   const float c = static_cast<float>(a.inv_t * 1.4426950408889634);
   float m = kTkLow, sum = 0.0f;
-  for (int64_t i = t * 8; i < a.vocab; i += kTkBlock * 8) {
-    const int n = a.vocab - i < 8 ? static_cast<int>(a.vocab - i) : 8;
-    float v[8];
-    tk_load8<DT>(a.s, base + i, n, v);
-    const uint32_t out = marks8(bits, i);
+  WavePart part{REST ? static_cast<double>(a.lse[r]) : -INFINITY, 0.0, 0.0, 0.0, -INFINITY, 0.0, 0.0f, 0.0f};
+  // The row's first loads are on their way while the listed tokens are marked and summed: the latter by the waves that
+  // have some, each with its own maxima, so that no wave waits for another before the row's end.
+  const auto listed = [&] {
+    for (int i = t; i < mark_words(a.vocab); i += BLK) bits[i] = 0;
+    __syncthreads();
+    mark_listed<BLK>(a, r, cut, bits, flags);
+    __syncthreads();
+    if (wave * 64 >= a.k) return;
+    const bool twice = all_flags<BLK>(flags) & 2;
+    for (int k = t; k < a.k; k += BLK) {
+      const int id = tk_id(a, r * a.k + k);
+      if (id < 0) continue;
+      if (!REST) part.nb = fmax(part.nb, load_as_f32(a.values, r * a.k + k, a.vdt) * a.inv_t);
+      part.ml = fmax(part.ml, load_as_f32(rows[0], id, DT) * a.inv_t);
+    }
+    double most[2] = {part.nb, part.ml};
+    lanes_max(most);
+    if (!REST) part.nb = most[0];
+    part.ml = most[1];
+    for (int k = t; k < a.k; k += BLK) {
+      const int id = tk_id(a, r * a.k + k);
+      if (id < 0) continue;
+      const double b = load_as_f32(a.values, r * a.k + k, a.vdt) * a.inv_t, s = load_as_f32(rows[0], id, DT) * a.inv_t;
+      const double e = part.nb == -INFINITY ? 0.0 : exp(b - part.nb);
+      if (!(e <= 0.0)) {
+        part.e0 += e;
+        part.e1 += e * (b - part.nb);
+        part.e2 += e * s;
+      }
+      if (REST && (!twice || first_of_id(a, r, k, id))) part.sl += exp_from(s, part.ml);
+    }
+    double x[4] = {part.e0, part.e1, part.e2, part.sl};
+    lanes_sum(x);
+    part.e0 = x[0], part.e1 = x[1], part.e2 = x[2], part.sl = x[3];
+  };
+  tk_stream<DT, BLK, kTkForwardU>(rows, cut, 0, listed, [&](int i, int, float (&x)[1][8]) {
+    float(&v)[8] = x[0];
     float top = m;
+    const uint32_t out = REST ? marks8(bits, cut, i) : 0;
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      if (out >> k & 1) v[k] = -INFINITY;
+      if (REST) {  // -inf where the bit is set
+        const uint32_t mask = static_cast<uint32_t>(static_cast<int32_t>(out << (31 - k)) >> 31);
+        v[k] = __uint_as_float((__float_as_uint(v[k]) & ~mask) | (mask & 0xff800000u));
+      }
       top = fmaxf(top, v[k]);
     }
     if (top > m) {
@@ -165,58 +300,63 @@ __global__ void __launch_bounds__(kTkBlock) top_kl_kernel(TopKlArgs a, double* _
     }
 #pragma unroll
     for (int k = 0; k < 8; ++k) sum += __builtin_amdgcn_exp2f((v[k] - m) * c);
+  });
+  part.m = m;
+  for (int off = 32; off > 0; off >>= 1) part.m = fmaxf(part.m, __shfl_xor(part.m, off, 64));
+  part.sum = sum == 0.0f ? 0.0f : sum * __builtin_amdgcn_exp2f((m - part.m) * c);
+  for (int off = 32; off > 0; off >>= 1) part.sum += __shfl_xor(part.sum, off, 64);
+  if (lane == 0) parts[wave] = part;
+  __syncthreads();
+  if (wave != 0) return;
+  // the waves' parts, one to a lane
+  constexpr int W = BLK / 64;
+  part = parts[lane % W];
+  double most[3] = {part.nb, part.ml, static_cast<double>(part.m) * a.inv_t};
+  lanes_max<W>(most);
+  const double nb = most[0], top = fmax(most[1], most[2]);
+  if (!REST && part.nb != nb) {
+    const double f = exp_from(part.nb, nb), d = part.nb - nb;
+    part.e1 = f == 0.0 ? 0.0 : f * (part.e1 + d * part.e0);
+    part.e0 = f == 0.0 ? 0.0 : f * part.e0;
+    part.e2 = f == 0.0 ? 0.0 : f * part.e2;
   }
-  // the listed ones, and the teacher's side
-  double bm = -INFINITY, am = -INFINITY;
-  for (int k = t; k < a.k; k += kTkBlock) {
-    const int64_t id = tk_id(a, r * a.k + k);
-    if (id < 0) continue;
-    bm = fmax(bm, load_as_f32(a.values, r * a.k + k, a.vdt) * a.inv_t);
-    am = fmax(am, static_cast<double>(load_as_f32(a.s, base + id, DT)));
-  }
-  const double top = block_max<kTkBlock>(fmax(am, m), part1);
-  if (!a.lse) bm = block_max<kTkBlock>(bm, part1);
-  double x[5] = {0.0, 0.0, 0.0, 0.0, 0.0};  // sum e, sum e (b - N0), sum e a, exponentials of the listed, of the rest
-  const double n0 = a.lse ? static_cast<double>(a.lse[r]) : bm;
-  for (int k = t; k < a.k; k += kTkBlock) {
-    const int64_t id = tk_id(a, r * a.k + k);
-    if (id < 0) continue;
-    const double b = load_as_f32(a.values, r * a.k + k, a.vdt) * a.inv_t;
-    const double s = load_as_f32(a.s, base + id, DT);
-    const double e = n0 == -INFINITY ? 0.0 : exp(b - n0);
-    if (!(e <= 0.0)) {
-      x[0] += e;
-      x[1] += e * (b - n0);
-      x[2] += e * (s * a.inv_t);
+  double x[5] = {part.e0, part.e1, part.e2, part.sum == 0.0f ? 0.0 : part.sum * exp(part.m * a.inv_t - top),
+                 part.sl == 0.0 ? 0.0 : part.sl * exp_from(part.ml, top)};
+  lanes_sum<W>(x);
+  const double e0 = x[0], e1 = x[1], e2 = x[2], rest = x[3], all = x[3] + x[4];
+  RowStats st{};
+  if (REST) {
+    st.r = e0 > 1.0 ? 0.0 : 1.0 - e0;
+    if (a.k >= a.vocab) {  // with every token listed there is no rest
+      int marked = 0;
+      for (int i = lane; i < mark_words(a.vocab); i += 64) marked += __popc(bits[i]);
+      for (int off = 32; off > 0; off >>= 1) marked += __shfl_xor(marked, off, 64);
+      if (marked == a.vocab) st.r = 0.0;
     }
-    bool first = true;
-    if (st.twice != 0.0)
-      for (int j = 0; j < k && first; ++j) first = tk_id(a, r * a.k + j) != id;
-    if (first) x[3] += s == -INFINITY ? 0.0 : exp((s - top) * a.inv_t);
   }
-  x[4] = sum == 0.0f ? 0.0 : static_cast<double>(sum) * exp((static_cast<double>(m) - top) * a.inv_t);
-  block_sum<5, kTkBlock>(x, part5);
-  if (t != 0) return;
-  st.z = top * a.inv_t + log(x[3] + x[4]);
-  st.zr = top * a.inv_t + log(x[4]);
-  double kl = 0.0;
-  if (a.lse) {
-    st.n = n0;
-    st.r = x[0] > 1.0 ? 0.0 : 1.0 - x[0];
-    int64_t listed = 0;  // with nothing left to hold the rest there is none
-    if (a.k >= a.vocab)
-      for (int64_t i = 0; i <= a.vocab / 32; ++i) listed += __popc(bits[i]);
-    if (listed >= a.vocab) st.r = 0.0;
-    st.p = x[0] + st.r;
-    kl = x[1] - x[2] + x[0] * st.z;
-    if (st.r != 0.0) kl += st.r * (log(st.r) - (st.zr - st.z));
-  } else if (x[0] != 0.0) {
-    st.n = n0 + log(x[0]);
-    st.p = 1.0;
-    kl = (x[1] - x[2]) / x[0] - log(x[0]) + st.z;
+  const double l = log(lane == 0 ? all : lane == 1 ? rest : REST ? st.r : e0);
+  if (!REST && e0 != 0.0) st.p = 1.0;
+  if (REST) st.p = e0 + st.r;
+  st.z = top + __shfl(l, 0, 64);
+  st.zr = top + __shfl(l, 1, 64);
+  st.n = nb + (REST ? 0.0 : __shfl(l, 2, 64));
+  double kl;
+  if (REST) {
+    kl = e1 - e2 + e0 * st.z;
+    if (st.r != 0.0) kl += st.r * (__shfl(l, 2, 64) - (st.zr - st.z));
+  } else {
+    kl = e0 == 0.0 ? 0.0 : (e1 - e2) / e0 - __shfl(l, 2, 64) + st.z;
   }
-  row_kl[r] = kl;
-  *reinterpret_cast<RowStats*>(stats + r * kTkStats) = st;
+  const int marked = all_flags<BLK>(flags);
+  if (!marked) {  // a row without entries adds nothing
+    st = RowStats{};
+    kl = 0.0;
+  }
+  st.twice = marked >> 1;
+  if (lane == 0) {
+    row_kl[r] = kl;
+    *reinterpret_cast<RowStats*>(stats + r * kTkStats) = st;
+  }
 }
 
 constexpr int kTkFinal = 1024;
@@ -249,22 +389,33 @@ __global__ void __launch_bounds__(kTkFinal) top_kl_dot_kernel(const double* __re
   if (threadIdx.x == 0) *dot = static_cast<float>(x[0]);
 }
 
-// What the gradient of a row needs of its sums: coefficients in f32 and Z in two parts, in the logits' units, so that
-// (s - hi) c - lo has the rounding of the difference only.
+// q = exp(s / T - Z) of a row: Z in two parts in the logits' units, hi near s where q is large.  The exponent in base 2,
+// (s - hi) c - lo, rounds in f32 by up to 2^-24 of itself: 1e-6 of q for a token of probability 1e-7, nothing beside
+// bf16's 2^-9; for f32 its whole part is split off and what s - hi and c round is carried along.
+template <int DT>
 struct RowGrad {
-  double factor;  // dL/da scale: g w T / sum w, of the logits: dL/ds
-  float hi, lo, c;
-  __device__ __forceinline__ RowGrad(const TopKlArgs& a, const RowStats& st, double f) : factor(f) {
-    const double z = st.z / a.inv_t;
+  float hi, lo, c, c_lo;
+  __device__ __forceinline__ RowGrad(const TopKlArgs& a, const RowStats& st) {
+    const double z = st.z / a.inv_t, k = a.inv_t * 1.4426950408889634;
     hi = static_cast<float>(z);
-    lo = static_cast<float>((z - static_cast<double>(hi)) * a.inv_t * 1.4426950408889634);
-    c = static_cast<float>(a.inv_t * 1.4426950408889634);
+    lo = static_cast<float>((z - static_cast<double>(hi)) * k);
+    c = static_cast<float>(k);
+    c_lo = static_cast<float>(k - static_cast<double>(c));
   }
-  __device__ __forceinline__ float q(float s) const { return __builtin_amdgcn_exp2f(fmaf(s - hi, c, -lo)); }
+  __device__ __forceinline__ float q(float s) const {
+    const float d = s - hi;
+    if constexpr (DT == SF_DTYPE_BF16) return __builtin_amdgcn_exp2f(fmaf(d, c, -lo));
+    const float back = d - s;  // d + e = s - hi exactly
+    const float e = (s - (d - back)) - (hi + back);
+    const float n = rintf(d * c);
+    const float f = fmaf(d, c, -n) + fmaf(e, c, fmaf(d, c_lo, -lo));
+    // below 2^-126 nothing is left to be exact about, and -inf has no parts
+    return n > -126.0f ? ldexpf(__builtin_amdgcn_exp2f(f), static_cast<int>(n)) : __builtin_amdgcn_exp2f(d * c);
+  }
 };
 
 // Probability that the row's record gives to the id of entry k: p_k, and those of entries with the same id.
-__device__ __forceinline__ double listed_p(const TopKlArgs& a, const RowStats& st, int64_t r, int k, int64_t id) {
+__device__ __forceinline__ double listed_p(const TopKlArgs& a, const RowStats& st, int64_t r, int k, int id) {
   if (st.twice == 0.0) return exp(load_as_f32(a.values, r * a.k + k, a.vdt) * a.inv_t - st.n);
   double p = 0.0;
   for (int j = 0; j < a.k; ++j)
@@ -272,112 +423,151 @@ __device__ __forceinline__ double listed_p(const TopKlArgs& a, const RowStats& s
   return p;
 }
 
-template <int DT>
-__global__ void __launch_bounds__(kTkBlock) top_kl_backward_kernel(TopKlArgs a, const double* __restrict__ stats,
+template <int DT, int BLK>
+__global__ void __launch_bounds__(BLK) top_kl_backward_kernel(TopKlArgs a, const double* __restrict__ stats,
                                                                    const double* __restrict__ norm,
                                                                    const float* __restrict__ grad_out,
                                                                    void* __restrict__ gs) {
-  const int64_t r = blockIdx.x, out = r * a.vocab;
+  // from the last row on: the forward read these last, and the caches hold them
+  const int64_t r = gridDim.x - 1 - blockIdx.x;
   const int t = threadIdx.x;
+  void* out = const_cast<void*>(row_at<DT>(gs, r * a.vocab));
   const double w = a.weights ? static_cast<double>(a.weights[r]) : 1.0, f = *norm * w * static_cast<double>(*grad_out);
   RowStats st{};
   if (w != 0.0) st = *reinterpret_cast<const RowStats*>(stats + r * kTkStats);
   if (f == 0.0 || st.p == 0.0) {
     const float zero[8] = {};
-    for (int64_t i = t * 8; i < a.vocab; i += kTkBlock * 8)
-      tk_store8<DT>(gs, out + i, a.vocab - i < 8 ? static_cast<int>(a.vocab - i) : 8, zero);
+    for (int i = t * 8; i < a.vocab; i += BLK * 8) tk_store8<DT>(out, i, a.vocab - i < 8 ? a.vocab - i : 8, zero);
     return;
   }
-  const int64_t base = (r / a.inner) * a.s0 + (r % a.inner) * a.s1;
-  const RowGrad g(a, st, f);
+  const RowGrad<DT> g(a, st);
   const float coef = static_cast<float>(f * (st.p - (st.r != 0.0 ? st.r * exp(st.z - st.zr) : 0.0)));
-  for (int64_t i = t * 8; i < a.vocab; i += kTkBlock * 8) {
-    const int n = a.vocab - i < 8 ? static_cast<int>(a.vocab - i) : 8;
-    float v[8];
-    tk_load8<DT>(a.s, base + i, n, v);
+  const void* rows[1] = {row_at<DT>(a.s, (r / a.inner) * a.s0 + (r % a.inner) * a.s1)};
+  const Cut cut = Cut::of<DT, BLK>(rows[0], a.vocab);
+  // the listed tokens' own gradient, formed while the row is on its way and written when the row is
+  const auto listed = [&](int k, int id) {
+    const double q = exp(load_as_f32(rows[0], id, DT) * a.inv_t - st.z);
+    return static_cast<float>(f * (st.p * q - listed_p(a, st, r, k, id)));
+  };
+  int id0 = -1;
+  float g0 = 0.0f;
+  const auto first = [&] {
+    if (t < a.k) id0 = tk_id(a, r * a.k + t);
+    if (id0 >= 0) g0 = listed(t, id0);
+  };
+  tk_stream<DT, BLK, kTkBackwardU>(rows, cut, 0, first, [&](int i, int n, float (&x)[1][8]) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = coef * g.q(v[k]);
-    tk_store8<DT>(gs, out + i, n, v);
-  }
-  __syncthreads();  // the listed tokens are written again, with their own gradient
-  for (int k = t; k < a.k; k += kTkBlock) {
-    const int64_t id = tk_id(a, r * a.k + k);
-    if (id < 0) continue;
-    const double q = exp(load_as_f32(a.s, base + id, DT) * a.inv_t - st.z);
-    store_from_f32(gs, out + id, DT, static_cast<float>(f * (st.p * q - listed_p(a, st, r, k, id))));
+    for (int k = 0; k < 8; ++k) x[0][k] = coef * g.q(x[0][k]);
+    tk_store8<DT>(out, i, n, x[0]);
+  });
+  __syncthreads();
+  if (id0 >= 0) store_from_f32(out, id0, DT, g0);
+  for (int k = t + BLK; k < a.k; k += BLK) {
+    const int id = tk_id(a, r * a.k + k);
+    if (id >= 0) store_from_f32(out, id, DT, listed(k, id));
   }
 }
 
 // Along u (rows contiguous): h_j, and the row's u . dL/ds at an upstream gradient of 1.
 template <int DT>
-__global__ void __launch_bounds__(kTkBlock) top_kl_second_kernel(TopKlArgs a, const double* __restrict__ stats,
-                                                                 const double* __restrict__ norm,
-                                                                 const float* __restrict__ grad_out,
-                                                                 const void* __restrict__ u, void* __restrict__ hs,
-                                                                 double* __restrict__ row_dot) {
+__global__ void __launch_bounds__(kTkSecond) top_kl_second_kernel(TopKlArgs a, const double* __restrict__ stats,
+                                                                  const double* __restrict__ norm,
+                                                                  const float* __restrict__ grad_out,
+                                                                  const void* __restrict__ u, void* __restrict__ hs,
+                                                                  double* __restrict__ row_dot) {
+  constexpr int BLK = kTkSecond, H = DT == SF_DTYPE_BF16 ? 6 : 3;
   extern __shared__ uint32_t bits[];
-  __shared__ double part[kTkBlock / 64][3];
-  const int64_t r = blockIdx.x, out = r * a.vocab;
+  __shared__ double part[BLK / 64][3];
+  __shared__ int flags[BLK / 64];
+  const int64_t r = gridDim.x - 1 - blockIdx.x;
   const int t = threadIdx.x;
+  void* out = const_cast<void*>(row_at<DT>(hs, r * a.vocab));
   const double share = *norm * (a.weights ? static_cast<double>(a.weights[r]) : 1.0);
   RowStats st{};
   if (share != 0.0) st = *reinterpret_cast<const RowStats*>(stats + r * kTkStats);
   if (share == 0.0 || st.p == 0.0) {
     const float zero[8] = {};
-    for (int64_t i = t * 8; i < a.vocab; i += kTkBlock * 8)
-      tk_store8<DT>(hs, out + i, a.vocab - i < 8 ? static_cast<int>(a.vocab - i) : 8, zero);
+    for (int i = t * 8; i < a.vocab; i += BLK * 8) tk_store8<DT>(out, i, a.vocab - i < 8 ? a.vocab - i : 8, zero);
     if (t == 0) row_dot[r] = 0.0;
     return;
   }
   const double f = share * static_cast<double>(*grad_out) * a.inv_t;
-  const int64_t base = (r / a.inner) * a.s0 + (r % a.inner) * a.s1;
-  const RowGrad g(a, st, f);
-  if (t == 0) bits[a.vocab / 32 + 1] = 0;
-  mark_listed<kTkBlock>(a, r, bits);
+  const RowGrad<DT> g(a, st);
+  const void* rows[2] = {row_at<DT>(a.s, (r / a.inner) * a.s0 + (r % a.inner) * a.s1), row_at<DT>(u, r * a.vocab)};
+  const Cut cut = Cut::of<DT, BLK>(rows[0], a.vocab);
+  Raw8<DT> raw[H][2];  // the thread's first pieces stay in registers
+#pragma unroll
+  for (int p = 0; p < H; ++p)
+    if (p < cut.n) {
+      raw[p][0].load(rows[0], cut.at<BLK>(p));
+      raw[p][1].load(rows[1], cut.at<BLK>(p));
+    }
+  for (int i = t; i < mark_words(a.vocab); i += BLK) bits[i] = 0;
+  __syncthreads();
+  mark_listed<BLK>(a, r, cut, bits, flags);
+  __syncthreads();
+  // the listed tokens, while the row is on its way
+  double x[3] = {0.0, 0.0, 0.0};  // u . q unlisted, listed; u . p
+  int id0 = -1;
+  double q0 = 0.0, w0 = 0.0;
+  for (int k = t; k < a.k; k += BLK) {
+    const int id = tk_id(a, r * a.k + k);
+    if (id < 0) continue;
+    const double q = exp(load_as_f32(rows[0], id, DT) * a.inv_t - st.z), w = load_as_f32(rows[1], id, DT);
+    if (k == t) id0 = id, q0 = q, w0 = w;
+    x[2] += w * exp(load_as_f32(a.values, r * a.k + k, a.vdt) * a.inv_t - st.n);
+    if (st.twice == 0.0 || first_of_id(a, r, k, id)) x[1] += w * q;
+  }
   float rest = 0.0f;
-  for (int64_t i = t * 8; i < a.vocab; i += kTkBlock * 8) {
-    const int n = a.vocab - i < 8 ? static_cast<int>(a.vocab - i) : 8;
-    float v[8], w[8];
-    tk_load8<DT>(a.s, base + i, n, v);
-    tk_load8<DT>(u, out + i, n, w);
-    const uint32_t skip = marks8(bits, i);
+  const auto dot = [&](int i, int m, float (&x)[2][8]) {
+    const uint32_t skip = marks8(bits, cut, i);
 #pragma unroll
     for (int k = 0; k < 8; ++k)
-      if (k < n && !(skip >> k & 1)) rest = fmaf(w[k], g.q(v[k]), rest);
-  }
-  double x[3] = {static_cast<double>(rest), 0.0, 0.0};  // u . q unlisted, listed; u . p
-  for (int k = t; k < a.k; k += kTkBlock) {
-    const int64_t id = tk_id(a, r * a.k + k);
-    if (id < 0) continue;
-    const double w = load_as_f32(u, out + id, DT);
-    x[2] += w * exp(load_as_f32(a.values, r * a.k + k, a.vdt) * a.inv_t - st.n);
-    bool first = true;
-    if (st.twice != 0.0)
-      for (int j = 0; j < k && first; ++j) first = tk_id(a, r * a.k + j) != id;
-    if (first) x[1] += w * exp(load_as_f32(a.s, base + id, DT) * a.inv_t - st.z);
-  }
-  block_sum<3, kTkBlock>(x, part);
+      if (k < m && !(skip >> k & 1)) rest = fmaf(x[1][k], g.q(x[0][k]), rest);
+  };
+  const auto kept = [&](auto&& use) {
+#pragma unroll
+    for (int p = 0; p < H; ++p)
+      if (p < cut.n) {
+        float x[2][8];
+        raw[p][0].get(x[0]);
+        raw[p][1].get(x[1]);
+        use(cut.at<BLK>(p), 8, x);
+      }
+  };
+  kept(dot);
+  tk_stream<DT, BLK, 1>(rows, cut, H, [] {}, dot);
+  x[0] = static_cast<double>(rest);
+  block_sum<3, BLK>(x, part);
   const double kappa = st.r != 0.0 ? exp(st.z - st.zr) : 0.0, uq = x[0] + x[1];
   if (t == 0) row_dot[r] = share * (st.p * uq - x[2] - st.r * kappa * x[0]);
   const float A = static_cast<float>(f * (st.p - st.r * kappa));
   const float B = static_cast<float>(f * (st.p * uq - st.r * kappa * kappa * x[0]));
-  for (int64_t i = t * 8; i < a.vocab; i += kTkBlock * 8) {
-    const int n = a.vocab - i < 8 ? static_cast<int>(a.vocab - i) : 8;
-    float v[8], w[8];
-    tk_load8<DT>(a.s, base + i, n, v);
-    tk_load8<DT>(u, out + i, n, w);
+  const auto write = [&](int i, int m, float (&x)[2][8]) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = g.q(v[k]) * fmaf(A, w[k], -B);
-    tk_store8<DT>(hs, out + i, n, v);
-  }
+    for (int k = 0; k < 8; ++k) x[0][k] = g.q(x[0][k]) * fmaf(A, x[1][k], -B);
+    tk_store8<DT>(out, i, m, x[0]);
+  };
+  kept(write);
+  tk_stream<DT, BLK, 1>(rows, cut, H, [] {}, write);
   __syncthreads();
-  for (int k = t; k < a.k; k += kTkBlock) {
-    const int64_t id = tk_id(a, r * a.k + k);
+  if (id0 >= 0) store_from_f32(out, id0, DT, static_cast<float>(f * st.p * q0 * (w0 - uq)));
+  for (int k = t + BLK; k < a.k; k += BLK) {
+    const int id = tk_id(a, r * a.k + k);
     if (id < 0) continue;
-    const double q = exp(load_as_f32(a.s, base + id, DT) * a.inv_t - st.z);
-    const double w = load_as_f32(u, out + id, DT);
-    store_from_f32(hs, out + id, DT, static_cast<float>(f * st.p * q * (w - uq)));
+    const double q = exp(load_as_f32(rows[0], id, DT) * a.inv_t - st.z), w = load_as_f32(rows[1], id, DT);
+    store_from_f32(out, id, DT, static_cast<float>(f * st.p * q * (w - uq)));
   }
+}
+
+constexpr int64_t kTkFewRows = 512;  // fewer rows than this take more threads each
+
+template <typename F>
+void tk_dispatch(int dtype, F&& launch) {
+  if (dtype == SF_DTYPE_F32)
+    launch(std::integral_constant<int, SF_DTYPE_F32>{});
+  else
+    launch(std::integral_constant<int, SF_DTYPE_BF16>{});
 }
 
 int top_kl_args(const sf_top_kl_desc* desc, const char* what, TopKlArgs& a) {
@@ -397,7 +587,7 @@ int top_kl_args(const sf_top_kl_desc* desc, const char* what, TopKlArgs& a) {
   SF_CHECK_ARG(d.temperature > 0.0f && d.temperature <= 3.0e38f, "%s: temperature %g", what, d.temperature);
   a.s = d.logits, a.s0 = d.outer_stride, a.s1 = d.row_stride, a.inner = d.inner;
   a.values = d.values, a.ids = d.ids, a.lse = d.lse, a.weights = d.weights;
-  a.vocab = d.vocab, a.k = static_cast<int>(d.k), a.vdt = d.value_dtype, a.id_bytes = d.id_bytes;
+  a.vocab = static_cast<int>(d.vocab), a.k = static_cast<int>(d.k), a.vdt = d.value_dtype, a.id_bytes = d.id_bytes;
   a.inv_t = 1.0 / static_cast<double>(d.temperature);
   return SF_OK;
 }
@@ -423,12 +613,22 @@ extern "C" int sf_top_kl_forward(const sf_top_kl_desc* desc, float* loss, void* 
                "sf_top_kl_forward: workspace too small");
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(desc->rows));
-  const size_t lds = (static_cast<size_t>(a.vocab) / 32 + 2) * 4;
+  const size_t lds = static_cast<size_t>(mark_words(a.vocab)) * 4;
   double* row_kl = static_cast<double*>(workspace);
-  if (desc->dtype == SF_DTYPE_F32)
-    top_kl_kernel<SF_DTYPE_F32><<<grid, kTkBlock, lds, st>>>(a, desc->stats, row_kl);
-  else
-    top_kl_kernel<SF_DTYPE_BF16><<<grid, kTkBlock, lds, st>>>(a, desc->stats, row_kl);
+  tk_dispatch(desc->dtype, [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    auto with = [&](auto blk) {
+      constexpr int BLK = decltype(blk)::value;
+      if (a.lse)
+        top_kl_kernel<DT, BLK, true><<<grid, BLK, lds, st>>>(a, desc->stats, row_kl);
+      else
+        top_kl_kernel<DT, BLK, false><<<grid, BLK, lds, st>>>(a, desc->stats, row_kl);
+    };
+    if (desc->rows < kTkFewRows)
+      with(std::integral_constant<int, 1024>{});
+    else
+      with(std::integral_constant<int, 256>{});
+  });
   top_kl_final_kernel<<<1, kTkFinal, 0, st>>>(row_kl, a.weights, desc->rows, desc->temperature, loss, desc->norm);
   return launch_status("sf_top_kl_forward");
 }
@@ -439,10 +639,13 @@ extern "C" int sf_top_kl_backward(const sf_top_kl_desc* desc, const float* grad_
   SF_CHECK_ARG(grad_out && grad_logits, "sf_top_kl_backward: null pointer");
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(desc->rows));
-  if (desc->dtype == SF_DTYPE_F32)
-    top_kl_backward_kernel<SF_DTYPE_F32><<<grid, kTkBlock, 0, st>>>(a, desc->stats, desc->norm, grad_out, grad_logits);
-  else
-    top_kl_backward_kernel<SF_DTYPE_BF16><<<grid, kTkBlock, 0, st>>>(a, desc->stats, desc->norm, grad_out, grad_logits);
+  tk_dispatch(desc->dtype, [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    if (desc->rows < kTkFewRows)
+      top_kl_backward_kernel<DT, 1024><<<grid, 1024, 0, st>>>(a, desc->stats, desc->norm, grad_out, grad_logits);
+    else
+      top_kl_backward_kernel<DT, 512><<<grid, 512, 0, st>>>(a, desc->stats, desc->norm, grad_out, grad_logits);
+  });
   return launch_status("sf_top_kl_backward");
 }
 
@@ -457,13 +660,12 @@ extern "C" int sf_top_kl_double_backward(const sf_top_kl_desc* desc, const float
   double* row_dot = static_cast<double*>(workspace);
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(desc->rows));
-  const size_t lds = (static_cast<size_t>(a.vocab) / 32 + 2) * 4;
-  if (desc->dtype == SF_DTYPE_F32)
-    top_kl_second_kernel<SF_DTYPE_F32><<<grid, kTkBlock, lds, st>>>(a, desc->stats, desc->norm, grad_out, grad_grad,
-                                                                    grad2_logits, row_dot);
-  else
-    top_kl_second_kernel<SF_DTYPE_BF16><<<grid, kTkBlock, lds, st>>>(a, desc->stats, desc->norm, grad_out, grad_grad,
-                                                                     grad2_logits, row_dot);
+  const size_t lds = static_cast<size_t>(mark_words(a.vocab)) * 4;
+  tk_dispatch(desc->dtype, [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    top_kl_second_kernel<DT><<<grid, kTkSecond, lds, st>>>(a, desc->stats, desc->norm, grad_out, grad_grad,
+                                                           grad2_logits, row_dot);
+  });
   if (dot) top_kl_dot_kernel<<<1, kTkFinal, 0, st>>>(row_dot, desc->rows, dot);
   return launch_status("sf_top_kl_double_backward");
 }

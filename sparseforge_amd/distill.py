@@ -33,7 +33,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib as L
 from . import profiling as _prof
-from .linear import apply_in_backward
+from .linear import apply_in_backward, transforms_active
 
 
 class _KL(torch.autograd.Function):
@@ -157,68 +157,72 @@ def top_logits(logits: torch.Tensor, k: int, temperature=2) -> TopLogits:
     lse = torch.empty(lead, dtype=torch.float32, device=dev)
     desc = L.TOP_LOGITS_DESC.pack(logits.data_ptr(), outer, step, inner, rows, V, k, values.data_ptr(), ids.data_ptr(),
                                   lse.data_ptr(), temperature, dt)
-    with torch.cuda.device_of(logits), _prof.region("sf_top_logits", rows * V * logits.element_size(), "B", dev):
+    with L.on(dev), _prof.region("sf_top_logits", rows * V * logits.element_size(), "B", dev):
         L.check(L.lib().sf_top_logits(desc, L.stream(dev)), "sf_top_logits")
     return TopLogits(values, ids, lse, temperature)
 
 
-def _top_kl_desc(s, values, ids, lse, weights, stats, norm, temperature):
+def _top_kl_desc(s, values, ids, lse, weights, state, temperature):
+    """The descriptor, and s or the copy of it that has to live until the call."""
     s, outer, step, inner, rows = L.rows_of(s)
-    desc = L.TOP_KL_DESC.pack(s.data_ptr(), outer, step, inner, rows, s.shape[-1], values.data_ptr(), ids.data_ptr(),
-                              values.shape[-1], L.ptr(lse) or 0, L.ptr(weights) or 0, stats.data_ptr(),
-                              norm.data_ptr(), temperature, L.dtype_code(s), L.dtype_code(values), ids.element_size())
-    return desc, s  # s, which may be a copy, has to live until the call
+    at = state.data_ptr()  # the norm, then the rows' sums
+    return L.TOP_KL_DESC.pack(s.data_ptr(), outer, step, inner, rows, s.shape[-1], values.data_ptr(), ids.data_ptr(),
+                              values.shape[-1], L.ptr(lse) or 0, L.ptr(weights) or 0, at + 8, at, temperature,
+                              L.dtype_code(s), L.dtype_code(values), ids.element_size()), s
+
+
+def _top_kl_forward(s, values, ids, lse, weights, temperature: float):
+    dev, lib, rows = s.device, L.lib(), s.shape[:-1].numel()
+    loss = torch.empty((), dtype=torch.float32, device=dev)
+    state = torch.empty(1 + int(lib.sf_top_kl_stats_size(rows)) // 8, dtype=torch.float64, device=dev)
+    ws = torch.empty(int(lib.sf_top_kl_workspace_size(rows)), dtype=torch.uint8, device=dev)
+    desc, keep = _top_kl_desc(s, values, ids, lse, weights, state, temperature)
+    with L.on(dev), _prof.region("sf_top_kl_forward", s.numel() * s.element_size(), "B", dev):
+        L.check(lib.sf_top_kl_forward(desc, loss.data_ptr(), ws.data_ptr(), ws.numel(), L.stream(dev)),
+                "sf_top_kl_forward")
+    return loss, state
 
 
 class _TopKL(torch.autograd.Function):
     @staticmethod
     def forward(ctx, s, values, ids, lse, weights, temperature: float):
-        dev, rows, lib = s.device, s.shape[:-1].numel(), L.lib()
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        stats = torch.empty(int(lib.sf_top_kl_stats_size(rows)) // 8, dtype=torch.float64, device=dev)
-        norm = torch.empty(1, dtype=torch.float64, device=dev)
-        ws = torch.empty(int(lib.sf_top_kl_workspace_size(rows)), dtype=torch.uint8, device=dev)
-        desc, keep = _top_kl_desc(s, values, ids, lse, weights, stats, norm, temperature)
-        with torch.cuda.device_of(s), _prof.region("sf_top_kl_forward", s.numel() * s.element_size(), "B", dev):
-            L.check(lib.sf_top_kl_forward(desc, loss.data_ptr(), ws.data_ptr(), ws.numel(), L.stream(dev)),
-                    "sf_top_kl_forward")
-        ctx.save_for_backward(s, values, ids, lse, weights, stats, norm)
+        loss, state = _top_kl_forward(s, values, ids, lse, weights, temperature)
+        ctx.save_for_backward(s, values, ids, lse, weights, state)
         ctx.temperature = temperature
         return loss
 
     @staticmethod
     def backward(ctx, g):
         # a Function of its own, as the whole KL's gradient: the Hutchinson probe differentiates it
-        return (apply_in_backward(_TopKLGrad, *ctx.saved_tensors, g, ctx.temperature), None, None, None, None, None)
+        return apply_in_backward(_TopKLGrad, *ctx.saved_tensors, g, ctx.temperature), None, None, None, None, None
 
 
 class _TopKLGrad(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, s, values, ids, lse, weights, stats, norm, g, temperature: float):
+    def forward(ctx, s, values, ids, lse, weights, state, g, temperature: float):
         dev = s.device
         gs = torch.empty_like(s, memory_format=torch.contiguous_format)
-        desc, keep = _top_kl_desc(s, values, ids, lse, weights, stats, norm, temperature)
-        with torch.cuda.device_of(s), _prof.region("sf_top_kl_backward", 2 * s.numel() * s.element_size(), "B", dev):
+        desc, keep = _top_kl_desc(s, values, ids, lse, weights, state, temperature)
+        with L.on(dev), _prof.region("sf_top_kl_backward", 2 * s.numel() * s.element_size(), "B", dev):
             L.check(L.lib().sf_top_kl_backward(desc, g.data_ptr(), gs.data_ptr(), L.stream(dev)), "sf_top_kl_backward")
-        ctx.save_for_backward(s, values, ids, lse, weights, stats, norm, g)
+        ctx.save_for_backward(s, values, ids, lse, weights, state, g)
         ctx.temperature = temperature
         return gs
 
     @staticmethod
     @once_differentiable
     def backward(ctx, u):
-        s, values, ids, lse, weights, stats, norm, g = ctx.saved_tensors
+        s, values, ids, lse, weights, state, g = ctx.saved_tensors
         dev, lib, u = s.device, L.lib(), u.contiguous()
         hs = torch.empty_like(s, memory_format=torch.contiguous_format)
-        dot = torch.empty((), dtype=torch.float32, device=dev) if ctx.needs_input_grad[7] else None
+        dot = torch.empty((), dtype=torch.float32, device=dev) if ctx.needs_input_grad[6] else None
         ws = torch.empty(int(lib.sf_top_kl_workspace_size(s.shape[:-1].numel())), dtype=torch.uint8, device=dev)
-        desc, keep = _top_kl_desc(s, values, ids, lse, weights, stats, norm, ctx.temperature)
-        with (torch.cuda.device_of(s),
-              _prof.region("sf_top_kl_double_backward", 3 * s.numel() * s.element_size(), "B", dev)):
+        desc, keep = _top_kl_desc(s, values, ids, lse, weights, state, ctx.temperature)
+        with L.on(dev), _prof.region("sf_top_kl_double_backward", 3 * s.numel() * s.element_size(), "B", dev):
             L.check(lib.sf_top_kl_double_backward(desc, g.data_ptr(), u.data_ptr(), hs.data_ptr(), L.ptr(dot),
                                                   ws.data_ptr(), ws.numel(), L.stream(dev)),
                     "sf_top_kl_double_backward")
-        return hs, None, None, None, None, None, None, dot, None
+        return hs, None, None, None, None, None, dot, None
 
 
 def top_kl_loss(student_logits: torch.Tensor, teacher: TopLogits, temperature=2, *,
@@ -249,6 +253,15 @@ def top_kl_loss(student_logits: torch.Tensor, teacher: TopLogits, temperature=2,
         raise ValueError(f"top_kl_loss: the record's log-sum-exp is at temperature {at}, the loss at {temperature}")
     if lead.numel() == 0:
         return student_logits.sum(dtype=torch.float32)
-    values, ids, lse, weights = (t.detach().contiguous() if t is not None else None
-                                 for t in (values, ids, lse, weights))
-    return _TopKL.apply(student_logits, values, ids, lse, weights, temperature)
+    args = (student_logits, _given(values), _given(ids), _given(lse), _given(weights), temperature)
+    if not (student_logits.requires_grad and torch.is_grad_enabled()) and not transforms_active():
+        return _top_kl_forward(*args)[0]
+    return _TopKL.apply(*args)
+
+
+def _given(t: torch.Tensor | None) -> torch.Tensor | None:
+    """An input that takes no gradient, contiguous."""
+    if t is None:
+        return None
+    t = t.detach() if t.requires_grad else t
+    return t if t.is_contiguous() else t.contiguous()

@@ -136,7 +136,7 @@ def sample_logits(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.
     desc = L.SAMPLE_DESC.pack(logits.data_ptr(), logits.stride(0) if B > 1 else V, B, V, uniform.data_ptr(),
                               ids.data_ptr(), L.ptr(logp) or 0, temp[0], k[0], p[0], least[0], temp[1], p[1], least[1],
                               k[1], dt)
-    with torch.cuda.device_of(logits), _prof.region("sf_sample_logits", B * V * logits.element_size(), "B", dev):
+    with L.on(dev), _prof.region("sf_sample_logits", B * V * logits.element_size(), "B", dev):
         L.check(L.lib().sf_sample_logits(desc, L.stream(dev)), "sf_sample_logits")
     return (ids, logp) if logprobs else ids
 
