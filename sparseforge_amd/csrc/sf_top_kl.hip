@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(BLK) top_kl_kernel(TopKlArgs a, double* __rest
   const void* rows[1] = {row_at<DT>(a.s, (r / a.inner) * a.s0 + (r % a.inner) * a.s1)};
   const Cut cut = Cut::of<DT, BLK>(rows[0], a.vocab);
   const float c = static_cast<float>(a.inv_t * 1.4426950408889634);
-  float m = kTkLow, sum = 0.0f;
+  float m = kTkLow, sum = 0.0f, lost = 0.0f;
   WavePart part{REST ? static_cast<double>(a.lse[r]) : -INFINITY, 0.0, 0.0, 0.0, -INFINITY, 0.0, 0.0f, 0.0f};
   // The row's first loads are on their way while the listed tokens are marked and summed: the latter by the waves that
   // have some, each with its own maxima, so that no wave waits for another before the row's end.
@@ -295,11 +295,17 @@ __global__ void __launch_bounds__(BLK) top_kl_kernel(TopKlArgs a, double* __rest
       top = fmaxf(top, v[k]);
     }
     if (top > m) {
-      sum *= __builtin_amdgcn_exp2f((m - top) * c);
+      const float f = __builtin_amdgcn_exp2f((m - top) * c);
+      sum *= f;
+      lost *= f;
       m = top;
     }
 #pragma unroll
-    for (int k = 0; k < 8; ++k) sum += __builtin_amdgcn_exp2f((v[k] - m) * c);
+    for (int k = 0; k < 8; ++k) v[k] = __builtin_amdgcn_exp2f((v[k] - m) * c);
+    // hundreds of small terms beside a large one: what an addition rounds off is carried along
+    const float add = (((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]))) - lost, upto = sum + add;
+    lost = (upto - sum) - add;
+    sum = upto;
   });
   part.m = m;
   for (int off = 32; off > 0; off >>= 1) part.m = fmaxf(part.m, __shfl_xor(part.m, off, 64));
