@@ -438,6 +438,7 @@ int sf_kl_backward(const void* student, const void* teacher, int dtype, int64_t 
 /* ---- the top of a row of logits (no counterpart in the reference) ---- */
 
 #define SF_TOP_MAX_VOCAB 262144 /* longest rows */
+#define SF_TOP_MAX_ROWS 4194304 /* there are fewer rows than this */
 #define SF_TOP_MAX_K 1024       /* most entries that sf_top_logits gives */
 
 /*

@@ -13,7 +13,7 @@
 // One workgroup per row streams it once.  Listed tokens (at most a few hundred) are gathered and handled in f64.
 #include <type_traits>
 
-#include "sf_common.hpp"
+#include "sf_top.hpp"
 
 namespace sf {
 namespace {
@@ -47,25 +47,6 @@ __device__ __forceinline__ int tk_id(const TopKlArgs& a, int64_t at) {
   const int64_t id = a.id_bytes == 8 ? static_cast<const int64_t*>(a.ids)[at] : static_cast<const int32_t*>(a.ids)[at];
   return id >= 0 && id < a.vocab ? static_cast<int>(id) : -1;
 }
-
-// 8 elements from any element's address, as they are stored.
-template <int DT>
-struct Raw8 {
-  uint32_t w[DT == SF_DTYPE_BF16 ? 4 : 8];
-  __device__ __forceinline__ void load(const void* row, int i) {
-    __builtin_memcpy(w, static_cast<const char*>(row) + static_cast<int64_t>(i) * (DT == SF_DTYPE_BF16 ? 2 : 4),
-                     sizeof(w));
-  }
-  __device__ __forceinline__ void get(float (&v)[8]) const {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      if constexpr (DT == SF_DTYPE_BF16)
-        v[k] = __uint_as_float(k & 1 ? w[k / 2] & 0xffff0000u : w[k / 2] << 16);
-      else
-        v[k] = __uint_as_float(w[k]);
-    }
-  }
-};
 
 template <int DT>
 __device__ __forceinline__ void tk_store8(void* row, int i, int n, const float (&v)[8]) {
@@ -582,8 +563,9 @@ int top_kl_args(const sf_top_kl_desc* desc, const char* what, TopKlArgs& a) {
   SF_CHECK_ARG((d.dtype == SF_DTYPE_F32 || d.dtype == SF_DTYPE_BF16) &&
                    (d.value_dtype == SF_DTYPE_F32 || d.value_dtype == SF_DTYPE_BF16),
                "%s: unknown dtype %d / %d", what, d.dtype, d.value_dtype);
-  SF_CHECK_ARG(d.rows > 0 && d.rows < (1ll << 31) && d.vocab > 0 && d.vocab <= SF_TOP_MAX_VOCAB,
-               "%s: %lld rows of %lld (at most %d)", what, (long long)d.rows, (long long)d.vocab, SF_TOP_MAX_VOCAB);
+  SF_CHECK_ARG(d.rows > 0 && d.rows < SF_TOP_MAX_ROWS && d.vocab > 0 && d.vocab <= SF_TOP_MAX_VOCAB,
+               "%s: %lld rows (fewer than %d) of %lld (at most %d)", what, (long long)d.rows, SF_TOP_MAX_ROWS,
+               (long long)d.vocab, SF_TOP_MAX_VOCAB);
   SF_CHECK_ARG(d.inner > 0 && d.rows % d.inner == 0 && d.outer_stride >= 0 && d.row_stride >= 0,
                "%s: rows in groups of %lld, strides %lld, %lld", what, (long long)d.inner, (long long)d.outer_stride,
                (long long)d.row_stride);

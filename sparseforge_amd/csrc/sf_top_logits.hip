@@ -1,100 +1,106 @@
 // The k largest logits of every row in falling order (equal ones by rising id), their ids, and the row's log-sum-exp at a
 // temperature: what is kept of a teacher for distillation, or answered as log-probabilities.
 //
-// One workgroup per row: it finds the k-th largest key, gathers what lies above it and the first of its equals, and sorts
-// these in LDS.
+// One workgroup per row, which it holds in registers if it fits: a pass for the maxima of the threads' parts, from which a
+// bound follows above which the k largest and few others lie (gather_top); a pass that gathers these in LDS and sums the
+// exponentials; then each candidate counts those before it, which is its place in the output.
+#include <type_traits>
+
 #include "sf_top.hpp"
 
 namespace sf {
 namespace {
 
-constexpr int kTlBlock = 1024;
-constexpr int kTlTiles = SF_TOP_MAX_VOCAB / (kTlBlock * 8);
-
 struct TopLogitsArgs {
   const void* x;
   int64_t s0, s1, inner;
-  int vocab, k, dt;
+  int vocab, k;
   double inv_t;
   void* values;
   int32_t* ids;
   float* lse;
 };
 
+// Entry `rank` of row r.
 template <int DT>
-__global__ void __launch_bounds__(kTlBlock) top_logits_kernel(TopLogitsArgs a) {
-  __shared__ u64 mass[256];
-  __shared__ uint32_t count[256];
-  __shared__ u64 sums[kTlTiles * (kTlBlock / 64)];
-  __shared__ u64 shared[3];
-  __shared__ float part[kTlBlock / 64];
-  __shared__ double partd[kTlBlock / 64];
-  __shared__ u64 found[SF_TOP_MAX_K];
-  __shared__ int at;
-  const int64_t r = blockIdx.x, base = (r / a.inner) * a.s0 + (r % a.inner) * a.s1;
+__device__ __forceinline__ void put(const TopLogitsArgs& a, const void* row, int64_t r, int rank, int id) {
+  a.ids[r * a.k + rank] = id;
+  if constexpr (DT == SF_DTYPE_F32)
+    static_cast<float*>(a.values)[r * a.k + rank] = static_cast<const float*>(row)[id];
+  else
+    static_cast<uint16_t*>(a.values)[r * a.k + rank] = static_cast<const uint16_t*>(row)[id];
+}
+
+// Any row: the k-th largest key by its bits, then the elements above it and the first of its equals.
+template <int DT, int BLK>
+__device__ __forceinline__ void top_of_any(const TopLogitsArgs& a, const void* row, int64_t r, AnyShared& any, TopShared& sh) {
   const int t = threadIdx.x, V = a.vocab;
-  float m = -INFINITY;
-  top_scan<DT, kTlBlock>(a.x, base, V, [&](int, int, int n, const float (&v)[8]) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (k < n) m = fmaxf(m, v[k]);
-  });
-  m = block_max_f<kTlBlock>(m, part);
-  const float c = static_cast<float>(a.inv_t * 1.4426950408889634);
-  const float ref = m == -INFINITY || m == INFINITY ? 0.0f : m;
-  float sum = 0.0f;
-  top_scan<DT, kTlBlock>(a.x, base, V, [&](int, int, int n, const float (&v)[8]) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (k < n) sum += __builtin_amdgcn_exp2f((v[k] - ref) * c);
-  });
-  double total = sum;
-  for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
-  if ((t & 63) == 0) partd[t >> 6] = total;
-  if (t == 0) at = 0;
-  const Border border = radix_border<DT, kTlBlock>(a.x, base, V, false, a.k, [](float) { return 0ull; }, mass, count,
-                                                   shared);
-  const int last = locate<DT, kTlBlock, kTlTiles>(
-                       a.x, base, V, [&](float x, int) { return static_cast<u64>(top_key<DT>(x) == border.key); },
-                       [&](u64) { return border.keep - 1; }, sums, shared)
+  const Border border = radix_border<DT, BLK>(row, V, false, a.k, [](float) { return 0ull; }, any);
+  const int last = locate<DT, BLK>(
+                       row, V, [&](float x, int) { return static_cast<u64>(top_key<DT>(x) == border.key); },
+                       [&](u64) { return border.keep - 1; }, any)
                        .id;
-  int size = 1;
-  while (size < a.k) size *= 2;
-  for (int i = t; i < size; i += kTlBlock) found[i] = 0;
+  if (t == 0) sh.n = 0;
   __syncthreads();
-  top_scan<DT, kTlBlock>(a.x, base, V, [&](int, int i, int n, const float (&v)[8]) {
+  top_scan<DT, BLK>(row, V, [&](int, int i, int n, const float (&v)[8]) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const uint32_t key = top_key<DT>(v[k]);
       if (k < n && (key > border.key || (key == border.key && i + k <= last)))
-        found[atomicAdd(&at, 1)] = static_cast<u64>(key) << 32 | static_cast<uint32_t>(~(i + k));
+        sh.found[atomicAdd(&sh.n, 1)] = candidate(v[k], i + k);
     }
   });
+  if (t == 0 && a.k % 2) sh.found[a.k] = 0;
   __syncthreads();
-  // bitonic sort, falling
-  for (int step = 2; step <= size; step *= 2)
-    for (int d = step / 2; d > 0; d /= 2) {
-      for (int i = t; i < size; i += kTlBlock) {
-        const int j = i ^ d;
-        if (j > i && (found[i] < found[j]) == ((i & step) == 0)) {
-          const u64 x = found[i];
-          found[i] = found[j];
-          found[j] = x;
-        }
-      }
-      __syncthreads();
+  for (int i = t; i < a.k; i += BLK) put<DT>(a, row, r, rank_of(sh.found[i], sh.found, a.k), candidate_id(sh.found[i]));
+}
+
+// H: pieces of 8 elements that a thread keeps in registers.
+template <int DT, int BLK, int H, int GROUPS>
+__global__ void __launch_bounds__(BLK) top_logits_kernel(TopLogitsArgs a) {
+  __shared__ TopShared sh;
+  __shared__ AnyShared any;
+  __shared__ double sums[BLK / 64];
+  const int64_t r = blockIdx.x;
+  const int t = threadIdx.x;
+  const Row<DT, BLK, H> row(static_cast<const char*>(a.x) + ((r / a.inner) * a.s0 + (r % a.inner) * a.s1) *
+                                                                (DT == SF_DTYPE_BF16 ? 2 : 4),
+                            a.vocab);
+  float best[GROUPS];
+  const float m = row_max(row, best, sh.edge[1]);
+  const float c = static_cast<float>(a.inv_t * 1.4426950408889634);
+  const float ref = m > -INFINITY && m < INFINITY ? m : 0.0f;
+  Bound bound{INFINITY, 1.0f, 0.0f};
+  if (ref == m) bound = top_bound<BLK>(best, m, a.k, sh);
+  float sum = 0.0f, lost = 0.0f;
+  uint32_t hits = 0;
+  row.each([&](int p, int, const float (&v)[8]) SF_INLINE {
+    if (bound.holds(max8(v))) hits |= 1u << p;
+    float e[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) e[k] = __builtin_amdgcn_exp2f((v[k] - ref) * c);
+    // hundreds of small terms beside a large one: what an addition rounds off is carried along
+    const float s = (((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]))) - lost, upto = sum + s;
+    lost = (upto - sum) - s;
+    sum = upto;
+  });
+  double total = sum;
+  for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
+  if ((t & 63) == 0) sums[t >> 6] = total;
+  const int n = ref == m ? gather(row, [&](float x) { return bound.holds(x); }, hits, sh) : 0;
+  if (n < a.k || n > kTopCandidates) {  // -inf, inf or NaN among the k, or too many equals
+    top_of_any<DT, BLK>(a, row.row, r, any, sh);
+  } else {
+    for (int i = t; i < n; i += BLK) {
+      const u64 own = sh.found[i];
+      const int rank = rank_of(own, sh.found, n);
+      if (rank < a.k) put<DT>(a, row.row, r, rank, candidate_id(own));
     }
-  for (int i = t; i < a.k; i += kTlBlock) {
-    const int id = static_cast<int>(~static_cast<uint32_t>(found[i]));
-    a.ids[r * a.k + i] = id;
-    if (DT == SF_DTYPE_F32)
-      static_cast<float*>(a.values)[r * a.k + i] = static_cast<const float*>(a.x)[base + id];
-    else
-      static_cast<uint16_t*>(a.values)[r * a.k + i] = static_cast<const uint16_t*>(a.x)[base + id];
   }
+  __syncthreads();
   if (t == 0 && a.lse) {
     total = 0.0;
-    for (int w = 0; w < kTlBlock / 64; ++w) total += partd[w];
+    for (int w = 0; w < BLK / 64; ++w) total += sums[w];
     a.lse[r] = static_cast<float>(ref * a.inv_t + log(total));
   }
 }
@@ -108,9 +114,9 @@ extern "C" int sf_top_logits(const sf_top_logits_desc* desc, void* stream) {
   SF_CHECK_ARG(desc, "sf_top_logits: null descriptor");
   const sf_top_logits_desc& d = *desc;
   SF_CHECK_ARG(d.dtype == SF_DTYPE_F32 || d.dtype == SF_DTYPE_BF16, "sf_top_logits: unknown dtype %d", d.dtype);
-  SF_CHECK_ARG(d.rows >= 0 && d.rows < (1ll << 31) && d.vocab > 0 && d.vocab <= SF_TOP_MAX_VOCAB,
-               "sf_top_logits: %lld rows of %lld (at most %d)", (long long)d.rows, (long long)d.vocab,
-               SF_TOP_MAX_VOCAB);
+  SF_CHECK_ARG(d.rows >= 0 && d.rows < SF_TOP_MAX_ROWS && d.vocab > 0 && d.vocab <= SF_TOP_MAX_VOCAB,
+               "sf_top_logits: %lld rows (fewer than %d) of %lld (at most %d)", (long long)d.rows, SF_TOP_MAX_ROWS,
+               (long long)d.vocab, SF_TOP_MAX_VOCAB);
   SF_CHECK_ARG(d.k >= 1 && d.k <= d.vocab && d.k <= SF_TOP_MAX_K, "sf_top_logits: the %lld largest of %lld (at most %d)",
                (long long)d.k, (long long)d.vocab, SF_TOP_MAX_K);
   SF_CHECK_ARG(d.inner > 0 && d.rows % d.inner == 0 && d.outer_stride >= 0 && d.row_stride >= 0,
@@ -126,9 +132,16 @@ extern "C" int sf_top_logits(const sf_top_logits_desc* desc, void* stream) {
   a.values = d.values, a.ids = d.ids, a.lse = d.lse;
   const dim3 grid(static_cast<unsigned>(d.rows));
   hipStream_t st = static_cast<hipStream_t>(stream);
+  auto with = [&](auto dt) {
+    constexpr int DT = decltype(dt)::value;
+    if (d.rows >= 512 && d.k <= 128 && d.vocab <= 256 * 8 * 32)
+      top_logits_kernel<DT, 256, DT == SF_DTYPE_BF16 ? 16 : 8, 1><<<grid, 256, 0, st>>>(a);
+    else
+      top_logits_kernel<DT, 1024, 8, 2><<<grid, 1024, 0, st>>>(a);
+  };
   if (d.dtype == SF_DTYPE_BF16)
-    top_logits_kernel<SF_DTYPE_BF16><<<grid, kTlBlock, 0, st>>>(a);
+    with(std::integral_constant<int, SF_DTYPE_BF16>{});
   else
-    top_logits_kernel<SF_DTYPE_F32><<<grid, kTlBlock, 0, st>>>(a);
+    with(std::integral_constant<int, SF_DTYPE_F32>{});
   return launch_status("sf_top_logits");
 }
