@@ -4,9 +4,8 @@
 //   top-k keeps the first k; top-p of these the fewest first tokens that hold p of their weight; min-p those of at least
 //   min_p times the largest weight.  All three keep a first part of that order.
 //   the token is the first, by id, at which the weight of the kept tokens up to it exceeds u times their whole weight.
-// Weights are formed in f64 and summed as integers of 2^-F, F = 62 - log2 of the vocabulary (45 for 131072 tokens): sums
-// do not depend on their order, and what a cumulative sum is off by (about 2^-F of the largest weight) decides a draw
-// once in 1e8 draws; sums of f32 exponentials would decide one in thousands over large vocabularies.
+// Weights are formed in f64 and summed as integers of 2^-F, F = 44 (43 above 131072 tokens): sums do not depend on their order.  A cumulative share is off by 2e-12 (the exponential's polynomial) at most, which decides
+// one draw in 4e6 from 131072 equal tokens; shares from f32 exponentials, off by 1e-7, would decide one in a hundred.
 //
 // One workgroup per row, which it holds in registers if it fits.  With top-k up to 1024 the row's largest are gathered in
 // LDS (gather_top) and the rest happens among them.  Without it, top-p's border is the place in a histogram of weights by
@@ -14,12 +13,12 @@
 // the thread's.
 #include <type_traits>
 
+#include "sf_mfma.hpp"
 #include "sf_top.hpp"
 
 namespace sf {
 namespace {
 
-constexpr int kSpBlock = 1024;
 constexpr int kSpBins = 2048;
 
 struct SampleArgs {
@@ -35,6 +34,7 @@ struct SampleArgs {
   const float* min_p;
   float temp1, top_p1, min_p1;
   int top_k1, bits;  // bits: F
+  double poly[8];    // (2^f - 1) / f, the polynomial of degree 7 through its values at the Chebyshev points
 };
 
 // A row's settings.
@@ -49,30 +49,32 @@ struct Settings {
 };
 
 // Weights exp((x - top) / T) as integers of 2^-bits (bits <= 51); 2^bits exactly for the largest logit, which is finite.
+// The polynomial's coefficients come from the kernel's arguments, that is in scalar registers.
 struct Weight {
   double top, c;  // c: log2(e) / T
   int bits;
-  __device__ __forceinline__ u64 operator()(float x) const {
+  const double (&poly)[8];
+  // before it is rounded
+  __device__ __forceinline__ double scaled(float x) const {
     // 2^z = 2^n 2^f, f in [-1/2, 1/2]: n is in the low bits of the sum with 1.5 * 2^52.  -inf ends at the smallest z.
     constexpr double kRound = 6755399441055744.0;
     const double z = fmax((static_cast<double>(x) - top) * c, -64.0);
     const double rounded = z + kRound;
     const double f = z - (rounded - kRound);
-    // (2^f - 1) / f, the polynomial of degree 8 through its values at the Chebyshev points: 4e-14 of 2^f
-    double p = 0x1.b63880a30e9ffp-24;
-    p = fma(p, f, 0x1.63d136366db24p-20);
-    p = fma(p, f, 0x1.ffcb9515a8016p-17);
-    p = fma(p, f, 0x1.4308ac85aa947p-13);
-    p = fma(p, f, 0x1.5d87fe86fe88ep-10);
-    p = fma(p, f, 0x1.3b2ab7181b755p-7);
-    p = fma(p, f, 0x1.c6b08d7047e52p-5);
-    p = fma(p, f, 0x1.ebfbdff823cedp-3);
-    p = fma(p, f, 0x1.62e42fefa39efp-1);
+    double p = poly[7];
+#pragma unroll
+    for (int i = 6; i >= 0; --i) p = fma(p, f, poly[i]);
     p = fma(p, f, 1.0);
-    const u64 scaled = static_cast<u64>(__double_as_longlong(p)) +
-                       (static_cast<u64>(static_cast<uint32_t>(__double_as_longlong(rounded)) + bits) << 52);
-    // with 2^52 added the low bits are the rounded integer
-    return static_cast<u64>(__double_as_longlong(__longlong_as_double(scaled) + 4503599627370496.0)) & 0xfffffffffffffull;
+    return __longlong_as_double(static_cast<u64>(__double_as_longlong(p)) +
+                                (static_cast<u64>(static_cast<uint32_t>(__double_as_longlong(rounded)) + bits) << 52));
+  }
+  __device__ __forceinline__ u64 operator()(float x) const { return whole(scaled(x) + kWhole); }
+
+  // A number added to 2^52 is rounded to an integer, which is in the sum's low bits; so are the sums of up to 2^52 / 2^bits
+  // weights that start there.
+  static constexpr double kWhole = 4503599627370496.0;
+  static __device__ __forceinline__ u64 whole(double x) {
+    return static_cast<u64>(__double_as_longlong(x)) & 0xfffffffffffffull;
   }
 };
 
@@ -140,16 +142,24 @@ struct SampleShared {
   u64 before[kTopCandidates];
   int id[SF_TOP_MAX_K];
   float logit[SF_TOP_MAX_K];
-  u64 part[2][kSpBlock / 64];
+  u64 part[2][16];
   u64 total, base, last;
   int count, bin;
 };
 
-// Among the row's n largest, which sh.top.found holds: top-k, top-p, min-p and the draw.
+// Among the row's n largest, which sh.top.found holds: top-k, top-p, min-p and the draw, by the first THREADS threads (64:
+// the first wave, which waits for nobody).
+template <int THREADS>
 __device__ __forceinline__ void sample_found(const SampleArgs& a, const Settings& s, int64_t r, const Weight& weight,
                                              int n, SampleShared& sh) {
+  const auto meet = [] SF_INLINE {
+    if constexpr (THREADS == 64)
+      wave_lds_fence();
+    else
+      __syncthreads();
+  };
   const int t = threadIdx.x;
-  for (int i = t; i < n; i += kSpBlock) {
+  for (int i = t; i < n; i += THREADS) {
     const u64 own = sh.top.found[i];
     const int rank = rank_of(own, sh.top.found, n);
     if (rank < s.k) {
@@ -158,23 +168,41 @@ __device__ __forceinline__ void sample_found(const SampleArgs& a, const Settings
       sh.id[rank] = candidate_id(own);
     }
   }
-  if (t == 0) sh.total = 0, sh.count = 0;
-  __syncthreads();
+  meet();
   const int k = s.k < n ? static_cast<int>(s.k) : n;
   const u64 w = t < k ? sh.weight[t] : 0;
-  const u64 upto = block_scan<kSpBlock>(w, sh.part[0]);
-  u64 all = 0;
-  for (int i = 0; i < kSpBlock / 64; ++i) all += sh.part[0][i];
-  const bool kept = t < k && (s.p >= 1.0 || upto - w < share_up(s.p, all)) && static_cast<double>(w) >= s.least;
-  if (kept) {
-    atomicMax(&sh.total, upto);
-    atomicMax(&sh.count, t + 1);
+  u64 upto = wave_scan(w), all;
+  if constexpr (THREADS == 64) {
+    all = last_lane(upto);
+  } else {
+    if ((t & 63) == 63) sh.part[0][t >> 6] = upto;
+    if (t == 0) sh.total = 0, sh.count = 0;
+    __syncthreads();
+    all = 0;
+    for (int i = 0; i < THREADS / 64; ++i) {
+      if (i == t >> 6) upto += all;
+      all += sh.part[0][i];
+    }
   }
-  __syncthreads();
+  const bool kept = t < k && (s.p >= 1.0 || upto - w < share_up(s.p, all)) && static_cast<double>(w) >= s.least;
+  int count;
+  u64 total;
+  if constexpr (THREADS == 64) {
+    count = __popcll(__ballot(kept));
+    total = __shfl(upto, count - 1, 64);
+  } else {
+    if (kept) {
+      atomicMax(&sh.total, upto);
+      atomicMax(&sh.count, t + 1);
+    }
+    __syncthreads();
+    count = sh.count, total = sh.total;
+  }
   if (!kept) return;
-  const int id = sh.id[t], count = sh.count;
-  const u64 total = sh.total, want = share_down(s.u, total);
+  const int id = sh.id[t];
+  const u64 want = share_down(s.u, total);
   u64 sum = 0;
+#pragma unroll 4
   for (int i = 0; i < count; ++i) sum += sh.id[i] <= id ? sh.weight[i] : 0;
   if (sum - w <= want && want < sum) put_token(a, s, r, id, sh.logit[t], total);
 }
@@ -183,40 +211,48 @@ __device__ __forceinline__ void sample_found(const SampleArgs& a, const Settings
 struct Bins {
   float top, scale;
   __device__ __forceinline__ int of(float x) const {
-    const float y = (top - x) * scale;
-    return y < kSpBins - 1 ? static_cast<int>(y) : kSpBins - 1;
+    return static_cast<int>(fminf((top - x) * scale, static_cast<float>(kSpBins - 1)));
+  }
+  // The logits of a bin lie between these (and others may).
+  __device__ __forceinline__ void range(int bin, float& low, float& high) const {
+    const float a = (static_cast<float>(bin) - 0.01f) / scale, b = (static_cast<float>(bin) + 1.01f) / scale;
+    const float off = 1e-6f * (fabsf(top) + b);
+    high = top - a + off;
+    low = bin == kSpBins - 1 ? -INFINITY : top - b - off;
   }
 };
 
-// What top-k and top-p keep: up to this candidate in the order of logits.
+// The last element, in the order of logits, that top-k and top-p keep.
 struct Last {
-  u64 c;
-  __device__ __forceinline__ bool keeps(float x, int id) const { return candidate(x, id) >= c; }
+  float x = -INFINITY;
+  int id = INT32_MAX;
+  __device__ __forceinline__ bool keeps(float y, int i) const { return (y > x) | ((y == x) & (i <= id)); }
 };
 
 // The last element, in the order of logits, at which the sum of amount(x, id) before it is below want(whole sum): found in
 // last.  False: more than kTopCandidates are in the bin where that happens.  A sum that stays below takes in everything.
-template <int DT, int H, typename M, typename A>
-__device__ __forceinline__ bool border_of(const Row<DT, kSpBlock, H>& row, const Bins& bins, M&& amount, A&& want,
+template <int DT, int BLK, int H, typename M, typename A>
+__device__ __forceinline__ bool border_of(Row<DT, BLK, H>& row, const Bins& bins, M&& amount, A&& want,
                                           Last& last, SampleShared& sh) {
-  constexpr int kEach = kSpBins / kSpBlock;
+  constexpr int kEach = kSpBins / BLK;
   const int t = threadIdx.x;
-  for (int i = t; i < kSpBins; i += kSpBlock) sh.weight[i] = 0;
+  for (int i = t; i < kSpBins; i += BLK) sh.weight[i] = 0;
   if (t == 0) sh.bin = -1, sh.top.n = 0;
   __syncthreads();
-  row.each([&](int, int i, const float (&v)[8]) SF_INLINE {
+  row.each_looped([&](int, int i, const float (&v)[8]) SF_INLINE {
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
       const u64 w = amount(v[k], i + k);
-      if (w) atomicAdd(&sh.weight[bins.of(v[k])], w);
+      if (w != 0) atomicAdd(&sh.weight[bins.of(v[k])], w);
+      if (k % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // four at a time: eight take more registers than there are
     }
   });
   __syncthreads();
   u64 own[kEach], sum = 0;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) sum += own[i] = sh.weight[t * kEach + i];
-  u64 upto = block_scan<kSpBlock>(sum, sh.part[0]) - sum, total = 0;
-  for (int i = 0; i < kSpBlock / 64; ++i) total += sh.part[0][i];
+  u64 upto = block_scan<BLK>(sum, sh.part[0]) - sum, total = 0;
+  for (int i = 0; i < BLK / 64; ++i) total += sh.part[0][i];
   const u64 target = want(total);
 #pragma unroll
   for (int i = 0; i < kEach; ++i) {
@@ -227,23 +263,25 @@ __device__ __forceinline__ bool border_of(const Row<DT, kSpBlock, H>& row, const
   const int bin = sh.bin;
   if (bin < 0) return true;
   uint32_t hits = 0;
-  row.each([&](int p, int i, const float (&v)[8]) SF_INLINE {
+  float low, high;
+  bins.range(bin, low, high);
+  row.each([&](int p, int, const float (&v)[8]) SF_INLINE {
     bool any = false;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) any |= bins.of(v[k]) == bin;
+    for (int k = 0; k < 8; ++k) any |= __builtin_amdgcn_fmed3f(v[k], low, high) == v[k];
     if (any) hits |= 1u << p;
   });
   const int n = gather(row, [&](float x) { return bins.of(x) == bin; }, hits, sh.top);
   if (n > kTopCandidates) return false;
-  for (int i = t; i < n; i += kSpBlock) {
+  for (int i = t; i < n; i += BLK) {
     const u64 c = sh.top.found[i];
     sh.weight[i] = amount(candidate_logit(c), candidate_id(c));
     sh.before[i] = sh.base;
   }
   __syncthreads();
   // every candidate's sum before it, its terms shared by as many threads as there are
-  const int parts = n < kSpBlock ? kSpBlock / n : 1, size = (n + parts - 1) / parts;
-  for (int at = t; at < n * parts; at += kSpBlock) {
+  const int parts = n < BLK ? BLK / n : 1, size = (n + parts - 1) / parts;
+  for (int at = t; at < n * parts; at += BLK) {
     const int i = at % n, from = at / n * size, to = from + size < n ? from + size : n;
     const u64 c = sh.top.found[i];
     u64 sum = 0;
@@ -251,63 +289,83 @@ __device__ __forceinline__ bool border_of(const Row<DT, kSpBlock, H>& row, const
     atomicAdd(&sh.before[i], sum);
   }
   __syncthreads();
-  for (int i = t; i < n; i += kSpBlock)
+  for (int i = t; i < n; i += BLK)
     if (sh.before[i] < target && target <= sh.before[i] + sh.weight[i]) sh.last = sh.top.found[i];
   __syncthreads();
-  last.c = sh.last;
+  last = {candidate_logit(sh.last), candidate_id(sh.last)};
   return true;
 }
 
-// The draw among the elements with amount(x, id): the wave whose part of the row it falls in, then the thread.
-template <int DT, int H, typename M>
-__device__ __forceinline__ void draw(const SampleArgs& a, const Settings& s, int64_t r, const Row<DT, kSpBlock, H>& row,
-                                     float cut, M&& amount, SampleShared& sh) {
+// The draw among the elements that `last` keeps (ALL: every one): the wave whose part of the row it falls in, then the
+// thread.
+template <bool ALL, int DT, int BLK, int H>
+__device__ __forceinline__ void draw(const SampleArgs& a, const Settings& s, int64_t r, Row<DT, BLK, H>& row,
+                                     const Last& last, const Weight& weight, SampleShared& sh) {
   const int t = threadIdx.x;
-  u64 sum = 0;
-  row.each([&](int, int i, const float (&v)[8]) SF_INLINE {
-    if (max8(v) >= cut) {
+  double sum = Weight::kWhole;
+  row.each_looped([&](int, int i, const float (&v)[8]) SF_INLINE {
+    if (ALL || max8(v) >= last.x) {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) sum += amount(v[k], i + k);
+      for (int k = 0; k < 8; ++k) {
+        const double w = weight.scaled(v[k]);
+        sum += ALL || last.keeps(v[k], i + k) ? w : 0.0;
+        if (k % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
     }
   });
-  for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
-  if ((t & 63) == 0) sh.part[1][t >> 6] = sum;
+  const u64 part = wave_scan(Weight::whole(sum));
+  if ((t & 63) == 63) sh.part[1][t >> 6] = part;
   __syncthreads();
   u64 total = 0;
-  for (int w = 0; w < kSpBlock / 64; ++w) total += sh.part[1][w];
+  for (int w = 0; w < BLK / 64; ++w) total += sh.part[1][w];
   u64 left = share_down(s.u, total);
   int wave = 0;
-  for (; wave < kSpBlock / 64 - 1 && sh.part[1][wave] <= left; ++wave) left -= sh.part[1][wave];
+  for (; wave < BLK / 64 - 1 && sh.part[1][wave] <= left; ++wave) left -= sh.part[1][wave];
   // the wave's ids, one range for each thread
-  const int each = (row.pieces * 64 + kSpBlock - 1) / kSpBlock, from = row.wave_at(wave) + t * each * 8,
+  const int each = (row.pieces * 64 + BLK - 1) / BLK, from = row.wave_at(wave) + t * each * 8,
             end = row.wave_at(wave + 1);
+  const auto amount = [&](float x, int id) { return last.keeps(x, id) ? weight(x) : 0; };
   u64 mine = 0;
+#pragma unroll 1
   for (int i = from; i < from + each * 8 && i < end; i += 8) {
     Raw8<DT> raw;
     float v[8];
     row.fetch(raw, i);
     raw.get(v);
+#pragma unroll
     for (int k = 0; k < 8; ++k) mine += amount(v[k], i + k);
   }
-  u64 before = block_scan<kSpBlock>(mine, sh.part[0]) - mine;
-  if (before <= left && left < before + mine)
+  u64 before = block_scan<BLK>(mine, sh.part[0]) - mine;
+  if (before <= left && left < before + mine) {
+#pragma unroll 1
     for (int i = from; i < from + each * 8 && i < row.vocab; ++i) {
       const float x = load_as_f32(row.row, i, DT);
       const u64 w = amount(x, i);
       if (before <= left && left < before + w) put_token(a, s, r, i, x, total);
       before += w;
     }
+  }
 }
 
-template <int DT, int H>
-__global__ void __launch_bounds__(kSpBlock) sample_kernel(SampleArgs a) {
+// The smallest logit whose weight min-p keeps: among the 64 floats around m + T ln(min_p), one to a lane.
+__device__ __forceinline__ float least_logit(const Settings& s, const Weight& weight) {
+  const float near = static_cast<float>(s.top + s.temp * log(s.least / s.one));
+  if (!(near > -3.0e38f)) return -INFINITY;
+  const uint32_t key = ordered_key(near) + 32 - (threadIdx.x & 63);  // falling
+  const float x = __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+  const u64 kept = __ballot(x <= s.top && static_cast<double>(weight(x)) >= s.least);
+  return kept ? __shfl(x, 63 - __clzll(kept), 64) : s.top;
+}
+
+template <int DT, int BLK, int H>
+__global__ void __launch_bounds__(BLK) sample_kernel(SampleArgs a) {
   __shared__ union {
     SampleShared sh;
     AnyShared any;
   } lds;
   SampleShared& sh = lds.sh;
   const int64_t r = blockIdx.x;
-  const Row<DT, kSpBlock, H> row(static_cast<const char*>(a.x) + r * a.xs * (DT == SF_DTYPE_BF16 ? 2 : 4), a.vocab);
+  Row<DT, BLK, H> row(static_cast<const char*>(a.x) + r * a.xs * (DT == SF_DTYPE_BF16 ? 2 : 4), a.vocab);
   const float T = a.temp ? a.temp[r] : a.temp1, top_p = a.top_p ? a.top_p[r] : a.top_p1;
   const float min_p = a.min_p ? a.min_p[r] : a.min_p1;
   const int top_k = a.top_k ? a.top_k[r] : a.top_k1;
@@ -319,8 +377,15 @@ __global__ void __launch_bounds__(kSpBlock) sample_kernel(SampleArgs a) {
   s.p = !greedy && top_p < 1.0f ? static_cast<double>(top_p) : 1.0;
   s.one = ldexp(1.0, a.bits);
   s.least = (min_p > 1.0f ? 1.0 : min_p > 0.0f ? static_cast<double>(min_p) : 0.0) * s.one;
-  float best[2];
-  const float m = s.top = row_max(row, best, sh.top.edge[1]);
+  const bool among = s.k <= BLK && s.k < a.vocab;  // few enough to be gathered
+  const bool binned = !among && (s.k < a.vocab || s.p < 1.0);
+  float best[2], low = INFINITY;
+  const float m = s.top = row_max(row, best, sh.top.edge[1], [&](const float (&v)[8]) SF_INLINE {
+    if (binned) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) low = fminf(low, v[k] == -INFINITY ? INFINITY : v[k]);
+    }
+  });
   if (m != m || m == -INFINITY) {
     if (threadIdx.x == 0) {
       a.tokens[r] = -1;
@@ -328,63 +393,52 @@ __global__ void __launch_bounds__(kSpBlock) sample_kernel(SampleArgs a) {
     }
     return;
   }
-  const Weight weight{m, 1.4426950408889634 / static_cast<double>(s.temp), a.bits};
+  const Weight weight{m, 1.4426950408889634 / static_cast<double>(s.temp), a.bits, a.poly};
   bool done = m < INFINITY;
-  if (done && s.k <= SF_TOP_MAX_K && s.k < a.vocab) {
-    const Bound bound = top_bound<kSpBlock>(best, m, static_cast<int>(s.k), sh.top);
+  if (done && among) {
+    const Bound bound = top_bound<BLK>(best, m, static_cast<int>(s.k), sh.top);
     uint32_t hits = 0;
     row.each([&](int p, int, const float (&v)[8]) SF_INLINE {
       if (bound.holds(max8(v))) hits |= 1u << p;
     });
     const int n = gather(row, [&](float x) { return bound.holds(x); }, hits, sh.top);
     done = n > 0 && n <= kTopCandidates;
-    if (done) sample_found(a, s, r, weight, n, sh);
+    if (done && n > 64)
+      sample_found<BLK>(a, s, r, weight, n, sh);
+    else if (done && threadIdx.x < 64)
+      sample_found<64>(a, s, r, weight, n, sh);
   } else if (done) {
-    Last last{0};
-    if (s.k < a.vocab || s.p < 1.0) {
-      float low = INFINITY;
-      row.each([&](int, int, const float (&v)[8]) SF_INLINE {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) low = fminf(low, v[k] == -INFINITY ? INFINITY : v[k]);
-      });
-      for (int off = 32; off > 0; off >>= 1) low = fminf(low, __shfl_xor(low, off, 64));
+    Last last;
+    if (binned) {
+      low = last_lane(wave_scan(low, INFINITY, [](float a, float b) { return fminf(a, b); }));
       if ((threadIdx.x & 63) == 0) sh.top.edge[0][threadIdx.x >> 6] = low;
       __syncthreads();
-      for (int w = 0; w < kSpBlock / 64; ++w) low = fminf(low, sh.top.edge[0][w]);
+      for (int w = 0; w < BLK / 64; ++w) low = fminf(low, sh.top.edge[0][w]);
       // 2^-(F + 1) of the largest weight is 0
       const float range = fminf(m - low, static_cast<float>((a.bits + 1) * 0.6931471805599453 * s.temp));
       const Bins bins{m, fminf(kSpBins / range, 1e30f)};
-      if (s.k < a.vocab)
+      // by number for top-k, by weight among these for top-p
+#pragma unroll 1
+      for (int by_weight = s.k < a.vocab ? 0 : 1; done && by_weight < (s.p < 1.0 ? 2 : 1); ++by_weight) {
         done = border_of(
-            row, bins, [&](float x, int) -> u64 { return x > -INFINITY; },
-            [&](u64) { return static_cast<u64>(s.k); }, last, sh);
-      if (done && s.p < 1.0) {
+            row, bins,
+            [&](float x, int id) -> u64 { return !last.keeps(x, id) ? 0 : by_weight ? weight(x) : x > -INFINITY; },
+            [&](u64 total) { return by_weight ? share_up(s.p, total) : static_cast<u64>(s.k); }, last, sh);
         __syncthreads();
-        done = border_of(
-            row, bins, [&](float x, int id) -> u64 { return last.keeps(x, id) ? weight(x) : 0; },
-            [&](u64 total) { return share_up(s.p, total); }, last, sh);
       }
     }
-    if (done) {
-      // no element below this one is kept
-      float cut = last.c ? candidate_logit(last.c) : -INFINITY;
-      if (s.least > 0.0) {
-        const double d = s.temp * log(s.least / s.one);
-        cut = fmaxf(cut, static_cast<float>(m + d - 1e-6 * (fabs(m) + fabs(d))));
-      }
-      draw(
-          a, s, r, row, cut,
-          [&](float x, int id) -> u64 {
-            if (x < cut || !last.keeps(x, id)) return 0;
-            const u64 w = weight(x);
-            return static_cast<double>(w) >= s.least ? w : 0;
-          },
-          sh);
+    if (done && s.least > 0.0) {
+      const float x = least_logit(s, weight);
+      if (x > last.x) last = {x, INT32_MAX};
     }
+    if (done && last.x > -INFINITY)
+      draw<false>(a, s, r, row, last, weight, sh);
+    else if (done)
+      draw<true>(a, s, r, row, last, weight, sh);
   }
   if (!done) {
     __syncthreads();
-    sample_any<DT, kSpBlock>(a, s, r, row.row, weight, lds.any);
+    sample_any<DT, BLK>(a, s, r, row.row, weight, lds.any);
   }
 }
 
@@ -409,17 +463,25 @@ extern "C" int sf_sample_logits(const sf_sample_desc* desc, void* stream) {
   a.u = d.uniform, a.tokens = d.tokens, a.logprobs = d.logprobs;
   a.temp = d.temperature, a.top_k = d.top_k, a.top_p = d.top_p, a.min_p = d.min_p;
   a.temp1 = d.temperature_all, a.top_k1 = d.top_k_all, a.top_p1 = d.top_p_all, a.min_p1 = d.min_p_all;
-  a.bits = 62;  // sums of vocab weights of at most 2^bits stay below 2^62; the weights below 2^52
+  // 2e-12 of 2^f
+  constexpr double kPoly[8] = {0x1.62e42fef9cc69p-1,  0x1.ebfbdff82a734p-3,  0x1.c6b08da70cce3p-5,
+                               0x1.3b2ab70ad2565p-7,  0x1.5d877598350dep-10, 0x1.4308c7183d6a2p-13,
+                               0x1.00c0e4e15189cp-16, 0x1.63b2d7971923fp-20};
+  memcpy(a.poly, kPoly, sizeof(kPoly));
+  // Sums of vocab weights of at most 2^bits stay below 2^62, those of a thread, which has at most vocab / 512 and 256 of
+  // them, below 2^52.
+  a.bits = 61;
   for (int64_t n = 1; n < d.vocab; n *= 2) --a.bits;
-  if (a.bits > 50) a.bits = 50;
+  if (a.bits > 44) a.bits = 44;
   const dim3 grid(static_cast<unsigned>(d.rows));
   hipStream_t st = static_cast<hipStream_t>(stream);
   auto with = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    if (a.vocab <= kSpBlock * 8 * 4)
-      sample_kernel<DT, 4><<<grid, kSpBlock, 0, st>>>(a);
+    constexpr int H = DT == SF_DTYPE_BF16 ? 8 : 4;
+    if (a.vocab <= 512 * 8 * 8 && d.rows > 256)
+      sample_kernel<DT, 512, H><<<grid, 512, 0, st>>>(a);
     else
-      sample_kernel<DT, 8><<<grid, kSpBlock, 0, st>>>(a);
+      sample_kernel<DT, 1024, H><<<grid, 1024, 0, st>>>(a);
   };
   if (d.dtype == SF_DTYPE_BF16)
     with(std::integral_constant<int, SF_DTYPE_BF16>{});

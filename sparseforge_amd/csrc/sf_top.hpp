@@ -102,10 +102,45 @@ struct Row {
         raw[p].get(v);
         f(p, at(p), v);
       }
+    constexpr int kAhead = 4;  // pieces on their way
+    Raw8<DT> more[kAhead];
+    for (int q = H; q < pieces; q += kAhead) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (q + u < pieces) fetch(more[u], at(q + u));
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        if (q + u < pieces) {
+          more[u].get(v);
+          f(q + u, at(q + u), v);
+        }
+    }
+  }
+  // The same as a loop, for an f of a hundred instructions and more, of which H copies would not stay in the instruction
+  // cache: the first piece is taken and the others move up before it, which restores their order in the end.
+  template <typename F>
+  __device__ __forceinline__ void each_looped(F&& f) {
+    float v[8];
+#pragma unroll 1
+    for (int p = 0; p < H; ++p) {
+      const Raw8<DT> first = raw[0];
+#pragma unroll
+      for (int q = 0; q + 1 < H; ++q) raw[q] = raw[q + 1];
+      raw[H - 1] = first;
+      if (p < pieces) {
+        first.get(v);
+        f(p, at(p), v);
+      }
+    }
+    if (pieces <= H) return;
+    Raw8<DT> next[2];
+    fetch(next[0], at(H));
+    fetch(next[1], at(H + 1));
+#pragma unroll 1
     for (int p = H; p < pieces; ++p) {
-      Raw8<DT> more;
-      fetch(more, at(p));
-      more.get(v);
+      next[0].get(v);
+      next[0] = next[1];
+      fetch(next[1], at(p + 2));  // behind the last piece another wave's, or nothing: not used
       f(p, at(p), v);
     }
   }
@@ -117,16 +152,44 @@ __device__ __forceinline__ float max8(const float (&v)[8]) {
   return nan_max(nan_max(nan_max(v[0], v[1]), nan_max(v[2], v[3])), nan_max(nan_max(v[4], v[5]), nan_max(v[6], v[7])));
 }
 
-// Inclusive sum over a wave's lanes.
+// x of the lane that a DPP control names, `none` in lanes that it gives nothing.
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ uint32_t dpp(uint32_t x, uint32_t none) {
+  return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(none), static_cast<int>(x), CTRL, ROWS, 0xf, false));
+}
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ u64 dpp(u64 x, u64 none) {
+  return static_cast<u64>(dpp<CTRL, ROWS>(static_cast<uint32_t>(x >> 32), static_cast<uint32_t>(none >> 32))) << 32 |
+         dpp<CTRL, ROWS>(static_cast<uint32_t>(x), static_cast<uint32_t>(none));
+}
+template <int CTRL, int ROWS = 0xf>
+__device__ __forceinline__ float dpp(float x, float none) {
+  return __uint_as_float(dpp<CTRL, ROWS>(__float_as_uint(x), __float_as_uint(none)));
+}
+// op over a wave's lanes up to each one, by shifts within rows of 16 lanes and the rows' last lanes; every lane of the
+// wave has to be there.
+template <typename T, typename F>
+__device__ __forceinline__ T wave_scan(T x, T none, F&& op) {
+  x = op(x, dpp<0x111>(x, none));
+  x = op(x, dpp<0x112>(x, none));
+  x = op(x, dpp<0x114>(x, none));
+  x = op(x, dpp<0x118>(x, none));
+  x = op(x, dpp<0x142, 0xa>(x, none));
+  return op(x, dpp<0x143, 0xc>(x, none));
+}
 template <typename T>
 __device__ __forceinline__ T wave_scan(T x) {
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const T y = __shfl_up(x, off, 64);
-    if (static_cast<int>(threadIdx.x & 63) >= off) x += y;
-  }
-  return x;
+  return wave_scan(x, T(0), [](T a, T b) { return a + b; });
 }
+// The last lane's, in every one.
+__device__ __forceinline__ uint32_t last_lane(uint32_t x) {
+  return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(x), 63));
+}
+__device__ __forceinline__ float last_lane(float x) { return __uint_as_float(last_lane(__float_as_uint(x))); }
+__device__ __forceinline__ u64 last_lane(u64 x) {
+  return static_cast<u64>(last_lane(static_cast<uint32_t>(x >> 32))) << 32 | last_lane(static_cast<uint32_t>(x));
+}
+
 // Inclusive sum over a workgroup's threads.  part: of BLK / 64, not in use before or after without a barrier.
 template <int BLK, typename T>
 __device__ __forceinline__ T block_scan(T x, T* part) {
@@ -178,7 +241,7 @@ __device__ __forceinline__ Bound top_bound(const float (&best)[GROUPS], float m,
   float low = INFINITY;
 #pragma unroll
   for (int g = 0; g < GROUPS; ++g) low = fminf(low, best[g] == -INFINITY ? INFINITY : best[g]);
-  for (int off = 32; off > 0; off >>= 1) low = fminf(low, __shfl_xor(low, off, 64));
+  low = last_lane(wave_scan(low, INFINITY, [](float a, float b) { return fminf(a, b); }));
   if (lane == 0) sh.edge[0][wave] = low;
   for (int i = t; i < kTopBins; i += BLK) sh.bins[i] = 0;
   if (t == 0) sh.limit = ~0u, sh.n = 0;
@@ -233,13 +296,14 @@ __device__ __forceinline__ int gather(const Row<DT, BLK, H>& row, F&& wanted, ui
   return n;
 }
 
-// Maxima of the thread's groups of pieces; the row's, NaN if it has one, in every thread.
-template <int DT, int BLK, int H, int GROUPS>
-__device__ __forceinline__ float row_max(const Row<DT, BLK, H>& row, float (&best)[GROUPS], float* part) {
+// Maxima of the thread's groups of pieces; the row's, NaN if it has one, in every thread.  also(elements): of every piece.
+template <int DT, int BLK, int H, int GROUPS, typename F>
+__device__ __forceinline__ float row_max(const Row<DT, BLK, H>& row, float (&best)[GROUPS], float* part, F&& also) {
 #pragma unroll
   for (int g = 0; g < GROUPS; ++g) best[g] = -INFINITY;
   row.each([&](int p, int, const float (&v)[8]) SF_INLINE {
     const float x = max8(v);
+    also(v);
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g)
       if (GROUPS == 1 || p % GROUPS == g) best[g] = nan_max(best[g], x);
@@ -247,7 +311,7 @@ __device__ __forceinline__ float row_max(const Row<DT, BLK, H>& row, float (&bes
   float m = best[0];
 #pragma unroll
   for (int g = 1; g < GROUPS; ++g) m = nan_max(m, best[g]);
-  for (int off = 32; off > 0; off >>= 1) m = nan_max(m, __shfl_xor(m, off, 64));
+  m = last_lane(wave_scan(m, -INFINITY, [](float a, float b) { return nan_max(a, b); }));
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
   __syncthreads();
   m = part[0];
@@ -258,6 +322,7 @@ __device__ __forceinline__ float row_max(const Row<DT, BLK, H>& row, float (&bes
 // How many of the n candidates come before c; where n is odd found[n] is 0.
 __device__ __forceinline__ int rank_of(u64 c, const u64* found, int n) {
   int rank = 0;
+#pragma unroll 4
   for (int j = 0; j < n; j += 2) {
     const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(found + j);
     rank += (x.x > c ? 1 : 0) + (x.y > c ? 1 : 0);
@@ -266,36 +331,14 @@ __device__ __forceinline__ int rank_of(u64 c, const u64* found, int n) {
 }
 
 // ---------------------------------------------------------------------------
-// Passes that are right for every row, whatever its order and its equal values: a row's elements in tiles of 8 * BLK,
-// thread t holding elements [8 t, 8 t + 8) of a tile, so that tiles, waves and lanes follow each other in the order of
-// the ids.  Used where gather_top finds too many.
+// Passes that are right for every row, whatever its order and its equal values, for the rows in which gather() finds too
+// many: element by element from memory, in little code and few registers.  Thread t takes elements [8 t, 8 t + 8) of tiles
+// of 8 * BLK, so that tiles, waves and lanes follow each other in the order of the ids.
 // ---------------------------------------------------------------------------
 // A row's order as integers: larger logits have larger keys, -0 equals 0, NaN is largest.  bf16 needs 16 bits.
 template <int DT>
 __device__ __forceinline__ uint32_t top_key(float x) {
   return DT == SF_DTYPE_BF16 ? ordered_key(x) >> 16 : ordered_key(x);
-}
-
-template <int DT>
-__device__ __forceinline__ void top_load8(const void* row, int i, int n, float (&v)[8]) {
-  Raw8<DT> raw;
-  if (n == 8)
-    raw.load(row, i);
-  else
-    raw.load_some(row, i, n);
-  raw.get(v);
-}
-
-// f(tile, first id, number of elements, elements) over a row.
-template <int DT, int BLK, typename F>
-__device__ __forceinline__ void top_scan(const void* row, int vocab, F&& f) {
-  int tile = 0;
-  for (int i = threadIdx.x * 8; i < vocab; i += BLK * 8, ++tile) {
-    const int n = vocab - i < 8 ? vocab - i : 8;
-    float v[8];
-    top_load8<DT>(row, i, n, v);
-    f(tile, i, n, v);
-  }
 }
 
 constexpr int kAnySums = SF_TOP_MAX_VOCAB / 512;  // a sum for each wave and tile
@@ -314,45 +357,46 @@ struct Border {
 };
 
 // Finds in a row the key at which the count, or the weight, of the elements from the largest down reaches target
-// (1 .. total): passes of 8 bits from the top, each over the elements whose higher bits are the border's.
+// (1 .. total): passes of 8 bits from the top, each over the elements whose higher bits are the border's.  Afterwards
+// sh.mass and sh.count hold the border's own key's at its last 8 bits.
 template <int DT, int BLK, typename W>
-__device__ __forceinline__ Border radix_border(const void* row, int vocab, bool by_weight, u64 target, W&& weight, AnyShared& sh) {
-  u64(&mass)[256] = sh.mass, (&shared)[3] = sh.shared;
-  uint32_t(&count)[256] = sh.count;
+__device__ __forceinline__ Border radix_border(const void* row, int vocab, bool by_weight, u64 target, W&& weight,
+                                               AnyShared& sh) {
   constexpr int kBits = DT == SF_DTYPE_BF16 ? 16 : 32;
   uint32_t prefix = 0;
   u64 above = 0;
+#pragma unroll 1
   for (int shift = kBits - 8; shift >= 0; shift -= 8) {
-    for (int i = threadIdx.x; i < 256; i += BLK) mass[i] = 0, count[i] = 0;
+    for (int i = threadIdx.x; i < 256; i += BLK) sh.mass[i] = 0, sh.count[i] = 0;
     __syncthreads();
-    top_scan<DT, BLK>(row, vocab, [&](int, int, int n, const float (&v)[8]) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const uint32_t key = top_key<DT>(v[k]);
-        if (k < n && (static_cast<u64>(key) >> (shift + 8)) == prefix) {
-          atomicAdd(&count[key >> shift & 255], 1u);
-          atomicAdd(&mass[key >> shift & 255], weight(v[k]));
-        }
+#pragma unroll 1
+    for (int i = threadIdx.x; i < vocab; i += BLK) {
+      const float x = load_as_f32(row, i, DT);
+      const uint32_t key = top_key<DT>(x);
+      if ((static_cast<u64>(key) >> (shift + 8)) == prefix) {
+        atomicAdd(&sh.count[key >> shift & 255], 1u);
+        atomicAdd(&sh.mass[key >> shift & 255], weight(x));
       }
-    });
+    }
     __syncthreads();
     if (threadIdx.x == 0) {
       u64 left = target, over = above;
       int b = 255;
+#pragma unroll 1
       for (; b > 0; --b) {
-        const u64 here = by_weight ? mass[b] : count[b];
+        const u64 here = by_weight ? sh.mass[b] : sh.count[b];
         if (here >= left) break;
         left -= here;
-        over += mass[b];
+        over += sh.mass[b];
       }
-      shared[0] = b;
-      shared[1] = left;
-      shared[2] = over;
+      sh.shared[0] = b;
+      sh.shared[1] = left;
+      sh.shared[2] = over;
     }
     __syncthreads();
-    prefix = prefix << 8 | static_cast<uint32_t>(shared[0]);
-    target = shared[1];
-    above = shared[2];
+    prefix = prefix << 8 | static_cast<uint32_t>(sh.shared[0]);
+    target = sh.shared[1];
+    above = sh.shared[2];
     __syncthreads();
   }
   return {prefix, target, above};
@@ -366,63 +410,51 @@ struct Place {
 // The first id at which the weight of the ids up to it exceeds at(total weight).
 template <int DT, int BLK, typename W, typename A>
 __device__ __forceinline__ Place locate(const void* row, int vocab, W&& weight, A&& at, AnyShared& sh) {
-  u64(&sums)[kAnySums] = sh.sums, (&shared)[3] = sh.shared;
   constexpr int kWaves = BLK / 64;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int tiles = (vocab + BLK * 8 - 1) / (BLK * 8);
-  for (int tile = 0; tile < tiles; ++tile) {
-    const int i = tile * BLK * 8 + threadIdx.x * 8, n = vocab - i < 8 ? vocab - i : 8;
+  const auto sum_of = [&](int i) SF_INLINE {
     u64 s = 0;
-    if (n > 0) {
-      float v[8];
-      top_load8<DT>(row, i, n, v);
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (k < n) s += weight(v[k], i + k);
-    }
-    for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
-    if (lane == 0) sums[tile * kWaves + wave] = s;
+#pragma unroll 1
+    for (int k = i; k < i + 8 && k < vocab; ++k) s += weight(load_as_f32(row, k, DT), k);
+    return s;
+  };
+#pragma unroll 1
+  for (int tile = 0; tile < tiles; ++tile) {
+    const u64 s = wave_scan(sum_of(tile * BLK * 8 + threadIdx.x * 8));
+    if (lane == 63) sh.sums[tile * kWaves + wave] = s;
   }
   __syncthreads();
   if (threadIdx.x == 0) {
     u64 total = 0;
-    for (int j = 0; j < tiles * kWaves; ++j) total += sums[j];
+    for (int j = 0; j < tiles * kWaves; ++j) total += sh.sums[j];
     u64 left = at(total);
     int j = 0;
-    for (; j < tiles * kWaves && sums[j] <= left; ++j) left -= sums[j];
-    shared[0] = j;
-    shared[1] = left;
-    shared[2] = total;
+    for (; j < tiles * kWaves && sh.sums[j] <= left; ++j) left -= sh.sums[j];
+    sh.shared[0] = j;
+    sh.shared[1] = left;
+    sh.shared[2] = total;
   }
   __syncthreads();
-  const int j = static_cast<int>(shared[0]);
-  const u64 left = shared[1], total = shared[2];
+  const int j = static_cast<int>(sh.shared[0]);
+  const u64 left = sh.shared[1], total = sh.shared[2];
   __syncthreads();
   if (j >= tiles * kWaves) return {-1, total};
   if (wave == 0) {
-    const int i = (j / kWaves) * BLK * 8 + (j % kWaves) * 512 + lane * 8, n = vocab - i < 8 ? vocab - i : 8;
-    float v[8];
-    u64 w[8], s = 0;
-    if (n > 0) top_load8<DT>(row, i, n, v);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      w[k] = k < n ? weight(v[k], i + k) : 0;
-      s += w[k];
-    }
-    u64 upto = s;
-    for (int off = 1; off < 64; off <<= 1) {
-      const u64 x = __shfl_up(upto, off, 64);
-      if (lane >= off) upto += x;
-    }
+    const int i = (j / kWaves) * BLK * 8 + (j % kWaves) * 512 + lane * 8;
+    const u64 s = sum_of(i), upto = wave_scan(s);
     u64 before = upto - s;
-    if (before <= left && left < upto)
-      for (int k = 0; k < 8; ++k) {
-        if (before <= left && left < before + w[k]) shared[0] = i + k;
-        before += w[k];
+    if (before <= left && left < upto) {
+#pragma unroll 1
+      for (int k = i; k < i + 8 && k < vocab; ++k) {
+        const u64 w = weight(load_as_f32(row, k, DT), k);
+        if (before <= left && left < before + w) sh.shared[0] = k;
+        before += w;
       }
+    }
   }
   __syncthreads();
-  const int id = static_cast<int>(shared[0]);
+  const int id = static_cast<int>(sh.shared[0]);
   __syncthreads();
   return {id, total};
 }

@@ -42,14 +42,12 @@ __device__ __forceinline__ void top_of_any(const TopLogitsArgs& a, const void* r
                        .id;
   if (t == 0) sh.n = 0;
   __syncthreads();
-  top_scan<DT, BLK>(row, V, [&](int, int i, int n, const float (&v)[8]) {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const uint32_t key = top_key<DT>(v[k]);
-      if (k < n && (key > border.key || (key == border.key && i + k <= last)))
-        sh.found[atomicAdd(&sh.n, 1)] = candidate(v[k], i + k);
-    }
-  });
+#pragma unroll 1
+  for (int i = t; i < V; i += BLK) {
+    const float x = load_as_f32(row, i, DT);
+    const uint32_t key = top_key<DT>(x);
+    if (key > border.key || (key == border.key && i <= last)) sh.found[atomicAdd(&sh.n, 1)] = candidate(x, i);
+  }
   if (t == 0 && a.k % 2) sh.found[a.k] = 0;
   __syncthreads();
   for (int i = t; i < a.k; i += BLK) put<DT>(a, row, r, rank_of(sh.found[i], sh.found, a.k), candidate_id(sh.found[i]));
@@ -67,7 +65,7 @@ __global__ void __launch_bounds__(BLK) top_logits_kernel(TopLogitsArgs a) {
                                                                 (DT == SF_DTYPE_BF16 ? 2 : 4),
                             a.vocab);
   float best[GROUPS];
-  const float m = row_max(row, best, sh.edge[1]);
+  const float m = row_max(row, best, sh.edge[1], [](const float (&)[8]) {});
   const float c = static_cast<float>(a.inv_t * 1.4426950408889634);
   const float ref = m > -INFINITY && m < INFINITY ? m : 0.0f;
   Bound bound{INFINITY, 1.0f, 0.0f};
