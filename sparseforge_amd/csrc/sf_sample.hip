@@ -19,7 +19,7 @@
 namespace sf {
 namespace {
 
-constexpr int kSpBins = 2048;
+constexpr int kSpBins = 2048, kSpCandidates = 2048;
 
 struct SampleArgs {
   const void* x;
@@ -137,74 +137,77 @@ __device__ __forceinline__ void sample_any(const SampleArgs& a, const Settings& 
 }
 
 struct SampleShared {
-  TopShared top;
-  u64 weight[kSpBins];  // of the found in their order, or of bins
-  u64 before[kTopCandidates];
-  int id[SF_TOP_MAX_K];
-  float logit[SF_TOP_MAX_K];
+  TopShared<kSpCandidates> top;
+  u64 weight[kSpBins + 64];  // by place, or by bin; in the end a bin for each lane of what has no weight
+  u64 before[kSpCandidates];
   u64 part[2][16];
   u64 total, base, last;
   int count, bin;
 };
 
-// Among the row's n largest, which sh.top.found holds: top-k, top-p, min-p and the draw, by the first THREADS threads (64:
-// the first wave, which waits for nobody).
-template <int THREADS>
-__device__ __forceinline__ void sample_found(const SampleArgs& a, const Settings& s, int64_t r, const Weight& weight,
-                                             int n, SampleShared& sh) {
-  const auto meet = [] SF_INLINE {
-    if constexpr (THREADS == 64)
-      wave_lds_fence();
-    else
-      __syncthreads();
-  };
+// The draw by one wave among the row's n <= 64 largest, which sh.top.found holds in any order: top-k, top-p, min-p and the
+// token.
+__device__ __forceinline__ void sample_few(const SampleArgs& a, const Settings& s, int64_t r, const Weight& weight, int n,
+                                           SampleShared& sh) {
   const int t = threadIdx.x;
-  for (int i = t; i < n; i += THREADS) {
-    const u64 own = sh.top.found[i];
-    const int rank = rank_of(own, sh.top.found, n);
-    if (rank < s.k) {
-      sh.logit[rank] = candidate_logit(own);
-      sh.weight[rank] = weight(sh.logit[rank]);
-      sh.id[rank] = candidate_id(own);
-    }
-  }
-  meet();
+  const u64 own = t < n ? sh.top.found[t] : 0;
+  int rank = 0;
+#pragma unroll 8
+  for (int j = 0; j < n; ++j) rank += sh.top.found[j] > own ? 1 : 0;
+  if (t < n) sh.top.mixed[rank] = own;
+  wave_lds_fence();
   const int k = s.k < n ? static_cast<int>(s.k) : n;
-  const u64 w = t < k ? sh.weight[t] : 0;
-  u64 upto = wave_scan(w), all;
-  if constexpr (THREADS == 64) {
-    all = last_lane(upto);
-  } else {
-    if ((t & 63) == 63) sh.part[0][t >> 6] = upto;
-    if (t == 0) sh.total = 0, sh.count = 0;
-    __syncthreads();
-    all = 0;
-    for (int i = 0; i < THREADS / 64; ++i) {
-      if (i == t >> 6) upto += all;
-      all += sh.part[0][i];
-    }
-  }
-  const bool kept = t < k && (s.p >= 1.0 || upto - w < share_up(s.p, all)) && static_cast<double>(w) >= s.least;
-  int count;
-  u64 total;
-  if constexpr (THREADS == 64) {
-    count = __popcll(__ballot(kept));
-    total = __shfl(upto, count - 1, 64);
-  } else {
-    if (kept) {
-      atomicMax(&sh.total, upto);
-      atomicMax(&sh.count, t + 1);
-    }
-    __syncthreads();
-    count = sh.count, total = sh.total;
-  }
-  if (!kept) return;
-  const int id = sh.id[t];
-  const u64 want = share_down(s.u, total);
+  const u64 c = t < k ? sh.top.mixed[t] : 0;
+  const float x = candidate_logit(c);
+  const int id = candidate_id(c);
+  const u64 w = t < k ? weight(x) : 0, upto = wave_scan(w);
+  const bool kept = t < k && (s.p >= 1.0 || upto - w < share_up(s.p, last_lane(upto))) && static_cast<double>(w) >= s.least;
+  const int count = __popcll(__ballot(kept));
+  const u64 total = __shfl(upto, count - 1, 64), want = share_down(s.u, total);
+  sh.weight[t] = w;
+  wave_lds_fence();
   u64 sum = 0;
 #pragma unroll 4
-  for (int i = 0; i < count; ++i) sum += sh.id[i] <= id ? sh.weight[i] : 0;
-  if (sum - w <= want && want < sum) put_token(a, s, r, id, sh.logit[t], total);
+  for (int i = 0; i < count; ++i) sum += candidate_id(sh.top.mixed[i]) <= id ? sh.weight[i] : 0;
+  if (kept && sum - w <= want && want < sum) put_token(a, s, r, id, x, total);
+}
+
+// The same by the workgroup among the n largest in order.  Ids are drawn from by ranges: the range in which the sum passes
+// the drawn share, then the token among the kept ones of that range.
+template <int BLK>
+__device__ __forceinline__ void sample_sorted(const SampleArgs& a, const Settings& s, int64_t r, const Weight& weight,
+                                              int n, SampleShared& sh) {
+  const int t = threadIdx.x, k = s.k < n ? static_cast<int>(s.k) : n;  // k <= BLK
+  const u64 c = t < k ? sh.top.found[t] : 0;
+  const float x = candidate_logit(c);
+  const int id = candidate_id(c);
+  const u64 w = t < k ? weight(x) : 0;
+  sh.weight[t] = 0;
+  if (t == 0) sh.count = 0;
+  const u64 upto = block_scan<BLK>(w, sh.part[0]);
+  u64 all = 0;
+  for (int i = 0; i < BLK / 64; ++i) all += sh.part[0][i];
+  const bool kept = t < k && (s.p >= 1.0 || upto - w < share_up(s.p, all)) && static_cast<double>(w) >= s.least;
+  const int width = (a.vocab + BLK - 1) / BLK, range = id / width;
+  if (kept) atomicAdd(&sh.weight[range], w);
+  __syncthreads();
+  const u64 mine = sh.weight[t], end = block_scan<BLK>(mine, sh.part[1]);
+  u64 total = 0;
+  for (int i = 0; i < BLK / 64; ++i) total += sh.part[1][i];
+  const u64 want = share_down(s.u, total);
+  if (end - mine <= want && want < end) sh.bin = t, sh.base = end - mine;
+  __syncthreads();
+  if (kept && range == sh.bin) {
+    const int at = atomicAdd(&sh.count, 1);
+    sh.top.mixed[at] = c;
+    sh.before[at] = w;
+  }
+  __syncthreads();
+  if (kept && range == sh.bin) {
+    u64 sum = sh.base;
+    for (int i = 0; i < sh.count; ++i) sum += candidate_id(sh.top.mixed[i]) <= id ? sh.before[i] : 0;
+    if (sum - w <= want && want < sum) put_token(a, s, r, id, x, total);
+  }
 }
 
 // Places of logits in a histogram from the largest down; what has no weight ends in the last bin.
@@ -229,24 +232,35 @@ struct Last {
   __device__ __forceinline__ bool keeps(float y, int i) const { return (y > x) | ((y == x) & (i <= id)); }
 };
 
-// The last element, in the order of logits, at which the sum of amount(x, id) before it is below want(whole sum): found in
-// last.  False: more than kTopCandidates are in the bin where that happens.  A sum that stays below takes in everything.
-template <int DT, int BLK, int H, typename M, typename A>
-__device__ __forceinline__ bool border_of(Row<DT, BLK, H>& row, const Bins& bins, M&& amount, A&& want,
+// Adds the elements' weights (KIND 1), those that `last` keeps (KIND 2), or their number (KIND 0) to the bins.
+template <int KIND, int DT, int BLK, int H>
+__device__ __forceinline__ void fill_bins(Row<DT, BLK, H>& row, const Bins& bins, const Last& last, const Weight& weight,
+                                          SampleShared& sh) {
+  // what is added has no branch around it, so that several elements are on their way at a time
+  const int none = kSpBins + (threadIdx.x & 63);
+  row.each_looped([&](int, int i, const float (&v)[8]) SF_INLINE {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const u64 w = KIND == 0 ? 1 : weight(v[k]);
+      const bool counts = KIND == 2 ? last.keeps(v[k], i + k) & (v[k] > -INFINITY) : v[k] > -INFINITY;
+      atomicAdd(&sh.weight[counts ? bins.of(v[k]) : none], w);
+      if (k % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // four at a time: eight take more registers than there are
+    }
+  });
+}
+
+// The last element, in the order of logits, at which what the bins hold (see fill_bins) of the elements before it is below
+// want(whole sum): found in last.  amount(x, id): of one element.  False: more than kSpCandidates are in the bin where
+// that happens.  A sum that stays below takes in everything.
+template <int DT, int BLK, int H, typename P, typename M, typename A>
+__device__ __forceinline__ bool border_of(Row<DT, BLK, H>& row, const Bins& bins, P&& fill, M&& amount, A&& want,
                                           Last& last, SampleShared& sh) {
   constexpr int kEach = kSpBins / BLK;
   const int t = threadIdx.x;
   for (int i = t; i < kSpBins; i += BLK) sh.weight[i] = 0;
   if (t == 0) sh.bin = -1, sh.top.n = 0;
   __syncthreads();
-  row.each_looped([&](int, int i, const float (&v)[8]) SF_INLINE {
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const u64 w = amount(v[k], i + k);
-      if (w != 0) atomicAdd(&sh.weight[bins.of(v[k])], w);
-      if (k % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // four at a time: eight take more registers than there are
-    }
-  });
+  fill();
   __syncthreads();
   u64 own[kEach], sum = 0;
 #pragma unroll
@@ -262,17 +276,24 @@ __device__ __forceinline__ bool border_of(Row<DT, BLK, H>& row, const Bins& bins
   __syncthreads();
   const int bin = sh.bin;
   if (bin < 0) return true;
-  uint32_t hits = 0;
   float low, high;
   bins.range(bin, low, high);
-  row.each([&](int p, int, const float (&v)[8]) SF_INLINE {
+  row.each_looped([&](int, int i, const float (&v)[8]) SF_INLINE {
     bool any = false;
 #pragma unroll
     for (int k = 0; k < 8; ++k) any |= __builtin_amdgcn_fmed3f(v[k], low, high) == v[k];
-    if (any) hits |= 1u << p;
+    if (any) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (v[k] > -INFINITY && bins.of(v[k]) == bin) {
+          const int at = atomicAdd(&sh.top.n, 1);
+          if (at < kSpCandidates) sh.top.found[at] = candidate(v[k], i + k);
+        }
+    }
   });
-  const int n = gather(row, [&](float x) { return bins.of(x) == bin; }, hits, sh.top);
-  if (n > kTopCandidates) return false;
+  __syncthreads();
+  const int n = sh.top.n;
+  if (n > kSpCandidates) return false;
   for (int i = t; i < n; i += BLK) {
     const u64 c = sh.top.found[i];
     sh.weight[i] = amount(candidate_logit(c), candidate_id(c));
@@ -285,6 +306,7 @@ __device__ __forceinline__ bool border_of(Row<DT, BLK, H>& row, const Bins& bins
     const int i = at % n, from = at / n * size, to = from + size < n ? from + size : n;
     const u64 c = sh.top.found[i];
     u64 sum = 0;
+#pragma unroll 4
     for (int j = from; j < to; ++j) sum += sh.top.found[j] > c ? sh.weight[j] : 0;
     atomicAdd(&sh.before[i], sum);
   }
@@ -303,12 +325,23 @@ __device__ __forceinline__ void draw(const SampleArgs& a, const Settings& s, int
                                      const Last& last, const Weight& weight, SampleShared& sh) {
   const int t = threadIdx.x;
   double sum = Weight::kWhole;
+  // of the pieces behind last.id only what is larger than last.x
+  const uint32_t key = ordered_key(last.x) + 1;
+  const float above = last.x == INFINITY ? INFINITY : __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
   row.each_looped([&](int, int i, const float (&v)[8]) SF_INLINE {
-    if (ALL || max8(v) >= last.x) {
+    const float least = i > last.id ? above : last.x;
+    if (ALL || max8(v) >= least) {
+      float x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = ALL || v[k] >= least ? v[k] : -INFINITY;
+      if (!ALL && i <= last.id && last.id < i + 7) {  // the piece that it ends in
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (!last.keeps(x[k], i + k)) x[k] = -INFINITY;
+      }
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        const double w = weight.scaled(v[k]);
-        sum += ALL || last.keeps(v[k], i + k) ? w : 0.0;
+        sum += weight.scaled(x[k]);  // -inf: 2^-20, which the sum of integers does not see
         if (k % 4 == 3) __builtin_amdgcn_sched_barrier(0);
       }
     }
@@ -358,7 +391,7 @@ __device__ __forceinline__ float least_logit(const Settings& s, const Weight& we
 }
 
 template <int DT, int BLK, int H>
-__global__ void __launch_bounds__(BLK) sample_kernel(SampleArgs a) {
+__global__ void __launch_bounds__(BLK, 4) sample_kernel(SampleArgs a) {
   __shared__ union {
     SampleShared sh;
     AnyShared any;
@@ -402,11 +435,13 @@ __global__ void __launch_bounds__(BLK) sample_kernel(SampleArgs a) {
       if (bound.holds(max8(v))) hits |= 1u << p;
     });
     const int n = gather(row, [&](float x) { return bound.holds(x); }, hits, sh.top);
-    done = n > 0 && n <= kTopCandidates;
-    if (done && n > 64)
-      sample_found<BLK>(a, s, r, weight, n, sh);
-    else if (done && threadIdx.x < 64)
-      sample_found<64>(a, s, r, weight, n, sh);
+    done = n > 0 && n <= kSpCandidates;
+    if (done && n > 64) {
+      sort_found<BLK>(bound, n, sh.top);
+      sample_sorted<BLK>(a, s, r, weight, n, sh);
+    } else if (done && threadIdx.x < 64) {
+      sample_few(a, s, r, weight, n, sh);
+    }
   } else if (done) {
     Last last;
     if (binned) {
@@ -418,11 +453,20 @@ __global__ void __launch_bounds__(BLK) sample_kernel(SampleArgs a) {
       const float range = fminf(m - low, static_cast<float>((a.bits + 1) * 0.6931471805599453 * s.temp));
       const Bins bins{m, fminf(kSpBins / range, 1e30f)};
       // by number for top-k, by weight among these for top-p
+      const bool cut = s.k < a.vocab;
 #pragma unroll 1
-      for (int by_weight = s.k < a.vocab ? 0 : 1; done && by_weight < (s.p < 1.0 ? 2 : 1); ++by_weight) {
+      for (int by_weight = cut ? 0 : 1; done && by_weight < (s.p < 1.0 ? 2 : 1); ++by_weight) {
         done = border_of(
             row, bins,
-            [&](float x, int id) -> u64 { return !last.keeps(x, id) ? 0 : by_weight ? weight(x) : x > -INFINITY; },
+            [&]() SF_INLINE {
+              if (!by_weight)
+                fill_bins<0>(row, bins, last, weight, sh);
+              else if (!cut)
+                fill_bins<1>(row, bins, last, weight, sh);
+              else
+                fill_bins<2>(row, bins, last, weight, sh);
+            },
+            [&](float x, int id) -> u64 { return !last.keeps(x, id) ? 0 : by_weight ? weight(x) : 1; },
             [&](u64 total) { return by_weight ? share_up(s.p, total) : static_cast<u64>(s.k); }, last, sh);
         __syncthreads();
       }

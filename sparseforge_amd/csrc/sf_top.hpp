@@ -213,11 +213,14 @@ __device__ __forceinline__ float candidate_logit(u64 c) {
 }
 
 constexpr int kTopBins = 1024;
-constexpr int kTopCandidates = 2048;
 
+// CAP: candidates that there is room for.
+template <int CAP>
 struct TopShared {
+  static constexpr int kCap = CAP;
   uint32_t bins[kTopBins];
-  u64 found[kTopCandidates];
+  u64 found[CAP], mixed[CAP];
+  uint32_t start[kTopBins + 1];
   uint32_t part[16];
   float edge[2][16];
   uint32_t limit;
@@ -234,8 +237,8 @@ struct Bound {
 
 // best: the thread's groups' maxima (no NaN, not inf), m: the row's.  Where fewer than k groups have anything above -inf
 // the bound takes everything above it.  sh.n is 0 afterwards.
-template <int BLK, int GROUPS>
-__device__ __forceinline__ Bound top_bound(const float (&best)[GROUPS], float m, int k, TopShared& sh) {
+template <int BLK, int GROUPS, int CAP>
+__device__ __forceinline__ Bound top_bound(const float (&best)[GROUPS], float m, int k, TopShared<CAP>& sh) {
   const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
   constexpr int kEach = kTopBins / BLK;
   float low = INFINITY;
@@ -271,10 +274,10 @@ __device__ __forceinline__ Bound top_bound(const float (&best)[GROUPS], float m,
 }
 
 // Gathers into sh.found the elements that wanted(x) holds for, of the thread's pieces whose bit is set in hits, and returns
-// how many there are in all (sh.n has to be 0 before); more than kTopCandidates: too many (equal ones, most likely), and not all are there.  The pieces
+// how many there are in all (sh.n has to be 0 before); more than CAP: too many (equal ones, most likely), and not all are there.  The pieces
 // come from the caches: eight tests for each piece in registers are more code than the instruction cache holds.
-template <int DT, int BLK, int H, typename F>
-__device__ __forceinline__ int gather(const Row<DT, BLK, H>& row, F&& wanted, uint32_t hits, TopShared& sh) {
+template <int DT, int BLK, int H, int CAP, typename F>
+__device__ __forceinline__ int gather(const Row<DT, BLK, H>& row, F&& wanted, uint32_t hits, TopShared<CAP>& sh) {
   while (hits) {
     const int i = row.at(__ffs(hits) - 1);
     hits &= hits - 1;
@@ -286,14 +289,49 @@ __device__ __forceinline__ int gather(const Row<DT, BLK, H>& row, F&& wanted, ui
     for (int j = 0; j < 8; ++j)
       if (wanted(v[j])) {
         const int at = atomicAdd(&sh.n, 1);
-        if (at < kTopCandidates) sh.found[at] = candidate(v[j], i + j);
+        if (at < CAP) sh.found[at] = candidate(v[j], i + j);
       }
   }
   __syncthreads();
-  const int n = sh.n;
-  if (threadIdx.x == 0 && n < kTopCandidates && n % 2) sh.found[n] = 0;  // rank_of reads two at a time
+  return sh.n;
+}
+
+// Orders sh.found[0 .. n), elements within the bound: counted into the bound's bins, then placed among those of their bin.
+template <int BLK, int CAP>
+__device__ __forceinline__ void sort_found(const Bound& bound, int n, TopShared<CAP>& sh) {
+  constexpr int kEach = kTopBins / BLK;
+  const int t = threadIdx.x;
+  const auto bin_of = [&](u64 c) SF_INLINE {
+    return static_cast<int>(fminf((bound.m - candidate_logit(c)) * bound.scale, static_cast<float>(kTopBins - 1)));
+  };
+  for (int i = t; i < kTopBins; i += BLK) sh.bins[i] = 0;
   __syncthreads();
-  return n;
+  for (int i = t; i < n; i += BLK) atomicAdd(&sh.bins[bin_of(sh.found[i])], 1u);
+  __syncthreads();
+  uint32_t own[kEach], sum = 0;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) sum += own[i] = sh.bins[t * kEach + i];
+  uint32_t at = block_scan<BLK>(sum, sh.part) - sum;
+#pragma unroll
+  for (int i = 0; i < kEach; ++i) {
+    sh.bins[t * kEach + i] = sh.start[t * kEach + i] = at;
+    at += own[i];
+  }
+  if (t == 0) sh.start[kTopBins] = n;
+  __syncthreads();
+  for (int i = t; i < n; i += BLK) {
+    const u64 c = sh.found[i];
+    sh.mixed[atomicAdd(&sh.bins[bin_of(c)], 1u)] = c;
+  }
+  __syncthreads();
+  for (int i = t; i < n; i += BLK) {
+    const u64 c = sh.mixed[i];
+    const int bin = bin_of(c), from = sh.start[bin], to = sh.start[bin + 1];
+    int rank = from;
+    for (int j = from; j < to; ++j) rank += sh.mixed[j] > c ? 1 : 0;
+    sh.found[rank] = c;
+  }
+  __syncthreads();
 }
 
 // Maxima of the thread's groups of pieces; the row's, NaN if it has one, in every thread.  also(elements): of every piece.
@@ -317,17 +355,6 @@ __device__ __forceinline__ float row_max(const Row<DT, BLK, H>& row, float (&bes
   m = part[0];
   for (int w = 1; w < BLK / 64; ++w) m = nan_max(m, part[w]);
   return m;
-}
-
-// How many of the n candidates come before c; where n is odd found[n] is 0.
-__device__ __forceinline__ int rank_of(u64 c, const u64* found, int n) {
-  int rank = 0;
-#pragma unroll 4
-  for (int j = 0; j < n; j += 2) {
-    const ulonglong2 x = *reinterpret_cast<const ulonglong2*>(found + j);
-    rank += (x.x > c ? 1 : 0) + (x.y > c ? 1 : 0);
-  }
-  return rank;
 }
 
 // ---------------------------------------------------------------------------

@@ -3,7 +3,7 @@
 //
 // One workgroup per row, which it holds in registers if it fits: a pass for the maxima of the threads' parts, from which a
 // bound follows above which the k largest and few others lie (gather_top); a pass that gathers these in LDS and sums the
-// exponentials; then each candidate counts those before it, which is its place in the output.
+// exponentials; then orders them.
 #include <type_traits>
 
 #include "sf_top.hpp"
@@ -32,8 +32,9 @@ __device__ __forceinline__ void put(const TopLogitsArgs& a, const void* row, int
 }
 
 // Any row: the k-th largest key by its bits, then the elements above it and the first of its equals.
-template <int DT, int BLK>
-__device__ __forceinline__ void top_of_any(const TopLogitsArgs& a, const void* row, int64_t r, AnyShared& any, TopShared& sh) {
+template <int DT, int BLK, int CAP>
+__device__ __forceinline__ void top_of_any(const TopLogitsArgs& a, const void* row, int64_t r, AnyShared& any,
+                                           TopShared<CAP>& sh) {
   const int t = threadIdx.x, V = a.vocab;
   const Border border = radix_border<DT, BLK>(row, V, false, a.k, [](float) { return 0ull; }, any);
   const int last = locate<DT, BLK>(
@@ -48,15 +49,19 @@ __device__ __forceinline__ void top_of_any(const TopLogitsArgs& a, const void* r
     const uint32_t key = top_key<DT>(x);
     if (key > border.key || (key == border.key && i <= last)) sh.found[atomicAdd(&sh.n, 1)] = candidate(x, i);
   }
-  if (t == 0 && a.k % 2) sh.found[a.k] = 0;
   __syncthreads();
-  for (int i = t; i < a.k; i += BLK) put<DT>(a, row, r, rank_of(sh.found[i], sh.found, a.k), candidate_id(sh.found[i]));
+  for (int i = t; i < a.k; i += BLK) {
+    const u64 own = sh.found[i];
+    int rank = 0;
+    for (int j = 0; j < a.k; ++j) rank += sh.found[j] > own ? 1 : 0;
+    put<DT>(a, row, r, rank, candidate_id(own));
+  }
 }
 
-// H: pieces of 8 elements that a thread keeps in registers.
-template <int DT, int BLK, int H, int GROUPS>
+// H: pieces of 8 elements that a thread keeps in registers.  k is at most BLK * GROUPS / 2 and CAP.
+template <int DT, int BLK, int H, int GROUPS, int CAP>
 __global__ void __launch_bounds__(BLK) top_logits_kernel(TopLogitsArgs a) {
-  __shared__ TopShared sh;
+  __shared__ TopShared<CAP> sh;
   __shared__ AnyShared any;
   __shared__ double sums[BLK / 64];
   const int64_t r = blockIdx.x;
@@ -86,14 +91,11 @@ __global__ void __launch_bounds__(BLK) top_logits_kernel(TopLogitsArgs a) {
   for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
   if ((t & 63) == 0) sums[t >> 6] = total;
   const int n = ref == m ? gather(row, [&](float x) { return bound.holds(x); }, hits, sh) : 0;
-  if (n < a.k || n > kTopCandidates) {  // -inf, inf or NaN among the k, or too many equals
+  if (n < a.k || n > CAP) {  // -inf, inf or NaN among the k, or too many equals
     top_of_any<DT, BLK>(a, row.row, r, any, sh);
   } else {
-    for (int i = t; i < n; i += BLK) {
-      const u64 own = sh.found[i];
-      const int rank = rank_of(own, sh.found, n);
-      if (rank < a.k) put<DT>(a, row.row, r, rank, candidate_id(own));
-    }
+    sort_found<BLK>(bound, n, sh);
+    for (int i = t; i < a.k; i += BLK) put<DT>(a, row.row, r, i, candidate_id(sh.found[i]));
   }
   __syncthreads();
   if (t == 0 && a.lse) {
@@ -133,9 +135,9 @@ extern "C" int sf_top_logits(const sf_top_logits_desc* desc, void* stream) {
   auto with = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     if (d.rows >= 512 && d.k <= 128 && d.vocab <= 256 * 8 * 32)
-      top_logits_kernel<DT, 256, DT == SF_DTYPE_BF16 ? 16 : 8, 1><<<grid, 256, 0, st>>>(a);
+      top_logits_kernel<DT, 256, DT == SF_DTYPE_BF16 ? 16 : 8, 1, 512><<<grid, 256, 0, st>>>(a);
     else
-      top_logits_kernel<DT, 1024, 8, 2><<<grid, 1024, 0, st>>>(a);
+      top_logits_kernel<DT, 1024, 8, 2, 2048><<<grid, 1024, 0, st>>>(a);
   };
   if (d.dtype == SF_DTYPE_BF16)
     with(std::integral_constant<int, SF_DTYPE_BF16>{});
