@@ -216,7 +216,7 @@ struct Bins {
   __device__ __forceinline__ int of(float x) const {
     return static_cast<int>(fminf((top - x) * scale, static_cast<float>(kSpBins - 1)));
   }
-  // The logits of a bin lie between these (and others may).
+  // The logits of a bin lie between these (and a few beside it).
   __device__ __forceinline__ void range(int bin, float& low, float& high) const {
     const float a = (static_cast<float>(bin) - 0.01f) / scale, b = (static_cast<float>(bin) + 1.01f) / scale;
     const float off = 1e-6f * (fabsf(top) + b);
@@ -279,13 +279,13 @@ __device__ __forceinline__ bool border_of(Row<DT, BLK, H>& row, const Bins& bins
   float low, high;
   bins.range(bin, low, high);
   row.each_looped([&](int, int i, const float (&v)[8]) SF_INLINE {
-    bool any = false;
+    bool in[8], any = false;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) any |= __builtin_amdgcn_fmed3f(v[k], low, high) == v[k];
+    for (int k = 0; k < 8; ++k) any |= in[k] = __builtin_amdgcn_fmed3f(v[k], low, high) == v[k];
     if (any) {
 #pragma unroll
       for (int k = 0; k < 8; ++k)
-        if (v[k] > -INFINITY && bins.of(v[k]) == bin) {
+        if (in[k]) {
           const int at = atomicAdd(&sh.top.n, 1);
           if (at < kSpCandidates) sh.top.found[at] = candidate(v[k], i + k);
         }
@@ -296,7 +296,8 @@ __device__ __forceinline__ bool border_of(Row<DT, BLK, H>& row, const Bins& bins
   if (n > kSpCandidates) return false;
   for (int i = t; i < n; i += BLK) {
     const u64 c = sh.top.found[i];
-    sh.weight[i] = amount(candidate_logit(c), candidate_id(c));
+    const float x = candidate_logit(c);
+    sh.weight[i] = x > -INFINITY && bins.of(x) == bin ? amount(x, candidate_id(c)) : 0;  // others are beside the bin
     sh.before[i] = sh.base;
   }
   __syncthreads();
@@ -390,7 +391,8 @@ __device__ __forceinline__ float least_logit(const Settings& s, const Weight& we
   return kept ? __shfl(x, 63 - __clzll(kept), 64) : s.top;
 }
 
-template <int DT, int BLK, int H>
+// WHOLE: without top-k and top-p.
+template <int DT, int BLK, int H, bool WHOLE>
 __global__ void __launch_bounds__(BLK, 4) sample_kernel(SampleArgs a) {
   __shared__ union {
     SampleShared sh;
@@ -410,8 +412,8 @@ __global__ void __launch_bounds__(BLK, 4) sample_kernel(SampleArgs a) {
   s.p = !greedy && top_p < 1.0f ? static_cast<double>(top_p) : 1.0;
   s.one = ldexp(1.0, a.bits);
   s.least = (min_p > 1.0f ? 1.0 : min_p > 0.0f ? static_cast<double>(min_p) : 0.0) * s.one;
-  const bool among = s.k <= BLK && s.k < a.vocab;  // few enough to be gathered
-  const bool binned = !among && (s.k < a.vocab || s.p < 1.0);
+  const bool among = !WHOLE && s.k <= BLK && s.k < a.vocab;  // few enough to be gathered
+  const bool binned = !WHOLE && !among && (s.k < a.vocab || s.p < 1.0);
   float best[2], low = INFINITY;
   const float m = s.top = row_max(row, best, sh.top.edge[1], [&](const float (&v)[8]) SF_INLINE {
     if (binned) {
@@ -522,10 +524,17 @@ extern "C" int sf_sample_logits(const sf_sample_desc* desc, void* stream) {
   auto with = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     constexpr int H = DT == SF_DTYPE_BF16 ? 8 : 4;
-    if (a.vocab <= 512 * 8 * 8 && d.rows > 256)
-      sample_kernel<DT, 512, H><<<grid, 512, 0, st>>>(a);
+    const bool narrow = a.vocab <= 512 * 8 * 8 && d.rows > 256;
+    const bool whole = !a.temp && a.temp1 > 0.0f && !a.top_k && (a.top_k1 <= 0 || a.top_k1 >= a.vocab) && !a.top_p &&
+                       !(a.top_p1 < 1.0f);
+    if (narrow && whole)
+      sample_kernel<DT, 512, H, true><<<grid, 512, 0, st>>>(a);
+    else if (narrow)
+      sample_kernel<DT, 512, H, false><<<grid, 512, 0, st>>>(a);
+    else if (whole)
+      sample_kernel<DT, 1024, H, true><<<grid, 1024, 0, st>>>(a);
     else
-      sample_kernel<DT, 1024, H><<<grid, 1024, 0, st>>>(a);
+      sample_kernel<DT, 1024, H, false><<<grid, 1024, 0, st>>>(a);
   };
   if (d.dtype == SF_DTYPE_BF16)
     with(std::integral_constant<int, SF_DTYPE_BF16>{});
