@@ -4,7 +4,7 @@
 //   top-k keeps the first k; top-p of these the fewest first tokens that hold p of their weight; min-p those of at least
 //   min_p times the largest weight.  All three keep a first part of that order.
 //   the token is the first, by id, at which the weight of the kept tokens up to it exceeds u times their whole weight.
-// Weights are formed in f64 and summed as integers of 2^-F, F = 44 (43 above 131072 tokens): sums do not depend on their order.  A cumulative share is off by 2e-12 (the exponential's polynomial) at most, which decides
+// Weights are formed in f64 and summed as integers of 2^-F, F = 44 (43 above 65536 tokens, 42 above 131072): sums do not depend on their order.  A cumulative share is off by 2e-12 (the exponential's polynomial) at most, which decides
 // one draw in 4e6 from 131072 equal tokens; shares from f32 exponentials, off by 1e-7, would decide one in a hundred.
 //
 // One workgroup per row, which it holds in registers if it fits.  With top-k up to 1024 the row's largest are gathered in
@@ -46,6 +46,19 @@ struct Settings {
   double p;      // 1: all
   double one;    // 2^F
   double least;  // the smallest weight that min-p keeps
+
+  __device__ __forceinline__ Settings(const SampleArgs& a, int64_t r) : top(0.0f) {
+    const float T = a.temp ? a.temp[r] : a.temp1, top_p = a.top_p ? a.top_p[r] : a.top_p1;
+    const float min_p = a.min_p ? a.min_p[r] : a.min_p1;
+    const int top_k = a.top_k ? a.top_k[r] : a.top_k1;
+    const bool greedy = !(T > 0.0f);
+    u = a.u[r];
+    temp = greedy ? 1.0f : T;
+    k = greedy ? 1 : top_k <= 0 || top_k > a.vocab ? a.vocab : top_k;
+    p = !greedy && top_p < 1.0f ? static_cast<double>(top_p) : 1.0;
+    one = ldexp(1.0, a.bits);
+    least = (min_p > 1.0f ? 1.0 : min_p > 0.0f ? static_cast<double>(min_p) : 0.0) * one;
+  }
 };
 
 // Weights exp((x - top) / T) as integers of 2^-bits (bits <= 51); 2^bits exactly for the largest logit, which is finite.
@@ -95,6 +108,13 @@ __device__ __forceinline__ void put_token(const SampleArgs& a, const Settings& s
   if (!a.logprobs) return;
   const double d = x == s.top ? 0.0 : (static_cast<double>(x) - s.top) / static_cast<double>(s.temp);
   a.logprobs[r] = static_cast<float>(d - log(static_cast<double>(total) / s.one));
+}
+
+// A row that holds a NaN, or nothing above -inf.
+__device__ __forceinline__ void put_none(const SampleArgs& a, int64_t r, float m) {
+  if (threadIdx.x != 0) return;
+  a.tokens[r] = -1;
+  if (a.logprobs) a.logprobs[r] = m;
 }
 
 // Any row, by passes over the bits of its logits.
@@ -207,6 +227,51 @@ __device__ __forceinline__ void sample_sorted(const SampleArgs& a, const Setting
     u64 sum = sh.base;
     for (int i = 0; i < sh.count; ++i) sum += candidate_id(sh.top.mixed[i]) <= id ? sh.before[i] : 0;
     if (sum - w <= want && want < sum) put_token(a, s, r, id, x, total);
+  }
+}
+
+template <int BLK>
+__device__ __forceinline__ void sample_found(const SampleArgs& a, const Settings& s, int64_t r, const Weight& weight,
+                                             const Bound& bound, int n, SampleShared& sh) {
+  if (n > 64) {
+    sort_found<BLK>(bound, n, sh.top);
+    sample_sorted<BLK>(a, s, r, weight, n, sh);
+  } else if (threadIdx.x < 64) {
+    sample_few(a, s, r, weight, n, sh);
+  }
+}
+
+// Every row with top-k, of at most BLK (or at temperature 0): the row is read once.
+template <int DT, int BLK, int G>
+__global__ void __launch_bounds__(BLK) sample_top_k_kernel(SampleArgs a) {
+  __shared__ union {
+    SampleShared sh;
+    AnyShared any;
+  } lds;
+  SampleShared& sh = lds.sh;
+  const int64_t r = blockIdx.x;
+  const RowAt<DT, BLK> row(static_cast<const char*>(a.x) + r * a.xs * (DT == SF_DTYPE_BF16 ? 2 : 4), a.vocab);
+  Settings s(a, r);
+  float best[G];
+  read_row(row, best, [](const float (&)[8]) {});
+  float m = best[0];
+#pragma unroll
+  for (int g = 1; g < G; ++g) m = nan_max(m, best[g]);
+  m = s.top = row_max<BLK>(m, sh.top.edge[1]);
+  if (!(m > -INFINITY)) {
+    put_none(a, r, m);
+    return;
+  }
+  const Weight weight{m, 1.4426950408889634 / static_cast<double>(s.temp), a.bits, a.poly};
+  int n = 0;
+  if (m < INFINITY) {
+    const Bound bound = bound_of<BLK>(best, m, static_cast<int>(s.k), sh.top);
+    n = gather<G>(row, bound, hits_of(best, bound), sh.top);
+    if (n > 0 && n <= kSpCandidates) sample_found<BLK>(a, s, r, weight, bound, n, sh);
+  }
+  if (n == 0 || n > kSpCandidates) {
+    __syncthreads();
+    sample_any<DT, BLK>(a, s, r, row.row, weight, lds.any);
   }
 }
 
@@ -401,31 +466,24 @@ __global__ void __launch_bounds__(BLK, 4) sample_kernel(SampleArgs a) {
   SampleShared& sh = lds.sh;
   const int64_t r = blockIdx.x;
   Row<DT, BLK, H> row(static_cast<const char*>(a.x) + r * a.xs * (DT == SF_DTYPE_BF16 ? 2 : 4), a.vocab);
-  const float T = a.temp ? a.temp[r] : a.temp1, top_p = a.top_p ? a.top_p[r] : a.top_p1;
-  const float min_p = a.min_p ? a.min_p[r] : a.min_p1;
-  const int top_k = a.top_k ? a.top_k[r] : a.top_k1;
-  const bool greedy = !(T > 0.0f);
-  Settings s;
-  s.u = a.u[r];
-  s.temp = greedy ? 1.0f : T;
-  s.k = greedy ? 1 : top_k <= 0 || top_k > a.vocab ? a.vocab : top_k;
-  s.p = !greedy && top_p < 1.0f ? static_cast<double>(top_p) : 1.0;
-  s.one = ldexp(1.0, a.bits);
-  s.least = (min_p > 1.0f ? 1.0 : min_p > 0.0f ? static_cast<double>(min_p) : 0.0) * s.one;
+  Settings s(a, r);
   const bool among = !WHOLE && s.k <= BLK && s.k < a.vocab;  // few enough to be gathered
   const bool binned = !WHOLE && !among && (s.k < a.vocab || s.p < 1.0);
-  float best[2], low = INFINITY;
-  const float m = s.top = row_max(row, best, sh.top.edge[1], [&](const float (&v)[8]) SF_INLINE {
+  float best[2] = {-INFINITY, -INFINITY}, low = INFINITY;
+  row.each([&](int p, int, const float (&v)[8]) SF_INLINE {
+    const float x = max8(v);
+    if (p % 2)
+      best[1] = nan_max(best[1], x);
+    else
+      best[0] = nan_max(best[0], x);
     if (binned) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) low = fminf(low, v[k] == -INFINITY ? INFINITY : v[k]);
     }
   });
-  if (m != m || m == -INFINITY) {
-    if (threadIdx.x == 0) {
-      a.tokens[r] = -1;
-      if (a.logprobs) a.logprobs[r] = m;
-    }
+  const float m = s.top = row_max<BLK>(nan_max(best[0], best[1]), sh.top.edge[1]);
+  if (!(m > -INFINITY)) {
+    put_none(a, r, m);
     return;
   }
   const Weight weight{m, 1.4426950408889634 / static_cast<double>(s.temp), a.bits, a.poly};
@@ -436,14 +494,9 @@ __global__ void __launch_bounds__(BLK, 4) sample_kernel(SampleArgs a) {
     row.each([&](int p, int, const float (&v)[8]) SF_INLINE {
       if (bound.holds(max8(v))) hits |= 1u << p;
     });
-    const int n = gather(row, [&](float x) { return bound.holds(x); }, hits, sh.top);
+    const int n = gather<32>(row, bound, hits, sh.top);
     done = n > 0 && n <= kSpCandidates;
-    if (done && n > 64) {
-      sort_found<BLK>(bound, n, sh.top);
-      sample_sorted<BLK>(a, s, r, weight, n, sh);
-    } else if (done && threadIdx.x < 64) {
-      sample_few(a, s, r, weight, n, sh);
-    }
+    if (done) sample_found<BLK>(a, s, r, weight, bound, n, sh);
   } else if (done) {
     Last last;
     if (binned) {
@@ -514,9 +567,8 @@ extern "C" int sf_sample_logits(const sf_sample_desc* desc, void* stream) {
                                0x1.3b2ab70ad2565p-7,  0x1.5d877598350dep-10, 0x1.4308c7183d6a2p-13,
                                0x1.00c0e4e15189cp-16, 0x1.63b2d7971923fp-20};
   memcpy(a.poly, kPoly, sizeof(kPoly));
-  // Sums of vocab weights of at most 2^bits stay below 2^62, those of a thread, which has at most vocab / 512 and 256 of
-  // them, below 2^52.
-  a.bits = 61;
+  // The sums of a thread, which has at most 256 weights of at most 2^bits, and vocab / 512, stay below 2^52.
+  a.bits = 60;
   for (int64_t n = 1; n < d.vocab; n *= 2) --a.bits;
   if (a.bits > 44) a.bits = 44;
   const dim3 grid(static_cast<unsigned>(d.rows));
@@ -524,10 +576,15 @@ extern "C" int sf_sample_logits(const sf_sample_desc* desc, void* stream) {
   auto with = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
     constexpr int H = DT == SF_DTYPE_BF16 ? 8 : 4;
-    const bool narrow = a.vocab <= 512 * 8 * 8 && d.rows > 256;
+    const bool narrow = d.rows > 256 && a.vocab <= (DT == SF_DTYPE_BF16 ? 131072 : 65536);
     const bool whole = !a.temp && a.temp1 > 0.0f && !a.top_k && (a.top_k1 <= 0 || a.top_k1 >= a.vocab) && !a.top_p &&
                        !(a.top_p1 < 1.0f);
-    if (narrow && whole)
+    const bool top_k = (!a.top_k && a.top_k1 > 0 && a.top_k1 <= (narrow ? 512 : 1024)) || (!a.temp && !(a.temp1 > 0.0f));
+    if (narrow && top_k)
+      sample_top_k_kernel<DT, 512, 8><<<grid, 512, 0, st>>>(a);
+    else if (top_k)
+      sample_top_k_kernel<DT, 1024, 8><<<grid, 1024, 0, st>>>(a);
+    else if (narrow && whole)
       sample_kernel<DT, 512, H, true><<<grid, 512, 0, st>>>(a);
     else if (narrow)
       sample_kernel<DT, 512, H, false><<<grid, 512, 0, st>>>(a);

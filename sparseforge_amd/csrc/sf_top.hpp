@@ -51,15 +51,15 @@ struct Raw8 {
   }
 };
 
-// A row in front of a workgroup of BLK threads.  Each wave has a range of the ids of its own, `pieces` times 512 long; of
-// piece p of a wave (at most 32), lane l holds 8 ids.  The first H pieces stay in registers, the others are read again by every pass
-// over the row.  What lies behind the row is -inf.
-template <int DT, int BLK, int H>
-struct Row {
+// A row in front of a workgroup of BLK threads.  Each wave has a range of the ids of its own, `pieces` (at most 32) times
+// 512 long; of piece p of a wave, lane l has 8 ids.  What lies behind the row is -inf.
+template <int DT, int BLK>
+struct RowAt {
   const void* row;
   int vocab, pieces;
-  Raw8<DT> raw[H];
 
+  __device__ __forceinline__ RowAt(const void* row_, int vocab_)
+      : row(row_), vocab(vocab_), pieces((vocab_ + BLK * 8 - 1) / (BLK * 8)) {}
   __device__ __forceinline__ int wave_at(int wave) const { return wave * pieces * 512; }
   __device__ __forceinline__ int at(int p) const {
     return wave_at(threadIdx.x >> 6) + p * 512 + (threadIdx.x & 63) * 8;
@@ -71,8 +71,21 @@ struct Row {
     else
       to.load_some(row, i, n);
   }
-  __device__ __forceinline__ Row(const void* row_, int vocab_) : row(row_), vocab(vocab_) {
-    pieces = (vocab + BLK * 8 - 1) / (BLK * 8);
+};
+
+// One that stays: the first H pieces in registers, the others are read again by every pass over the row.
+template <int DT, int BLK, int H>
+struct Row : RowAt<DT, BLK> {
+  using Base = RowAt<DT, BLK>;
+  using Base::at;
+  using Base::fetch;
+  using Base::pieces;
+  using Base::row;
+  using Base::vocab;
+  using Base::wave_at;
+  Raw8<DT> raw[H];
+
+  __device__ __forceinline__ Row(const void* row_, int vocab_) : Base(row_, vocab_) {
 #pragma unroll
     for (int p = 0; p < H; ++p)
       if (p < pieces) {
@@ -145,6 +158,8 @@ struct Row {
     }
   }
 };
+
+constexpr float kTopLow = -3.402823466e38f;  // start of a running maximum: finite, so that -inf minus it is not NaN
 
 // The larger of two, NaN if either is (v_maximum3_f32 takes two of these).
 __device__ __forceinline__ float nan_max(float a, float b) { return __builtin_elementwise_maximum(a, b); }
@@ -273,24 +288,27 @@ __device__ __forceinline__ Bound top_bound(const float (&best)[GROUPS], float m,
   return {m, scale, sh.limit == ~0u ? INFINITY : static_cast<float>(sh.limit + 1)};
 }
 
-// Gathers into sh.found the elements that wanted(x) holds for, of the thread's pieces whose bit is set in hits, and returns
-// how many there are in all (sh.n has to be 0 before); more than CAP: too many (equal ones, most likely), and not all are there.  The pieces
-// come from the caches: eight tests for each piece in registers are more code than the instruction cache holds.
-template <int DT, int BLK, int H, int CAP, typename F>
-__device__ __forceinline__ int gather(const Row<DT, BLK, H>& row, F&& wanted, uint32_t hits, TopShared<CAP>& sh) {
+// Gathers into sh.found the elements within the bound of the thread's pieces p for which bit p % G of hits is set, and
+// returns how many there are in all (sh.n has to be 0 before); more than CAP: too many (equal ones, most likely), and not
+// all are there.  A thread has few such pieces and takes them from the caches.
+template <int G, int DT, int BLK, int CAP>
+__device__ __forceinline__ int gather(const RowAt<DT, BLK>& row, const Bound& bound, uint32_t hits, TopShared<CAP>& sh) {
   while (hits) {
-    const int i = row.at(__ffs(hits) - 1);
-    hits &= hits - 1;
-    Raw8<DT> raw;
-    float v[8];
-    row.fetch(raw, i);
-    raw.get(v);
+#pragma unroll 1
+    for (int p = __ffs(hits) - 1; p < row.pieces; p += G) {
+      const int i = row.at(p);
+      Raw8<DT> raw;
+      float v[8];
+      row.fetch(raw, i);
+      raw.get(v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (wanted(v[j])) {
-        const int at = atomicAdd(&sh.n, 1);
-        if (at < CAP) sh.found[at] = candidate(v[j], i + j);
-      }
+      for (int j = 0; j < 8; ++j)
+        if (bound.holds(v[j])) {
+          const int at = atomicAdd(&sh.n, 1);
+          if (at < CAP) sh.found[at] = candidate(v[j], i + j);
+        }
+    }
+    hits &= hits - 1;
   }
   __syncthreads();
   return sh.n;
@@ -334,27 +352,73 @@ __device__ __forceinline__ void sort_found(const Bound& bound, int n, TopShared<
   __syncthreads();
 }
 
-// Maxima of the thread's groups of pieces; the row's, NaN if it has one, in every thread.  also(elements): of every piece.
-template <int DT, int BLK, int H, int GROUPS, typename F>
-__device__ __forceinline__ float row_max(const Row<DT, BLK, H>& row, float (&best)[GROUPS], float* part, F&& also) {
-#pragma unroll
-  for (int g = 0; g < GROUPS; ++g) best[g] = -INFINITY;
-  row.each([&](int p, int, const float (&v)[8]) SF_INLINE {
-    const float x = max8(v);
-    also(v);
-#pragma unroll
-    for (int g = 0; g < GROUPS; ++g)
-      if (GROUPS == 1 || p % GROUPS == g) best[g] = nan_max(best[g], x);
-  });
-  float m = best[0];
-#pragma unroll
-  for (int g = 1; g < GROUPS; ++g) m = nan_max(m, best[g]);
+// The largest of the threads' m, NaN if one is, in every thread.
+template <int BLK>
+__device__ __forceinline__ float row_max(float m, float* part) {
   m = last_lane(wave_scan(m, -INFINITY, [](float a, float b) { return nan_max(a, b); }));
   if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = m;
   __syncthreads();
   m = part[0];
   for (int w = 1; w < BLK / 64; ++w) m = nan_max(m, part[w]);
   return m;
+}
+
+// Reads a row once: the maxima of the thread's G groups of pieces (piece p is in group p % G), and also(elements) for every
+// piece, four pieces on their way at a time.
+template <int G, int DT, int BLK, typename F>
+__device__ __forceinline__ void read_row(const RowAt<DT, BLK>& row, float (&best)[G], F&& also) {
+#pragma unroll
+  for (int g = 0; g < G; ++g) best[g] = -INFINITY;
+#pragma unroll 1
+  for (int q = 0; q < row.pieces; q += G)
+#pragma unroll
+    for (int g = 0; g < G; g += 4)
+      if (q + g < row.pieces) {
+        Raw8<DT> raw[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          if (row.at(q + g + u) + 8 <= row.vocab && q + g + u < row.pieces)
+            raw[u].load(row.row, row.at(q + g + u));
+          else
+            raw[u].empty();
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          float v[8];
+          raw[u].get(v);
+          best[g + u] = nan_max(best[g + u], max8(v));
+          also(v);
+        }
+      }
+  if (row.vocab % 8 != 0) {  // one thread has a piece that the row ends in
+    const int i = row.vocab / 8 * 8 - row.wave_at(threadIdx.x >> 6);
+    if (i >= 0 && i < row.pieces * 512 && i % 512 / 8 == static_cast<int>(threadIdx.x & 63)) {
+      Raw8<DT> raw;
+      float v[8];
+      raw.load_some(row.row, row.vocab / 8 * 8, row.vocab % 8);
+      raw.get(v);
+      const float x = max8(v);
+#pragma unroll
+      for (int g = 0; g < G; ++g)
+        if (i / 512 % G == g) best[g] = nan_max(best[g], x);
+      also(v);
+    }
+  }
+}
+// The bound for k elements from the groups' maxima of read_row, taken together to two a thread.
+template <int BLK, int G, int CAP>
+__device__ __forceinline__ Bound bound_of(const float (&best)[G], float m, int k, TopShared<CAP>& sh) {
+  float two[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+  for (int g = 0; g < G; ++g) two[g & 1] = fmaxf(two[g & 1], best[g]);
+  return top_bound<BLK>(two, m, k, sh);
+}
+template <int G>
+__device__ __forceinline__ uint32_t hits_of(const float (&best)[G], const Bound& bound) {
+  uint32_t hits = 0;
+#pragma unroll
+  for (int g = 0; g < G; ++g) hits |= bound.holds(best[g]) ? 1u << g : 0u;
+  return hits;
 }
 
 // ---------------------------------------------------------------------------

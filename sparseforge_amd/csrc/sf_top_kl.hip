@@ -20,8 +20,7 @@ namespace {
 
 constexpr int kTkForwardU = 3, kTkBackwardU = 4;  // pieces of a row a thread loads before using them
 constexpr int kTkSecond = 512;
-constexpr int kTkStats = 6;  // f64 of a row that the backward needs
-constexpr float kTkLow = -3.0e38f;  // start of a running maximum: finite, so that -inf minus it is -inf and not NaN
+constexpr int kTkStats = 8;  // f64 of a row's RowStats
 
 struct TopKlArgs {
   const void* s;
@@ -35,10 +34,15 @@ struct TopKlArgs {
   double inv_t;
 };
 
+// What the backward needs of a row.  Z = top / T + lz and Z_r = top / T + lzr, N = nb + ln: in two parts, so that rows of
+// huge logits (all at the type's lowest value, say) keep their differences.
 struct RowStats {
-  double z, zr, n, p, r;  // Z, Z_r, N, P, r; in units of a
-  double twice;           // an id is listed more than once
+  double top, lz, lzr;
+  double nb, ln;
+  double p, r;
+  double twice;  // an id is listed more than once
 };
+static_assert(sizeof(RowStats) == kTkStats * sizeof(double), "stats of a row");
 
 // Words of a row's marks.
 __host__ __device__ __forceinline__ int mark_words(int vocab) { return (vocab + 8) / 32 + 1; }
@@ -202,13 +206,15 @@ __device__ __forceinline__ bool first_of_id(const TopKlArgs& a, int64_t r, int k
 
 // What a wave finds of a row.
 struct WavePart {
-  double nb, e0, e1, e2;  // listed: sums of e = exp(b - nb), of e (b - nb), of e a
+  double nb, e0, e1, e2;  // listed: sums of e = exp(b - nb), of e (b - nb), of e (s - ml)
   double ml, sl;          // listed students: maximum and sum of exponentials
   float m, sum;           // tokens of the stream: maximum and sum of exponentials
 };
 
-// exp(x - top) for sums whose maximum is top; nothing counts 0.
-__device__ __forceinline__ double exp_from(double x, double top) { return x == -INFINITY ? 0.0 : exp(x - top); }
+// exp((x - top) / T) for sums whose maximum is top; nothing counts 0.
+__device__ __forceinline__ double exp_from(double x, double top, double inv_t) {
+  return x == -INFINITY ? 0.0 : exp((x - top) * inv_t);
+}
 
 // REST: with the teacher's log-sum-exp; the stream then leaves out the listed tokens.
 template <int DT, int BLK, bool REST>
@@ -226,7 +232,7 @@ __global__ void __launch_bounds__(BLK) top_kl_kernel(TopKlArgs a, double* __rest
   const void* rows[1] = {row_at<DT>(a.s, (r / a.inner) * a.s0 + (r % a.inner) * a.s1)};
   const Cut cut = Cut::of<DT, BLK>(rows[0], a.vocab);
   const float c = static_cast<float>(a.inv_t * 1.4426950408889634);
-  float m = kTkLow, sum = 0.0f, lost = 0.0f;
+  float m = kTopLow, sum = 0.0f, lost = 0.0f;
   WavePart part{REST ? static_cast<double>(a.lse[r]) : -INFINITY, 0.0, 0.0, 0.0, -INFINITY, 0.0, 0.0f, 0.0f};
   // The row's first loads are on their way while the listed tokens are marked and summed: the latter by the waves that
   // have some, each with its own maxima, so that no wave waits for another before the row's end.
@@ -241,7 +247,7 @@ __global__ void __launch_bounds__(BLK) top_kl_kernel(TopKlArgs a, double* __rest
       const int id = tk_id(a, r * a.k + k);
       if (id < 0) continue;
       if (!REST) part.nb = fmax(part.nb, load_as_f32(a.values, r * a.k + k, a.vdt) * a.inv_t);
-      part.ml = fmax(part.ml, load_as_f32(rows[0], id, DT) * a.inv_t);
+      part.ml = fmax(part.ml, static_cast<double>(load_as_f32(rows[0], id, DT)));
     }
     double most[2] = {part.nb, part.ml};
     lanes_max(most);
@@ -250,14 +256,14 @@ __global__ void __launch_bounds__(BLK) top_kl_kernel(TopKlArgs a, double* __rest
     for (int k = t; k < a.k; k += BLK) {
       const int id = tk_id(a, r * a.k + k);
       if (id < 0) continue;
-      const double b = load_as_f32(a.values, r * a.k + k, a.vdt) * a.inv_t, s = load_as_f32(rows[0], id, DT) * a.inv_t;
+      const double b = load_as_f32(a.values, r * a.k + k, a.vdt) * a.inv_t, s = load_as_f32(rows[0], id, DT);
       const double e = part.nb == -INFINITY ? 0.0 : exp(b - part.nb);
       if (!(e <= 0.0)) {
         part.e0 += e;
         part.e1 += e * (b - part.nb);
-        part.e2 += e * s;
+        part.e2 += s == -INFINITY ? -INFINITY : e * (s - part.ml);
       }
-      if (REST && (!twice || first_of_id(a, r, k, id))) part.sl += exp_from(s, part.ml);
+      if (REST && (!twice || first_of_id(a, r, k, id))) part.sl += exp_from(s, part.ml, a.inv_t);
     }
     double x[4] = {part.e0, part.e1, part.e2, part.sl};
     lanes_sum(x);
@@ -298,19 +304,21 @@ __global__ void __launch_bounds__(BLK) top_kl_kernel(TopKlArgs a, double* __rest
   // the waves' parts, one to a lane
   constexpr int W = BLK / 64;
   part = parts[lane % W];
-  double most[3] = {part.nb, part.ml, static_cast<double>(part.m) * a.inv_t};
+  double most[3] = {part.nb, part.ml, static_cast<double>(part.m)};
   lanes_max<W>(most);
   const double nb = most[0], top = fmax(most[1], most[2]);
+  if (part.e0 != 0.0) part.e2 += part.e0 * (part.ml == -INFINITY ? 0.0 : part.ml - top);
   if (!REST && part.nb != nb) {
-    const double f = exp_from(part.nb, nb), d = part.nb - nb;
+    const double f = exp_from(part.nb, nb, 1.0), d = part.nb - nb;
     part.e1 = f == 0.0 ? 0.0 : f * (part.e1 + d * part.e0);
     part.e0 = f == 0.0 ? 0.0 : f * part.e0;
     part.e2 = f == 0.0 ? 0.0 : f * part.e2;
   }
-  double x[5] = {part.e0, part.e1, part.e2, part.sum == 0.0f ? 0.0 : part.sum * exp(part.m * a.inv_t - top),
-                 part.sl == 0.0 ? 0.0 : part.sl * exp_from(part.ml, top)};
+  double x[5] = {part.e0, part.e1, part.e2,
+                 part.sum == 0.0f ? 0.0 : part.sum * exp((static_cast<double>(part.m) - top) * a.inv_t),
+                 part.sl == 0.0 ? 0.0 : part.sl * exp_from(part.ml, top, a.inv_t)};
   lanes_sum<W>(x);
-  const double e0 = x[0], e1 = x[1], e2 = x[2], rest = x[3], all = x[3] + x[4];
+  const double e0 = x[0], e1 = x[1], e2 = x[2] * a.inv_t, rest = x[3], all = x[3] + x[4];
   RowStats st{};
   if (REST) {
     st.r = e0 > 1.0 ? 0.0 : 1.0 - e0;
@@ -324,15 +332,17 @@ __global__ void __launch_bounds__(BLK) top_kl_kernel(TopKlArgs a, double* __rest
   const double l = log(lane == 0 ? all : lane == 1 ? rest : REST ? st.r : e0);
   if (!REST && e0 != 0.0) st.p = 1.0;
   if (REST) st.p = e0 + st.r;
-  st.z = top + __shfl(l, 0, 64);
-  st.zr = top + __shfl(l, 1, 64);
-  st.n = nb + (REST ? 0.0 : __shfl(l, 2, 64));
+  st.top = top;
+  st.lz = __shfl(l, 0, 64);
+  st.lzr = __shfl(l, 1, 64);
+  st.nb = nb;
+  st.ln = REST ? 0.0 : __shfl(l, 2, 64);
   double kl;
   if (REST) {
-    kl = e1 - e2 + e0 * st.z;
-    if (st.r != 0.0) kl += st.r * (__shfl(l, 2, 64) - (st.zr - st.z));
+    kl = e1 - e2 + e0 * st.lz;
+    if (st.r != 0.0) kl += st.r * (__shfl(l, 2, 64) - (st.lzr - st.lz));
   } else {
-    kl = e0 == 0.0 ? 0.0 : (e1 - e2) / e0 - __shfl(l, 2, 64) + st.z;
+    kl = e0 == 0.0 ? 0.0 : (e1 - e2) / e0 - st.ln + st.lz;
   }
   const int marked = all_flags<BLK>(flags);
   if (!marked) {  // a row without entries adds nothing
@@ -376,18 +386,20 @@ __global__ void __launch_bounds__(kTkFinal) top_kl_dot_kernel(const double* __re
   if (threadIdx.x == 0) *dot = static_cast<float>(x[0]);
 }
 
-// q = exp(s / T - Z) of a row: Z in two parts in the logits' units, hi near s where q is large.  The exponent in base 2,
-// (s - hi) c - lo, rounds in f32 by up to 2^-24 of itself: 1e-6 of q for a token of probability 1e-7, nothing beside
-// bf16's 2^-9; for f32 its whole part is split off and what s - hi and c round is carried along.
+// q = exp(s / T - Z) of a row.  The exponent in base 2, (s - top) c - lo, rounds in f32 by up to 2^-24 of itself: 1e-6 of
+// q for a token of probability 1e-7, nothing beside bf16's 2^-9; for f32 its whole part is split off and what s - top and c
+// round is carried along.
 template <int DT>
 struct RowGrad {
-  float hi, lo, c, c_lo;
+  float hi, lo, c, c_lo, whole, part;  // lo = whole + part
   __device__ __forceinline__ RowGrad(const TopKlArgs& a, const RowStats& st) {
-    const double z = st.z / a.inv_t, k = a.inv_t * 1.4426950408889634;
-    hi = static_cast<float>(z);
-    lo = static_cast<float>((z - static_cast<double>(hi)) * k);
+    const double k = a.inv_t * 1.4426950408889634, l = st.lz * 1.4426950408889634;
+    hi = static_cast<float>(st.top);
+    lo = static_cast<float>(l);
     c = static_cast<float>(k);
     c_lo = static_cast<float>(k - static_cast<double>(c));
+    whole = static_cast<float>(rint(l));
+    part = static_cast<float>(l - rint(l));
   }
   __device__ __forceinline__ float q(float s) const {
     const float d = s - hi;
@@ -395,18 +407,27 @@ struct RowGrad {
     const float back = d - s;  // d + e = s - hi exactly
     const float e = (s - (d - back)) - (hi + back);
     const float n = rintf(d * c);
-    const float f = fmaf(d, c, -n) + fmaf(e, c, fmaf(d, c_lo, -lo));
+    const float f = fmaf(d, c, -n) + fmaf(e, c, fmaf(d, c_lo, -part));
     // below 2^-126 nothing is left to be exact about, and -inf has no parts
-    return n > -126.0f ? ldexpf(__builtin_amdgcn_exp2f(f), static_cast<int>(n)) : __builtin_amdgcn_exp2f(d * c);
+    return n - whole > -126.0f ? ldexpf(__builtin_amdgcn_exp2f(f), static_cast<int>(n - whole))
+                               : __builtin_amdgcn_exp2f(fmaf(d, c, -lo));
   }
 };
 
+// The same in f64, and the listed probability of entry k's own value.
+__device__ __forceinline__ double q_of(const TopKlArgs& a, const RowStats& st, float s) {
+  return exp((static_cast<double>(s) - st.top) * a.inv_t - st.lz);
+}
+__device__ __forceinline__ double p_of(const TopKlArgs& a, const RowStats& st, int64_t at) {
+  return exp((load_as_f32(a.values, at, a.vdt) * a.inv_t - st.nb) - st.ln);
+}
+
 // Probability that the row's record gives to the id of entry k: p_k, and those of entries with the same id.
 __device__ __forceinline__ double listed_p(const TopKlArgs& a, const RowStats& st, int64_t r, int k, int id) {
-  if (st.twice == 0.0) return exp(load_as_f32(a.values, r * a.k + k, a.vdt) * a.inv_t - st.n);
+  if (st.twice == 0.0) return p_of(a, st, r * a.k + k);
   double p = 0.0;
   for (int j = 0; j < a.k; ++j)
-    if (tk_id(a, r * a.k + j) == id) p += exp(load_as_f32(a.values, r * a.k + j, a.vdt) * a.inv_t - st.n);
+    if (tk_id(a, r * a.k + j) == id) p += p_of(a, st, r * a.k + j);
   return p;
 }
 
@@ -428,12 +449,12 @@ __global__ void __launch_bounds__(BLK) top_kl_backward_kernel(TopKlArgs a, const
     return;
   }
   const RowGrad<DT> g(a, st);
-  const float coef = static_cast<float>(f * (st.p - (st.r != 0.0 ? st.r * exp(st.z - st.zr) : 0.0)));
+  const float coef = static_cast<float>(f * (st.p - (st.r != 0.0 ? st.r * exp(st.lz - st.lzr) : 0.0)));
   const void* rows[1] = {row_at<DT>(a.s, (r / a.inner) * a.s0 + (r % a.inner) * a.s1)};
   const Cut cut = Cut::of<DT, BLK>(rows[0], a.vocab);
   // the listed tokens' own gradient, formed while the row is on its way and written when the row is
   const auto listed = [&](int k, int id) {
-    const double q = exp(load_as_f32(rows[0], id, DT) * a.inv_t - st.z);
+    const double q = q_of(a, st, load_as_f32(rows[0], id, DT));
     return static_cast<float>(f * (st.p * q - listed_p(a, st, r, k, id)));
   };
   int id0 = -1;
@@ -500,9 +521,9 @@ __global__ void __launch_bounds__(kTkSecond) top_kl_second_kernel(TopKlArgs a, c
   for (int k = t; k < a.k; k += BLK) {
     const int id = tk_id(a, r * a.k + k);
     if (id < 0) continue;
-    const double q = exp(load_as_f32(rows[0], id, DT) * a.inv_t - st.z), w = load_as_f32(rows[1], id, DT);
+    const double q = q_of(a, st, load_as_f32(rows[0], id, DT)), w = load_as_f32(rows[1], id, DT);
     if (k == t) id0 = id, q0 = q, w0 = w;
-    x[2] += w * exp(load_as_f32(a.values, r * a.k + k, a.vdt) * a.inv_t - st.n);
+    x[2] += w * p_of(a, st, r * a.k + k);
     if (st.twice == 0.0 || first_of_id(a, r, k, id)) x[1] += w * q;
   }
   float rest = 0.0f;
@@ -526,7 +547,7 @@ __global__ void __launch_bounds__(kTkSecond) top_kl_second_kernel(TopKlArgs a, c
   tk_stream<DT, BLK, 1>(rows, cut, H, [] {}, dot);
   x[0] = static_cast<double>(rest);
   block_sum<3, BLK>(x, part);
-  const double kappa = st.r != 0.0 ? exp(st.z - st.zr) : 0.0, uq = x[0] + x[1];
+  const double kappa = st.r != 0.0 ? exp(st.lz - st.lzr) : 0.0, uq = x[0] + x[1];
   if (t == 0) row_dot[r] = share * (st.p * uq - x[2] - st.r * kappa * x[0]);
   const float A = static_cast<float>(f * (st.p - st.r * kappa));
   const float B = static_cast<float>(f * (st.p * uq - st.r * kappa * kappa * x[0]));
@@ -542,7 +563,7 @@ __global__ void __launch_bounds__(kTkSecond) top_kl_second_kernel(TopKlArgs a, c
   for (int k = t + BLK; k < a.k; k += BLK) {
     const int id = tk_id(a, r * a.k + k);
     if (id < 0) continue;
-    const double q = exp(load_as_f32(rows[0], id, DT) * a.inv_t - st.z), w = load_as_f32(rows[1], id, DT);
+    const double q = q_of(a, st, load_as_f32(rows[0], id, DT)), w = load_as_f32(rows[1], id, DT);
     store_from_f32(out, id, DT, static_cast<float>(f * st.p * q * (w - uq)));
   }
 }

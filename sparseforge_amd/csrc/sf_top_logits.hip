@@ -1,9 +1,9 @@
 // The k largest logits of every row in falling order (equal ones by rising id), their ids, and the row's log-sum-exp at a
 // temperature: what is kept of a teacher for distillation, or answered as log-probabilities.
 //
-// One workgroup per row, which it holds in registers if it fits: a pass for the maxima of the threads' parts, from which a
-// bound follows above which the k largest and few others lie (gather_top); a pass that gathers these in LDS and sums the
-// exponentials; then orders them.
+// One workgroup per row reads it once, for the sum of exponentials and the maxima of the threads' pieces.  From these follows
+// a bound above which the k largest and few others lie (top_bound), whose pieces are taken again from the caches.  The
+// candidates are ordered in LDS.
 #include <type_traits>
 
 #include "sf_top.hpp"
@@ -58,50 +58,63 @@ __device__ __forceinline__ void top_of_any(const TopLogitsArgs& a, const void* r
   }
 }
 
-// H: pieces of 8 elements that a thread keeps in registers.  k is at most BLK * GROUPS / 2 and CAP.
-template <int DT, int BLK, int H, int GROUPS, int CAP>
+// k is at most BLK (two groups' maxima a thread) and below CAP.
+template <int DT, int BLK, int G, int CAP>
 __global__ void __launch_bounds__(BLK) top_logits_kernel(TopLogitsArgs a) {
   __shared__ TopShared<CAP> sh;
   __shared__ AnyShared any;
   __shared__ double sums[BLK / 64];
   const int64_t r = blockIdx.x;
   const int t = threadIdx.x;
-  const Row<DT, BLK, H> row(static_cast<const char*>(a.x) + ((r / a.inner) * a.s0 + (r % a.inner) * a.s1) *
-                                                                (DT == SF_DTYPE_BF16 ? 2 : 4),
-                            a.vocab);
-  float best[GROUPS];
-  const float m = row_max(row, best, sh.edge[1], [](const float (&)[8]) {});
+  const RowAt<DT, BLK> row(static_cast<const char*>(a.x) + ((r / a.inner) * a.s0 + (r % a.inner) * a.s1) *
+                                                               (DT == SF_DTYPE_BF16 ? 2 : 4),
+                           a.vocab);
   const float c = static_cast<float>(a.inv_t * 1.4426950408889634);
-  const float ref = m > -INFINITY && m < INFINITY ? m : 0.0f;
-  Bound bound{INFINITY, 1.0f, 0.0f};
-  if (ref == m) bound = top_bound<BLK>(best, m, a.k, sh);
-  float sum = 0.0f, lost = 0.0f;
-  uint32_t hits = 0;
-  row.each([&](int p, int, const float (&v)[8]) SF_INLINE {
-    if (bound.holds(max8(v))) hits |= 1u << p;
+  float top = kTopLow, sum = 0.0f, lost = 0.0f, best[G];
+  read_row(row, best, [&](const float (&v)[8]) SF_INLINE {
+    float x = top;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) x = fmaxf(x, v[k]);
+    if (x > top) {
+      const float f = __builtin_amdgcn_exp2f((top - x) * c);
+      sum *= f;
+      lost *= f;
+      top = x;
+    }
     float e[8];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) e[k] = __builtin_amdgcn_exp2f((v[k] - ref) * c);
+    for (int k = 0; k < 8; ++k) e[k] = __builtin_amdgcn_exp2f((v[k] - top) * c);
     // hundreds of small terms beside a large one: what an addition rounds off is carried along
     const float s = (((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]))) - lost, upto = sum + s;
     lost = (upto - sum) - s;
     sum = upto;
   });
-  double total = sum;
+  float m = best[0];
+#pragma unroll
+  for (int g = 1; g < G; ++g) m = nan_max(m, best[g]);
+  m = row_max<BLK>(m, sh.edge[1]);
+  const bool plain = m > -INFINITY && m < INFINITY;
+  int n = 0;
+  double total = sum == 0.0f || !plain ? 0.0 : static_cast<double>(sum * __builtin_amdgcn_exp2f((top - m) * c));
   for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
   if ((t & 63) == 0) sums[t >> 6] = total;
-  const int n = ref == m ? gather(row, [&](float x) { return bound.holds(x); }, hits, sh) : 0;
+  Bound bound;
+  if (plain) {
+    bound = bound_of<BLK>(best, m, a.k, sh);
+    n = gather<G>(row, bound, hits_of(best, bound), sh);
+  } else {
+    __syncthreads();
+  }
+  if (t == 0 && a.lse) {
+    total = 0.0;
+    for (int w = 0; w < BLK / 64; ++w) total += sums[w];
+    a.lse[r] = plain ? static_cast<float>(m * a.inv_t + log(total)) : m;
+  }
   if (n < a.k || n > CAP) {  // -inf, inf or NaN among the k, or too many equals
     top_of_any<DT, BLK>(a, row.row, r, any, sh);
   } else {
     sort_found<BLK>(bound, n, sh);
     for (int i = t; i < a.k; i += BLK) put<DT>(a, row.row, r, i, candidate_id(sh.found[i]));
-  }
-  __syncthreads();
-  if (t == 0 && a.lse) {
-    total = 0.0;
-    for (int w = 0; w < BLK / 64; ++w) total += sums[w];
-    a.lse[r] = static_cast<float>(ref * a.inv_t + log(total));
   }
 }
 
@@ -134,10 +147,16 @@ extern "C" int sf_top_logits(const sf_top_logits_desc* desc, void* stream) {
   hipStream_t st = static_cast<hipStream_t>(stream);
   auto with = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    if (d.rows >= 512 && d.k <= 128 && d.vocab <= 256 * 8 * 32)
-      top_logits_kernel<DT, 256, DT == SF_DTYPE_BF16 ? 16 : 8, 1, 512><<<grid, 256, 0, st>>>(a);
+    // Threads to a row: many where every CU has at most one, fewer where rows can cover each other's waits, the fewest
+    // for rows that these hold whole (bf16, k 20, us with 1024, 512 and 256 threads: 100 x 32000 13, 14 and 16; 1024 x
+    // 32000 43, 26 and 26; 3000 x 32000 109, 55 and 51; f32 1024 x 50257 66, 55 and 63).  Long rows in f32 are read twice
+    // in any case (1024 x 131072 151 and 157).
+    if (d.rows >= 1024 && d.k <= 128 && d.vocab <= 256 * 8 * 32)
+      top_logits_kernel<DT, 256, 16, 512><<<grid, 256, 0, st>>>(a);
+    else if (d.rows > 256 && d.k <= 512 && d.vocab <= 512 * 8 * 32)
+      top_logits_kernel<DT, 512, 8, 2048><<<grid, 512, 0, st>>>(a);
     else
-      top_logits_kernel<DT, 1024, 8, 2, 2048><<<grid, 1024, 0, st>>>(a);
+      top_logits_kernel<DT, 1024, 8, 2048><<<grid, 1024, 0, st>>>(a);
   };
   if (d.dtype == SF_DTYPE_BF16)
     with(std::integral_constant<int, SF_DTYPE_BF16>{});

@@ -1,6 +1,6 @@
 """logits.sample_logits (sf_sample_logits) against its definition in float64: the same token everywhere.
 
-The kernel's exponentials are off by 2.2e-12 of themselves, and summed rounded to 2^-F of the largest, F = min(44, 61 -
+The kernel's exponentials are off by 2.2e-12 of themselves, and summed rounded to 2^-F of the largest, F = min(44, 60 -
 ceil(log2 V)): a cumulative share is off by 2.2e-12 and V 2^-(F + 1) of the largest weight's, that where the roundings all
 go one way, which they do not.  The inputs are fixed, and no draw of theirs lies within 1e-9 of a token's edge (asserted),
 except where weights are equal and the sums exact.  Log-probabilities: float64 rounded once, 2^-24 of the value, and the
@@ -70,7 +70,7 @@ def check(x, u, settings, edges=True):
     B, V = x.shape
     assert ids.dtype == torch.int64 and ids.shape == (B,) and logp.dtype == torch.float32 and logp.shape == (B,)
     assert torch.equal(ids, sample_logits(x, u, **settings))
-    F = min(44, 61 - math.ceil(math.log2(V)))
+    F = min(44, 60 - math.ceil(math.log2(V)))
     for b in range(B):
         at = {n: (s[b].item() if torch.is_tensor(s) else s) for n, s in settings.items()}
         want, lp, edge = reference(x[b].cpu(), u[b].item(), **at)

@@ -264,6 +264,20 @@ def test_what_is_not_finite_shows(cuda_device):
     check(t, 2.0)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rest", [True, False])
+def test_tokens_masked_by_the_lowest_value(cuda_device, dtype, rest):
+    """The type's lowest value in place of -inf: tokens of no probability among others, equal tokens alone."""
+    t = _inputs(cuda_device, (4,), 777, 6, dtype, rest=rest, padded=False, weighted=False)
+    lowest = torch.finfo(dtype).min
+    keep = t["s"].clone()
+    t["s"][1, 100:700] = lowest
+    t["s"][1] = torch.where(torch.zeros(777, dtype=torch.bool, device=cuda_device)
+                            .index_fill_(0, t["ids"][1].long(), True), keep[1], t["s"][1])
+    t["s"][2] = lowest
+    check(t, 2.0, hvp=False)
+
+
 def test_agrees_with_the_whole_teacher(cuda_device):
     """With every token recorded the loss is chunked_kl_loss'."""
     from sparseforge_amd.distill import chunked_kl_loss, top_kl_loss, top_logits
