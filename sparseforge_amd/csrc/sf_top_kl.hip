@@ -52,19 +52,30 @@ __device__ __forceinline__ int tk_id(const TopKlArgs& a, int64_t at) {
   return id >= 0 && id < a.vocab ? static_cast<int>(id) : -1;
 }
 
-template <int DT>
+// PAST: past the caches.
+template <int DT, bool PAST>
 __device__ __forceinline__ void tk_store8(void* row, int i, int n, const float (&v)[8]) {
+  typedef uint32_t u32x4u __attribute__((ext_vector_type(4), aligned(2)));
   if (n == 8) {
-    uint32_t w[DT == SF_DTYPE_BF16 ? 4 : 8];
+    u32x4u* to = reinterpret_cast<u32x4u*>(static_cast<char*>(row) +
+                                           static_cast<int64_t>(i) * (DT == SF_DTYPE_BF16 ? 2 : 4));
+    const auto put = [](u32x4u* q, const u32x4u& w) {
+      if constexpr (PAST)
+        __builtin_nontemporal_store(w, q);
+      else
+        *q = w;
+    };
     if constexpr (DT == SF_DTYPE_BF16) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        w[k] = static_cast<uint32_t>(f32_to_bf16(v[2 * k])) | static_cast<uint32_t>(f32_to_bf16(v[2 * k + 1])) << 16;
+      const auto two = [&](int k) {
+        return static_cast<uint32_t>(f32_to_bf16(v[k])) | static_cast<uint32_t>(f32_to_bf16(v[k + 1])) << 16;
+      };
+      put(to, u32x4u{two(0), two(2), two(4), two(6)});
     } else {
 #pragma unroll
-      for (int k = 0; k < 8; ++k) w[k] = __float_as_uint(v[k]);
+      for (int k = 0; k < 8; k += 4)
+        put(to + k / 4, u32x4u{__float_as_uint(v[k]), __float_as_uint(v[k + 1]), __float_as_uint(v[k + 2]),
+                               __float_as_uint(v[k + 3])});
     }
-    __builtin_memcpy(static_cast<char*>(row) + static_cast<int64_t>(i) * (DT == SF_DTYPE_BF16 ? 2 : 4), w, sizeof(w));
   } else {
     for (int k = 0; k < n; ++k) store_from_f32(row, i + k, DT, v[k]);
   }
@@ -431,7 +442,7 @@ __device__ __forceinline__ double listed_p(const TopKlArgs& a, const RowStats& s
   return p;
 }
 
-template <int DT, int BLK>
+template <int DT, int BLK, bool PAST>
 __global__ void __launch_bounds__(BLK) top_kl_backward_kernel(TopKlArgs a, const double* __restrict__ stats,
                                                                    const double* __restrict__ norm,
                                                                    const float* __restrict__ grad_out,
@@ -445,7 +456,7 @@ __global__ void __launch_bounds__(BLK) top_kl_backward_kernel(TopKlArgs a, const
   if (w != 0.0) st = *reinterpret_cast<const RowStats*>(stats + r * kTkStats);
   if (f == 0.0 || st.p == 0.0) {
     const float zero[8] = {};
-    for (int i = t * 8; i < a.vocab; i += BLK * 8) tk_store8<DT>(out, i, a.vocab - i < 8 ? a.vocab - i : 8, zero);
+    for (int i = t * 8; i < a.vocab; i += BLK * 8) tk_store8<DT, PAST>(out, i, a.vocab - i < 8 ? a.vocab - i : 8, zero);
     return;
   }
   const RowGrad<DT> g(a, st);
@@ -466,7 +477,7 @@ __global__ void __launch_bounds__(BLK) top_kl_backward_kernel(TopKlArgs a, const
   tk_stream<DT, BLK, kTkBackwardU>(rows, cut, 0, first, [&](int i, int n, float (&x)[1][8]) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[0][k] = coef * g.q(x[0][k]);
-    tk_store8<DT>(out, i, n, x[0]);
+    tk_store8<DT, PAST>(out, i, n, x[0]);
   });
   __syncthreads();
   if (id0 >= 0) store_from_f32(out, id0, DT, g0);
@@ -477,7 +488,7 @@ __global__ void __launch_bounds__(BLK) top_kl_backward_kernel(TopKlArgs a, const
 }
 
 // Along u (rows contiguous): h_j, and the row's u . dL/ds at an upstream gradient of 1.
-template <int DT>
+template <int DT, bool PAST>
 __global__ void __launch_bounds__(kTkSecond) top_kl_second_kernel(TopKlArgs a, const double* __restrict__ stats,
                                                                   const double* __restrict__ norm,
                                                                   const float* __restrict__ grad_out,
@@ -495,7 +506,7 @@ __global__ void __launch_bounds__(kTkSecond) top_kl_second_kernel(TopKlArgs a, c
   if (share != 0.0) st = *reinterpret_cast<const RowStats*>(stats + r * kTkStats);
   if (share == 0.0 || st.p == 0.0) {
     const float zero[8] = {};
-    for (int i = t * 8; i < a.vocab; i += BLK * 8) tk_store8<DT>(out, i, a.vocab - i < 8 ? a.vocab - i : 8, zero);
+    for (int i = t * 8; i < a.vocab; i += BLK * 8) tk_store8<DT, PAST>(out, i, a.vocab - i < 8 ? a.vocab - i : 8, zero);
     if (t == 0) row_dot[r] = 0.0;
     return;
   }
@@ -554,7 +565,7 @@ __global__ void __launch_bounds__(kTkSecond) top_kl_second_kernel(TopKlArgs a, c
   const auto write = [&](int i, int m, float (&x)[2][8]) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[0][k] = g.q(x[0][k]) * fmaf(A, x[1][k], -B);
-    tk_store8<DT>(out, i, m, x[0]);
+    tk_store8<DT, PAST>(out, i, m, x[0]);
   };
   kept(write);
   tk_stream<DT, BLK, 1>(rows, cut, H, [] {}, write);
@@ -570,12 +581,23 @@ __global__ void __launch_bounds__(kTkSecond) top_kl_second_kernel(TopKlArgs a, c
 
 constexpr int64_t kTkFewRows = 512;  // fewer rows than this take more threads each
 
+// launch(data type, whether what it writes passes the caches).  A gradient that the last-level cache (256 MB) does not hold
+// beside the logits is not found there by who reads it next, and what of it stays there has to be written back while the
+// next pass reads: forward and backward by turns, 4096 x 32000 bf16 143 us past the caches and 167 through them, 2048 x
+// 131072 270 and 314; 1024 x 32000 (66 MB) 45 and 43.
 template <typename F>
-void tk_dispatch(int dtype, F&& launch) {
-  if (dtype == SF_DTYPE_F32)
-    launch(std::integral_constant<int, SF_DTYPE_F32>{});
+void tk_dispatch(const sf_top_kl_desc& d, F&& launch) {
+  const bool past = d.rows * d.vocab * (d.dtype == SF_DTYPE_F32 ? 4 : 2) > (128ll << 20);
+  const auto with = [&](auto dt) {
+    if (past)
+      launch(dt, std::true_type{});
+    else
+      launch(dt, std::false_type{});
+  };
+  if (d.dtype == SF_DTYPE_F32)
+    with(std::integral_constant<int, SF_DTYPE_F32>{});
   else
-    launch(std::integral_constant<int, SF_DTYPE_BF16>{});
+    with(std::integral_constant<int, SF_DTYPE_BF16>{});
 }
 
 int top_kl_args(const sf_top_kl_desc* desc, const char* what, TopKlArgs& a) {
@@ -624,7 +646,7 @@ extern "C" int sf_top_kl_forward(const sf_top_kl_desc* desc, float* loss, void* 
   const dim3 grid(static_cast<unsigned>(desc->rows));
   const size_t lds = static_cast<size_t>(mark_words(a.vocab)) * 4;
   double* row_kl = static_cast<double*>(workspace);
-  tk_dispatch(desc->dtype, [&](auto dt) {
+  tk_dispatch(*desc, [&](auto dt, auto) {
     constexpr int DT = decltype(dt)::value;
     auto with = [&](auto blk) {
       constexpr int BLK = decltype(blk)::value;
@@ -648,12 +670,13 @@ extern "C" int sf_top_kl_backward(const sf_top_kl_desc* desc, const float* grad_
   SF_CHECK_ARG(grad_out && grad_logits, "sf_top_kl_backward: null pointer");
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(desc->rows));
-  tk_dispatch(desc->dtype, [&](auto dt) {
+  tk_dispatch(*desc, [&](auto dt, auto past) {
     constexpr int DT = decltype(dt)::value;
+    constexpr bool PAST = decltype(past)::value;
     if (desc->rows < kTkFewRows)
-      top_kl_backward_kernel<DT, 1024><<<grid, 1024, 0, st>>>(a, desc->stats, desc->norm, grad_out, grad_logits);
+      top_kl_backward_kernel<DT, 1024, PAST><<<grid, 1024, 0, st>>>(a, desc->stats, desc->norm, grad_out, grad_logits);
     else
-      top_kl_backward_kernel<DT, 512><<<grid, 512, 0, st>>>(a, desc->stats, desc->norm, grad_out, grad_logits);
+      top_kl_backward_kernel<DT, 512, PAST><<<grid, 512, 0, st>>>(a, desc->stats, desc->norm, grad_out, grad_logits);
   });
   return launch_status("sf_top_kl_backward");
 }
@@ -670,10 +693,9 @@ extern "C" int sf_top_kl_double_backward(const sf_top_kl_desc* desc, const float
   hipStream_t st = static_cast<hipStream_t>(stream);
   const dim3 grid(static_cast<unsigned>(desc->rows));
   const size_t lds = static_cast<size_t>(mark_words(a.vocab)) * 4;
-  tk_dispatch(desc->dtype, [&](auto dt) {
-    constexpr int DT = decltype(dt)::value;
-    top_kl_second_kernel<DT><<<grid, kTkSecond, lds, st>>>(a, desc->stats, desc->norm, grad_out, grad_grad,
-                                                           grad2_logits, row_dot);
+  tk_dispatch(*desc, [&](auto dt, auto past) {
+    top_kl_second_kernel<decltype(dt)::value, decltype(past)::value><<<grid, kTkSecond, lds, st>>>(
+        a, desc->stats, desc->norm, grad_out, grad_grad, grad2_logits, row_dot);
   });
   if (dot) top_kl_dot_kernel<<<1, kTkFinal, 0, st>>>(row_dot, desc->rows, dot);
   return launch_status("sf_top_kl_double_backward");
