@@ -3,7 +3,7 @@
 A step takes the new tokens of every sequence through the model once: queries and keys are turned to their positions
 (rotary.rotary_embed), keys and values go into a cache of 8-bit codes and the queries attend over it
 (kv_cache.KVCache8), and the last token's logits are penalised, biased and masked (logits.process_logits) before the
-next one is picked.  The reference has no such path: it scores text by running whole sequences
+next one is picked or drawn (logits.sample_logits).  The reference has no such path: it scores text by running whole sequences
 (legacy/eval_wiki_ppl.py:548-651).
 """
 from __future__ import annotations
@@ -12,7 +12,7 @@ import torch
 
 from .kv_cache import KVCache8
 from .llama import LlamaDecoder, swiglu
-from .logits import process_logits
+from .logits import process_logits, sample_logits
 from .rotary import rotary_cos_sin, rotary_embed
 
 
@@ -75,7 +75,8 @@ class Generator:
 @torch.no_grad()
 def generate(model: LlamaDecoder, prompts: torch.Tensor, new_tokens: int, lengths: torch.Tensor | None = None, *,
              repetition=1.0, presence=0.0, frequency=0.0, bias: torch.Tensor | None = None, allowed=None, pick=None,
-             end_token: int | None = None, chunk: int = 2048) -> tuple[torch.Tensor, torch.Tensor]:
+             end_token: int | None = None, chunk: int = 2048, temperature=None, top_k=0, top_p=1.0, min_p=0.0,
+             generator: torch.Generator | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """Continue prompts [B, S] (the first lengths[b], at least one, of a row; what pads a row is not looked at) by up to
     new_tokens tokens each.
 
@@ -83,11 +84,15 @@ def generate(model: LlamaDecoder, prompts: torch.Tensor, new_tokens: int, length
     tokens that is; what lies past a row's length has no meaning.  The penalties, bias and allowed are process_logits',
     with the prompt and the answer so far as the history;
     allowed may be a function of (tokens, lengths) that gives the mask of a step.  pick turns logits [B, V] into ids
-    [B]: the most likely token (the lowest id among equals) where None.  A sequence stops after end_token, and where
-    its mask or bias lets nothing follow; the logits that pick sees of one that has stopped are zeros.  Prompts are
-    taken `chunk` tokens at a time."""
+    [B]: the most likely token (the lowest id among equals) where None.  With a temperature tokens are drawn instead, by
+    logits.sample_logits with top_k, top_p and min_p and random numbers from `generator` (the device's own where None),
+    one for each sequence and token.  A sequence stops after end_token, and where its mask or bias lets nothing follow,
+    a drawn one also where its logits hold a NaN; the logits that pick sees of one that has stopped are zeros.  Prompts
+    are taken `chunk` tokens at a time."""
     if prompts.dim() != 2 or prompts.shape[1] < 1 or prompts.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"generate: prompts must be ids [B, S], got {prompts.dtype} {tuple(prompts.shape)}")
+    if pick is not None and temperature is not None:
+        raise ValueError("generate: pick and a temperature both say how tokens are chosen")
     if new_tokens < 0 or chunk < 1:
         raise ValueError(f"generate: {new_tokens} new tokens, chunks of {chunk}")
     B, S = prompts.shape
@@ -110,14 +115,19 @@ def generate(model: LlamaDecoder, prompts: torch.Tensor, new_tokens: int, length
         logits = out if logits is None else torch.where((counts > 0)[:, None], out, logits)
     alive = torch.ones(B, dtype=torch.int32, device=dev)
     shaped = allowed is not None or bias is not None
-    stops = shaped or end_token is not None
+    drawn = temperature is not None
+    stops = shaped or drawn or end_token is not None
     for i in range(new_tokens):
         mask = allowed(tokens, lengths) if callable(allowed) else allowed
         logits = process_logits(logits, tokens, lengths, repetition=repetition, presence=presence,
                                 frequency=frequency, bias=bias, allowed=mask, out=logits)
         if shaped:
             alive = alive * ~(logits == float("-inf")).all(-1)
-        if pick is None:
+        if drawn:
+            uniform = torch.rand(B, device=dev, generator=generator)
+            ids = sample_logits(logits, uniform, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
+            alive = alive * (ids >= 0)
+        elif pick is None:
             ids = logits.argmax(-1)
         else:
             ids = pick(logits.masked_fill(alive[:, None] == 0, 0.0) if stops else logits)

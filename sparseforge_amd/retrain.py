@@ -9,6 +9,7 @@ FSDP/DDP, no GradScaler: bf16 needs none):
       frozen masks, so every micro-batch adds the same value)
   for each micro-batch (X, Y):                                   (:1996)
       logits, task, layerwise, kl = Distill_Model(X, Y)          (:2022)
+          (or from the teacher's top logits alone: teacher_top, recorded batches)
       loss = h_task * task + h_kl * kl (+ h_sq * layerwise)       (:2025-2028)
       loss += penalty
       loss /= grad_accum                                         (:2067)
@@ -53,6 +54,7 @@ class RetrainConfig:
     autocast_dtype: torch.dtype | None = torch.bfloat16
     lr: float = 1e-4
     decay: float = 0.0
+    teacher_top: int = 0  # distil from this many of the teacher's logits a token (0: from all of them)
 
 
 @dataclass
@@ -82,11 +84,14 @@ def lambda_mid_at(cfg: RetrainConfig, iter_num: int) -> float:
 
 
 class RetrainStep:
-    """Callable step over (student, teacher, optimizer); `batches` is a list of grad_accum (X, Y) pairs."""
+    """Callable step over (student, teacher, optimizer); `batches` is a list of grad_accum (X, Y) pairs.
+
+    A batch may be (X, Y, record), the record being the teacher's logits of X as distill.top_logits gives them (at the
+    default temperature of 2): then no teacher runs, and where every batch has one the teacher may be None."""
 
     def __init__(self, student, teacher, optimizer, cfg: RetrainConfig, timed: bool = False, on_grads=None):
         self.student = student
-        self.model = Distill_Model(student, teacher)
+        self.model = Distill_Model(student, teacher, top=cfg.teacher_top)
         self.optimizer = optimizer
         self.cfg = cfg
         self.timed = timed
@@ -118,12 +123,12 @@ class RetrainStep:
                 pen, _cur = U.sparsity_penalty(self.student, target_sparsity=cfg.sparsity_ratio,
                                                alpha=cfg.sparsity_alpha)
                 penalty = penalty + pen
-        for micro, (X, Y) in enumerate(batches):
+        for micro, (X, Y, *record) in enumerate(batches):
             last = micro == cfg.grad_accum - 1
             ctx = (torch.autocast("cuda", dtype=cfg.autocast_dtype) if cfg.autocast_dtype is not None
                    else torch.autocast("cuda", enabled=False))
             with ctx:
-                _logits, task, layerwise, kl = self.model(X, Y)
+                _logits, task, layerwise, kl = self.model(X, Y, *record)
                 if task is None:
                     task = 0.0
                 if layerwise is None:

@@ -679,16 +679,22 @@ class SparseLinear(nn.Linear):
 
 
 class Distill_Model(torch.nn.Module):
-    """Student/teacher distillation wrapper (legacy/sparse_modeling.py:1669-1838)."""
+    """Student/teacher distillation wrapper (legacy/sparse_modeling.py:1669-1838).
 
-    def __init__(self, model, teacher=None, output_hidden_state=False):
+    Beyond the reference: with top > 0 the KL is that from the teacher's `top` largest logits and the probability of all
+    other tokens together (distill.top_kl_loss); forward also takes such a record of the teacher's (distill.TopLogits) as
+    teacher_top, and then runs no teacher, which may be None."""
+
+    def __init__(self, model, teacher=None, output_hidden_state=False, top=0):
         super().__init__()
         self.student = model
         self.teacher = teacher
+        self.top = int(top)
         self.student.config.output_hidden_state = output_hidden_state
-        self.teacher.config.output_hidden_state = output_hidden_state
         self.output_hidden_state = output_hidden_state
-        self.teacher.eval()
+        if teacher is not None:
+            self.teacher.config.output_hidden_state = output_hidden_state
+            self.teacher.eval()
 
     def _teacher_forward(self, idx, targets):
         with torch.no_grad():
@@ -702,7 +708,14 @@ class Distill_Model(torch.nn.Module):
                 targets_t = targets.to(device=tdev) if targets.device != tdev else targets
             return self.teacher(idx_t, targets_t)
 
-    def forward(self, idx, targets=None):
+    def forward(self, idx, targets=None, teacher_top=None):
+        if teacher_top is not None:
+            from .distill import top_kl_loss
+
+            if self.output_hidden_state:
+                raise ValueError("Distill_Model: a record of the teacher's logits has no hidden states")
+            student_logits, task_loss, _ = self.student(idx, targets)
+            return student_logits, task_loss, None, top_kl_loss(student_logits, teacher_top)
         if self.teacher is None:
             student_logits, task_loss, _ = self.student(idx, targets)
             return student_logits, task_loss, None, torch.tensor(0.0, device=idx.device)
@@ -717,12 +730,19 @@ class Distill_Model(torch.nn.Module):
                 layerwise = self.layerwise_loss(student_hidden, teacher_hidden)
             else:
                 layerwise = 0.0
-            return student_logits, task_loss, layerwise, self.kl_loss(student_logits, teacher_logits)
+            return student_logits, task_loss, layerwise, self._kl(student_logits, teacher_logits)
         student_logits, task_loss, _ = self.student(idx, targets)
         teacher_logits, _, _ = self._teacher_forward(idx, targets)
         if teacher_logits.device != student_logits.device:
             teacher_logits = teacher_logits.to(device=student_logits.device, dtype=student_logits.dtype)
-        return student_logits, task_loss, None, self.kl_loss(student_logits, teacher_logits)
+        return student_logits, task_loss, None, self._kl(student_logits, teacher_logits)
+
+    def _kl(self, student_logits, teacher_logits):
+        if not self.top:
+            return self.kl_loss(student_logits, teacher_logits)
+        from .distill import top_kl_loss, top_logits
+
+        return top_kl_loss(student_logits, top_logits(teacher_logits, self.top))
 
     def kl_loss(self, student_logits, teacher_logits, temperature=2):
         """KL(P_teacher || Q_student) at temperature T, logits clamped to +-100 (:1749-1828)."""
