@@ -402,3 +402,29 @@ def test_results_do_not_vary(cuda_device):
         if first is None:
             first = loss.detach(), g
         assert torch.equal(first[0], loss.detach()) and torch.equal(first[1], g)
+
+
+def test_plain_and_recorded_backward_agree(cuda_device):
+    """A plain backward pass and one that records give the same gradients; forward mode and vmap are refused, not passed
+    by."""
+    from torch.autograd import forward_ad
+
+    from sparseforge_amd.distill import TopLogits, top_kl_loss
+
+    t = _inputs(cuda_device, (7,), 300, 5, torch.float32)
+    teacher = TopLogits(t["values"], t["ids"], _lse(t, 2.0), 2.0)
+    s = t["s"].requires_grad_(True)
+    loss = top_kl_loss(s, teacher, weights=t["weights"])
+    a, = torch.autograd.grad(loss, s, retain_graph=True)
+    b, = torch.autograd.grad(loss, s, create_graph=True)
+    assert b.requires_grad and not a.requires_grad and torch.equal(a, b.detach())
+    with torch.no_grad():
+        assert torch.equal(loss.detach(), top_kl_loss(s, teacher, weights=t["weights"]))
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(s.detach(), torch.ones_like(s))
+        with pytest.raises(NotImplementedError):
+            top_kl_loss(dual, teacher, weights=t["weights"])
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(lambda x: top_kl_loss(x, teacher))(s.detach()[None])
+    with pytest.raises(RuntimeError):
+        torch.func.grad(lambda x: top_kl_loss(x, teacher))(s.detach())
