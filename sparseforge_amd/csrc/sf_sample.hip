@@ -581,7 +581,7 @@ extern "C" int sf_sample_logits(const sf_sample_desc* desc, void* stream) {
                        !(a.top_p1 < 1.0f);
     const bool top_k = (!a.top_k && a.top_k1 > 0 && a.top_k1 <= (narrow ? 512 : 1024)) || (!a.temp && !(a.temp1 > 0.0f));
     if (narrow && top_k)
-      sample_top_k_kernel<DT, 512, 8><<<grid, 512, 0, st>>>(a);
+      sample_top_k_kernel<DT, 512, 16><<<grid, 512, 0, st>>>(a);
     else if (top_k)
       sample_top_k_kernel<DT, 1024, 8><<<grid, 1024, 0, st>>>(a);
     else if (narrow && whole)

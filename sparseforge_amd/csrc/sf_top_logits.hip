@@ -151,10 +151,13 @@ extern "C" int sf_top_logits(const sf_top_logits_desc* desc, void* stream) {
     // for rows that these hold whole (bf16, k 20, us with 1024, 512 and 256 threads: 100 x 32000 13, 14 and 16; 1024 x
     // 32000 43, 26 and 26; 3000 x 32000 109, 55 and 51; f32 1024 x 50257 66, 55 and 63).  Long rows in f32 are read twice
     // in any case (1024 x 131072 151 and 157).
-    if (d.rows >= 1024 && d.k <= 128 && d.vocab <= 256 * 8 * 32)
-      top_logits_kernel<DT, 256, 16, 512><<<grid, 256, 0, st>>>(a);
-    else if (d.rows > 256 && d.k <= 512 && d.vocab <= 512 * 8 * 32)
-      top_logits_kernel<DT, 512, 8, 2048><<<grid, 512, 0, st>>>(a);
+    // Threads to a row: many where a CU has at most one row, fewer where rows can cover each other's waits (us with 1024,
+    // 512 and 256 threads, k 20: bf16 100 x 32000 14, 14 and 17; 1024 x 32000 31, 27 and 24; 3000 x 32000 71, 55 and 49;
+    // f32 3000 x 50257 112, 110 and 117; 509 x 131072 with k 500 70 and 75).
+    if (DT == SF_DTYPE_BF16 && d.rows > 512 && d.k <= 128 && d.vocab <= 256 * 8 * 32)
+      top_logits_kernel<SF_DTYPE_BF16, 256, 16, 512><<<grid, 256, 0, st>>>(a);
+    else if (d.rows > 256 && d.k <= 512 && d.vocab <= (DT == SF_DTYPE_BF16 ? 131072 : 65536))
+      top_logits_kernel<DT, 512, 16, 2048><<<grid, 512, 0, st>>>(a);
     else
       top_logits_kernel<DT, 1024, 8, 2048><<<grid, 1024, 0, st>>>(a);
   };
