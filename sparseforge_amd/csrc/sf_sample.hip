@@ -285,8 +285,8 @@ struct Bins {
   __device__ __forceinline__ void range(int bin, float& low, float& high) const {
     const float a = (static_cast<float>(bin) - 0.01f) / scale, b = (static_cast<float>(bin) + 1.01f) / scale;
     const float off = 1e-6f * (fabsf(top) + b);
-    high = top - a + off;
-    low = bin == kSpBins - 1 ? -INFINITY : top - b - off;
+    high = fminf(top - a + off, -kTopLow);
+    low = bin == kSpBins - 1 ? kTopLow : fmaxf(top - b - off, kTopLow);
   }
 };
 
@@ -314,19 +314,50 @@ __device__ __forceinline__ void fill_bins(Row<DT, BLK, H>& row, const Bins& bins
   });
 }
 
-// The last element, in the order of logits, at which what the bins hold (see fill_bins) of the elements before it is below
-// want(whole sum): found in last.  amount(x, id): of one element.  False: more than kSpCandidates are in the bin where
-// that happens.  A sum that stays below takes in everything.
-template <int DT, int BLK, int H, typename P, typename M, typename A>
-__device__ __forceinline__ bool border_of(Row<DT, BLK, H>& row, const Bins& bins, P&& fill, M&& amount, A&& want,
-                                          Last& last, SampleShared& sh) {
+// The float above x, which is not inf.
+__device__ __forceinline__ float float_above(float x) {
+  const uint32_t key = ordered_key(x) + 1;
+  return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+}
+
+// The weight of the thread's elements from `from` up (ALL: of every one), as a sum that starts at 2^52.  Those of
+// [low, high], which is below, are gathered in sh.top.found.
+template <bool ALL, int DT, int BLK, int H>
+__device__ __forceinline__ double sum_from(Row<DT, BLK, H>& row, float from, float low, float high,
+                                           const Weight& weight, SampleShared& sh) {
+  double sum = Weight::kWhole;
+  row.each_looped([&](int, int i, const float (&v)[8]) SF_INLINE {
+    const float largest = max8(v);
+    if (!ALL && largest >= low) {
+      bool in[8], any = false;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) any |= in[k] = (v[k] >= low) & (v[k] <= high);
+      if (any) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (in[k]) {
+            const int at = atomicAdd(&sh.top.n, 1);
+            if (at < kSpCandidates) sh.top.found[at] = candidate(v[k], i + k);
+          }
+      }
+    }
+    if (ALL || largest >= from) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        sum += weight.scaled(ALL || v[k] >= from ? v[k] : -INFINITY);  // 2^-20, which the sum of integers does not see
+        if (k % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  });
+  return sum;
+}
+
+// The place in the bins (see fill_bins) at which the sum of what they hold reaches want(whole sum): sh.bin and the sum
+// before it in sh.base, which comes back with the target.  -1: the sum stays below.
+template <int BLK, typename W>
+__device__ __forceinline__ u64 bin_of_sum(W&& want, SampleShared& sh) {
   constexpr int kEach = kSpBins / BLK;
   const int t = threadIdx.x;
-  for (int i = t; i < kSpBins; i += BLK) sh.weight[i] = 0;
-  if (t == 0) sh.bin = -1, sh.top.n = 0;
-  __syncthreads();
-  fill();
-  __syncthreads();
   u64 own[kEach], sum = 0;
 #pragma unroll
   for (int i = 0; i < kEach; ++i) sum += own[i] = sh.weight[t * kEach + i];
@@ -339,30 +370,17 @@ __device__ __forceinline__ bool border_of(Row<DT, BLK, H>& row, const Bins& bins
     upto += own[i];
   }
   __syncthreads();
-  const int bin = sh.bin;
-  if (bin < 0) return true;
-  float low, high;
-  bins.range(bin, low, high);
-  row.each_looped([&](int, int i, const float (&v)[8]) SF_INLINE {
-    bool in[8], any = false;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) any |= in[k] = __builtin_amdgcn_fmed3f(v[k], low, high) == v[k];
-    if (any) {
-#pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (in[k]) {
-          const int at = atomicAdd(&sh.top.n, 1);
-          if (at < kSpCandidates) sh.top.found[at] = candidate(v[k], i + k);
-        }
-    }
-  });
-  __syncthreads();
-  const int n = sh.top.n;
-  if (n > kSpCandidates) return false;
+  return target;
+}
+
+// Among the n gathered elements, which hold all of the bin, the last one before which the sum is below target.
+template <int BLK, typename M>
+__device__ __forceinline__ Last last_of(const Bins& bins, int n, u64 target, M&& amount, SampleShared& sh) {
+  const int t = threadIdx.x, bin = sh.bin;
   for (int i = t; i < n; i += BLK) {
     const u64 c = sh.top.found[i];
     const float x = candidate_logit(c);
-    sh.weight[i] = x > -INFINITY && bins.of(x) == bin ? amount(x, candidate_id(c)) : 0;  // others are beside the bin
+    sh.weight[i] = bins.of(x) == bin ? amount(x, candidate_id(c)) : 0;  // others are beside the bin
     sh.before[i] = sh.base;
   }
   __syncthreads();
@@ -380,41 +398,15 @@ __device__ __forceinline__ bool border_of(Row<DT, BLK, H>& row, const Bins& bins
   for (int i = t; i < n; i += BLK)
     if (sh.before[i] < target && target <= sh.before[i] + sh.weight[i]) sh.last = sh.top.found[i];
   __syncthreads();
-  last = {candidate_logit(sh.last), candidate_id(sh.last)};
-  return true;
+  return {candidate_logit(sh.last), candidate_id(sh.last)};
 }
 
-// The draw among the elements that `last` keeps (ALL: every one): the wave whose part of the row it falls in, then the
-// thread.
-template <bool ALL, int DT, int BLK, int H>
-__device__ __forceinline__ void draw(const SampleArgs& a, const Settings& s, int64_t r, Row<DT, BLK, H>& row,
+// The draw among the elements that `last` keeps, whose weight by wave is in sh.part[1]: the wave whose part of the row it
+// falls in, then the thread.
+template <int DT, int BLK, int H>
+__device__ __forceinline__ void draw(const SampleArgs& a, const Settings& s, int64_t r, const Row<DT, BLK, H>& row,
                                      const Last& last, const Weight& weight, SampleShared& sh) {
   const int t = threadIdx.x;
-  double sum = Weight::kWhole;
-  // of the pieces behind last.id only what is larger than last.x
-  const uint32_t key = ordered_key(last.x) + 1;
-  const float above = last.x == INFINITY ? INFINITY : __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
-  row.each_looped([&](int, int i, const float (&v)[8]) SF_INLINE {
-    const float least = i > last.id ? above : last.x;
-    if (ALL || max8(v) >= least) {
-      float x[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) x[k] = ALL || v[k] >= least ? v[k] : -INFINITY;
-      if (!ALL && i <= last.id && last.id < i + 7) {  // the piece that it ends in
-#pragma unroll
-        for (int k = 0; k < 8; ++k)
-          if (!last.keeps(x[k], i + k)) x[k] = -INFINITY;
-      }
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        sum += weight.scaled(x[k]);  // -inf: 2^-20, which the sum of integers does not see
-        if (k % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-      }
-    }
-  });
-  const u64 part = wave_scan(Weight::whole(sum));
-  if ((t & 63) == 63) sh.part[1][t >> 6] = part;
-  __syncthreads();
   u64 total = 0;
   for (int w = 0; w < BLK / 64; ++w) total += sh.part[1][w];
   u64 left = share_down(s.u, total);
@@ -469,19 +461,18 @@ __global__ void __launch_bounds__(BLK, 4) sample_kernel(SampleArgs a) {
   Settings s(a, r);
   const bool among = !WHOLE && s.k <= BLK && s.k < a.vocab;  // few enough to be gathered
   const bool binned = !WHOLE && !among && (s.k < a.vocab || s.p < 1.0);
-  float best[2] = {-INFINITY, -INFINITY}, low = INFINITY;
+  float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY}, low = INFINITY;
   row.each([&](int p, int, const float (&v)[8]) SF_INLINE {
     const float x = max8(v);
-    if (p % 2)
-      best[1] = nan_max(best[1], x);
-    else
-      best[0] = nan_max(best[0], x);
+#pragma unroll
+    for (int g = 0; g < 4; ++g)
+      if (p % 4 == g) best[g] = nan_max(best[g], x);
     if (binned) {
 #pragma unroll
       for (int k = 0; k < 8; ++k) low = fminf(low, v[k] == -INFINITY ? INFINITY : v[k]);
     }
   });
-  const float m = s.top = row_max<BLK>(nan_max(best[0], best[1]), sh.top.edge[1]);
+  const float m = s.top = row_max<BLK>(nan_max(nan_max(best[0], best[1]), nan_max(best[2], best[3])), sh.top.edge[1]);
   if (!(m > -INFINITY)) {
     put_none(a, r, m);
     return;
@@ -489,51 +480,79 @@ __global__ void __launch_bounds__(BLK, 4) sample_kernel(SampleArgs a) {
   const Weight weight{m, 1.4426950408889634 / static_cast<double>(s.temp), a.bits, a.poly};
   bool done = m < INFINITY;
   if (done && among) {
-    const Bound bound = top_bound<BLK>(best, m, static_cast<int>(s.k), sh.top);
-    uint32_t hits = 0;
-    row.each([&](int p, int, const float (&v)[8]) SF_INLINE {
-      if (bound.holds(max8(v))) hits |= 1u << p;
-    });
-    const int n = gather<32>(row, bound, hits, sh.top);
+    const Bound bound = bound_of<BLK>(best, m, static_cast<int>(s.k), sh.top);
+    const int n = gather<4>(row, bound, hits_of(best, bound), sh.top);
     done = n > 0 && n <= kSpCandidates;
     if (done) sample_found<BLK>(a, s, r, weight, bound, n, sh);
   } else if (done) {
     Last last;
-    if (binned) {
-      low = last_lane(wave_scan(low, INFINITY, [](float a, float b) { return fminf(a, b); }));
-      if ((threadIdx.x & 63) == 0) sh.top.edge[0][threadIdx.x >> 6] = low;
-      __syncthreads();
-      for (int w = 0; w < BLK / 64; ++w) low = fminf(low, sh.top.edge[0][w]);
-      // 2^-(F + 1) of the largest weight is 0
-      const float range = fminf(m - low, static_cast<float>((a.bits + 1) * 0.6931471805599453 * s.temp));
-      const Bins bins{m, fminf(kSpBins / range, 1e30f)};
-      // by number for top-k, by weight among these for top-p
-      const bool cut = s.k < a.vocab;
-#pragma unroll 1
-      for (int by_weight = cut ? 0 : 1; done && by_weight < (s.p < 1.0 ? 2 : 1); ++by_weight) {
-        done = border_of(
-            row, bins,
-            [&]() SF_INLINE {
-              if (!by_weight)
-                fill_bins<0>(row, bins, last, weight, sh);
-              else if (!cut)
-                fill_bins<1>(row, bins, last, weight, sh);
-              else
-                fill_bins<2>(row, bins, last, weight, sh);
-            },
-            [&](float x, int id) -> u64 { return !last.keeps(x, id) ? 0 : by_weight ? weight(x) : 1; },
-            [&](u64 total) { return by_weight ? share_up(s.p, total) : static_cast<u64>(s.k); }, last, sh);
+    const float least = s.least > 0.0 ? least_logit(s, weight) : -INFINITY;
+    double sum = 0.0;
+    if (WHOLE && least == -INFINITY) {
+      sum = sum_from<true>(row, 0.0f, 0.0f, 0.0f, weight, sh);
+    } else {
+      Bins bins{m, 0.0f};
+      if (binned) {
+        low = last_lane(wave_scan(low, INFINITY, [](float a, float b) { return fminf(a, b); }));
+        if ((threadIdx.x & 63) == 0) sh.top.edge[0][threadIdx.x >> 6] = low;
         __syncthreads();
+        for (int w = 0; w < BLK / 64; ++w) low = fminf(low, sh.top.edge[0][w]);
+        // 2^-(F + 1) of the largest weight is 0
+        const float range = fminf(m - low, static_cast<float>((a.bits + 1) * 0.6931471805599453 * s.temp));
+        bins.scale = fminf(kSpBins / range, 1e30f);
+      }
+      // by number for top-k, by weight among these for top-p
+      const bool cut = s.k < a.vocab, among_p = s.p < 1.0;
+      bool by_weight = !cut;
+      while (true) {
+        u64 target = 0;
+        float low = INFINITY, high = -INFINITY;
+        if (binned) {
+          for (int i = threadIdx.x; i < kSpBins; i += BLK) sh.weight[i] = 0;
+          if (threadIdx.x == 0) sh.bin = -1, sh.top.n = 0;
+          __syncthreads();
+          if (!by_weight)
+            fill_bins<0>(row, bins, last, weight, sh);
+          else if (!cut)
+            fill_bins<1>(row, bins, last, weight, sh);
+          else
+            fill_bins<2>(row, bins, last, weight, sh);
+          __syncthreads();
+          target = bin_of_sum<BLK>(
+              [&](u64 total) { return by_weight ? share_up(s.p, total) : static_cast<u64>(s.k); }, sh);
+          if (sh.bin >= 0) bins.range(sh.bin, low, high);
+        }
+        // the weight above the bin, for the draw, in the pass that gathers the bin
+        const bool at_end = by_weight || !among_p;
+        sum = sum_from<false>(row, at_end ? fmaxf(float_above(high), least) : INFINITY, low, high, weight, sh);
+        if (!binned) break;
+        __syncthreads();
+        const int n = sh.top.n;
+        done = n <= kSpCandidates;
+        if (done && n > 0)
+          last = last_of<BLK>(
+              bins, n, target,
+              [&](float x, int id) -> u64 { return !last.keeps(x, id) ? 0 : by_weight ? weight(x) : 1; }, sh);
+        if (!done || at_end) break;
+        by_weight = true;
       }
     }
-    if (done && s.least > 0.0) {
-      const float x = least_logit(s, weight);
-      if (x > last.x) last = {x, INT32_MAX};
+    if (done) {
+      const u64 part = wave_scan(Weight::whole(sum));
+      if ((threadIdx.x & 63) == 63) sh.part[1][threadIdx.x >> 6] = part;
+      __syncthreads();
+      if (least > last.x) last = {least, INT32_MAX};
+      if (binned) {
+        for (int i = threadIdx.x; i < sh.top.n; i += BLK) {
+          const u64 c = sh.top.found[i];
+          const float x = candidate_logit(c);
+          const int id = candidate_id(c);
+          if (last.keeps(x, id)) atomicAdd(&sh.part[1][id / (row.pieces * 512)], weight(x));
+        }
+        __syncthreads();
+      }
+      draw(a, s, r, row, last, weight, sh);
     }
-    if (done && last.x > -INFINITY)
-      draw<false>(a, s, r, row, last, weight, sh);
-    else if (done)
-      draw<true>(a, s, r, row, last, weight, sh);
   }
   if (!done) {
     __syncthreads();
@@ -575,7 +594,7 @@ extern "C" int sf_sample_logits(const sf_sample_desc* desc, void* stream) {
   hipStream_t st = static_cast<hipStream_t>(stream);
   auto with = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    constexpr int H = DT == SF_DTYPE_BF16 ? 8 : 4;
+    constexpr int H = DT == SF_DTYPE_BF16 ? 8 : 4, kFew = H / 2;
     const bool narrow = d.rows > 256 && a.vocab <= (DT == SF_DTYPE_BF16 ? 131072 : 65536);
     const bool whole = !a.temp && a.temp1 > 0.0f && !a.top_k && (a.top_k1 <= 0 || a.top_k1 >= a.vocab) && !a.top_p &&
                        !(a.top_p1 < 1.0f);
@@ -587,11 +606,11 @@ extern "C" int sf_sample_logits(const sf_sample_desc* desc, void* stream) {
     else if (narrow && whole)
       sample_kernel<DT, 512, H, true><<<grid, 512, 0, st>>>(a);
     else if (narrow)
-      sample_kernel<DT, 512, H, false><<<grid, 512, 0, st>>>(a);
+      sample_kernel<DT, 512, kFew, false><<<grid, 512, 0, st>>>(a);
     else if (whole)
       sample_kernel<DT, 1024, H, true><<<grid, 1024, 0, st>>>(a);
     else
-      sample_kernel<DT, 1024, H, false><<<grid, 1024, 0, st>>>(a);
+      sample_kernel<DT, 1024, kFew, false><<<grid, 1024, 0, st>>>(a);
   };
   if (d.dtype == SF_DTYPE_BF16)
     with(std::integral_constant<int, SF_DTYPE_BF16>{});
