@@ -34,6 +34,7 @@ struct SampleArgs {
   const float* min_p;
   float temp1, top_p1, min_p1;
   int top_k1, bits;  // bits: F
+  double round;      // 1.5 * 2^52 + F
   double poly[8];    // (2^f - 1) / f, the polynomial of degree 7 through its values at the Chebyshev points
 };
 
@@ -61,25 +62,28 @@ struct Settings {
   }
 };
 
-// Weights exp((x - top) / T) as integers of 2^-bits (bits <= 51); 2^bits exactly for the largest logit, which is finite.
-// The polynomial's coefficients come from the kernel's arguments, that is in scalar registers.
+// Weights exp((x - top) / T) as integers of 2^-F (F <= 44); 2^F exactly for the largest logit, which is finite.  The
+// constants come from the kernel's arguments, that is in scalar registers.
 struct Weight {
   double top, c;  // c: log2(e) / T
-  int bits;
+  const double& round;
   const double (&poly)[8];
   // before it is rounded
   __device__ __forceinline__ double scaled(float x) const {
-    // 2^z = 2^n 2^f, f in [-1/2, 1/2]: n is in the low bits of the sum with 1.5 * 2^52.  -inf ends at the smallest z.
-    constexpr double kRound = 6755399441055744.0;
+    // 2^z = 2^n 2^f, f in [-1/2, 1/2]: n + F is in the low bits of the sum with 1.5 * 2^52 + F.  -inf ends at the smallest
+    // z.  The last bit, 2^-8 of a unit at most, is set: nothing lies half way between integers, where a sum would round
+    // another way than the weight alone.
     const double z = fmax((static_cast<double>(x) - top) * c, -64.0);
-    const double rounded = z + kRound;
-    const double f = z - (rounded - kRound);
+    const double rounded = z + round;
+    const double f = z - (rounded - round);
     double p = poly[7];
 #pragma unroll
     for (int i = 6; i >= 0; --i) p = fma(p, f, poly[i]);
     p = fma(p, f, 1.0);
-    return __longlong_as_double(static_cast<u64>(__double_as_longlong(p)) +
-                                (static_cast<u64>(static_cast<uint32_t>(__double_as_longlong(rounded)) + bits) << 52));
+    const u64 as = static_cast<u64>(__double_as_longlong(p));
+    const uint32_t n = static_cast<uint32_t>(__double_as_longlong(rounded));
+    return __longlong_as_double(static_cast<u64>(static_cast<uint32_t>(as >> 32) + (n << 20)) << 32 |
+                                (static_cast<uint32_t>(as) | 1u));
   }
   __device__ __forceinline__ u64 operator()(float x) const { return whole(scaled(x) + kWhole); }
 
@@ -161,7 +165,7 @@ struct SampleShared {
   u64 weight[kSpBins + 64];  // by place, or by bin; in the end a bin for each lane of what has no weight
   u64 before[kSpCandidates];
   u64 part[2][16];
-  u64 total, base, last;
+  u64 base, last;
   int count, bin;
 };
 
@@ -262,7 +266,7 @@ __global__ void __launch_bounds__(BLK) sample_top_k_kernel(SampleArgs a) {
     put_none(a, r, m);
     return;
   }
-  const Weight weight{m, 1.4426950408889634 / static_cast<double>(s.temp), a.bits, a.poly};
+  const Weight weight{m, 1.4426950408889634 / static_cast<double>(s.temp), a.round, a.poly};
   int n = 0;
   if (m < INFINITY) {
     const Bound bound = bound_of<BLK>(best, m, static_cast<int>(s.k), sh.top);
@@ -477,7 +481,7 @@ __global__ void __launch_bounds__(BLK, 4) sample_kernel(SampleArgs a) {
     put_none(a, r, m);
     return;
   }
-  const Weight weight{m, 1.4426950408889634 / static_cast<double>(s.temp), a.bits, a.poly};
+  const Weight weight{m, 1.4426950408889634 / static_cast<double>(s.temp), a.round, a.poly};
   bool done = m < INFINITY;
   if (done && among) {
     const Bound bound = bound_of<BLK>(best, m, static_cast<int>(s.k), sh.top);
@@ -590,6 +594,7 @@ extern "C" int sf_sample_logits(const sf_sample_desc* desc, void* stream) {
   a.bits = 60;
   for (int64_t n = 1; n < d.vocab; n *= 2) --a.bits;
   if (a.bits > 44) a.bits = 44;
+  a.round = 6755399441055744.0 + a.bits;
   const dim3 grid(static_cast<unsigned>(d.rows));
   hipStream_t st = static_cast<hipStream_t>(stream);
   auto with = [&](auto dt) {

@@ -144,7 +144,7 @@ def sample_logits(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.
 def _setting(x, name: str, low, high, B: int, dev, dtype=torch.float32) -> tuple:
     """A setting as the kernel takes it: a pointer to one for each row, or a number."""
     if not isinstance(x, torch.Tensor):
-        if not low <= x <= high:
+        if not low <= x <= high or (dtype == torch.int32 and int(x) != x):
             raise ValueError(f"sample_logits: a {name} of {x}")
         return 0, int(x) if dtype == torch.int32 else float(x)
     if x.device != dev:

@@ -250,3 +250,105 @@ def test_captured_and_replayed(cuda_device):
         for (t, k), out in zip(((0.9, 0), (0.7, 60), (0.0, 0)), outs):
             again = sample_logits(x, u, top_p=top_p, temperature=t, top_k=k, logprobs=True)
             assert torch.equal(out[0], again[0]) and torch.equal(out[1], again[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_the_whole_weight_ends_at_the_last_kept_token(cuda_device, dtype):
+    """A number that counts as the last below 1 (2^-24 of the weight is more than any token's here but the largest) draws
+    the last kept token of every row: sums by wave and by token agree to the unit."""
+    from sparseforge_amd.logits import sample_logits
+
+    g = torch.Generator(device=cuda_device).manual_seed(12)
+    x = (torch.randn(3000, 4001, generator=g, device=cuda_device) * 2).to(dtype)
+    u = torch.ones(3000, device=cuda_device)
+    assert bool((sample_logits(x, u) == 4000).all())
+    assert bool((sample_logits(x, u, temperature=1.3, min_p=1e-12) == 4000).all())
+    # few kept: the last id among the largest n that hold the share, counted in float64
+    order = torch.sort(x.double(), dim=-1, descending=True, stable=True)
+    w = (order.values - order.values[:, :1]).exp()
+    before = torch.cumsum(w, -1) - w
+    kept = before < _f32(0.75) * w.sum(-1, keepdim=True)
+    want = torch.where(kept, order.indices, -1).amax(-1)
+    assert torch.equal(sample_logits(x, u, top_p=0.75), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_extreme_temperatures_and_logits(cuda_device, dtype):
+    from sparseforge_amd.logits import sample_logits
+
+    low, high = torch.finfo(dtype).min, torch.finfo(dtype).max
+    x = torch.tensor([[low, high, low, 0.0], [low, low, low, low], [0.0, 1.0, 1.0, -math.inf], [high, high, low, -high]],
+                     device=cuda_device).to(dtype)
+    u = torch.full((4,), 0.6, device=cuda_device)
+    for p in (1.0, 0.9):
+        for k in (0, 3):
+            assert sample_logits(x, u, temperature=1e-42, top_p=p, top_k=k).tolist() == [1, 2 if k == 0 else 1, 2, 1]
+    # at an infinite temperature all above -inf are alike
+    assert sample_logits(x, u, temperature=math.inf).tolist() == [2, 2, 1, 2]
+    assert sample_logits(x, u, temperature=math.inf, min_p=1.0).tolist() == [2, 2, 1, 2]
+
+
+def test_whole_numbers_for_top_k(cuda_device):
+    from sparseforge_amd.logits import sample_logits
+
+    x, u = torch.zeros(2, 8, device=cuda_device), torch.zeros(2, device=cuda_device)
+    with pytest.raises(ValueError):
+        sample_logits(x, u, top_k=2.5)
+    assert sample_logits(x, u, top_k=2.0).tolist() == [0, 0]
+
+
+@pytest.mark.parametrize("dtype,settings", [(torch.bfloat16, {}), (torch.bfloat16, {"top_k": 40, "top_p": 0.9}),
+                                            (torch.float32, {"top_p": 0.8})])
+def test_rows_behind_2_31_elements(cuda_device, dtype, settings):
+    """The last rows of logits whose offsets pass 32 bits, also in bytes beyond 4 GB, and of a wide stride."""
+    from sparseforge_amd.logits import sample_logits
+
+    B, V = 8300, 262144 if dtype == torch.bfloat16 else 262143
+    x = torch.zeros(B, V, dtype=dtype, device=cuda_device)
+    g = torch.Generator(device=cuda_device).manual_seed(3)
+    x[-3:] = _logits(g, 3, V, dtype, cuda_device)
+    u = torch.rand(B, generator=g, device=cuda_device)
+    ids = sample_logits(x, u, **settings)
+    assert torch.equal(ids[-3:], sample_logits(x[-3:].clone(), u[-3:], **settings))
+    far = torch.as_strided(x, (3, 5000), (V * (B - 3) // 2, 1))
+    assert torch.equal(sample_logits(far, u[:3], **settings), sample_logits(far.contiguous(), u[:3], **settings))
+
+
+def test_on_another_stream_and_beside_another_draw(cuda_device):
+    """Draws on two streams at once equal those in turn."""
+    from sparseforge_amd.logits import sample_logits
+
+    g = torch.Generator(device=cuda_device).manual_seed(6)
+    x = [_logits(g, 40, 50257, torch.float32, cuda_device) for _ in range(2)]
+    u = torch.rand(40, generator=g, device=cuda_device)
+    want = [sample_logits(y, u, top_p=0.9) for y in x]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(4):
+        for y, stream, out in zip(x, streams, got):
+            with torch.cuda.stream(stream):
+                out.append(sample_logits(y, u, top_p=0.9))
+    torch.cuda.synchronize()
+    for w, out in zip(want, got):
+        assert all(torch.equal(w, o) for o in out)
+
+
+def test_penalties_then_a_draw(cuda_device):
+    """process_logits and sample_logits as a step of generation uses them: the mask's tokens only, -1 where it leaves none."""
+    from sparseforge_amd.logits import process_logits, sample_logits
+
+    g = torch.Generator(device=cuda_device).manual_seed(8)
+    B, V = 6, 32000
+    x = _logits(g, B, V, torch.bfloat16, cuda_device)
+    history = torch.randint(0, V, (B, 50), generator=g, device=cuda_device)
+    allowed = torch.rand(B, V, generator=g, device=cuda_device) < 0.01
+    allowed[2] = False
+    y = process_logits(x, history, repetition=1.3, allowed=allowed)
+    u = torch.rand(B, generator=g, device=cuda_device)
+    for settings in ({}, {"top_k": 30}, {"top_k": 500, "top_p": 0.7}, {"top_p": 0.99, "min_p": 0.01}):
+        ids = sample_logits(y, u, temperature=0.9, **settings)
+        assert int(ids[2]) == -1
+        ok = torch.arange(B, device=cuda_device) != 2
+        assert bool(allowed[ok].gather(1, ids[ok, None]).all())
+        check(y, u, {"temperature": 0.9, **settings})
