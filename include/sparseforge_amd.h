@@ -440,13 +440,15 @@ int sf_kl_backward(const void* student, const void* teacher, int dtype, int64_t 
 #define SF_TOP_MAX_VOCAB 262144 /* longest rows */
 #define SF_TOP_MAX_ROWS 4194304 /* there are fewer rows than this */
 #define SF_TOP_MAX_K 1024       /* most entries that sf_top_logits gives */
+#define SF_TOP_MAX_ENTRIES 4096 /* most entries of a row that sf_top_kl_* take */
 
 /*
  * The k largest logits of every row, falling, equal ones by rising id (NaN
  * above all, -0 equal to 0), with their ids, and the log-sum-exp of the row at
  * `temperature`.  Row r lies at (r / inner) * outer_stride + (r % inner) *
  * row_stride elements.  values [rows, k] (the logits' dtype), ids int32 [rows,
- * k], lse f32 [rows] or null.
+ * k], lse f32 [rows] or null.  Temperatures here and below lie in
+ * 1e-30 .. 1e30.
  */
 typedef struct sf_top_logits_desc {
   const void* logits;

@@ -501,9 +501,9 @@ __global__ void __launch_bounds__(kTkSecond) top_kl_second_kernel(TopKlArgs a, c
   const int64_t r = gridDim.x - 1 - blockIdx.x;
   const int t = threadIdx.x;
   void* out = const_cast<void*>(row_at<DT>(hs, r * a.vocab));
-  const double share = *norm * (a.weights ? static_cast<double>(a.weights[r]) : 1.0);
+  const double w = a.weights ? static_cast<double>(a.weights[r]) : 1.0, share = *norm * w;
   RowStats st{};
-  if (share != 0.0) st = *reinterpret_cast<const RowStats*>(stats + r * kTkStats);
+  if (w != 0.0) st = *reinterpret_cast<const RowStats*>(stats + r * kTkStats);
   if (share == 0.0 || st.p == 0.0) {
     const float zero[8] = {};
     for (int i = t * 8; i < a.vocab; i += BLK * 8) tk_store8<DT, PAST>(out, i, a.vocab - i < 8 ? a.vocab - i : 8, zero);
@@ -528,14 +528,14 @@ __global__ void __launch_bounds__(kTkSecond) top_kl_second_kernel(TopKlArgs a, c
   // the listed tokens, while the row is on its way
   double x[3] = {0.0, 0.0, 0.0};  // u . q unlisted, listed; u . p
   int id0 = -1;
-  double q0 = 0.0, w0 = 0.0;
+  double q0 = 0.0, u0 = 0.0;
   for (int k = t; k < a.k; k += BLK) {
     const int id = tk_id(a, r * a.k + k);
     if (id < 0) continue;
-    const double q = q_of(a, st, load_as_f32(rows[0], id, DT)), w = load_as_f32(rows[1], id, DT);
-    if (k == t) id0 = id, q0 = q, w0 = w;
-    x[2] += w * p_of(a, st, r * a.k + k);
-    if (st.twice == 0.0 || first_of_id(a, r, k, id)) x[1] += w * q;
+    const double q = q_of(a, st, load_as_f32(rows[0], id, DT)), y = load_as_f32(rows[1], id, DT);
+    if (k == t) id0 = id, q0 = q, u0 = y;
+    x[2] += y * p_of(a, st, r * a.k + k);
+    if (st.twice == 0.0 || first_of_id(a, r, k, id)) x[1] += y * q;
   }
   float rest = 0.0f;
   const auto dot = [&](int i, int m, float (&x)[2][8]) {
@@ -570,12 +570,12 @@ __global__ void __launch_bounds__(kTkSecond) top_kl_second_kernel(TopKlArgs a, c
   kept(write);
   tk_stream<DT, BLK, 1>(rows, cut, H, [] {}, write);
   __syncthreads();
-  if (id0 >= 0) store_from_f32(out, id0, DT, static_cast<float>(f * st.p * q0 * (w0 - uq)));
+  if (id0 >= 0) store_from_f32(out, id0, DT, static_cast<float>(f * st.p * q0 * (u0 - uq)));
   for (int k = t + BLK; k < a.k; k += BLK) {
     const int id = tk_id(a, r * a.k + k);
     if (id < 0) continue;
-    const double q = q_of(a, st, load_as_f32(rows[0], id, DT)), w = load_as_f32(rows[1], id, DT);
-    store_from_f32(out, id, DT, static_cast<float>(f * st.p * q * (w - uq)));
+    const double q = q_of(a, st, load_as_f32(rows[0], id, DT)), y = load_as_f32(rows[1], id, DT);
+    store_from_f32(out, id, DT, static_cast<float>(f * st.p * q * (y - uq)));
   }
 }
 
@@ -612,10 +612,11 @@ int top_kl_args(const sf_top_kl_desc* desc, const char* what, TopKlArgs& a) {
   SF_CHECK_ARG(d.inner > 0 && d.rows % d.inner == 0 && d.outer_stride >= 0 && d.row_stride >= 0,
                "%s: rows in groups of %lld, strides %lld, %lld", what, (long long)d.inner, (long long)d.outer_stride,
                (long long)d.row_stride);
-  SF_CHECK_ARG(d.k >= 0 && d.k <= d.vocab, "%s: %lld entries of %lld", what, (long long)d.k, (long long)d.vocab);
+  SF_CHECK_ARG(d.k >= 0 && d.k <= d.vocab && d.k <= SF_TOP_MAX_ENTRIES, "%s: %lld entries of %lld (at most %d)", what,
+               (long long)d.k, (long long)d.vocab, SF_TOP_MAX_ENTRIES);
   SF_CHECK_ARG(d.id_bytes == 4 || d.id_bytes == 8, "%s: ids must be int32 or int64", what);
   SF_CHECK_ARG(d.logits && ((d.values && d.ids) || d.k == 0) && d.stats && d.norm, "%s: null pointer", what);
-  SF_CHECK_ARG(d.temperature > 0.0f && d.temperature <= 3.0e38f, "%s: temperature %g", what, d.temperature);
+  SF_CHECK_ARG(d.temperature >= 1.0e-30f && d.temperature <= 1.0e30f, "%s: temperature %g", what, d.temperature);
   a.s = d.logits, a.s0 = d.outer_stride, a.s1 = d.row_stride, a.inner = d.inner;
   a.values = d.values, a.ids = d.ids, a.lse = d.lse, a.weights = d.weights;
   a.vocab = static_cast<int>(d.vocab), a.k = static_cast<int>(d.k), a.vdt = d.value_dtype, a.id_bytes = d.id_bytes;

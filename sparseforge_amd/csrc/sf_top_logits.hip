@@ -135,7 +135,7 @@ extern "C" int sf_top_logits(const sf_top_logits_desc* desc, void* stream) {
   SF_CHECK_ARG(d.inner > 0 && d.rows % d.inner == 0 && d.outer_stride >= 0 && d.row_stride >= 0,
                "sf_top_logits: rows in groups of %lld, strides %lld, %lld", (long long)d.inner,
                (long long)d.outer_stride, (long long)d.row_stride);
-  SF_CHECK_ARG(d.temperature > 0.0f && d.temperature <= 3.0e38f, "sf_top_logits: temperature %g", d.temperature);
+  SF_CHECK_ARG(d.temperature >= 1.0e-30f && d.temperature <= 1.0e30f, "sf_top_logits: temperature %g", d.temperature);
   if (d.rows == 0) return SF_OK;
   SF_CHECK_ARG(d.logits && d.values && d.ids, "sf_top_logits: null pointer");
   TopLogitsArgs a;
@@ -147,10 +147,6 @@ extern "C" int sf_top_logits(const sf_top_logits_desc* desc, void* stream) {
   hipStream_t st = static_cast<hipStream_t>(stream);
   auto with = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
-    // Threads to a row: many where every CU has at most one, fewer where rows can cover each other's waits, the fewest
-    // for rows that these hold whole (bf16, k 20, us with 1024, 512 and 256 threads: 100 x 32000 13, 14 and 16; 1024 x
-    // 32000 43, 26 and 26; 3000 x 32000 109, 55 and 51; f32 1024 x 50257 66, 55 and 63).  Long rows in f32 are read twice
-    // in any case (1024 x 131072 151 and 157).
     // Threads to a row: many where a CU has at most one row, fewer where rows can cover each other's waits (us with 1024,
     // 512 and 256 threads, k 20: bf16 100 x 32000 14, 14 and 17; 1024 x 32000 31, 27 and 24; 3000 x 32000 71, 55 and 49;
     // f32 3000 x 50257 112, 110 and 117; 509 x 131072 with k 500 70 and 75).

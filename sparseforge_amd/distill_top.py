@@ -130,13 +130,16 @@ def top_kl_loss(student_logits: torch.Tensor, teacher: TopLogits, temperature=2,
     the same rows, as float32 (see the module).
 
     weights: float32 [..], 1 where None; rows of weight 0 (prompts, padding) are not looked at and take a zero gradient.
-    Rows without entries add 0; without any weight the loss is 0.  An id that is listed twice counts twice.  Logits are
+    Rows without entries add 0; without any weight the loss is 0.  An id that is listed twice counts twice.  A row has at
+    most 4096 entries, and no more than V.  Logits are
     not clamped and nothing is dropped: what is not finite shows in the loss.  Only the student takes a gradient."""
     values, ids, lse, at = teacher
     dev = L.require_device_only(student_logits, values, ids, lse, weights)
     L.dtype_code(student_logits)
     L.dtype_code(values)
-    lead, V = student_logits.shape[:-1], student_logits.shape[-1]
+    if student_logits.dim() < 1:
+        raise ValueError("top_kl_loss: the logits must be [.., V], got a number")
+    lead = student_logits.shape[:-1]
     if ids.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"top_kl_loss: the ids are {ids.dtype} (int32 / int64 only)")
     if values.shape != ids.shape or values.shape[:-1] != lead:

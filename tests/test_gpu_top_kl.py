@@ -428,3 +428,97 @@ def test_plain_and_recorded_backward_agree(cuda_device):
         torch.func.vmap(lambda x: top_kl_loss(x, teacher))(s.detach()[None])
     with pytest.raises(RuntimeError):
         torch.func.grad(lambda x: top_kl_loss(x, teacher))(s.detach())
+
+
+def test_rows_of_no_weight_beside_a_weight_that_is_nan(cuda_device):
+    """A NaN among the weights shows in the rows that count; rows of weight 0 still take zeros."""
+    from sparseforge_amd.distill import TopLogits, top_kl_loss
+
+    t = _inputs(cuda_device, (4,), 900, 6, torch.float32, padded=False, weighted=False)
+    weights = torch.tensor([1.0, 0.0, math.nan, 0.0], device=cuda_device)
+    s = t["s"].requires_grad_(True)
+    loss = top_kl_loss(s, TopLogits(t["values"], t["ids"], _lse(t, 2.0), 2.0), weights=weights)
+    g, = torch.autograd.grad(loss, s, create_graph=True)
+    h, = torch.autograd.grad(g, s, torch.ones_like(g))
+    for y in (g, h):
+        assert bool((y[[1, 3]] == 0).all()) and bool(y[[0, 2]].isnan().any(-1).all())
+
+
+def test_shapes_that_are_refused(cuda_device):
+    from sparseforge_amd.distill import TopLogits, top_kl_loss
+
+    v, i = torch.zeros(2, 5000, device=cuda_device), torch.zeros(2, 5000, dtype=torch.int32, device=cuda_device)
+    with pytest.raises(ValueError):
+        top_kl_loss(torch.zeros(2, 6000, device=cuda_device), TopLogits(v, i))  # too many entries
+    with pytest.raises(ValueError):
+        top_kl_loss(torch.zeros(2, 0, device=cuda_device), TopLogits(v[:, :0], i[:, :0]))
+    with pytest.raises(ValueError):
+        top_kl_loss(torch.zeros((), device=cuda_device), TopLogits(v[0, :1], i[0, :1]))
+    # no entries at all: nothing to learn
+    s = torch.randn(2, 30, device=cuda_device, requires_grad=True)
+    loss = top_kl_loss(s, TopLogits(v[:, :0], i[:, :0], torch.zeros(2, device=cuda_device), 2.0))
+    assert float(loss) == 0.0 and bool((torch.autograd.grad(loss, s)[0] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_behind_2_31_elements(cuda_device, dtype):
+    """The last rows of logits whose offsets pass 32 bits, with their gradient and second derivative."""
+    from sparseforge_amd.distill import TopLogits, top_kl_loss
+
+    B, V, k = 8300, 262144 if dtype == torch.bfloat16 else 262143, 12
+    t = _inputs(cuda_device, (3,), V, k, dtype, padded=False, weighted=False)
+    lse = _lse(t, 2.0)
+    s = torch.zeros(B, V, dtype=dtype, device=cuda_device)
+    s[-3:] = t["s"]
+    ids = torch.full((B, k), -1, dtype=torch.int32, device=cuda_device)
+    values, all_lse = torch.zeros(B, k, dtype=dtype, device=cuda_device), torch.zeros(B, device=cuda_device)
+    weights = torch.zeros(B, device=cuda_device)
+    ids[-3:], values[-3:], all_lse[-3:], weights[-3:] = t["ids"], t["values"], lse, 1.0
+    weights[5] = 1.0  # counts, without entries
+    u = torch.zeros_like(s)
+    u[-3:] = torch.randn(3, V, generator=t["g"], device=cuda_device).to(dtype)
+    s.requires_grad_(True)
+    loss = top_kl_loss(s, TopLogits(values, ids, all_lse, 2.0), weights=weights)
+    g, = torch.autograd.grad(loss, s, create_graph=True)
+    h, = torch.autograd.grad(g, s, u)
+    few = torch.cat([s.detach()[5:6], s.detach()[-3:]]).requires_grad_(True)
+    pick = [5, B - 3, B - 2, B - 1]
+    alone = top_kl_loss(few, TopLogits(values[pick], ids[pick], all_lse[pick], 2.0))
+    g1, = torch.autograd.grad(alone, few, create_graph=True)
+    h1, = torch.autograd.grad(g1, few, u[pick])
+    # other threads to a row: the sums of float32 exponentials differ in their order
+    bar = 2.0 ** -23 * (3 * (math.log(V) + 1) + 10 + V / 256) * 4
+    assert abs(float(loss.detach()) - float(alone.detach())) <= 4 * bar
+    for big, small in ((g.detach(), g1.detach()), (h, h1)):
+        step = torch.finfo(dtype).eps
+        near = (big[-3:].double() - small[1:].double()).abs()
+        assert bool((near <= (bar + step) * small[1:].double().abs() + bar * small.double().abs().amax(-1)[1:, None]).all())
+        for part in big[:-3].split(1000):
+            assert not bool((part != 0).any())
+
+
+def test_record_then_distil(cuda_device):
+    """top_logits' record of a teacher, kept in float32 or as it is, and the loss from it, against the definition; on a
+    stream of its own beside another."""
+    from sparseforge_amd.distill import TopLogits, top_kl_loss, top_logits
+
+    g = torch.Generator(device=cuda_device).manual_seed(21)
+    teacher = (torch.randn(2, 9, 32000, generator=g, device=cuda_device) * 3).bfloat16()
+    student = (teacher.float() + torch.randn(2, 9, 32000, generator=g, device=cuda_device)).bfloat16()
+    for k in (1, 50, 1000):
+        record = top_logits(teacher, k, 1.5)
+        t = {"s": student.clone(), "values": record.values, "ids": record.ids, "weights": None}
+        want = _loss(student.view(18, -1).double(), t, record.lse, 1.5)
+        dZ = 2.0 ** -24 * (3 * (math.log(32000) + 1) + 2 + 32000 / 256 + 8)
+        for values in (record.values, record.values.float()):
+            kept = TopLogits(values, record.ids.long(), record.lse, 1.5)
+            got = top_kl_loss(student, kept, 1.5)
+            assert abs(float(got) - float(want)) <= 1.5 ** 2 * 2 * dZ + 2.0 ** -24 * abs(float(want))
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        torch.cuda.synchronize()
+        outs = []
+        for stream in streams * 3:
+            with torch.cuda.stream(stream):
+                outs.append(top_kl_loss(student, top_logits(teacher, k, 1.5), 1.5))
+        torch.cuda.synchronize()
+        assert all(float(o) == float(outs[0]) for o in outs)

@@ -122,3 +122,50 @@ def test_captured_and_replayed(cuda_device):
         torch.cuda.synchronize()
         again = top_logits(x, 64)
         assert all(torch.equal(a, b) for a, b in zip(out[:3], again[:3]))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_behind_2_31_elements(cuda_device, dtype):
+    """The last rows of logits whose offsets pass 32 bits."""
+    from sparseforge_amd.distill import top_logits
+
+    B, V = 8300, 262144 if dtype == torch.bfloat16 else 262143
+    x = torch.zeros(B, V, dtype=dtype, device=cuda_device)
+    g = torch.Generator(device=cuda_device).manual_seed(3)
+    x[:, 7:1000:31] = 1.0
+    x[-3:] = (torch.randn(3, V, generator=g, device=cuda_device) * 3).to(dtype)
+    top = top_logits(x, 20)
+    alone = top_logits(x[-3:].clone(), 20)
+    assert torch.equal(top.ids[-3:], alone.ids) and torch.equal(top.values[-3:], alone.values)
+    assert torch.equal(top.lse[-3:], alone.lse)
+    assert bool((top.ids[:-3] == torch.arange(7, 7 + 31 * 20, 31, device=cuda_device)).all())
+
+
+def test_far_apart_and_at_the_ends_of_the_temperatures(cuda_device):
+    from sparseforge_amd.distill import top_logits
+
+    x = torch.tensor([[0.0, 1.0, -2.0], [3e38, -3e38, 0.0]], device=cuda_device)
+    for T in (1e-30, 1e-3, 1e30):
+        top = top_logits(x, 2, T)
+        assert top.ids.tolist() == [[1, 0], [0, 2]]
+        want = torch.logsumexp(x.double() / T, -1).float()
+        assert torch.allclose(top.lse, want, rtol=1e-6, atol=1e-6)
+
+
+def test_on_two_streams(cuda_device):
+    from sparseforge_amd.distill import top_logits
+
+    g = torch.Generator(device=cuda_device).manual_seed(6)
+    x = [torch.randn(300, 50257, generator=g, device=cuda_device) for _ in range(2)]
+    want = [top_logits(y, 50) for y in x]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(4):
+        for y, stream, out in zip(x, streams, got):
+            with torch.cuda.stream(stream):
+                out.append(top_logits(y, 50))
+    torch.cuda.synchronize()
+    for w, out in zip(want, got):
+        for o in out:
+            assert torch.equal(w.ids, o.ids) and torch.equal(w.values, o.values) and torch.equal(w.lse, o.lse)

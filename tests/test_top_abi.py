@@ -100,3 +100,18 @@ def test_rows_of_a_view():
         flat = torch.as_strided(y, (rows // inner, inner, t.shape[-1]), (outer, step, 1), y.storage_offset())
         assert torch.equal(flat.reshape(t.shape), t)
     assert L.rows_of(x[:, :-1])[0].data_ptr() == x.data_ptr() and L.rows_of(x[:0])[4] == 0
+
+
+def test_limits_of_temperatures_and_entries():
+    """Temperatures whose reciprocal float32 does not hold, and lists that are too long, are refused."""
+    from sparseforge_amd import _lib as L
+
+    lib = L.load()
+    for T in (1e-39, 1e-31, 1e31, 3.4e38):
+        d = L.TOP_LOGITS_DESC.pack(SOME, 0, 8, 2, 2, 2000, 3, SOME, SOME, 0, T, L.DT_F32)
+        assert lib.sf_top_logits(d, None) == L.SF_ERR_INVALID
+    for T, k in ((1e-39, 3), (3.4e38, 3), (1.0, 4097)):
+        d = L.TOP_KL_DESC.pack(SOME, 0, 8, 2, 2, 50000, SOME, SOME, k, 0, 0, SOME, SOME, T, L.DT_F32, L.DT_F32, 4)
+        assert lib.sf_top_kl_forward(d, SOME, SOME, 1 << 20, None) == L.SF_ERR_INVALID
+        assert lib.sf_top_kl_backward(d, SOME, SOME, None) == L.SF_ERR_INVALID
+        assert lib.sf_top_kl_double_backward(d, SOME, SOME, SOME, None, SOME, 1 << 20, None) == L.SF_ERR_INVALID
