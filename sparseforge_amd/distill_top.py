@@ -13,6 +13,7 @@ and the loss T^2 sum w KL / sum w over the rows.  It can be differentiated twice
 """
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import NamedTuple
 
 import torch
@@ -64,20 +65,25 @@ def top_logits(logits: torch.Tensor, k: int, temperature=2) -> TopLogits:
 def _top_kl_desc(s, values, ids, lse, weights, state, temperature):
     """The descriptor, and s or the copy of it that has to live until the call."""
     s, outer, step, inner, rows = L.rows_of(s)
-    at = state.data_ptr()  # the norm, then the rows' sums
+    at = state.data_ptr()  # the norm, the rows' sums, the forward's workspace
     return L.TOP_KL_DESC.pack(s.data_ptr(), outer, step, inner, rows, s.shape[-1], values.data_ptr(), ids.data_ptr(),
                               values.shape[-1], L.ptr(lse) or 0, L.ptr(weights) or 0, at + 8, at, temperature,
                               L.dtype_code(s), L.dtype_code(values), ids.element_size()), s
 
 
+@lru_cache(maxsize=64)
+def _sizes(rows: int) -> tuple[int, int]:
+    """Bytes of the rows' sums and of the workspace."""
+    return int(L.lib().sf_top_kl_stats_size(rows)), int(L.lib().sf_top_kl_workspace_size(rows))
+
+
 def _top_kl_forward(s, values, ids, lse, weights, temperature: float):
-    dev, lib, rows = s.device, L.lib(), s.shape[:-1].numel()
+    dev, (stats, ws) = s.device, _sizes(s.shape[:-1].numel())
     loss = torch.empty((), dtype=torch.float32, device=dev)
-    state = torch.empty(1 + int(lib.sf_top_kl_stats_size(rows)) // 8, dtype=torch.float64, device=dev)
-    ws = torch.empty(int(lib.sf_top_kl_workspace_size(rows)), dtype=torch.uint8, device=dev)
+    state = torch.empty(1 + (stats + ws) // 8, dtype=torch.float64, device=dev)  # an allocation costs 1.5 us
     desc, keep = _top_kl_desc(s, values, ids, lse, weights, state, temperature)
     with L.on(dev), _prof.region("sf_top_kl_forward", s.numel() * s.element_size(), "B", dev):
-        L.check(lib.sf_top_kl_forward(desc, loss.data_ptr(), ws.data_ptr(), ws.numel(), L.stream(dev)),
+        L.check(L.lib().sf_top_kl_forward(desc, loss.data_ptr(), state.data_ptr() + 8 + stats, ws, L.stream(dev)),
                 "sf_top_kl_forward")
     return loss, state
 
@@ -112,14 +118,14 @@ class _TopKLGrad(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, u):
         s, values, ids, lse, weights, state, g = ctx.saved_tensors
-        dev, lib, u = s.device, L.lib(), u.contiguous()
+        dev, u = s.device, u.contiguous()
         hs = torch.empty_like(s, memory_format=torch.contiguous_format)
         dot = torch.empty((), dtype=torch.float32, device=dev) if ctx.needs_input_grad[6] else None
-        ws = torch.empty(int(lib.sf_top_kl_workspace_size(s.shape[:-1].numel())), dtype=torch.uint8, device=dev)
+        ws = torch.empty(_sizes(s.shape[:-1].numel())[1], dtype=torch.uint8, device=dev)
         desc, keep = _top_kl_desc(s, values, ids, lse, weights, state, ctx.temperature)
         with L.on(dev), _prof.region("sf_top_kl_double_backward", 3 * s.numel() * s.element_size(), "B", dev):
-            L.check(lib.sf_top_kl_double_backward(desc, g.data_ptr(), u.data_ptr(), hs.data_ptr(), L.ptr(dot),
-                                                  ws.data_ptr(), ws.numel(), L.stream(dev)),
+            L.check(L.lib().sf_top_kl_double_backward(desc, g.data_ptr(), u.data_ptr(), hs.data_ptr(), L.ptr(dot),
+                                                      ws.data_ptr(), ws.numel(), L.stream(dev)),
                     "sf_top_kl_double_backward")
         return hs, None, None, None, None, None, dot, None
 
