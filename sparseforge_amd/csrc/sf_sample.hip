@@ -4,13 +4,22 @@
 //   top-k keeps the first k; top-p of these the fewest first tokens that hold p of their weight; min-p those of at least
 //   min_p times the largest weight.  All three keep a first part of that order.
 //   the token is the first, by id, at which the weight of the kept tokens up to it exceeds u times their whole weight.
-// Weights are formed in f64 and summed as integers of 2^-F, F = 44 (43 above 65536 tokens, 42 above 131072): sums do not depend on their order.  A cumulative share is off by 2e-12 (the exponential's polynomial) at most, which decides
-// one draw in 4e6 from 131072 equal tokens; shares from f32 exponentials, off by 1e-7, would decide one in a hundred.
+// Weights are formed in f64 and summed as integers of 2^-F, F = 44 (43 above 65536 tokens, 42 above 131072), so that no
+// sum depends on its order.  A cumulative share is off by 2e-12 (the exponential's polynomial) at most, which decides one
+// draw in 4e6 from 131072 equal tokens; shares from f32 exponentials, off by 1e-7, would decide one in a hundred.
 //
-// One workgroup per row, which it holds in registers if it fits.  With top-k up to 1024 the row's largest are gathered in
-// LDS (gather_top) and the rest happens among them.  Without it, top-p's border is the place in a histogram of weights by
-// logit where their sum reaches p, resolved among the tokens of that bin; the draw finds the wave's part of the row, then
-// the thread's.
+// One workgroup per row.  With top-k up to 1024 the row is read once, for the maxima of its pieces; the pieces above the
+// bound that follows from these are taken again, their largest gathered in LDS, and the rest happens among them.  Without
+// it, top-p's border is the place in a histogram of weights by logit where their sum reaches p, resolved among the tokens
+// of that bin, which are gathered while the weight above the bin is summed; the draw finds the wave's part of the row,
+// then the thread's.
+//
+// Few rows are bound by their chain of passes and barriers (4 x 32000 bf16, k 50: 9.8 us; 48 x 50257 f32 with settings of
+// their own: 17), many without top-k by the vector unit, which forms a weight in 23 instructions for 64 elements: 1024 x
+// 32000 bf16 without limits 41 us (vector unit 0.72 busy), 256 x 131072 f32 with top-p 0.95 107 us (three passes, 0.60
+// busy, half of the cycles of LDS lost to bins that collide).  1024 x 32000 bf16 with k 50: 30 us.  Tried for top-p: a
+// histogram with f32 exponentials that the next pass's exact sums confirm, 117 us with sums of 64 bits, 256 with the float
+// additions of LDS.
 #include <type_traits>
 
 #include "sf_mfma.hpp"
@@ -590,7 +599,7 @@ extern "C" int sf_sample_logits(const sf_sample_desc* desc, void* stream) {
                                0x1.3b2ab70ad2565p-7,  0x1.5d877598350dep-10, 0x1.4308c7183d6a2p-13,
                                0x1.00c0e4e15189cp-16, 0x1.63b2d7971923fp-20};
   memcpy(a.poly, kPoly, sizeof(kPoly));
-  // The sums of a thread, which has at most 256 weights of at most 2^bits, and vocab / 512, stay below 2^52.
+  // The sums of a thread, which has at most vocab / 512 weights of at most 2^bits, stay below 2^52.
   a.bits = 60;
   for (int64_t n = 1; n < d.vocab; n *= 2) --a.bits;
   if (a.bits > 44) a.bits = 44;
@@ -599,8 +608,15 @@ extern "C" int sf_sample_logits(const sf_sample_desc* desc, void* stream) {
   hipStream_t st = static_cast<hipStream_t>(stream);
   auto with = [&](auto dt) {
     constexpr int DT = decltype(dt)::value;
+    // Pieces that stay in registers: with the code of every setting half as many, as more are spilled (us with 12, 8, 4
+    // and 2 of bf16 and half of that of f32, top-p 0.9: 1024 x 32000 bf16 108, 87, 86 and 86; 1024 x 50257 f32 171, 155,
+    // 147 and 154).
     constexpr int H = DT == SF_DTYPE_BF16 ? 8 : 4, kFew = H / 2;
-    const bool narrow = d.rows > 256 && a.vocab <= (DT == SF_DTYPE_BF16 ? 131072 : 65536);
+    // Threads to a row: 1024 where a CU has at most one row, 512 where two cover each other's waits (us: 64 x 50257 f32 k
+    // 50 17 and 20, 64 x 131072 bf16 top-p 0.9 80 and 96; 300 x 32000 bf16 k 400 31 and 22, 1024 x 50257 f32 top-p 0.9 178
+    // and 149, 1024 x 131072 f32 k 400 164 and 150, without limits 209 and 209; 300 x 262144 bf16 without limits 141 and
+    // 148).
+    const bool narrow = d.rows > 256;
     const bool whole = !a.temp && a.temp1 > 0.0f && !a.top_k && (a.top_k1 <= 0 || a.top_k1 >= a.vocab) && !a.top_p &&
                        !(a.top_p1 < 1.0f);
     const bool top_k = (!a.top_k && a.top_k1 > 0 && a.top_k1 <= (narrow ? 512 : 1024)) || (!a.temp && !(a.temp1 > 0.0f));

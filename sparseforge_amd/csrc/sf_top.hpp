@@ -51,8 +51,8 @@ struct Raw8 {
   }
 };
 
-// A row in front of a workgroup of BLK threads.  Each wave has a range of the ids of its own, `pieces` (at most 32) times
-// 512 long; of piece p of a wave, lane l has 8 ids.  What lies behind the row is -inf.
+// A row in front of a workgroup of BLK threads.  Each wave has a range of the ids of its own, `pieces` times 512 long; of
+// piece p of a wave, lane l has 8 ids.  What lies behind the row is -inf.
 template <int DT, int BLK>
 struct RowAt {
   const void* row;
@@ -170,7 +170,8 @@ __device__ __forceinline__ float max8(const float (&v)[8]) {
 // x of the lane that a DPP control names, `none` in lanes that it gives nothing.
 template <int CTRL, int ROWS = 0xf>
 __device__ __forceinline__ uint32_t dpp(uint32_t x, uint32_t none) {
-  return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(static_cast<int>(none), static_cast<int>(x), CTRL, ROWS, 0xf, false));
+  return static_cast<uint32_t>(
+      __builtin_amdgcn_update_dpp(static_cast<int>(none), static_cast<int>(x), CTRL, ROWS, 0xf, false));
 }
 template <int CTRL, int ROWS = 0xf>
 __device__ __forceinline__ u64 dpp(u64 x, u64 none) {

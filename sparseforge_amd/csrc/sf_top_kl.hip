@@ -10,7 +10,13 @@
 //   h_j = q_j ((P - r kappa) u_j - (P U - r kappa^2 U_r))  [unlisted],   P q_j (u_j - U)  [listed].
 // The rest's sums are formed without the listed tokens (one bit for each of the vocabulary in LDS), not as a difference.
 //
-// One workgroup per row streams it once.  Listed tokens (at most a few hundred) are gathered and handled in f64.
+// One workgroup per row streams it once forward and once backward (twice along u); listed tokens are gathered and handled
+// in f64 while the row is on its way.  Row sums are f32 exponentials in compensated sums, joined in f64; stats and losses
+// are f64.  Bound by memory: forward and backward by turns 4096 x 32000 bf16, k 64, 143 us (two reads and a write of 262
+// MB: 5.5 TB/s, what a copy reaches), 2048 x 131072 269 (6.0 TB/s, part of the second read from the last-level cache),
+// 2046 x 50257 f32 with rows of odd alignment 202 (6.1 TB/s); along u 1024 x 32000 45 (two rows read, one written, 4.4
+// TB/s).  64 x 32000 forward 7 us and 3 for the sum over the rows.  Two products of log-softmax over the vocabulary, as the
+// formula stands, take ten passes and more.
 #include <type_traits>
 
 #include "sf_top.hpp"
@@ -18,7 +24,13 @@
 namespace sf {
 namespace {
 
-constexpr int kTkForwardU = 3, kTkBackwardU = 4;  // pieces of a row a thread loads before using them
+// Pieces of a row that a thread loads before it uses them: bytes on their way against registers.  Forward and backward by
+// turns, us: 4096 x 32000 bf16 142 with 3 and 4 pieces, 146 with 2 and 2; 2046 x 50257 f32, whose pieces are twice as
+// long, 212 and 202.
+template <int DT>
+constexpr int kTkForwardU = DT == SF_DTYPE_BF16 ? 3 : 2;
+template <int DT>
+constexpr int kTkBackwardU = DT == SF_DTYPE_BF16 ? 4 : 2;
 constexpr int kTkSecond = 512;
 constexpr int kTkStats = 8;  // f64 of a row's RowStats
 
@@ -280,7 +292,7 @@ __global__ void __launch_bounds__(BLK) top_kl_kernel(TopKlArgs a, double* __rest
     lanes_sum(x);
     part.e0 = x[0], part.e1 = x[1], part.e2 = x[2], part.sl = x[3];
   };
-  tk_stream<DT, BLK, kTkForwardU>(rows, cut, 0, listed, [&](int i, int, float (&x)[1][8]) {
+  tk_stream<DT, BLK, kTkForwardU<DT>>(rows, cut, 0, listed, [&](int i, int, float (&x)[1][8]) {
     float(&v)[8] = x[0];
     float top = m;
     const uint32_t out = REST ? marks8(bits, cut, i) : 0;
@@ -462,7 +474,7 @@ __global__ void __launch_bounds__(BLK) top_kl_backward_kernel(TopKlArgs a, const
   const RowGrad<DT> g(a, st);
   const float coef = static_cast<float>(f * (st.p - (st.r != 0.0 ? st.r * exp(st.lz - st.lzr) : 0.0)));
   const void* rows[1] = {row_at<DT>(a.s, (r / a.inner) * a.s0 + (r % a.inner) * a.s1)};
-  const Cut cut = Cut::of<DT, BLK>(rows[0], a.vocab);
+  const Cut cut = Cut::of<DT, BLK>(out, a.vocab);  // whole 16 bytes are written rather than read
   // the listed tokens' own gradient, formed while the row is on its way and written when the row is
   const auto listed = [&](int k, int id) {
     const double q = q_of(a, st, load_as_f32(rows[0], id, DT));
@@ -474,7 +486,7 @@ __global__ void __launch_bounds__(BLK) top_kl_backward_kernel(TopKlArgs a, const
     if (t < a.k) id0 = tk_id(a, r * a.k + t);
     if (id0 >= 0) g0 = listed(t, id0);
   };
-  tk_stream<DT, BLK, kTkBackwardU>(rows, cut, 0, first, [&](int i, int n, float (&x)[1][8]) {
+  tk_stream<DT, BLK, kTkBackwardU<DT>>(rows, cut, 0, first, [&](int i, int n, float (&x)[1][8]) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[0][k] = coef * g.q(x[0][k]);
     tk_store8<DT, PAST>(out, i, n, x[0]);
@@ -487,7 +499,9 @@ __global__ void __launch_bounds__(BLK) top_kl_backward_kernel(TopKlArgs a, const
   }
 }
 
-// Along u (rows contiguous): h_j, and the row's u . dL/ds at an upstream gradient of 1.
+// Along u (rows contiguous): h_j, and the row's u . dL/ds at an upstream gradient of 1.  Of the pieces that both passes need
+// the first H of a thread stay in registers: 4096 x 32000 bf16 167 us with 6, 185 with 2; 2046 x 50257 f32 248 with 3,
+// 259 with 1.
 template <int DT, bool PAST>
 __global__ void __launch_bounds__(kTkSecond) top_kl_second_kernel(TopKlArgs a, const double* __restrict__ stats,
                                                                   const double* __restrict__ norm,
@@ -579,7 +593,10 @@ __global__ void __launch_bounds__(kTkSecond) top_kl_second_kernel(TopKlArgs a, c
   }
 }
 
-constexpr int64_t kTkFewRows = 512;  // fewer rows than this take more threads each
+// With at most one row for each CU a row takes 1024 threads; with more, 256 forward and 512 backward, whose waits cover each
+// other.  Forward and backward by turns, us: 64 x 32000 bf16 15.8 and 17.9, 256 x 50257 f32 35 and 39; 400 x 32000 bf16
+// 30.6 and 26.3, 400 x 50257 f32 53 and 50, 4096 x 32000 bf16 193 and 143 (256 threads backward too: 150).
+constexpr int64_t kTkFewRows = 256;
 
 // launch(data type, whether what it writes passes the caches).  A gradient that the last-level cache (256 MB) does not hold
 // beside the logits is not found there by who reads it next, and what of it stays there has to be written back while the
@@ -656,7 +673,7 @@ extern "C" int sf_top_kl_forward(const sf_top_kl_desc* desc, float* loss, void* 
       else
         top_kl_kernel<DT, BLK, false><<<grid, BLK, lds, st>>>(a, desc->stats, row_kl);
     };
-    if (desc->rows < kTkFewRows)
+    if (desc->rows <= kTkFewRows)
       with(std::integral_constant<int, 1024>{});
     else
       with(std::integral_constant<int, 256>{});
@@ -674,7 +691,7 @@ extern "C" int sf_top_kl_backward(const sf_top_kl_desc* desc, const float* grad_
   tk_dispatch(*desc, [&](auto dt, auto past) {
     constexpr int DT = decltype(dt)::value;
     constexpr bool PAST = decltype(past)::value;
-    if (desc->rows < kTkFewRows)
+    if (desc->rows <= kTkFewRows)
       top_kl_backward_kernel<DT, 1024, PAST><<<grid, 1024, 0, st>>>(a, desc->stats, desc->norm, grad_out, grad_logits);
     else
       top_kl_backward_kernel<DT, 512, PAST><<<grid, 512, 0, st>>>(a, desc->stats, desc->norm, grad_out, grad_logits);

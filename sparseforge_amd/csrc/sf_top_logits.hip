@@ -3,7 +3,12 @@
 //
 // One workgroup per row reads it once, for the sum of exponentials and the maxima of the threads' pieces.  From these follows
 // a bound above which the k largest and few others lie (top_bound), whose pieces are taken again from the caches.  The
-// candidates are ordered in LDS.
+// candidates are ordered in LDS: counted into bins, placed, ranked among those of their bin.  Rows in which that finds too
+// many or too few (equal values, infinities, NaN) are looked through by the bits of their logits instead.
+//
+// 4096 x 32000 bf16, k 64: 60 us (262 MB at 4.4 TB/s; the vector unit is 0.86 busy: an exponential and a fourth of a
+// compensated sum for each element beside the maxima); 509 x 131072 f32, k 500: 63 us (267 MB at 4.2 TB/s); 16 x 32000
+// bf16, k 20: 10 us, a chain of some ten barriers.  Every row by the bits of its logits: 589, 404 and 71 us.
 #include <type_traits>
 
 #include "sf_top.hpp"
