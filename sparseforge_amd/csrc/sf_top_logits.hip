@@ -8,7 +8,8 @@
 //
 // 4096 x 32000 bf16, k 64: 60 us (262 MB at 4.4 TB/s; the vector unit is 0.86 busy: an exponential and a fourth of a
 // compensated sum for each element beside the maxima); 509 x 131072 f32, k 500: 63 us (267 MB at 4.2 TB/s); 16 x 32000
-// bf16, k 20: 10 us, a chain of some ten barriers.  Every row by the bits of its logits: 589, 404 and 71 us.
+// bf16, k 20: 10 us, a chain of some ten barriers.  With four passes over the bits of every row's logits: 589, 404 and 71
+// us.
 #include <type_traits>
 
 #include "sf_top.hpp"
@@ -48,19 +49,17 @@ __device__ __forceinline__ void top_of_any(const TopLogitsArgs& a, const void* r
                        .id;
   if (t == 0) sh.n = 0;
   __syncthreads();
-#pragma unroll 1
-  for (int i = t; i < V; i += BLK) {
-    const float x = load_as_f32(row, i, DT);
-    const uint32_t key = top_key<DT>(x);
-    if (key > border.key || (key == border.key && i <= last)) sh.found[atomicAdd(&sh.n, 1)] = candidate(x, i);
-  }
+  each_any<DT, BLK>(row, V, [&](int i, int n, const float (&v)[8]) SF_INLINE {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const uint32_t key = top_key<DT>(v[k]);
+      if (k < n && (key > border.key || (key == border.key && i + k <= last)))
+        sh.found[atomicAdd(&sh.n, 1)] = candidate(v[k], i + k);
+    }
+  });
   __syncthreads();
-  for (int i = t; i < a.k; i += BLK) {
-    const u64 own = sh.found[i];
-    int rank = 0;
-    for (int j = 0; j < a.k; ++j) rank += sh.found[j] > own ? 1 : 0;
-    put<DT>(a, row, r, rank, candidate_id(own));
-  }
+  sort_all<BLK>(sh.found, a.k);
+  for (int i = t; i < a.k; i += BLK) put<DT>(a, row, r, i, candidate_id(sh.found[i]));
 }
 
 // k is at most BLK (two groups' maxima a thread) and below CAP.
@@ -118,7 +117,7 @@ __global__ void __launch_bounds__(BLK) top_logits_kernel(TopLogitsArgs a) {
   if (n < a.k || n > CAP) {  // -inf, inf or NaN among the k, or too many equals
     top_of_any<DT, BLK>(a, row.row, r, any, sh);
   } else {
-    sort_found<BLK>(bound, n, sh);
+    sort_found<BLK>(bound, m, n, sh);
     for (int i = t; i < a.k; i += BLK) put<DT>(a, row.row, r, i, candidate_id(sh.found[i]));
   }
 }

@@ -352,3 +352,27 @@ def test_penalties_then_a_draw(cuda_device):
         ok = torch.arange(B, device=cuda_device) != 2
         assert bool(allowed[ok].gather(1, ids[ok, None]).all())
         check(y, u, {"temperature": 0.9, **settings})
+
+
+@pytest.mark.parametrize("settings", [{"top_k": 40}, {"top_k": 300, "top_p": 0.9}, {"top_k": 900, "temperature": 1.5},
+                                      {"top_k": 2500, "top_p": 0.95}, {"top_p": 0.9}, {"top_p": 0.999}],
+                         ids=lambda s: "-".join(f"{k}{v}" for k, v in s.items()))
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_logits_far_from_all_others(cuda_device, dtype, settings):
+    """Masks of -1e4, 1e9 and the type's lowest value, lone large logits, clusters, differences below 1e-30; alone and in
+    rows enough for fewer threads each, which draw the same."""
+    from sparseforge_amd.logits import sample_logits
+
+    g = torch.Generator(device=cuda_device).manual_seed(17)
+    V = 30011
+    n = torch.randn(V, generator=g, device=cuda_device) * 2
+    i = torch.arange(V, device=cuda_device)
+    few = torch.rand(V, generator=g, device=cuda_device) < 0.05
+    rows = [torch.where(few, n, low) for low in (-1e4, -1e9, torch.finfo(dtype).min)]
+    rows += [torch.where(i % 4001 == 7, 1e4, n), torch.where(i < 700, 100.0 + n, n), n * 1e-44, (n * 4).round(),
+             torch.where(few, 1.0, -1e30), torch.where(few, n - 30.0, torch.finfo(dtype).min), n * 0.5 + 12.0]
+    x = torch.stack(rows).to(dtype)
+    u = torch.rand(len(rows), generator=g, device=cuda_device)
+    check(x, u, settings, edges=False)
+    many = sample_logits(x.repeat(30, 1), u.repeat(30), **settings)
+    assert torch.equal(many, sample_logits(x, u, **settings).repeat(30))

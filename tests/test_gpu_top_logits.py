@@ -169,3 +169,25 @@ def test_on_two_streams(cuda_device):
     for w, out in zip(want, got):
         for o in out:
             assert torch.equal(w.ids, o.ids) and torch.equal(w.values, o.values) and torch.equal(w.lse, o.lse)
+
+
+def _far_apart(dev, dtype, V=30011):
+    """Rows in which some logits lie far from all others, or hardly apart."""
+    g = torch.Generator(device=dev).manual_seed(17)
+    n = torch.randn(V, generator=g, device=dev) * 2
+    i = torch.arange(V, device=dev)
+    few = torch.rand(V, generator=g, device=dev) < 0.05
+    rows = [torch.where(few, n, low) for low in (-1e4, -1e9, -3e38, torch.finfo(dtype).min)]
+    rows += [torch.where(i % 4001 == 7, 1e4, n), torch.where(i % 97 == 7, 3e38, n), torch.where(i < 700, 100.0 + n, n),
+             torch.where(i < 700, 100.0 + n, torch.where(few, n, -1e30)), n * 1e-44, torch.where(few, n * 1e-40, -1e30),
+             torch.where(i == 5, 3e38, torch.where(few, n * 1e-40, -3e38)), (n * 4).round(), torch.where(few, 1.0, -1e30),
+             n + torch.where(i % 2 == 0, 1e6, -1e6), torch.where(i < 1500, 2.0 + n * 1e-3, n * 1e-3 - 30.0)]
+    return torch.stack(rows).to(dtype)
+
+
+@pytest.mark.parametrize("copies", [1, 40])  # with 1024 threads a row, with 512 and 256
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_logits_far_from_all_others(cuda_device, dtype, copies):
+    x = _far_apart(cuda_device, dtype).repeat(copies, 1)
+    for k in (1, 20, 128, 300, 1000):
+        check(x, k, 1.0)
