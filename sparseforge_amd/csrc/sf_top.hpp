@@ -485,8 +485,8 @@ __device__ __forceinline__ uint32_t hits_of(const float (&best)[G], const Bound&
 
 // ---------------------------------------------------------------------------
 // Passes that are right for every row, whatever its order and its equal values, for the rows in which gather() finds too
-// many (512 rows of 131072 equal bf16 logits: k 20 250 us, k 50 drawn 290, top-p 0.9 drawn 550).  Thread t takes elements [8 t, 8 t + 8) of tiles of 8 * BLK, so that tiles, waves and lanes follow each other in the
-// order of the ids.
+// many (512 rows of 131072 equal bf16 logits: k 20 250 us, k 50 drawn 290, top-p 0.9 drawn 550).  Thread t takes elements
+// [8 t, 8 t + 8) of tiles of 8 * BLK, so that tiles, waves and lanes follow each other in the order of the ids.
 // ---------------------------------------------------------------------------
 // A row's order as integers: larger logits have larger keys, -0 equals 0, NaN is largest.  bf16 needs 16 bits.
 template <int DT>

@@ -93,6 +93,12 @@ def generate(model: LlamaDecoder, prompts: torch.Tensor, new_tokens: int, length
         raise ValueError(f"generate: prompts must be ids [B, S], got {prompts.dtype} {tuple(prompts.shape)}")
     if pick is not None and temperature is not None:
         raise ValueError("generate: pick and a temperature both say how tokens are chosen")
+    if temperature is None:
+        given = {"top_k": (top_k, 0), "top_p": (top_p, 1.0), "min_p": (min_p, 0.0)}
+        unused = [n for n, (x, none) in given.items() if torch.is_tensor(x) or x != none]
+        unused += ["generator"] if generator is not None else []
+        if unused:
+            raise ValueError(f"generate: {', '.join(unused)} without a temperature, which draws tokens")
     if new_tokens < 0 or chunk < 1:
         raise ValueError(f"generate: {new_tokens} new tokens, chunks of {chunk}")
     B, S = prompts.shape

@@ -85,3 +85,14 @@ def test_refusals(cuda_device):
     for bad in ({"temperature": -1.0}, {"temperature": 1.0, "top_p": 2.0}, {"temperature": 1.0, "top_k": -1}):
         with pytest.raises(ValueError):
             generate(m, prompts, 2, **bad)
+
+
+def test_settings_without_a_temperature_are_refused(cuda_device):
+    from sparseforge_amd.generate import generate
+
+    model, prompts = _model(cuda_device), torch.ones(2, 3, dtype=torch.int64, device=cuda_device)
+    for bad in ({"top_k": 5}, {"top_p": 0.9}, {"min_p": 0.1}, {"top_p": torch.ones(2, device=cuda_device)},
+                {"generator": torch.Generator(device=cuda_device)}):
+        with pytest.raises(ValueError, match="temperature"):
+            generate(model, prompts, 2, **bad)
+    generate(model, prompts, 2, top_k=0, top_p=1.0, min_p=0.0)

@@ -522,3 +522,65 @@ def test_record_then_distil(cuda_device):
                 outs.append(top_kl_loss(student, top_logits(teacher, k, 1.5), 1.5))
         torch.cuda.synchronize()
         assert all(float(o) == float(outs[0]) for o in outs)
+
+
+def test_captured_second_derivative(cuda_device):
+    """Loss, gradient and the second derivative's product in one graph, beside another graph of the same tensors, replayed in
+    turn on new logits and weights with eager work between."""
+    from sparseforge_amd.distill import TopLogits, top_kl_loss
+
+    t = _inputs(cuda_device, (6,), 5001, 30, torch.float32, padded=False)
+    teacher = TopLogits(t["values"], t["ids"], _lse(t, 2.0), 2.0)
+    s, weights = t["s"].clone().requires_grad_(True), t["weights"].clone()
+    u = torch.randn(s.shape, generator=t["g"], device=cuda_device)
+
+    def step():
+        loss = top_kl_loss(s, teacher, weights=weights)
+        g, = torch.autograd.grad(loss, s, create_graph=True)
+        h, = torch.autograd.grad(g, s, u)
+        return loss.detach(), g.detach(), h
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for graph in graphs:
+        with torch.cuda.graph(graph):
+            outs.append(step())
+    for _ in range(3):
+        with torch.no_grad():
+            s.copy_(torch.randn(s.shape, generator=t["g"], device=cuda_device) * 2)
+            weights.copy_(torch.rand(weights.shape, generator=t["g"], device=cuda_device))
+            weights[2] = 0.0
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        want = step()
+        for out in outs:
+            for a, b in zip(out, want):
+                assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_logits_next_to_the_row_are_left(cuda_device, dtype):
+    """Gradients are written to their rows alone, whatever the alignment: rows of odd lengths beside others."""
+    from sparseforge_amd import _lib as L
+    from sparseforge_amd.distill_top import _top_kl_desc, _top_kl_forward
+
+    for V in (1, 7, 8, 9, 130, 4099):
+        t = _inputs(cuda_device, (5,), V, 1, dtype, padded=False, weighted=False)
+        lse = _lse(t, 2.0)
+        ids = t["ids"].contiguous()
+        loss, state = _top_kl_forward(t["s"], t["values"], ids, lse, None, 2.0)
+        one = torch.ones((), device=cuda_device)
+        guard = torch.full((5 * V + 64,), 7.0, dtype=dtype, device=cuda_device)
+        desc, keep = _top_kl_desc(t["s"], t["values"], ids, lse, None, state, 2.0)
+        for at in (0, 1, 8, 13):
+            guard.fill_(7.0)
+            out = guard[32 + at:32 + at + 5 * V]
+            L.check(L.lib().sf_top_kl_backward(desc, one.data_ptr(), out.data_ptr(), L.stream(t["s"].device)), "backward")
+            assert bool((guard[:32 + at] == 7.0).all()) and bool((guard[32 + at + 5 * V:] == 7.0).all())
+            assert bool(out.isfinite().all()) and not bool((out == 7.0).any())
