@@ -17,7 +17,7 @@
 // Few rows are bound by their chain of passes and barriers (4 x 32000 bf16, k 50: 9.8 us; 48 x 50257 f32 with settings of
 // their own: 17), many without top-k by the vector unit, which forms a weight in 23 instructions for 64 elements: 1024 x
 // 32000 bf16 without limits 41 us (vector unit 0.72 busy), 256 x 131072 f32 with top-p 104 us (three passes, 0.60
-// busy, half of the cycles of LDS lost to bins that collide).  1024 x 32000 bf16 with k 50: 30 us.  Tried for top-p: a
+// busy, half of the cycles of LDS lost to bins that collide).  1024 x 32000 bf16 with k 100: 28 us.  Tried for top-p: a
 // histogram with f32 exponentials that the next pass's exact sums confirm, 117 us with sums of 64 bits, 256 with the float
 // additions of LDS.
 #include <type_traits>
@@ -169,19 +169,23 @@ __device__ __forceinline__ void sample_any(const SampleArgs& a, const Settings& 
   if (threadIdx.x == 0) put_token(a, s, r, at.id, load_as_f32(row, at.id, DT), at.total);
 }
 
-struct SampleShared {
-  TopShared<kSpCandidates> top;
-  u64 weight[kSpBins + 64];  // by place, or by bin; in the end a bin for each lane of what has no weight
-  u64 before[kSpCandidates];
+// CAP: candidates, BINS: bins of weight, or tokens that are drawn from.
+template <int CAP, int BINS>
+struct SampleLds {
+  TopShared<CAP> top;
+  u64 weight[BINS + 64];  // by place, or by bin; in the end a bin for each lane of what has no weight
+  u64 before[BINS];
   u64 part[2][16];
   u64 base, last;
   int count, bin;
 };
+using SampleShared = SampleLds<kSpCandidates, kSpBins>;
 
 // The draw by one wave among the row's n <= 64 largest, which sh.top.found holds in any order: top-k, top-p, min-p and the
 // token.
+template <typename S>
 __device__ __forceinline__ void sample_few(const SampleArgs& a, const Settings& s, int64_t r, const Weight& weight, int n,
-                                           SampleShared& sh) {
+                                           S& sh) {
   const int t = threadIdx.x;
   const u64 own = t < n ? sh.top.found[t] : 0;
   int rank = 0;
@@ -207,9 +211,9 @@ __device__ __forceinline__ void sample_few(const SampleArgs& a, const Settings& 
 
 // The same by the workgroup among the n largest in order.  Ids are drawn from by ranges: the range in which the sum passes
 // the drawn share, then the token among the kept ones of that range.
-template <int BLK>
+template <int BLK, typename S>
 __device__ __forceinline__ void sample_sorted(const SampleArgs& a, const Settings& s, int64_t r, const Weight& weight,
-                                              int n, SampleShared& sh) {
+                                              int n, S& sh) {
   const int t = threadIdx.x, k = s.k < n ? static_cast<int>(s.k) : n;  // k <= BLK
   const u64 c = t < k ? sh.top.found[t] : 0;
   const float x = candidate_logit(c);
@@ -243,9 +247,9 @@ __device__ __forceinline__ void sample_sorted(const SampleArgs& a, const Setting
   }
 }
 
-template <int BLK>
+template <int BLK, typename S>
 __device__ __forceinline__ void sample_found(const SampleArgs& a, const Settings& s, int64_t r, const Weight& weight,
-                                             const Bound& bound, int n, SampleShared& sh) {
+                                             const Bound& bound, int n, S& sh) {
   if (n > 64) {
     sort_found<BLK>(bound, s.top, n, sh.top);
     sample_sorted<BLK>(a, s, r, weight, n, sh);
@@ -254,14 +258,14 @@ __device__ __forceinline__ void sample_found(const SampleArgs& a, const Settings
   }
 }
 
-// Every row with top-k, of at most BLK (or at temperature 0): the row is read once.
-template <int DT, int BLK, int G>
+// Every row with top-k, of at most BLK and less than CAP (or at temperature 0): the row is read once.
+template <int DT, int BLK, int G, int CAP>
 __global__ void __launch_bounds__(BLK) sample_top_k_kernel(SampleArgs a) {
   __shared__ union {
-    SampleShared sh;
+    SampleLds<CAP, BLK> sh;
     AnyShared any;
   } lds;
-  SampleShared& sh = lds.sh;
+  auto& sh = lds.sh;
   const int64_t r = blockIdx.x;
   const RowAt<DT, BLK> row(static_cast<const char*>(a.x) + r * a.xs * (DT == SF_DTYPE_BF16 ? 2 : 4), a.vocab);
   Settings s(a, r);
@@ -280,9 +284,9 @@ __global__ void __launch_bounds__(BLK) sample_top_k_kernel(SampleArgs a) {
   if (m < INFINITY) {
     const Bound bound = bound_of<BLK>(best, m, static_cast<int>(s.k), sh.top);
     n = gather<G>(row, bound, hits_of(best, bound), sh.top);
-    if (n > 0 && n <= kSpCandidates) sample_found<BLK>(a, s, r, weight, bound, n, sh);
+    if (n > 0 && n <= CAP) sample_found<BLK>(a, s, r, weight, bound, n, sh);
   }
-  if (n == 0 || n > kSpCandidates) {
+  if (n == 0 || n > CAP) {
     __syncthreads();
     sample_any<DT, BLK>(a, s, r, row.row, weight, lds.any);
   }
@@ -637,11 +641,16 @@ extern "C" int sf_sample_logits(const sf_sample_desc* desc, void* stream) {
     const bool narrow = d.rows > 256;
     const bool whole = !a.temp && a.temp1 > 0.0f && !a.top_k && (a.top_k1 <= 0 || a.top_k1 >= a.vocab) && !a.top_p &&
                        !(a.top_p1 < 1.0f);
-    const bool top_k = (!a.top_k && a.top_k1 > 0 && a.top_k1 <= (narrow ? 512 : 1024)) || (!a.temp && !(a.temp1 > 0.0f));
-    if (narrow && top_k)
-      sample_top_k_kernel<DT, 512, 16><<<grid, 512, 0, st>>>(a);
-    else if (top_k)
-      sample_top_k_kernel<DT, 1024, 8><<<grid, 1024, 0, st>>>(a);
+    const int k = !a.temp && !(a.temp1 > 0.0f) ? 1 : a.top_k || a.top_k1 <= 0 ? INT32_MAX : a.top_k1;
+    // 256 where many rows each give few candidates (us, k 100, with 512 and 256: 3000 x 8192 bf16 63 and 34, 600 x 32000
+    // bf16 27 and 23, 3000 x 32000 f32 103 and 85, 1024 x 65536 bf16 44 and 43, 300 x 65536 bf16 23 and 28, 1024 x 131072
+    // bf16 74 and 78).
+    if (d.rows > 512 && k <= 128 && a.vocab <= 65536)
+      sample_top_k_kernel<DT, 256, 16, 512><<<grid, 256, 0, st>>>(a);
+    else if (narrow && k <= 512)
+      sample_top_k_kernel<DT, 512, 16, 2048><<<grid, 512, 0, st>>>(a);
+    else if (!narrow && k <= 1024)
+      sample_top_k_kernel<DT, 1024, 8, 2048><<<grid, 1024, 0, st>>>(a);
     else if (narrow && whole)
       sample_kernel<DT, 512, H, true><<<grid, 512, 0, st>>>(a);
     else if (narrow)
