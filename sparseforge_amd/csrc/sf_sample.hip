@@ -332,10 +332,7 @@ __device__ __forceinline__ void fill_bins(Row<DT, BLK, H>& row, const Bins& bins
 }
 
 // The float above x, which is not inf.
-__device__ __forceinline__ float float_above(float x) {
-  const uint32_t key = ordered_key(x) + 1;
-  return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
-}
+__device__ __forceinline__ float float_above(float x) { return key_float(ordered_key(x) + 1); }
 
 // The weight of the thread's elements from `from` up (ALL: of every one), as a sum that starts at 2^52.  Those of
 // [low, high], which is below, are gathered in sh.top.found.
@@ -473,14 +470,27 @@ __device__ __forceinline__ void draw(const SampleArgs& a, const Settings& s, int
   }
 }
 
-// The smallest logit whose weight min-p keeps: among the 64 floats around m + T ln(min_p), one to a lane.
+// The smallest logit whose weight min-p keeps, for s.least above 0.  It lies between a float that is not kept and one that is,
+// in the order of their keys: 64 floats around m + T ln((ceil(least) - 1/2) / 2^F), where a weight rounds to what is asked for,
+// nearly always hold both; next to 0, where floats lie closer than weights differ, the gap between the two is cut by 65 until
+// they are neighbours, six times more at most.
 __device__ __forceinline__ float least_logit(const Settings& s, const Weight& weight) {
-  const float near = static_cast<float>(s.top + s.temp * log(s.least / s.one));
-  if (!(near > -3.0e38f)) return -INFINITY;
-  const uint32_t key = ordered_key(near) + 32 - (threadIdx.x & 63);  // falling
-  const float x = __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
-  const u64 kept = __ballot(x <= s.top && static_cast<double>(weight(x)) >= s.least);
-  return kept ? __shfl(x, 63 - __clzll(kept), 64) : s.top;
+  const int lane = threadIdx.x & 63;
+  uint32_t low = ordered_key(-INFINITY), high = __builtin_amdgcn_readfirstlane(ordered_key(s.top));
+  const double near = s.top + s.temp * log((ceil(s.least) - 0.5) / s.one);
+  uint32_t from = ordered_key(static_cast<float>(fmax(near, static_cast<double>(kTopLow)))) - 32, step = 1;
+#pragma unroll 1
+  while (high - low > 1) {
+    const int64_t at = static_cast<int64_t>(from) + static_cast<int64_t>(step) * lane;
+    const uint32_t key = at <= low ? low : at >= high ? high : static_cast<uint32_t>(at);
+    const u64 kept = __ballot(key == high || (key > low && static_cast<double>(weight(key_float(key))) >= s.least));
+    const int first = kept ? __ffsll(kept) - 1 : 64;
+    if (first > 0) low = __builtin_amdgcn_readlane(key, first - 1);
+    if (first < 64) high = __builtin_amdgcn_readlane(key, first);
+    step = (high - low + 64) / 65;
+    from = low + step;
+  }
+  return key_float(high);
 }
 
 // WHOLE: without top-k and top-p.

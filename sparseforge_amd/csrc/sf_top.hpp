@@ -223,10 +223,11 @@ __device__ __forceinline__ u64 candidate(float x, int id) {
   return static_cast<u64>(ordered_key(x)) << 32 | static_cast<uint32_t>(~id);
 }
 __device__ __forceinline__ int candidate_id(u64 c) { return static_cast<int>(~static_cast<uint32_t>(c)); }
-__device__ __forceinline__ float candidate_logit(u64 c) {
-  const uint32_t key = static_cast<uint32_t>(c >> 32);
+// The float of an ordered_key.
+__device__ __forceinline__ float key_float(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
+__device__ __forceinline__ float candidate_logit(u64 c) { return key_float(static_cast<uint32_t>(c >> 32)); }
 
 constexpr int kTopBins = 1024;
 
