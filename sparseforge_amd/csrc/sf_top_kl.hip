@@ -5,10 +5,13 @@
 //   N = log sum_k exp b_k (then the row is renormalised, r = 0), or the given lse (then r = 1 - sum p, not below 0)
 //   KL = sum_k p_k (log p_k - log q_(i_k)) + r (log r - log q_rest),   q_rest = sum over unlisted j of q_j
 //   dKL/da_j = P q_j - p_j - r q_j / q_rest [j unlisted],              P = sum p + r
-// With Z_r the log-sum-exp of the unlisted tokens and kappa = exp(Z - Z_r) the gradient of an unlisted token is
-// (P - r kappa) q_j: one exponential.  Its derivative along u: with U = sum u_j q_j and U_r = the same over the unlisted,
-//   h_j = q_j ((P - r kappa) u_j - (P U - r kappa^2 U_r))  [unlisted],   P q_j (u_j - U)  [listed].
-// The rest's sums are formed without the listed tokens (one bit for each of the vocabulary in LDS), not as a difference.
+// With Z_r the log-sum-exp of the unlisted tokens, rho_j = exp(a_j - Z_r) and G = exp(Z_r - Z) the gradient of an unlisted
+// token is (P G - r) rho_j: one exponential, and no factor above 1, however little probability the rest has (of q_j and exp(Z -
+// Z_r) float32 holds neither from a gap of 88 on).  Its derivative along u: with U = sum u_j q_j over the vocabulary and U_r =
+// sum u_j rho_j over the unlisted,
+//   h_j = rho_j ((P G - r) u_j - (P G U - r U_r))  [unlisted],   P q_j (u_j - U)  [listed].
+// The rest's sums are formed without the listed tokens (one bit for each of the vocabulary in LDS), not as a difference, and
+// from the rest's own maximum.
 //
 // One workgroup per row streams it once forward and once backward (twice along u); listed tokens are gathered and handled
 // in f64 while the row is on its way.  Row sums are f32 exponentials in compensated sums, joined in f64; stats and losses
@@ -32,7 +35,7 @@ constexpr int kTkForwardU = DT == SF_DTYPE_BF16 ? 3 : 2;
 template <int DT>
 constexpr int kTkBackwardU = DT == SF_DTYPE_BF16 ? 4 : 2;
 constexpr int kTkSecond = 512;
-constexpr int kTkStats = 8;  // f64 of a row's RowStats
+constexpr int kTkStats = 9;  // f64 of a row's RowStats
 
 struct TopKlArgs {
   const void* s;
@@ -46,15 +49,20 @@ struct TopKlArgs {
   double inv_t;
 };
 
-// What the backward needs of a row.  Z = top / T + lz and Z_r = top / T + lzr, N = nb + ln: in two parts, so that rows of
+// What the backward needs of a row.  Z = top / T + lz and Z_r = rest_top / T + lzr, N = nb + ln: in two parts, so that rows of
 // huge logits (all at the type's lowest value, say) keep their differences.
 struct RowStats {
-  double top, lz, lzr;
+  double top, lz, rest_top, lzr;
   double nb, ln;
   double p, r;
   double twice;  // an id is listed more than once
 };
 static_assert(sizeof(RowStats) == kTkStats * sizeof(double), "stats of a row");
+
+// Z_r - Z
+__device__ __forceinline__ double rest_gap(const TopKlArgs& a, const RowStats& st) {
+  return (st.rest_top - st.top) * a.inv_t + (st.lzr - st.lz);
+}
 
 // Words of a row's marks.
 __host__ __device__ __forceinline__ int mark_words(int vocab) { return (vocab + 8) / 32 + 1; }
@@ -329,7 +337,7 @@ __global__ void __launch_bounds__(BLK) top_kl_kernel(TopKlArgs a, double* __rest
   part = parts[lane % W];
   double most[3] = {part.nb, part.ml, static_cast<double>(part.m)};
   lanes_max<W>(most);
-  const double nb = most[0], top = fmax(most[1], most[2]);
+  const double nb = most[0], rest_top = most[2], top = fmax(most[1], rest_top);
   if (part.e0 != 0.0) part.e2 += part.e0 * (part.ml == -INFINITY ? 0.0 : part.ml - top);
   if (!REST && part.nb != nb) {
     const double f = exp_from(part.nb, nb, 1.0), d = part.nb - nb;
@@ -338,10 +346,11 @@ __global__ void __launch_bounds__(BLK) top_kl_kernel(TopKlArgs a, double* __rest
     part.e2 = f == 0.0 ? 0.0 : f * part.e2;
   }
   double x[5] = {part.e0, part.e1, part.e2,
-                 part.sum == 0.0f ? 0.0 : part.sum * exp((static_cast<double>(part.m) - top) * a.inv_t),
+                 part.sum == 0.0f ? 0.0 : part.sum * exp((static_cast<double>(part.m) - rest_top) * a.inv_t),
                  part.sl == 0.0 ? 0.0 : part.sl * exp_from(part.ml, top, a.inv_t)};
   lanes_sum<W>(x);
-  const double e0 = x[0], e1 = x[1], e2 = x[2] * a.inv_t, rest = x[3], all = x[3] + x[4];
+  const double e0 = x[0], e1 = x[1], e2 = x[2] * a.inv_t, rest = x[3];
+  const double all = rest * exp((rest_top - top) * a.inv_t) + x[4];
   RowStats st{};
   if (REST) {
     st.r = e0 > 1.0 ? 0.0 : 1.0 - e0;
@@ -356,6 +365,7 @@ __global__ void __launch_bounds__(BLK) top_kl_kernel(TopKlArgs a, double* __rest
   if (!REST && e0 != 0.0) st.p = 1.0;
   if (REST) st.p = e0 + st.r;
   st.top = top;
+  st.rest_top = rest_top;
   st.lz = __shfl(l, 0, 64);
   st.lzr = __shfl(l, 1, 64);
   st.nb = nb;
@@ -363,7 +373,7 @@ __global__ void __launch_bounds__(BLK) top_kl_kernel(TopKlArgs a, double* __rest
   double kl;
   if (REST) {
     kl = e1 - e2 + e0 * st.lz;
-    if (st.r != 0.0) kl += st.r * (__shfl(l, 2, 64) - (st.lzr - st.lz));
+    if (st.r != 0.0) kl += st.r * (__shfl(l, 2, 64) - rest_gap(a, st));
   } else {
     kl = e0 == 0.0 ? 0.0 : (e1 - e2) / e0 - st.ln + st.lz;
   }
@@ -409,15 +419,19 @@ __global__ void __launch_bounds__(kTkFinal) top_kl_dot_kernel(const double* __re
   if (threadIdx.x == 0) *dot = static_cast<float>(x[0]);
 }
 
-// q = exp(s / T - Z) of a row.  The exponent in base 2, (s - top) c - lo, rounds in f32 by up to 2^-24 of itself: 1e-6 of
-// q for a token of probability 1e-7, nothing beside bf16's 2^-9; for f32 its whole part is split off and what s - top and c
-// round is carried along.
+// Of a row's unlisted tokens: with a rest rho = exp(s / T - Z_r) and `share` = G, else q = exp(s / T - Z) and 1.  The exponent
+// in base 2, (s - top) c - lo, rounds in f32 by up to 2^-24 of itself: 1e-6 of q for a token of probability 1e-7, nothing
+// beside bf16's 2^-9; for f32 its whole part is split off and what s - top and c round is carried along.  Of listed tokens it
+// may be inf.
 template <int DT>
 struct RowGrad {
+  double share;
   float hi, lo, c, c_lo, whole, part;  // lo = whole + part
   __device__ __forceinline__ RowGrad(const TopKlArgs& a, const RowStats& st) {
-    const double k = a.inv_t * 1.4426950408889634, l = st.lz * 1.4426950408889634;
-    hi = static_cast<float>(st.top);
+    const bool rest = st.r != 0.0;
+    const double k = a.inv_t * 1.4426950408889634, l = (rest ? st.lzr : st.lz) * 1.4426950408889634;
+    share = rest ? exp(rest_gap(a, st)) : 1.0;
+    hi = static_cast<float>(rest ? st.rest_top : st.top);
     lo = static_cast<float>(l);
     c = static_cast<float>(k);
     c_lo = static_cast<float>(k - static_cast<double>(c));
@@ -472,7 +486,7 @@ __global__ void __launch_bounds__(BLK) top_kl_backward_kernel(TopKlArgs a, const
     return;
   }
   const RowGrad<DT> g(a, st);
-  const float coef = static_cast<float>(f * (st.p - (st.r != 0.0 ? st.r * exp(st.lz - st.lzr) : 0.0)));
+  const float coef = static_cast<float>(f * (st.p * g.share - st.r));
   const void* rows[1] = {row_at<DT>(a.s, (r / a.inner) * a.s0 + (r % a.inner) * a.s1)};
   const Cut cut = Cut::of<DT, BLK>(out, a.vocab);  // whole 16 bytes are written rather than read
   // the listed tokens' own gradient, formed while the row is on its way and written when the row is
@@ -540,7 +554,7 @@ __global__ void __launch_bounds__(kTkSecond) top_kl_second_kernel(TopKlArgs a, c
   mark_listed<BLK>(a, r, cut, bits, flags);
   __syncthreads();
   // the listed tokens, while the row is on its way
-  double x[3] = {0.0, 0.0, 0.0};  // u . q unlisted, listed; u . p
+  double x[3] = {0.0, 0.0, 0.0};  // u . rho unlisted (see RowGrad), u . q listed; u . p
   int id0 = -1;
   double q0 = 0.0, u0 = 0.0;
   for (int k = t; k < a.k; k += BLK) {
@@ -572,10 +586,10 @@ __global__ void __launch_bounds__(kTkSecond) top_kl_second_kernel(TopKlArgs a, c
   tk_stream<DT, BLK, 1>(rows, cut, H, [] {}, dot);
   x[0] = static_cast<double>(rest);
   block_sum<3, BLK>(x, part);
-  const double kappa = st.r != 0.0 ? exp(st.lz - st.lzr) : 0.0, uq = x[0] + x[1];
-  if (t == 0) row_dot[r] = share * (st.p * uq - x[2] - st.r * kappa * x[0]);
-  const float A = static_cast<float>(f * (st.p - st.r * kappa));
-  const float B = static_cast<float>(f * (st.p * uq - st.r * kappa * kappa * x[0]));
+  const double uq = g.share * x[0] + x[1];
+  if (t == 0) row_dot[r] = share * (st.p * uq - x[2] - st.r * x[0]);
+  const float A = static_cast<float>(f * (st.p * g.share - st.r));
+  const float B = static_cast<float>(f * (st.p * g.share * uq - st.r * x[0]));
   const auto write = [&](int i, int m, float (&x)[2][8]) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) x[0][k] = g.q(x[0][k]) * fmaf(A, x[1][k], -B);
