@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(BLK) top_kl_kernel(TopKlArgs a, double* __rest
       const int id = tk_id(a, r * a.k + k);
       if (id < 0) continue;
       const double b = load_as_f32(a.values, r * a.k + k, a.vdt) * a.inv_t, s = load_as_f32(rows[0], id, DT);
-      const double e = part.nb == -INFINITY ? 0.0 : exp(b - part.nb);
+      const double e = !REST && part.nb == -INFINITY ? 0.0 : exp(b - part.nb);
       if (!(e <= 0.0)) {
         part.e0 += e;
         part.e1 += e * (b - part.nb);

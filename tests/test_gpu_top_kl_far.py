@@ -132,3 +132,24 @@ def test_rows_of_both_kinds_and_no_rest(cuda_device):
     w, = torch.autograd.grad(want, flat)
     assert abs(loss.item() - want.item()) <= 1e-5 + 1e-6 * abs(want.item())
     assert bool(((g.detach().double() - w).abs() <= 1e-5 * w.abs() + 1e-7).all()) and bool(h.isfinite().all())
+
+
+def test_a_teacher_without_any_probability_shows(cuda_device):
+    """A record of a row that is -inf throughout has a log-sum-exp of -inf: neither its entries nor the rest have a
+    probability, and the loss and the row's gradient say so.  With a weight of 0 it is not looked at."""
+    from sparseforge_amd.distill import top_kl_loss, top_logits
+
+    g = torch.Generator(device=cuda_device).manual_seed(4)
+    teacher = torch.randn(4, 500, generator=g, device=cuda_device)
+    teacher[2] = -math.inf
+    s = torch.randn(4, 500, generator=g, device=cuda_device, requires_grad=True)
+    record = top_logits(teacher, 7)
+    assert float(record.lse[2]) == -math.inf
+    loss = top_kl_loss(s, record)
+    assert not math.isfinite(loss.item())
+    grad, = torch.autograd.grad(loss, s)
+    assert not bool(grad[2].isfinite().any())
+    weights = torch.tensor([1.0, 1.0, 0.0, 1.0], device=cuda_device)
+    loss = top_kl_loss(s, record, weights=weights)
+    grad, = torch.autograd.grad(loss, s)
+    assert math.isfinite(loss.item()) and bool(grad.isfinite().all()) and bool((grad[2] == 0).all())
