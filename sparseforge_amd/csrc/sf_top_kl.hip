@@ -288,7 +288,7 @@ __global__ void __launch_bounds__(BLK) top_kl_kernel(TopKlArgs a, double* __rest
       const int id = tk_id(a, r * a.k + k);
       if (id < 0) continue;
       const double b = load_as_f32(a.values, r * a.k + k, a.vdt) * a.inv_t, s = load_as_f32(rows[0], id, DT);
-      const double e = !REST && part.nb == -INFINITY ? 0.0 : exp(b - part.nb);
+      const double e = !REST && b == -INFINITY ? 0.0 : exp(b - part.nb);  // NaN where b is, whatever the maximum says
       if (!(e <= 0.0)) {
         part.e0 += e;
         part.e1 += e * (b - part.nb);
@@ -340,10 +340,10 @@ __global__ void __launch_bounds__(BLK) top_kl_kernel(TopKlArgs a, double* __rest
   const double nb = most[0], rest_top = most[2], top = fmax(most[1], rest_top);
   if (part.e0 != 0.0) part.e2 += part.e0 * (part.ml == -INFINITY ? 0.0 : part.ml - top);
   if (!REST && part.nb != nb) {
-    const double f = exp_from(part.nb, nb, 1.0), d = part.nb - nb;
-    part.e1 = f == 0.0 ? 0.0 : f * (part.e1 + d * part.e0);
-    part.e0 = f == 0.0 ? 0.0 : f * part.e0;
-    part.e2 = f == 0.0 ? 0.0 : f * part.e2;
+    const double f = exp_from(part.nb, nb, 1.0), d = part.nb - nb, none = 0.0 * part.e0;  // 0, or NaN
+    part.e1 = f == 0.0 ? none : f * (part.e1 + d * part.e0);
+    part.e2 = f == 0.0 ? none : f * part.e2;
+    part.e0 = f == 0.0 ? none : f * part.e0;
   }
   double x[5] = {part.e0, part.e1, part.e2,
                  part.sum == 0.0f ? 0.0 : part.sum * exp((static_cast<double>(part.m) - rest_top) * a.inv_t),

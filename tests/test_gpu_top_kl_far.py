@@ -153,3 +153,33 @@ def test_a_teacher_without_any_probability_shows(cuda_device):
     loss = top_kl_loss(s, record, weights=weights)
     grad, = torch.autograd.grad(loss, s)
     assert math.isfinite(loss.item()) and bool(grad.isfinite().all()) and bool((grad[2] == 0).all())
+
+
+@pytest.mark.parametrize("rest", [True, False])
+@pytest.mark.parametrize("entries", [1, 200])
+def test_a_teachers_nan_shows(cuda_device, rest, entries):
+    """Whichever entries of a row are NaN, all of them among these, or all that one part of the workgroup has."""
+    from sparseforge_amd.distill import TopLogits, top_kl_loss
+
+    g = torch.Generator(device=cuda_device).manual_seed(5)
+    s = torch.randn(3, 700, generator=g, device=cuda_device, requires_grad=True)
+    ids = torch.rand(3, 700, generator=g, device=cuda_device).argsort(-1)[:, :entries].int()
+    values = torch.randn(3, entries, generator=g, device=cuda_device)
+    lse = torch.logsumexp(values, -1) + 0.1 if rest else None
+    for part in (slice(None), slice(0, 64), slice(64, 128), slice(entries - 1, entries)):
+        bad = values.clone()
+        bad[1, part] = math.nan
+        if not bool(bad.isnan().any()):
+            continue
+        loss = top_kl_loss(s, TopLogits(bad, ids, lse, 2.0 if rest else None))
+        assert math.isnan(loss.item())
+        grad, = torch.autograd.grad(loss, s)
+        assert bool(grad[1].isnan().any()) and bool(grad[[0, 2]].isfinite().all())
+    # entries of -inf have no probability, and without a log-sum-exp a row of nothing else adds nothing
+    none = values.clone()
+    none[1] = -math.inf
+    if not rest:
+        loss = top_kl_loss(s, TopLogits(none, ids))
+        two = top_kl_loss(s[[0, 2]], TopLogits(values[[0, 2]], ids[[0, 2]]))
+        assert abs(loss.item() - two.item() * 2 / 3) <= 1e-6 * two.item()
+        assert bool((torch.autograd.grad(loss, s)[0][1] == 0).all())
