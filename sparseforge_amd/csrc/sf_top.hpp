@@ -244,7 +244,8 @@ struct TopShared {
   int n;
 };
 
-// A bound above which at least k elements of a row lie, and few others: those with (m - x) * scale < limit.  Its place
+// A bound above which at least k elements of a row lie, and few others: those with half(x) * scale < limit, half(x) being
+// half of m - x: the whole is more than a float where logits lie at both ends of the type.  Its place
 // comes from the maxima of the threads' groups of the row: the k-th largest of these is one, and a histogram over [the
 // lowest, the highest] finds its bin.  With at least 2 k groups about 1.4 k elements lie above it.  Where many groups share
 // that bin (some logits lie far from all others: a mask of -1e4 or of the type's lowest value, say) the histogram is made
@@ -253,7 +254,8 @@ struct TopShared {
 struct Bound {
   float m, scale, limit;
   float low;  // the lowest group of those above the bound, about
-  __device__ __forceinline__ bool holds(float x) const { return (m - x) * scale < limit; }
+  __device__ __forceinline__ bool holds(float x) const { return half_below(0.5f * m, x) * scale < limit; }
+  static __device__ __forceinline__ float half_below(float half_m, float x) { return fmaf(-0.5f, x, half_m); }
 };
 
 // best: the thread's groups' maxima (no NaN, not inf), m: the row's.  Where fewer than k groups have anything above -inf
@@ -276,10 +278,9 @@ __device__ __forceinline__ Bound top_bound(const float (&best)[GROUPS], float m,
     if (t == 0) sh.limit = ~0u, sh.n = 0;
     __syncthreads();
     for (int w = 0; w < BLK / 64; ++w) low = fminf(low, sh.edge[0][w]);
-    // logits at both ends of the type are more than its largest apart
-    const float scale = fminf((kTopBins - 1) / fminf(top - low, -kTopLow), 1e30f);
+    const float half_top = 0.5f * top, scale = fminf((kTopBins - 1) / Bound::half_below(half_top, low), 2e30f);
     const auto bin_of = [&](float x) SF_INLINE {
-      return static_cast<int>(fminf((top - x) * scale, static_cast<float>(kTopBins - 1)));
+      return static_cast<int>(fminf(Bound::half_below(half_top, x) * scale, static_cast<float>(kTopBins - 1)));
     };
 #pragma unroll
     for (int g = 0; g < GROUPS; ++g)
@@ -298,8 +299,8 @@ __device__ __forceinline__ Bound top_bound(const float (&best)[GROUPS], float m,
     __syncthreads();
     const uint32_t limit = sh.limit;
     if (limit == ~0u) return {m, 1.0f, INFINITY, low};
-    if (again == 0 || static_cast<int>(sh.start[0]) <= 16 + k / 4) 
-      return {top, scale, static_cast<float>(limit + 1), fmaxf(low, top - static_cast<float>(limit + 1) / scale)};
+    if (again == 0 || static_cast<int>(sh.start[0]) <= 16 + k / 4)
+      return {top, scale, static_cast<float>(limit + 1), fmaxf(low, top - 2.0f * (static_cast<float>(limit + 1) / scale))};
     above = sh.start[1];
     float first = -INFINITY, last = INFINITY;
 #pragma unroll
@@ -314,7 +315,7 @@ __device__ __forceinline__ Bound top_bound(const float (&best)[GROUPS], float m,
     __syncthreads();
     low = INFINITY, top = -INFINITY;
     for (int w = 0; w < BLK / 64; ++w) low = fminf(low, sh.edge[0][w]), top = fmaxf(top, sh.edge[1][w]);
-    if (low == top) return {top, 1e30f, 1.0f, low};  // equal ones, and what is larger
+    if (low == top) return {top, 2e30f, 1.0f, low};  // equal ones, and what is larger
   }
 }
 
