@@ -234,7 +234,6 @@ constexpr int kTopBins = 1024;
 // CAP: candidates that there is room for.
 template <int CAP>
 struct TopShared {
-  static constexpr int kCap = CAP;
   uint32_t bins[kTopBins];
   u64 found[CAP], mixed[CAP];
   uint32_t start[kTopBins + 1];
