@@ -87,11 +87,12 @@ class RetrainStep:
     """Callable step over (student, teacher, optimizer); `batches` is a list of grad_accum (X, Y) pairs.
 
     A batch may be (X, Y, record), the record being the teacher's logits of X as distill.top_logits gives them (at the
-    default temperature of 2): then no teacher runs, and where every batch has one the teacher may be None."""
+    default temperature of 2): then no teacher runs, and where every batch has one (or hardness_kldiv is 0) the teacher may
+    be None."""
 
     def __init__(self, student, teacher, optimizer, cfg: RetrainConfig, timed: bool = False, on_grads=None):
         self.student = student
-        self.model = Distill_Model(student, teacher, top=cfg.teacher_top)
+        self.model = Distill_Model(student, teacher, top=cfg.teacher_top if teacher is not None else 0)
         self.optimizer = optimizer
         self.cfg = cfg
         self.timed = timed
@@ -110,6 +111,8 @@ class RetrainStep:
         cfg = self.cfg
         if len(batches) != cfg.grad_accum:
             raise ValueError(f"expected {cfg.grad_accum} micro-batches, got {len(batches)}")
+        if self.model.teacher is None and cfg.hardness_kldiv and any(len(b) < 3 or b[2] is None for b in batches):
+            raise ValueError("RetrainStep: there is no teacher, and a batch has no record of one")
         ev: dict = {}
         lam = lambda_mid_at(cfg, iter_num)
         total = 0.0

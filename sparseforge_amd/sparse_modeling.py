@@ -683,7 +683,8 @@ class Distill_Model(torch.nn.Module):
 
     Beyond the reference: with top > 0 the KL is that from the teacher's `top` largest logits and the probability of all
     other tokens together (distill.top_kl_loss); forward also takes such a record of the teacher's (distill.TopLogits) as
-    teacher_top, and then runs no teacher, which may be None."""
+    teacher_top, and then runs no teacher, which may be None.  Without a teacher and a record the KL is 0, and with top > 0
+    the call is refused."""
 
     def __init__(self, model, teacher=None, output_hidden_state=False, top=0):
         super().__init__()
@@ -717,6 +718,8 @@ class Distill_Model(torch.nn.Module):
             student_logits, task_loss, _ = self.student(idx, targets)
             return student_logits, task_loss, None, top_kl_loss(student_logits, teacher_top)
         if self.teacher is None:
+            if self.top:
+                raise ValueError(f"Distill_Model: the KL from the teacher's top {self.top} needs a teacher or a record")
             student_logits, task_loss, _ = self.student(idx, targets)
             return student_logits, task_loss, None, torch.tensor(0.0, device=idx.device)
         if self.output_hidden_state:
