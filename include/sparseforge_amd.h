@@ -471,8 +471,9 @@ int sf_top_logits(const sf_top_logits_desc* desc, void* stream);
  *   below 0) with lse, else 0; q_rest = sum of q over the unlisted tokens
  *   KL = sum_k p_k (log p_k - log q_(i_k)) + r (log r - log q_rest)
  *   loss = T^2 sum_rows w KL / sum_rows w      (w = weights, null: 1)
- * Rows of weight 0 are not looked at; rows without entries add 0; without any
- * weight the loss is 0.  An id that is listed twice counts twice.
+ * Rows of weight 0 are not looked at; rows without entries, or without lse and
+ * with entries of -inf alone, add 0; without any weight the loss is 0.  An id
+ * that is listed twice counts twice.
  * stats: device double[sf_top_kl_stats_size / 8] and norm: device double, both
  * written by the forward and read by the others.  Sums of rows are formed in
  * a fixed order.

@@ -246,7 +246,8 @@ struct TopShared {
 // A bound above which at least k elements of a row lie, and few others: those with half(x) * scale < limit, half(x) being
 // half of m - x: the whole is more than a float where logits lie at both ends of the type.  Its place
 // comes from the maxima of the threads' groups of the row: the k-th largest of these is one, and a histogram over [the
-// lowest, the highest] finds its bin.  With at least 2 k groups about 1.4 k elements lie above it.  Where many groups share
+// lowest, the highest] finds its bin.  With at least 2 k groups about 1.4 k elements lie above it, with hardly more than k
+// nearly all, and a row of less than 8 k logits has fewer: then the bound takes everything above -inf.  Where many groups share
 // that bin (some logits lie far from all others: a mask of -1e4 or of the type's lowest value, say) the histogram is made
 // again over what the bin holds: 512 rows of 131072 bf16, of which such a mask leaves one in 15, k 20: 39 us, 502 by the
 // bits of every logit, 37 without the mask.
@@ -486,7 +487,8 @@ __device__ __forceinline__ uint32_t hits_of(const float (&best)[G], const Bound&
 
 // ---------------------------------------------------------------------------
 // Passes that are right for every row, whatever its order and its equal values, for the rows in which gather() finds too
-// many (512 rows of 131072 equal bf16 logits: k 20 250 us, k 50 drawn 290, top-p 0.9 drawn 550).  Thread t takes elements
+// many (512 rows of 131072 equal bf16 logits: k 20 250 us, k 50 drawn 290, top-p 0.9 drawn 550; rows that have more than CAP
+// logits and not much more than 8 k: 256 x 8192 bf16, k 1000, 38 us, 15 with k 600).  Thread t takes elements
 // [8 t, 8 t + 8) of tiles of 8 * BLK, so that tiles, waves and lanes follow each other in the order of the ids.
 // ---------------------------------------------------------------------------
 // A row's order as integers: larger logits have larger keys, -0 equals 0, NaN is largest.  bf16 needs 16 bits.

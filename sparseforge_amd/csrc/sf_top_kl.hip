@@ -16,10 +16,10 @@
 // One workgroup per row streams it once forward and once backward (twice along u); listed tokens are gathered and handled
 // in f64 while the row is on its way.  Row sums are f32 exponentials in compensated sums, joined in f64; stats and losses
 // are f64.  Bound by memory: forward and backward by turns 4096 x 32000 bf16, k 64, 143 us (two reads and a write of 262
-// MB: 5.5 TB/s, what a copy reaches), 2048 x 131072 269 (6.0 TB/s, part of the second read from the last-level cache),
-// 2046 x 50257 f32 with rows of odd alignment 202 (6.1 TB/s); along u 1024 x 32000 45 (two rows read, one written, 4.4
-// TB/s).  64 x 32000 forward 7 us and 3 for the sum over the rows.  Two products of log-softmax over the vocabulary, as the
-// formula stands, take ten passes and more.
+// MB: 5.5 TB/s, what a copy reaches), 2048 x 131072 333 (4.8 TB/s; with a fifth of the rows of weight 0, whose zeros are
+// written alone, 270), 2046 x 50257 f32 with rows of odd alignment 248 (5.0 TB/s; 202 with three rows in ten of weight 0);
+// along u 1024 x 32000 46 (two rows read, one written, 4.3 TB/s).  64 x 32000 forward 7 us and 3 for the sum over the rows.
+// Two products of log-softmax over the vocabulary, as the formula stands, take ten passes and more.
 #include <type_traits>
 
 #include "sf_top.hpp"
@@ -29,7 +29,7 @@ namespace {
 
 // Pieces of a row that a thread loads before it uses them: bytes on their way against registers.  Forward and backward by
 // turns, us: 4096 x 32000 bf16 142 with 3 and 4 pieces, 146 with 2 and 2; 2046 x 50257 f32, whose pieces are twice as
-// long, 212 and 202.
+// long, three rows in ten of weight 0, 212 and 202.
 template <int DT>
 constexpr int kTkForwardU = DT == SF_DTYPE_BF16 ? 3 : 2;
 template <int DT>
@@ -514,8 +514,8 @@ __global__ void __launch_bounds__(BLK) top_kl_backward_kernel(TopKlArgs a, const
 }
 
 // Along u (rows contiguous): h_j, and the row's u . dL/ds at an upstream gradient of 1.  Of the pieces that both passes need
-// the first H of a thread stay in registers: 4096 x 32000 bf16 167 us with 6, 185 with 2; 2046 x 50257 f32 248 with 3,
-// 259 with 1.
+// the first H of a thread stay in registers: 4096 x 32000 bf16 167 us with 6, 185 with 2; 2046 x 50257 f32, three rows in
+// ten of weight 0, 248 with 3, 259 with 1 (every row: 307 with 3).
 template <int DT, bool PAST>
 __global__ void __launch_bounds__(kTkSecond) top_kl_second_kernel(TopKlArgs a, const double* __restrict__ stats,
                                                                   const double* __restrict__ norm,
@@ -615,7 +615,7 @@ constexpr int64_t kTkFewRows = 256;
 // launch(data type, whether what it writes passes the caches).  A gradient that the last-level cache (256 MB) does not hold
 // beside the logits is not found there by who reads it next, and what of it stays there has to be written back while the
 // next pass reads: forward and backward by turns, 4096 x 32000 bf16 143 us past the caches and 167 through them, 2048 x
-// 131072 270 and 314; 1024 x 32000 (66 MB) 45 and 43.
+// 131072, a fifth of the rows of weight 0, 270 and 314; 1024 x 32000 (66 MB) 45 and 43.
 template <typename F>
 void tk_dispatch(const sf_top_kl_desc& d, F&& launch) {
   const bool past = d.rows * d.vocab * (d.dtype == SF_DTYPE_F32 ? 4 : 2) > (128ll << 20);

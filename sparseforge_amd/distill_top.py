@@ -136,9 +136,10 @@ def top_kl_loss(student_logits: torch.Tensor, teacher: TopLogits, temperature=2,
     the same rows, as float32 (see the module).
 
     weights: float32 [..], 1 where None; rows of weight 0 (prompts, padding) are not looked at and take a zero gradient.
-    Rows without entries add 0; without any weight the loss is 0.  An id that is listed twice counts twice.  A row has at
-    most 4096 entries, and no more than V.  Logits are
-    not clamped and nothing is dropped: what is not finite shows in the loss.  Only the student takes a gradient."""
+    Rows without entries, or without a log-sum-exp and with entries of -inf alone, add 0; without any weight the loss is 0.
+    An id that is listed twice counts twice.  A row has at most 4096 entries, and no more than V.  Logits are not clamped
+    and nothing is dropped: what is not finite shows in the loss, a log-sum-exp of -inf (a teacher's row that is masked
+    throughout) too.  Only the student takes a gradient.  Temperatures lie in 1e-30 .. 1e30."""
     values, ids, lse, at = teacher
     dev = L.require_device_only(student_logits, values, ids, lse, weights)
     L.dtype_code(student_logits)

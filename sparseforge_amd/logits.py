@@ -113,7 +113,9 @@ def sample_logits(logits: torch.Tensor, uniform: torch.Tensor, *, temperature=1.
     their whole weight, its log-probability the logarithm of its share.  Temperature 0 takes the largest logit of the
     lowest id.  Each setting is a number, or a tensor [B] on the device (top_k int32, the others float32; what lies
     outside a setting's range there counts as its nearest end).  A row that holds a NaN, or nothing above -inf (a mask that
-    allows nothing), has no token: -1, with a log-probability of NaN or -inf.  V is at most 262144."""
+    allows nothing), has no token: -1, with a log-probability of NaN or -inf.  V is at most 262144.  Weights are whole
+    numbers of 2^-44 of the largest (2^-43, 2^-42 above 65536, 131072 tokens), and a min_p above 0 keeps what has one of at
+    least 1.  Forward only: the log-probabilities take no gradient."""
     dev = logits.device
     for t in (logits, uniform):
         if not t.is_cuda or t.get_device() != dev.index:
