@@ -183,3 +183,25 @@ def test_a_teachers_nan_shows(cuda_device, rest, entries):
         two = top_kl_loss(s[[0, 2]], TopLogits(values[[0, 2]], ids[[0, 2]]))
         assert abs(loss.item() - two.item() * 2 / 3) <= 1e-6 * two.item()
         assert bool((torch.autograd.grad(loss, s)[0][1] == 0).all())
+
+
+def test_gradients_that_pass_the_caches(cuda_device):
+    """More than 128 MB of them: four copies of 300 rows, whose listed tokens lie where float32 has no rho, have a fourth of
+    these rows' gradients and products to the bit, the listed tokens' written over what came before."""
+    from sparseforge_amd.distill import TopLogits, top_kl_loss
+
+    t = _inputs(cuda_device, (300,), 32000, 70, torch.float32, padded=False, weighted=False)
+    at, lse = t["ids"].long(), _lse(t, 1.0)
+    t["s"] = t["s"].scatter(1, at, t["s"].gather(1, at) + 150.0)
+    u = torch.randn(300, 32000, generator=t["g"], device=cuda_device)
+    seen = []
+    for copies in (1, 4):
+        s = t["s"].repeat(copies, 1).requires_grad_(True)
+        teacher = TopLogits(t["values"].repeat(copies, 1), t["ids"].repeat(copies, 1), lse.repeat(copies), 1.0)
+        g, = torch.autograd.grad(top_kl_loss(s, teacher, 1.0) * copies, s, create_graph=True)
+        h, = torch.autograd.grad(g, s, u.repeat(copies, 1))
+        seen.append((g.detach(), h))
+    for one, four in zip(*seen):
+        assert bool(one.isfinite().all()) and bool((one != 0).any())
+        for part in four.split(300):
+            assert torch.equal(part, one)
